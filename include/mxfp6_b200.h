@@ -26,7 +26,7 @@
 extern "C" {
 #endif
 
-#define MXFP6_B200_ABI_VERSION 5
+#define MXFP6_B200_ABI_VERSION 6
 
 #define MXFP6_DTYPE_F16 0
 #define MXFP6_DTYPE_BF16 1
@@ -467,6 +467,63 @@ int mxfp6_workspace_stats(int64_t out_stats[10]);
 int mxfp6_workspace_barriers_zero(int* all_zero);
 /* Drops every lane and returns the arena to its initial state (test helper). */
 int mxfp6_workspace_reset(void);
+
+/* ---- paged 8-bit KV cache, attention over it, rotary positions ----------- */
+
+/* The cache: E4M3 values [pages, kv_heads, page_size, head_dim] and UE8M0 scales
+ * [pages, kv_heads, page_size / 32], contiguous, values 16-byte aligned; page_size 32, 64 or
+ * 128, head_dim 64, 128 or 256, pages * kv_heads * page_size < 2^31.
+ * A batch: block_table [batch, table_width] int32 with table_stride elements between rows (an
+ * id outside [0, pages) names no page), seq_lens [batch] int32 = tokens of each sequence
+ * including the rows of this call, cu_seqlens [batch + 1] int32 or NULL (one row a sequence):
+ * rows [cu_seqlens[b], cu_seqlens[b + 1]) of the token tensors are the last positions of
+ * sequence b.  `tokens` = rows of the token tensors; rows behind cu_seqlens[batch] stay as they
+ * were.  The three arrays are device memory; no content of theirs leads out of bounds. */
+int mxfp6_kv_cache_write(uint8_t* k_values, uint8_t* v_values, uint8_t* k_scales,
+                         uint8_t* v_scales, int64_t pages, int kv_heads, int page_size,
+                         int head_dim, const int32_t* block_table, const int32_t* seq_lens,
+                         const int32_t* cu_seqlens, int64_t table_stride, int64_t tokens,
+                         int table_width, int batch, const void* k, const void* v, int dtype,
+                         int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride,
+                         int64_t v_head_stride, void* stream);
+/* k_out, v_out: contiguous [tokens, kv_heads, head_dim] of `dtype`, 16-byte aligned. */
+int mxfp6_kv_cache_read(const uint8_t* k_values, const uint8_t* v_values, const uint8_t* k_scales,
+                        const uint8_t* v_scales, int64_t pages, int kv_heads, int page_size,
+                        int head_dim, const int32_t* block_table, const int32_t* seq_lens,
+                        const int32_t* cu_seqlens, int64_t table_stride, int64_t tokens,
+                        int table_width, int batch, void* k_out, void* v_out, int dtype,
+                        void* stream);
+/* Scratch bytes of one attention call (0: none needed, -1: sizes it would refuse).
+ * max_context = table_width * page_size. */
+int64_t mxfp6_kv_cache_attention_workspace(int64_t batch, int64_t tokens, int64_t max_query_len,
+                                           int q_heads, int kv_heads, int head_dim, int dtype,
+                                           int64_t max_context);
+/* softmax(scale * q k^T) v per query head over the cached tokens of its sequence (up to the
+ * row's own position when causal != 0); strides in elements.  The workspace needs no
+ * initialisation; concurrent calls need one each. */
+int mxfp6_kv_cache_attention(const uint8_t* k_values, const uint8_t* v_values,
+                             const uint8_t* k_scales, const uint8_t* v_scales, int64_t pages,
+                             int kv_heads, int page_size, int head_dim,
+                             const int32_t* block_table, const int32_t* seq_lens,
+                             const int32_t* cu_seqlens, int64_t table_stride, int64_t tokens,
+                             int table_width, int batch, const void* q, void* out, int dtype,
+                             int q_heads, int64_t q_token_stride, int64_t q_head_stride,
+                             int64_t out_token_stride, int64_t out_head_stride,
+                             int64_t max_query_len, float scale, int causal, void* workspace,
+                             int64_t workspace_bytes, void* stream);
+/* Turns pair i of every head of q [tokens, q_heads, dim] and k [tokens, k_heads, dim] by
+ * positions[axis[i], token] * inv_freq[i] radians, i < half; out may be the input.  Pairs are
+ * (i, i + half), or (2 i, 2 i + 1) when adjacent != 0.  positions: int32, or int64 when
+ * wide_positions != 0.  Either tensor may have zero heads. */
+int mxfp6_rotary_multi_axis(const void* q, void* q_out, int q_heads, int64_t q_token_stride,
+                            int64_t q_head_stride, int64_t q_out_token_stride,
+                            int64_t q_out_head_stride, const void* k, void* k_out, int k_heads,
+                            int64_t k_token_stride, int64_t k_head_stride,
+                            int64_t k_out_token_stride, int64_t k_out_head_stride, int dtype,
+                            int64_t tokens, int dim, const void* positions,
+                            int64_t position_stride, int axes, int wide_positions,
+                            const double* inv_freq, const int32_t* axis, int half, int adjacent,
+                            void* stream);
 
 #ifdef __cplusplus
 }

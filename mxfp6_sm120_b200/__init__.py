@@ -105,6 +105,17 @@ from .qwen35 import (
     shared_expert_out,
 )
 
+from .kv_cache import (
+    KV_HEAD_DIMS,
+    KV_PAGE_SIZES,
+    PagedKVCache,
+    RotaryFrequencies,
+    kv_cache_attention,
+    kv_cache_read,
+    kv_cache_write,
+    rotary_frequencies,
+    rotary_multi_axis,
+)
 from .checkpoint import MoeLayerCheckpoint, TensorSource, load_linear, load_moe_layer
 from .adapter import MxFp6LinearKernel, MxFp6MoERunner
 from . import torch_ops  # registers torch.ops.mxfp6.* (the reference's dispatcher names)

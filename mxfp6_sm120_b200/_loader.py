@@ -20,6 +20,11 @@ _LIBRARY_PATH: Path | None = None
 _I64P = POINTER(c_int64)
 _IP = POINTER(c_int)
 
+# The paged KV cache (four pointers, pages, heads, page size, head size) and a batch of sequences
+# (block table, lengths, row offsets, table stride, rows, table width, sequences).
+_KV_CACHE = [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_int]
+_KV_BATCH = [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int, c_int]
+
 # name -> (restype, argtypes); every symbol declared in include/mxfp6_b200.h.
 SIGNATURES: dict[str, tuple] = {
     "mxfp6_b200_abi_version": (c_int, []),
@@ -192,6 +197,30 @@ SIGNATURES: dict[str, tuple] = {
         c_int,
         [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int64,
          c_int, c_int, c_int64, c_void_p],
+    ),
+    "mxfp6_kv_cache_write": (
+        c_int,
+        [*_KV_CACHE, *_KV_BATCH, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int64,
+         c_void_p],
+    ),
+    "mxfp6_kv_cache_read": (
+        c_int,
+        [*_KV_CACHE, *_KV_BATCH, c_void_p, c_void_p, c_int, c_void_p],
+    ),
+    "mxfp6_kv_cache_attention_workspace": (
+        c_int64,
+        [c_int64, c_int64, c_int64, c_int, c_int, c_int, c_int, c_int64],
+    ),
+    "mxfp6_kv_cache_attention": (
+        c_int,
+        [*_KV_CACHE, *_KV_BATCH, c_void_p, c_void_p, c_int, c_int, c_int64, c_int64, c_int64,
+         c_int64, c_int64, c_float, c_int, c_void_p, c_int64, c_void_p],
+    ),
+    "mxfp6_rotary_multi_axis": (
+        c_int,
+        [c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int,
+         c_int64, c_int64, c_int64, c_int64, c_int, c_int64, c_int, c_void_p, c_int64, c_int, c_int,
+         c_void_p, c_void_p, c_int, c_int, c_void_p],
     ),
     "mxfp6_workspace_begin_planning": (c_int, []),
     "mxfp6_workspace_finalize_planning": (c_int, [c_void_p, _I64P]),

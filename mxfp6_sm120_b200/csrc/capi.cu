@@ -7,6 +7,7 @@
 #include "../../include/mxfp6_b200.h"
 
 #include "gemm.cuh"
+#include "kv_cache.cuh"
 
 #include <algorithm>
 #include <map>
@@ -61,6 +62,16 @@ int unpack_scales(const uint8_t*, int64_t, int64_t, uint8_t*, cudaStream_t);
 int grouped_scale_offsets(const int64_t*, int, int64_t*, cudaStream_t);
 int pack_grouped_scales(const uint8_t*, const int64_t*, const int64_t*, int, int64_t, int64_t,
                         uint8_t*, cudaStream_t);
+
+int kv_cache_write(const KvCache&, const KvBatch&, const void*, const void*, int, const int64_t[4],
+                   cudaStream_t);
+int kv_cache_read(const KvCache&, const KvBatch&, void*, void*, int, cudaStream_t);
+int64_t kv_cache_attention_workspace(int64_t, int64_t, int64_t, int, int, int, int, int64_t);
+int kv_cache_attention(const KvCache&, const KvBatch&, const void*, void*, int, int,
+                       const int64_t[4], int64_t, float, int, void*, int64_t, cudaStream_t);
+int rotary_multi_axis(const void*, void*, int, const int64_t[4], const void*, void*, int,
+                      const int64_t[4], int, int64_t, int, const void*, int64_t, int, int,
+                      const double*, const int32_t*, int, int, cudaStream_t);
 
 int moe_topk_quant(const void*, const void*, int64_t, int, int, int, int, uint8_t*, uint8_t*,
                    uint8_t*, float*, int32_t*, cudaStream_t);
@@ -925,6 +936,79 @@ int mxfp6_workspace_reset(void) {
     g_arenas.erase(it);
   }
   return kOk;
+}
+
+int mxfp6_kv_cache_write(uint8_t* k_values, uint8_t* v_values, uint8_t* k_scales,
+                         uint8_t* v_scales, int64_t pages, int kv_heads, int page_size,
+                         int head_dim, const int32_t* block_table, const int32_t* seq_lens,
+                         const int32_t* cu_seqlens, int64_t table_stride, int64_t tokens,
+                         int table_width, int batch, const void* k, const void* v, int dtype,
+                         int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride,
+                         int64_t v_head_stride, void* stream) {
+  const int64_t strides[4] = {k_token_stride, k_head_stride, v_token_stride, v_head_stride};
+  return kv_cache_write(
+      KvCache{k_values, v_values, k_scales, v_scales, pages, kv_heads, page_size, head_dim},
+      KvBatch{block_table, seq_lens, cu_seqlens, table_stride, tokens, table_width, batch}, k, v,
+      dtype, strides, static_cast<cudaStream_t>(stream));
+}
+
+int mxfp6_kv_cache_read(const uint8_t* k_values, const uint8_t* v_values, const uint8_t* k_scales,
+                        const uint8_t* v_scales, int64_t pages, int kv_heads, int page_size,
+                        int head_dim, const int32_t* block_table, const int32_t* seq_lens,
+                        const int32_t* cu_seqlens, int64_t table_stride, int64_t tokens,
+                        int table_width, int batch, void* k_out, void* v_out, int dtype,
+                        void* stream) {
+  return kv_cache_read(
+      KvCache{const_cast<uint8_t*>(k_values), const_cast<uint8_t*>(v_values),
+              const_cast<uint8_t*>(k_scales), const_cast<uint8_t*>(v_scales), pages, kv_heads,
+              page_size, head_dim},
+      KvBatch{block_table, seq_lens, cu_seqlens, table_stride, tokens, table_width, batch}, k_out,
+      v_out, dtype, static_cast<cudaStream_t>(stream));
+}
+
+int64_t mxfp6_kv_cache_attention_workspace(int64_t batch, int64_t tokens, int64_t max_query_len,
+                                           int q_heads, int kv_heads, int head_dim, int dtype,
+                                           int64_t max_context) {
+  return kv_cache_attention_workspace(batch, tokens, max_query_len, q_heads, kv_heads, head_dim,
+                                      dtype, max_context);
+}
+
+int mxfp6_kv_cache_attention(const uint8_t* k_values, const uint8_t* v_values,
+                             const uint8_t* k_scales, const uint8_t* v_scales, int64_t pages,
+                             int kv_heads, int page_size, int head_dim,
+                             const int32_t* block_table, const int32_t* seq_lens,
+                             const int32_t* cu_seqlens, int64_t table_stride, int64_t tokens,
+                             int table_width, int batch, const void* q, void* out, int dtype,
+                             int q_heads, int64_t q_token_stride, int64_t q_head_stride,
+                             int64_t out_token_stride, int64_t out_head_stride,
+                             int64_t max_query_len, float scale, int causal, void* workspace,
+                             int64_t workspace_bytes, void* stream) {
+  const int64_t strides[4] = {q_token_stride, q_head_stride, out_token_stride, out_head_stride};
+  return kv_cache_attention(
+      KvCache{const_cast<uint8_t*>(k_values), const_cast<uint8_t*>(v_values),
+              const_cast<uint8_t*>(k_scales), const_cast<uint8_t*>(v_scales), pages, kv_heads,
+              page_size, head_dim},
+      KvBatch{block_table, seq_lens, cu_seqlens, table_stride, tokens, table_width, batch}, q, out,
+      dtype, q_heads, strides, max_query_len, scale, causal, workspace, workspace_bytes,
+      static_cast<cudaStream_t>(stream));
+}
+
+int mxfp6_rotary_multi_axis(const void* q, void* q_out, int q_heads, int64_t q_token_stride,
+                            int64_t q_head_stride, int64_t q_out_token_stride,
+                            int64_t q_out_head_stride, const void* k, void* k_out, int k_heads,
+                            int64_t k_token_stride, int64_t k_head_stride,
+                            int64_t k_out_token_stride, int64_t k_out_head_stride, int dtype,
+                            int64_t tokens, int dim, const void* positions,
+                            int64_t position_stride, int axes, int wide_positions,
+                            const double* inv_freq, const int32_t* axis, int half, int adjacent,
+                            void* stream) {
+  const int64_t q_strides[4] = {q_token_stride, q_head_stride, q_out_token_stride,
+                                q_out_head_stride};
+  const int64_t k_strides[4] = {k_token_stride, k_head_stride, k_out_token_stride,
+                                k_out_head_stride};
+  return rotary_multi_axis(q, q_out, q_heads, q_strides, k, k_out, k_heads, k_strides, dtype,
+                           tokens, dim, positions, position_stride, axes, wide_positions, inv_freq,
+                           axis, half, adjacent, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"
