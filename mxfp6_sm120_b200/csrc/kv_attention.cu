@@ -6,26 +6,17 @@
 //
 // First form: four warps per (token row, query head); each walks every fourth block of 32 tokens
 // with a running maximum and sum, and the four results are joined in a fixed order.
-#include "kv_cache.cuh"
-
-#include <cuda_fp8.h>
-#include <type_traits>
+#include "kv_attention.cuh"
 
 namespace mx {
+
+int launch_kv_decode(const AttentionArgs& a, int dtype, cudaStream_t stream);
+int64_t kv_decode_workspace(int64_t batch, int kv_heads, int head_dim, int rows, int64_t max_context);
+int* device_status_word(int device);
+
 namespace {
 
 constexpr int kWarps = 4;
-
-struct AttentionArgs {
-  KvCache cache;
-  KvBatch batch;
-  const void* q;
-  void* out;
-  int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;
-  int q_heads;
-  float scale_log2;  // softmax scale * log2(e)
-  int causal;
-};
 
 __device__ __forceinline__ float2 values2(uint32_t codes) {
   const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(codes & 0xffffu), __NV_E4M3);
@@ -154,7 +145,68 @@ void launch_rows(const AttentionArgs& a, cudaStream_t stream) {
   if (a.cache.head_dim == 256) kv_attention_rows_kernel<T, 256><<<grid, kWarps * 32, 0, stream>>>(a);
 }
 
+constexpr int kDecodeRows = 32;  // rows (tokens x group) of a sequence that the decode kernel takes
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                              const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                              const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeFn encode_fn() {
+  static EncodeFn fn = []() -> EncodeFn {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) !=
+            cudaSuccess ||
+        q != cudaDriverEntryPointSuccess) {
+      return nullptr;
+    }
+    return reinterpret_cast<EncodeFn>(p);
+  }();
+  return fn;
+}
+
 }  // namespace
+
+// The cache's values as rows of head_dim bytes, copied one page x 128 (64) columns at a time.
+int make_kv_map(CUtensorMap* map, const uint8_t* values, const KvCache& cache) {
+  EncodeFn fn = encode_fn();
+  if (fn == nullptr) {
+    set_error("cuTensorMapEncodeTiled is not available from the CUDA driver");
+    return kCudaError;
+  }
+  const cuuint64_t dims[2] = {(cuuint64_t)cache.head_dim,
+                              (cuuint64_t)(cache.pages * cache.kv_heads * cache.page_size)};
+  const cuuint64_t strides[1] = {(cuuint64_t)cache.head_dim};
+  const cuuint32_t inner = cache.head_dim < 128 ? cache.head_dim : 128;
+  const cuuint32_t box[2] = {inner, (cuuint32_t)cache.page_size};
+  const cuuint32_t estr[2] = {1, 1};
+  const CUresult rc = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(values), dims,
+                         strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         inner == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (rc != CUDA_SUCCESS) {
+    set_error("cuTensorMapEncodeTiled failed with CUresult %d for the cache", (int)rc);
+    return kCudaError;
+  }
+  return kOk;
+}
+
+int64_t kv_cache_attention_workspace(int64_t batch, int64_t tokens, int64_t max_query_len,
+                                     int q_heads, int kv_heads, int head_dim, int dtype,
+                                     int64_t max_context) {
+  (void)tokens;
+  (void)dtype;
+  if (batch < 1 || max_query_len < 1 || q_heads < 1 || kv_heads < 1 || q_heads % kv_heads != 0 ||
+      (head_dim != 64 && head_dim != 128 && head_dim != 256) || max_context < 1) {
+    return -1;
+  }
+  const int64_t rows = max_query_len * (q_heads / kv_heads);
+  if (rows > kDecodeRows) return 0;
+  return kv_decode_workspace(batch, kv_heads, head_dim, (int)rows, max_context);
+}
 
 int kv_cache_attention(const KvCache& cache, const KvBatch& batch, const void* q, void* out,
                        int dtype, int q_heads, const int64_t strides[4], int64_t max_query_len,
@@ -167,18 +219,40 @@ int kv_cache_attention(const KvCache& cache, const KvBatch& batch, const void* q
   MX_REQUIRE(max_query_len >= 1, "max_query_len must be positive");
   if (batch.tokens == 0) return kOk;
   MX_REQUIRE(q != nullptr && out != nullptr, "q and out must not be null");
-  (void)workspace;
-  (void)workspace_bytes;
-  AttentionArgs a{cache, batch, q, out, strides[0], strides[1], strides[2], strides[3], q_heads,
-                  scale * 1.4426950408889634f, causal};
+  const int64_t need = kv_cache_attention_workspace(
+      batch.batch, batch.tokens, max_query_len, q_heads, cache.kv_heads, cache.head_dim, dtype,
+      (int64_t)batch.table_width * cache.page_size);
+  MX_REQUIRE(workspace_bytes >= need && (need == 0 || aligned16(workspace)) &&
+                 (need == 0 || workspace != nullptr),
+             "the workspace must be 16-byte aligned and hold %lld bytes", (long long)need);
+  int device = 0;
+  MX_CUDA(cudaGetDevice(&device));
+  AttentionArgs a{};
+  a.cache = cache;
+  a.batch = batch;
+  a.q = q;
+  a.out = out;
+  a.partials = static_cast<float*>(workspace);
+  a.status = device_status_word(device);
+  if (a.status == nullptr) return kCudaError;
+  a.q_token_stride = strides[0];
+  a.q_head_stride = strides[1];
+  a.out_token_stride = strides[2];
+  a.out_head_stride = strides[3];
+  a.q_heads = q_heads;
+  a.group = q_heads / cache.kv_heads;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.causal = causal;
+  a.vector = aligned16(q) && strides[0] % 8 == 0 && strides[1] % 8 == 0;
+  const int64_t rows = max_query_len * a.group;
+  if (rows <= kDecodeRows) {
+    a.max_rows = (int)rows;
+    return launch_kv_decode(a, dtype, stream);
+  }
   if (dtype == kBF16) launch_rows<__nv_bfloat16>(a, stream);
   else launch_rows<__half>(a, stream);
   MX_CUDA(cudaGetLastError());
   return kOk;
-}
-
-int64_t kv_cache_attention_workspace(int64_t, int64_t, int64_t, int, int, int, int, int64_t) {
-  return 0;
 }
 
 }  // namespace mx

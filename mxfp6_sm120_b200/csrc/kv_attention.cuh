@@ -1,0 +1,91 @@
+// What the attention kernels over the paged 8-bit cache share: arguments, number formats, and
+// the walk of a CTA along its share of the (sequence, head, tile) work list.
+//
+// Numbers.  Keys and values enter the tensor cores as they lie in the cache (E4M3 under UE8M0
+// block scales, kind::mxf8f6f4).  The other operand of each product, 16-bit queries and 32-bit
+// weights, becomes a sum of E4M3 terms x = t0 + t1 / 16 (+ t2 / 256): a term keeps four
+// significant bits, rounding to nearest makes the remainder at most half a step (2^-4 relative to
+// the binade), so each further term takes four more.  Two terms hold a BF16 query (8 bits)
+// exactly, three an FP16 one (11 bits); for the weights the error is at most 2^-9 and 2^-14.  The
+// products of all terms accumulate in 32 bits.
+#pragma once
+
+#include "kv_cache.cuh"
+#include "ptx.cuh"
+#include "wait.cuh"
+
+#include <cuda_fp8.h>
+#include <type_traits>
+
+namespace mx {
+
+constexpr int kKvTile = 128;                       // cached tokens per tile
+constexpr int kKvTileBlocks = kKvTile / kKvBlock;  // scale blocks per tile
+
+struct AttentionArgs {
+  KvCache cache;
+  KvBatch batch;
+  const void* q;
+  void* out;
+  float* partials;  // workspace, see the kernels
+  int* status;
+  int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;
+  int q_heads;
+  int group;        // query heads per key head
+  float scale_log2; // softmax scale * log2(e)
+  int causal;
+  int max_rows;     // rows (tokens x group) a sequence may have to be this kernel's
+  int vector;       // q rows can be read sixteen bytes at a time
+};
+
+int make_kv_map(CUtensorMap* map, const uint8_t* values, const KvCache& cache);
+
+#ifdef __CUDACC__
+__device__ __forceinline__ uint32_t e4m3x2(float a, float b) {  // a in the low byte
+  return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+}
+__device__ __forceinline__ float2 e4m3x2_values(uint32_t codes) {
+  return __half22float2(__half2(
+      __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(codes & 0xffffu), __NV_E4M3)));
+}
+
+// E4M3 terms of two values: codes[t] holds both in its low sixteen bits.
+template <int kTerms>
+__device__ __forceinline__ void e4m3_terms(float a, float b, uint32_t (&codes)[kTerms]) {
+#pragma unroll
+  for (int t = 0; t < kTerms; ++t) {
+    codes[t] = e4m3x2(a, b);
+    if (t + 1 < kTerms) {
+      const float2 v = e4m3x2_values(codes[t]);
+      a = (a - v.x) * 16.0f;
+      b = (b - v.y) * 16.0f;
+    }
+  }
+}
+
+__device__ __forceinline__ float pow2_int(int e) {  // 2^e, -126 <= e <= 127
+  return __uint_as_float((uint32_t)(e + 127) << 23);
+}
+
+// A sequence as this kernel sees it: `tiles` is 0 when it has no rows or is another kernel's.
+struct KvSequence {
+  int64_t row;  // first token row
+  int rows;     // new tokens
+  int length;   // cached tokens that its rows may see
+  int64_t last; // unclamped position of its last row
+  int tiles;
+};
+__device__ __forceinline__ KvSequence kv_sequence(const AttentionArgs& a, int b) {
+  const KvSpan s = kv_span(a.batch, a.cache.page_size, b);
+  KvSequence q;
+  q.row = s.row;
+  q.rows = s.rows;
+  q.length = s.length;
+  q.last = (int64_t)a.batch.seq_lens[b] - 1;
+  const bool mine = s.rows > 0 && (int64_t)s.rows * a.group <= a.max_rows;
+  q.tiles = mine ? max(1, (s.length + kKvTile - 1) / kKvTile) : 0;
+  return q;
+}
+#endif
+
+}  // namespace mx

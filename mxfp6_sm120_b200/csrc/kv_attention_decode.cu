@@ -1,0 +1,907 @@
+// Attention of a few new rows per sequence over the paged 8-bit cache (decode, drafted tokens).
+//
+// Every cached byte is needed once and meets at most 32 query rows (new tokens x query heads of
+// its key head), so HBM bounds the kernel; the work is to keep the byte stream going and
+// everything else underneath it.
+//
+//  * Tokens are the M side of both products: S^T = K Q^T (128 tokens x rows) and
+//    O^T = V^T P^T (head_dim x rows).  K and V^T are read by tcgen05.mma straight from the TMA
+//    tiles (V as an MN-major operand), with the block scales of the cache as the hardware's block
+//    scales: no cached value passes through a register.  A token row is a lane of tensor memory.
+//  * Queries and weights are E4M3 terms (kv_attention.cuh).  The terms lie side by side along N,
+//    so that one pass of the K or V tile serves all of them, and are added in 32 bits afterwards.
+//    With at most 96 columns an MMA costs what its 128-row operand costs (about 33 ns).
+//  * Warps: 0-3 softmax (one lane per token), 4 TMA, 5 MMA, 6-7 quantise queries.  K(j+1) is
+//    multiplied before V(j), so the softmax of a tile overlaps the next tile's scores.
+//  * The list of (sequence, key head, tile of 128 tokens) is cut into equal shares, one per CTA
+//    (one per SM), whatever the lengths are: the cut follows the lengths on the device.  A CTA
+//    whose share covers all tiles of a (sequence, head) writes its rows; otherwise it leaves
+//    unnormalised rows with their maximum and sum, and a second kernel (launched as a
+//    programmatic dependent) joins them in the order of the tiles, so the result does not depend
+//    on timing.
+//  * Weights are scaled by 128 before they become E4M3 terms, so that small ones stay clear of
+//    E4M3's smallest step (the last of two terms ends at 2^-21 of the largest weight; at a scale
+//    of 16 a row whose softmax one token dominates was off by more than 2^-8 of its weights).
+//    E4M3 ends at 448, so the running maximum is raised when a tile exceeds it by 2^1.5.
+#include "kv_attention.cuh"
+
+#include <cstdlib>
+
+namespace mx {
+
+int* device_status_word(int device);
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kSoftmaxWarps = 4;
+constexpr int kTmaWarp = 4, kMmaWarp = 5, kQueryWarp = 6, kQueryWarps = 2;
+constexpr float kWeightScale = 128.0f;  // weights 0..1 become 0..128 before rounding
+constexpr float kSlackLog2 = 1.5f;      // and may reach 2^1.5 times that before the maximum moves
+constexpr int kMinTiles = 2;           // tiles a CTA takes at least, see the plan
+
+template <int D, int RP, int TERMS>
+struct DecodeCfg {
+  static constexpr int kN = RP * TERMS;              // columns of both products
+  static constexpr int kRowBytes = D < 128 ? D : 128;  // bytes of a token row in one sub-tile
+  static constexpr int kSubs = D / kRowBytes;
+  static constexpr int kSubBytes = kKvTile * kRowBytes;
+  static constexpr int kSlotBytes = kKvTile * D;     // a K or V tile
+  static constexpr int kQBytes = (kN * D + 1023) / 1024 * 1024;
+  static constexpr int kPBytes = kN * kKvTile;
+  static constexpr int kFixedBytes = 4096;
+  static constexpr int kBudget = 227 * 1024 - 1024;
+  static constexpr int kFit =
+      (kBudget - kFixedBytes - 2 * kQBytes - 2 * kPBytes) / (kSlotBytes + 512);
+  static constexpr int kSlots = kFit > 16 ? 16 : kFit;
+  static_assert(kSlots >= 4, "the ring needs two tiles of K and V");
+  static constexpr int kSmemBytes =
+      1024 + kSlots * (kSlotBytes + 512) + 2 * kQBytes + 2 * kPBytes + kFixedBytes;
+  // Tensor memory columns: two score tiles, the output halves, scales.
+  static constexpr int kHalves = D > 128 ? 2 : 1;
+  static constexpr int kOCol = 2 * kN;
+  static constexpr int kSfCol = kOCol + kHalves * kN;
+  static constexpr int kColsUsed = (kSfCol + 3) / 4 * 4 + 20;
+  static constexpr int kTmemCols = kColsUsed <= 64 ? 64 : kColsUsed <= 128 ? 128 : kColsUsed <= 256 ? 256 : 512;
+  static_assert(kColsUsed <= 512, "tensor memory");
+  static constexpr uint64_t kSwizzle = kRowBytes == 128 ? ptx::kSwizzle128 : ptx::kSwizzle64;
+  static constexpr int kGroup = 8 * kRowBytes;  // bytes of eight token rows
+  // Partial rows of one CTA end: RP rows of D values, then RP pairs (maximum, sum).
+  static constexpr int kPartialFloats = RP * D + 2 * RP;
+};
+
+// Share of the work list of one CTA, the same arithmetic in both kernels.
+struct Share {
+  int64_t total;  // tiles in all
+  int ctas;
+};
+__host__ __device__ __forceinline__ int64_t share_begin(const Share& s, int cta) {
+  return s.total * cta / s.ctas;
+}
+__device__ __forceinline__ Share share_of(int64_t total, int grid) {
+  Share s;
+  s.total = total;
+  // Fewer, larger shares while the list is short: joining costs more than a second tile.
+  const int64_t want = (total + kMinTiles - 1) / kMinTiles;
+  s.ctas = (int)(want < grid ? (want < 1 ? 1 : want) : grid);
+  return s;
+}
+
+// Sum of tiles over all sequences (one key head), by a full warp.
+__device__ __forceinline__ int64_t warp_total_tiles(const AttentionArgs& a, int lane) {
+  int64_t mine = 0;
+  for (int b = lane; b < a.batch.batch; b += 32) mine += kv_sequence(a, b).tiles;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+  return mine;
+}
+
+// A place in the work list and the sequence it belongs to.
+struct Cursor {
+  int b, head, tile;
+  KvSequence seq;
+  __device__ __forceinline__ void load(const AttentionArgs& a) { seq = kv_sequence(a, b); }
+  // Next tile; the caller knows that there is one.
+  __device__ __forceinline__ void next(const AttentionArgs& a) {
+    if (++tile < seq.tiles) return;
+    tile = 0;
+    if (++head < a.cache.kv_heads) return;
+    head = 0;
+    do {
+      if (++b >= a.batch.batch) {
+        b = a.batch.batch - 1;  // behind the end: only reached by look-ahead
+        seq.tiles = 1;
+        return;
+      }
+      seq = kv_sequence(a, b);
+    } while (seq.tiles == 0);
+  }
+};
+
+// The cursor at flattened tile `at` (< total), by a full warp; all lanes get it.
+__device__ __forceinline__ Cursor warp_locate(const AttentionArgs& a, int64_t at, int lane) {
+  Cursor c;
+  c.b = a.batch.batch - 1;
+  c.head = 0;
+  c.tile = 0;
+  int64_t before = 0;  // tiles of all heads of the sequences before this group of 32
+  for (int b0 = 0; b0 < a.batch.batch; b0 += 32) {
+    const int b = b0 + lane;
+    const int tiles = b < a.batch.batch ? kv_sequence(a, b).tiles : 0;
+    int64_t upto = (int64_t)tiles * a.cache.kv_heads;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t other = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += other;
+    }
+    const unsigned reached = __ballot_sync(0xffffffffu, before + upto > at);
+    if (reached != 0) {
+      const int l = __ffs(reached) - 1;
+      const int64_t first = before + __shfl_sync(0xffffffffu, upto, l) -
+                            (int64_t)__shfl_sync(0xffffffffu, tiles, l) * a.cache.kv_heads;
+      const int count = __shfl_sync(0xffffffffu, tiles, l);
+      c.b = b0 + l;
+      c.head = (int)((at - first) / count);
+      c.tile = (int)((at - first) % count);
+      break;
+    }
+    before += __shfl_sync(0xffffffffu, upto, 31);
+  }
+  c.load(a);
+  return c;
+}
+
+template <int RP>
+__device__ __forceinline__ void output_row(const AttentionArgs& a, const KvSequence& seq, int head,
+                                           int r, int64_t* offset) {
+  *offset = (seq.row + r / a.group) * a.out_token_stride +
+            (int64_t)(head * a.group + r % a.group) * a.out_head_stride;
+}
+
+template <int D, int RP, int TERMS>
+__global__ void __launch_bounds__(kThreads, 1)
+kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                 const AttentionArgs a) {
+  using C = DecodeCfg<D, RP, TERMS>;
+  using T = typename std::conditional<TERMS == 2, __nv_bfloat16, __half>::type;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* slots = smem;
+  uint8_t* q_tiles = slots + C::kSlots * C::kSlotBytes;        // two, [sub][column][row bytes]
+  uint8_t* p_tiles = q_tiles + 2 * C::kQBytes;                 // two, [column][128 tokens]
+  uint8_t* sf_tiles = p_tiles + 2 * C::kPBytes;                // scale atom of every slot
+  uint8_t* fixed = sf_tiles + C::kSlots * 512;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(fixed);
+  uint8_t* ones = fixed + 512;                                 // scale atom of factors of one
+  float* row_scale = reinterpret_cast<float*>(fixed + 1024);   // [2][RP]
+  float* red_max = row_scale + 2 * RP;                         // [2][4][RP]
+  float* red_sum = red_max + 8 * RP;                           // [4][RP]
+  Cursor* start = reinterpret_cast<Cursor*>(red_sum + 4 * RP);
+  int64_t* share_smem = reinterpret_cast<int64_t*>(start + 1);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(share_smem + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  static_assert(1024 + 14 * RP * 4 + sizeof(Cursor) + 64 <= C::kFixedBytes, "fixed area");
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t full0 = ptx::smem_u32(bars);
+  const uint32_t empty0 = full0 + 8 * C::kSlots;
+  const uint32_t sfull0 = empty0 + 8 * C::kSlots;  // two of each from here on
+  const uint32_t pfull0 = sfull0 + 16;
+  const uint32_t pvdone0 = pfull0 + 16;
+  const uint32_t qfull0 = pvdone0 + 16;
+  const uint32_t qempty0 = qfull0 + 16;
+  const uint32_t wsync = qempty0 + 16;             // among the softmax warps
+  static_assert(8 * (2 * 16 + 11) <= 512, "barriers");
+
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    for (int s = 0; s < C::kSlots; ++s) {
+      ptx::mbar_init(full0 + 8 * s, 33);  // expected bytes, and one arrival per lane for the scales
+      ptx::mbar_init(empty0 + 8 * s, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      ptx::mbar_init(sfull0 + 8 * i, 1);
+      ptx::mbar_init(pfull0 + 8 * i, kSoftmaxWarps);
+      ptx::mbar_init(pvdone0 + 8 * i, 1);
+      ptx::mbar_init(qfull0 + 8 * i, kQueryWarps);
+      ptx::mbar_init(qempty0 + 8 * i, 1 + kSoftmaxWarps);
+    }
+    ptx::mbar_init(wsync, kSoftmaxWarps);
+    ptx::fence_mbar_init();
+    ptx::prefetch_tensormap(&tm_k);
+    ptx::prefetch_tensormap(&tm_v);
+  }
+  if (threadIdx.x < 128) reinterpret_cast<uint32_t*>(ones)[threadIdx.x] = 0x7f7f7f7fu;
+  ptx::fence_proxy_async();
+  if (warp == kMmaWarp) {
+    ptx::tmem_alloc(ptx::smem_u32(tmem_slot), C::kTmemCols);
+    ptx::tmem_relinquish();
+  }
+  ptx::grid_launch_dependents();
+  ptx::grid_dependency_wait();
+  if (warp == 0) {
+    const Share s = share_of(warp_total_tiles(a, lane) * a.cache.kv_heads, (int)gridDim.x);
+    const int cta = (int)blockIdx.x;
+    const int64_t t0 = cta < s.ctas ? share_begin(s, cta) : 0;
+    const int64_t t1 = cta < s.ctas ? share_begin(s, cta + 1) : 0;
+    Cursor c;
+    if (t1 > t0) c = warp_locate(a, t0, lane);
+    if (lane == 0) {
+      share_smem[0] = t1 - t0;
+      if (t1 > t0) *start = c;
+    }
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int count = (int)share_smem[0];  // tiles of this CTA
+  const int per_page = a.cache.page_size / kKvBlock;
+
+  if (count > 0 && warp == kTmaWarp) {
+    // ---------------- TMA producer ----------------
+    // Tiles are fetched in the order of their use: K0, K1, V0, K2, V1, ...  Lane l looks up block
+    // l % 4 of tile l / 4 of a group of eight tiles; the next group's lookups are in flight while
+    // this group is copied.
+    Cursor mine = *start;
+    for (int i = 0; i < (lane >> 2); ++i) mine.next(a);
+    int64_t page = -1, next_page = -1;  // first scale / value block of this lane's block, or -1
+    uint32_t k_sf = 127, v_sf = 127, next_k = 127, next_v = 127;
+    auto lookup_page = [&]() -> int64_t {
+      const int block = mine.tile * kKvTileBlocks + (lane & 3);
+      if (block * kKvBlock >= mine.seq.length) return -1;
+      const int64_t p = kv_page(a.batch, a.cache, mine.b, block);
+      return p < 0 ? -1 : (p * a.cache.kv_heads + mine.head) * per_page + block % per_page;
+    };
+    page = lookup_page();
+    if (page >= 0) {
+      k_sf = a.cache.k_scales[page];
+      v_sf = a.cache.v_scales[page];
+    }
+    // The V tile of a group's last tile is copied after the next group's first K tile.
+    int64_t last_page = -1;
+    uint32_t last_v = 127;
+    int slot = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    // Copies one tile whose four blocks are known to lanes src .. src + 3.
+    auto copy = [&](bool is_v, int64_t lane_page, uint32_t lane_sf, int src) {
+      ok = ok && __all_sync(0xffffffffu, bounded_wait(empty0 + 8 * slot, phase ^ 1u, abort_flag,
+                                                      a.status, 401));
+      int64_t at[kKvTileBlocks];
+      uint32_t sf[kKvTileBlocks];
+#pragma unroll
+      for (int i = 0; i < kKvTileBlocks; ++i) {
+        at[i] = __shfl_sync(0xffffffffu, lane_page, src + i);
+        sf[i] = __shfl_sync(0xffffffffu, lane_sf, src + i);
+      }
+      if (!ok) return;
+      const uint32_t bar = full0 + 8 * slot;
+      // Scale atom: lane = row % 32.  Keys: row block c of 32 tokens has one factor for all of
+      // head_dim; values: every row has the factors of the four 32-token steps along K.
+      const uint4 word = is_v ? make_uint4(sf[0] | sf[1] << 8 | sf[2] << 16 | sf[3] << 24, 0, 0, 0)
+                              : make_uint4(sf[0] * 0x01010101u, sf[1] * 0x01010101u,
+                                           sf[2] * 0x01010101u, sf[3] * 0x01010101u);
+      uint4* atom = reinterpret_cast<uint4*>(sf_tiles + slot * 512);
+      atom[lane] = is_v ? make_uint4(word.x, word.x, word.x, word.x) : word;
+      ptx::fence_proxy_async();
+      ptx::mbar_arrive(bar);
+      if (ptx::elect_one()) {
+        // One copy per page and 128 columns; blocks of no page are left as they are.
+        uint32_t bytes = 0;
+        for (int i = 0; i < kKvTileBlocks; i += per_page)
+          if (at[i] >= 0) bytes += (uint32_t)(a.cache.page_size * D);
+        ptx::mbar_arrive_expect_tx(bar, bytes);
+        const uint32_t dst = ptx::smem_u32(slots + slot * C::kSlotBytes);
+        for (int i = 0; i < kKvTileBlocks; i += per_page) {
+          if (at[i] < 0) continue;
+#pragma unroll
+          for (int s = 0; s < C::kSubs; ++s)
+            ptx::tma_load_2d(dst + s * C::kSubBytes + i * kKvBlock * C::kRowBytes,
+                             is_v ? &tm_v : &tm_k, s * 128, (int)(at[i] * kKvBlock), bar);
+        }
+      }
+      __syncwarp();
+      if (++slot == C::kSlots) {
+        slot = 0;
+        phase ^= 1u;
+      }
+    };
+    for (int i0 = 0; ok && i0 < count; i0 += 8) {
+      const bool more = i0 + 8 < count;
+      if (more) {
+        for (int i = 0; i < 8; ++i) mine.next(a);
+        next_page = lookup_page();
+      }
+      for (int j = 0; ok && j < 8 && i0 + j < count; ++j) {
+        copy(false, page, k_sf, 4 * j);
+        if (j > 0) copy(true, page, v_sf, 4 * (j - 1));
+        else if (i0 > 0) copy(true, last_page, last_v, 28);
+        if (j == 3 && more) {
+          next_k = next_page >= 0 ? a.cache.k_scales[next_page] : 127u;
+          next_v = next_page >= 0 ? a.cache.v_scales[next_page] : 127u;
+        }
+      }
+      last_page = page;
+      last_v = v_sf;
+      page = next_page;
+      k_sf = next_k;
+      v_sf = next_v;
+    }
+    if (ok) copy(true, last_page, last_v, 4 * ((count - 1) & 7));
+  } else if (count > 0 && warp == kMmaWarp) {
+    // ---------------- MMA issuer ----------------
+    constexpr uint32_t kIdesc = ((uint32_t)(C::kN >> 3) << 17) | (1u << 23) | ((128u >> 4) << 24);
+    const uint32_t sf0 = tmem + (C::kSfCol + 3) / 4 * 4;  // K and V scales by tile parity, ones
+    const uint32_t ones_t = sf0 + 16;
+    if (ptx::elect_one()) ptx::tc_cp_32x128b_warpx4(ones_t, ptx::smem_desc_scale_atom(ptx::smem_u32(ones)));
+    __syncwarp();
+    Cursor scored = *start, summed = scored;  // tile of the last QK and PV issued
+    int segment = 0;                          // of `scored`
+    bool ok = true;
+    // Slot of K(i) is 2i - 1 (0 for the first), of V(i) 2i + 2 (2i + 1 for the last).
+    auto scores = [&](int i) {
+      const bool first = i == 0 || scored.tile == 0;
+      const bool last = i + 1 == count || scored.tile + 1 == scored.seq.tiles;
+      const int at = i == 0 ? 0 : 2 * i - 1;
+      const int slot = at % C::kSlots;
+      if (first)
+        ok = ok && __all_sync(0xffffffffu, bounded_wait(qfull0 + 8 * (segment & 1),
+                                                        (uint32_t)(segment >> 1) & 1u, abort_flag,
+                                                        a.status, 402));
+      ok = ok && __all_sync(0xffffffffu,
+                            bounded_wait(full0 + 8 * slot, (uint32_t)(at / C::kSlots) & 1u,
+                                         abort_flag, a.status, 403));
+      if (!ok) return;
+      ptx::tc_fence_after();
+      if (ptx::elect_one()) {
+        const uint32_t sf_t = sf0 + 8 * (i & 1);
+        ptx::tc_cp_32x128b_warpx4(sf_t, ptx::smem_desc_scale_atom(ptx::smem_u32(sf_tiles + slot * 512)));
+        const uint32_t k_s = ptx::smem_u32(slots + slot * C::kSlotBytes);
+        const uint32_t q_s = ptx::smem_u32(q_tiles + (segment & 1) * C::kQBytes);
+#pragma unroll
+        for (int s = 0; s < C::kSubs; ++s) {
+          const uint64_t ad = ptx::smem_desc(k_s + s * C::kSubBytes, 0, C::kGroup, C::kSwizzle);
+          const uint64_t bd = ptx::smem_desc(q_s + s * C::kN * C::kRowBytes, 0, C::kGroup, C::kSwizzle);
+#pragma unroll
+          for (int ks = 0; ks < C::kRowBytes / 32; ++ks)
+            ptx::tc_mma_mxf8f6f4(tmem + (i & 1) * C::kN, ad + 2 * ks, bd + 2 * ks, kIdesc, sf_t,
+                                 ones_t, (s > 0 || ks > 0) ? 1u : 0u);
+        }
+        ptx::tc_commit(empty0 + 8 * slot);
+        ptx::tc_commit(sfull0 + 8 * (i & 1));
+        if (last) ptx::tc_commit(qempty0 + 8 * (segment & 1));
+      }
+      __syncwarp();
+      if (last) ++segment;
+    };
+    scores(0);
+    for (int i = 0; ok && i < count; ++i) {
+      if (i + 1 < count) {
+        scored.next(a);
+        scores(i + 1);
+      }
+      const int at = i + 1 < count ? 2 * i + 2 : 2 * i + 1;
+      const int slot = at % C::kSlots;
+      ok = ok && __all_sync(0xffffffffu, bounded_wait(pfull0 + 8 * (i & 1), (uint32_t)(i >> 1) & 1u,
+                                                      abort_flag, a.status, 404));
+      ok = ok && __all_sync(0xffffffffu,
+                            bounded_wait(full0 + 8 * slot, (uint32_t)(at / C::kSlots) & 1u,
+                                         abort_flag, a.status, 405));
+      if (!ok) break;
+      ptx::tc_fence_after();
+      const bool first = i == 0 || summed.tile == 0;
+      if (ptx::elect_one()) {
+        const uint32_t sf_t = sf0 + 8 * (i & 1) + 4;
+        ptx::tc_cp_32x128b_warpx4(sf_t, ptx::smem_desc_scale_atom(ptx::smem_u32(sf_tiles + slot * 512)));
+        const uint32_t v_s = ptx::smem_u32(slots + slot * C::kSlotBytes);
+        const uint64_t bd =
+            ptx::smem_desc(ptx::smem_u32(p_tiles + (i & 1) * C::kPBytes), 0, 1024, ptx::kSwizzle128);
+#pragma unroll
+        for (int h = 0; h < C::kHalves; ++h) {
+          // V^T: 128 values of head_dim along M (MN-major), 32 tokens per step.  With a head of
+          // 64 the upper 64 rows of M are the next eight tokens' bytes: lanes nobody reads.
+          const uint64_t ad = ptx::smem_desc(v_s + h * C::kSubBytes, C::kGroup, C::kGroup, C::kSwizzle);
+#pragma unroll
+          for (int ks = 0; ks < kKvTileBlocks; ++ks) {
+            const uint32_t idesc = kIdesc | (1u << 15) | ((uint32_t)ks << 29);
+            ptx::tc_mma_mxf8f6f4(tmem + C::kOCol + h * C::kN, ad + ks * (kKvBlock * C::kRowBytes / 16),
+                                 bd + 2 * ks, idesc, sf_t, ones_t, (!first || ks > 0) ? 1u : 0u);
+          }
+        }
+        ptx::tc_commit(empty0 + 8 * slot);
+        ptx::tc_commit(pvdone0 + 8 * (i & 1));
+      }
+      __syncwarp();
+      if (i + 1 < count) summed.next(a);
+    }
+  } else if (count > 0 && warp >= kQueryWarp) {
+    // ---------------- query terms ----------------
+    Cursor c = *start;
+    int left = count;
+    bool ok = true;
+    for (int segment = 0; ok && left > 0; ++segment) {
+      const int buffer = segment & 1;
+      ok = __all_sync(0xffffffffu, bounded_wait(qempty0 + 8 * buffer, ((uint32_t)(segment >> 1) & 1u) ^ 1u,
+                                                abort_flag, a.status, 406));
+      if (!ok) break;
+      uint8_t* q_s = q_tiles + buffer * C::kQBytes;
+      const int rows = c.seq.rows * a.group;
+      constexpr int kPer = D / 32;  // values per lane
+#pragma unroll 1
+      for (int r = warp - kQueryWarp; r < RP; r += kQueryWarps) {
+        float v[kPer];
+        uint32_t top = 0;
+        constexpr uint32_t kInf = TERMS == 2 ? 0x7f80u : 0x7c00u;
+        const T* src = static_cast<const T*>(a.q) + (c.seq.row + r / a.group) * a.q_token_stride +
+                       (int64_t)(c.head * a.group + r % a.group) * a.q_head_stride + lane * kPer;
+        __align__(16) uint16_t raw[kPer];
+        if (r < rows) {
+          if (a.vector && kPer == 8) {
+            *reinterpret_cast<uint4*>(raw) = *reinterpret_cast<const uint4*>(src);
+          } else if (a.vector && kPer == 4) {
+            *reinterpret_cast<uint2*>(raw) = *reinterpret_cast<const uint2*>(src);
+          } else {
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) raw[i] = reinterpret_cast<const uint16_t*>(src)[i];
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) raw[i] = 0;
+        }
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+          top = max(top, (uint32_t)(raw[i] & 0x7fffu));
+          if constexpr (TERMS == 2) v[i] = __uint_as_float((uint32_t)raw[i] << 16);
+          else v[i] = __half2float(__ushort_as_half(raw[i]));
+        }
+        top = __reduce_max_sync(0xffffffffu, top);
+        const float most = TERMS == 2 ? __uint_as_float(top << 16)
+                                      : __half2float(__ushort_as_half((unsigned short)top));
+        // A row with an infinity or NaN has no scale: its scores become NaN.
+        const uint32_t bits = ue8m0_scale_bits_shift<8>(top < kInf ? most : 1.0f);
+        const float inverse = ue8m0_inverse(bits);
+        if (lane == 0) row_scale[buffer * RP + r] = top < kInf ? __uint_as_float(bits) : NAN;
+        uint32_t codes[TERMS][kPer / 2];
+#pragma unroll
+        for (int i = 0; i < kPer / 2; ++i) {
+          uint32_t t[TERMS];
+          e4m3_terms<TERMS>(v[2 * i] * inverse, v[2 * i + 1] * inverse, t);
+#pragma unroll
+          for (int k = 0; k < TERMS; ++k) codes[k][i] = t[k];
+        }
+        const int d0 = lane * kPer;
+#pragma unroll
+        for (int k = 0; k < TERMS; ++k) {
+          const int col = k * RP + r;
+          const int in_row = d0 % C::kRowBytes;
+          const int swizzle = C::kRowBytes == 128 ? (col & 7) : ((col >> 1) & 3);
+          uint8_t* dst = q_s + (d0 / C::kRowBytes) * C::kN * C::kRowBytes + col * C::kRowBytes +
+                         (((in_row >> 4) ^ swizzle) << 4) + (in_row & 15);
+          if constexpr (kPer == 8) {
+            *reinterpret_cast<uint2*>(dst) = make_uint2(codes[k][0] | codes[k][1] << 16,
+                                                        codes[k][2] | codes[k][3] << 16);
+          } else if constexpr (kPer == 4) {
+            *reinterpret_cast<uint32_t*>(dst) = codes[k][0] | codes[k][1] << 16;
+          } else {
+            *reinterpret_cast<uint16_t*>(dst) = (uint16_t)codes[k][0];
+          }
+        }
+      }
+      ptx::fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(qfull0 + 8 * buffer);
+      // On to the first tile of the next (sequence, head) of this share.
+      const int rest = min(left, c.seq.tiles - c.tile);
+      left -= rest;
+      c.tile = c.seq.tiles - 1;
+      if (left > 0) c.next(a);
+    }
+  } else if (count > 0 && warp < kSoftmaxWarps) {
+    // ---------------- softmax: lane = token of the tile ----------------
+    const int token = warp * 32 + lane;  // within the tile; warp = its scale block
+    const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
+    Cursor c = *start;
+    float top[RP], sum[RP], factor[RP];  // top: the same in all lanes
+    int segment = 0;
+    int segment_tile0 = c.tile;          // first tile of this CTA in the segment
+    bool ok = true;
+    // Barrier among the four warps; bounded like every other wait.
+    uint32_t wphase = 0;
+    auto warps_sync = [&]() -> bool {
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(wsync);
+      const bool done = bounded_wait(wsync, wphase, abort_flag, a.status, 413);
+      wphase ^= 1u;
+      return __all_sync(0xffffffffu, done);
+    };
+    auto block_named = [&](const Cursor& at) -> bool {
+      const int block = at.tile * kKvTileBlocks + warp;
+      return block * kKvBlock < at.seq.length && kv_page(a.batch, a.cache, at.b, block) >= 0;
+    };
+    bool named = block_named(c);
+    for (int i = 0; i < count; ++i) {
+      const bool first = i == 0 || c.tile == 0;
+      const bool last = i + 1 == count || c.tile + 1 == c.seq.tiles;
+      // The next tile's page lookup is in flight during this tile.
+      Cursor ahead = c;
+      bool named_ahead = false;
+      if (i + 1 < count) {
+        ahead.next(a);
+        named_ahead = block_named(ahead);
+      }
+      if (first) {
+        segment_tile0 = c.tile;
+        ok = bounded_wait(qfull0 + 8 * (segment & 1), (uint32_t)(segment >> 1) & 1u, abort_flag,
+                          a.status, 407);
+        if (!__all_sync(0xffffffffu, ok)) break;
+#pragma unroll
+        for (int r = 0; r < RP; ++r) {
+          factor[r] = row_scale[(segment & 1) * RP + r] * a.scale_log2;
+          top[r] = -INFINITY;
+          sum[r] = 0.0f;
+        }
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(qempty0 + 8 * (segment & 1));
+      }
+      // Tokens of this tile that exist, and how far the rows see.
+      const int64_t t0 = (int64_t)c.tile * kKvTile;
+      const int held = (int)min((int64_t)kKvTile, c.seq.length - t0);
+      const bool here = named && token < held;
+      if (!__all_sync(0xffffffffu, named && (warp + 1) * 32 <= held)) {
+        // Rows of V without a token may hold anything, NaN among them, and 0 * NaN is NaN: clear
+        // them once the tile has landed.
+        const int at = i + 1 < count ? 2 * i + 2 : 2 * i + 1;
+        const int slot = at % C::kSlots;
+        ok = bounded_wait(full0 + 8 * slot, (uint32_t)(at / C::kSlots) & 1u, abort_flag, a.status, 408);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        uint8_t* v_s = slots + slot * C::kSlotBytes;
+        for (int t = 0; t < 32; ++t) {
+          if (named && warp * 32 + t < held) continue;
+          for (int at16 = lane; at16 < D / 16; at16 += 32) {
+            const int s = at16 * 16 / C::kRowBytes, in_row = at16 % (C::kRowBytes / 16);
+            *reinterpret_cast<uint4*>(v_s + s * C::kSubBytes + (warp * 32 + t) * C::kRowBytes +
+                                      in_row * 16) = make_uint4(0, 0, 0, 0);
+          }
+        }
+        ptx::fence_proxy_async();
+      }
+      ok = bounded_wait(sfull0 + 8 * (i & 1), (uint32_t)(i >> 1) & 1u, abort_flag, a.status, 409);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      ptx::tc_fence_after();
+      float s[RP];
+#pragma unroll
+      for (int r0 = 0; r0 < RP; r0 += 8) {
+        uint32_t raw[TERMS][8];
+#pragma unroll
+        for (int k = 0; k < TERMS; ++k)
+          ptx::tmem_ld_x8(tmem + lane_base + (i & 1) * C::kN + k * RP + r0, raw[k]);
+        ptx::tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          float v = __uint_as_float(raw[TERMS - 1][j]);
+#pragma unroll
+          for (int k = TERMS - 2; k >= 0; --k) v = v * 0.0625f + __uint_as_float(raw[k][j]);
+          s[r0 + j] = here ? v * factor[r0 + j] : -INFINITY;
+        }
+      }
+      ptx::tc_fence_before();
+      if (a.causal && t0 + held > c.seq.last - c.seq.rows + 1) {
+#pragma unroll
+        for (int r = 0; r < RP; ++r)
+          if (t0 + token > c.seq.last - c.seq.rows + 1 + r / a.group) s[r] = -INFINITY;
+      }
+      // Largest score of the tile per row, over the four warps.
+      float* mine = red_max + (i & 1) * 4 * RP;
+#pragma unroll
+      for (int r = 0; r < RP; ++r) {
+        const float m = ptx::warp_max(s[r]);
+        if (lane == (r & 31)) mine[warp * RP + r] = m;
+      }
+      if (!warps_sync()) break;
+      bool raise = false;
+      float next[RP];
+#pragma unroll
+      for (int r = 0; r < RP; ++r) {
+        const float m = fmaxf(fmaxf(mine[r], mine[RP + r]), fmaxf(mine[2 * RP + r], mine[3 * RP + r]));
+        next[r] = m > top[r] + kSlackLog2 || (top[r] == -INFINITY && m > top[r]) ? m : top[r];
+        raise = raise || next[r] != top[r];
+      }
+      if (raise) {  // the same in all threads of the four warps
+        if (c.tile != segment_tile0) {
+          // The output so far shrinks; the last PV of this segment has to be done.
+          ok = bounded_wait(pvdone0 + 8 * ((i - 1) & 1), (uint32_t)((i - 1) >> 1) & 1u, abort_flag,
+                            a.status, 410);
+          if (!__all_sync(0xffffffffu, ok)) break;
+          ptx::tc_fence_after();
+#pragma unroll
+          for (int h = 0; h < C::kHalves; ++h) {
+#pragma unroll
+            for (int c0 = 0; c0 < C::kN; c0 += 8) {
+              uint32_t o[8];
+              const uint32_t at = tmem + lane_base + C::kOCol + h * C::kN + c0;
+              ptx::tmem_ld_x8(at, o);
+              ptx::tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                const int r = (c0 + j) % RP;
+                const float f = next[r] == top[r] ? 1.0f : exp2f(top[r] - next[r]);
+                o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+              }
+              ptx::tmem_st_x8(at, o);
+            }
+          }
+          ptx::tmem_st_wait();
+          ptx::tc_fence_before();
+        }
+#pragma unroll
+        for (int r = 0; r < RP; ++r) {
+          if (next[r] != top[r]) sum[r] *= exp2f(top[r] - next[r]);
+          top[r] = next[r];
+        }
+      }
+      if (i >= 2) {  // PV(i - 2) has read the buffer that this tile's weights go to
+        ok = bounded_wait(pvdone0 + 8 * (i & 1), (uint32_t)((i - 2) >> 1) & 1u, abort_flag, a.status, 411);
+        if (!__all_sync(0xffffffffu, ok)) break;
+      }
+      uint8_t* p_s = p_tiles + (i & 1) * C::kPBytes + (token & 15);
+#pragma unroll
+      for (int r = 0; r < RP; r += 2) {
+        float p[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          p[j] = exp2f(s[r + j] - (top[r + j] == -INFINITY ? 0.0f : top[r + j]));
+          sum[r + j] += p[j];
+        }
+        uint32_t codes[TERMS];
+        e4m3_terms<TERMS>(p[0] * kWeightScale, p[1] * kWeightScale, codes);
+#pragma unroll
+        for (int k = 0; k < TERMS; ++k) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int col = k * RP + r + j;
+            p_s[col * 128 + (((token >> 4) ^ (col & 7)) << 4)] = (uint8_t)(codes[k] >> (8 * j));
+          }
+        }
+      }
+      ptx::fence_proxy_async();
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(pfull0 + 8 * (i & 1));
+      if (last) {
+        // ---- the segment's rows: sums over the tokens, then the output of this CTA's tiles ----
+#pragma unroll
+        for (int r = 0; r < RP; ++r) {
+          float v = sum[r];
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+          if (lane == (r & 31)) red_sum[warp * RP + r] = v;
+        }
+        if (!warps_sync()) break;
+        ok = bounded_wait(pvdone0 + 8 * (i & 1), (uint32_t)(i >> 1) & 1u, abort_flag, a.status, 412);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        ptx::tc_fence_after();
+        const int rows = c.seq.rows * a.group;
+        const bool whole = segment_tile0 == 0 && c.tile + 1 == c.seq.tiles;
+        // A share that begins inside a (sequence, head) uses the CTA's first partial slot for it,
+        // one that ends inside the second.
+        float* part = a.partials + (int64_t)(2 * blockIdx.x + (segment_tile0 != 0 ? 0 : 1)) *
+                                       C::kPartialFloats;
+#pragma unroll 1
+        for (int r0 = 0; r0 < RP; r0 += 8) {
+#pragma unroll
+          for (int h = 0; h < C::kHalves; ++h) {
+            uint32_t raw[TERMS][8];
+#pragma unroll
+            for (int k = 0; k < TERMS; ++k)
+              ptx::tmem_ld_x8(tmem + lane_base + C::kOCol + h * C::kN + k * RP + r0, raw[k]);
+            ptx::tmem_ld_wait();
+            const int d = h * 128 + token;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const int r = r0 + j;
+              float v = __uint_as_float(raw[TERMS - 1][j]);
+#pragma unroll
+              for (int k = TERMS - 2; k >= 0; --k) v = v * 0.0625f + __uint_as_float(raw[k][j]);
+              v *= 1.0f / kWeightScale;
+              if (r < rows && d < D) {
+                if (whole) {
+                  const float l = red_sum[r] + red_sum[RP + r] + red_sum[2 * RP + r] + red_sum[3 * RP + r];
+                  int64_t at;
+                  output_row<RP>(a, c.seq, c.head, r, &at);
+                  v = l == 0.0f ? 0.0f : v / l;
+                  T* out = static_cast<T*>(a.out) + at + d;
+                  if constexpr (TERMS == 2) *out = __float2bfloat16_rn(v);
+                  else *out = __float2half_rn(v);
+                } else {
+                  part[r * D + d] = v;
+                }
+              }
+            }
+          }
+        }
+        if (!whole) {
+#pragma unroll
+          for (int r = 0; r < RP; ++r)
+            if (token == r) {
+              part[RP * D + 2 * r] = top[r];
+              part[RP * D + 2 * r + 1] =
+                  red_sum[r] + red_sum[RP + r] + red_sum[2 * RP + r] + red_sum[3 * RP + r];
+            }
+        }
+        ptx::tc_fence_before();
+        // red_sum is written again by the next segment.
+        if (!warps_sync()) break;
+        ++segment;
+      }
+      c = ahead;
+      named = named_ahead;
+    }
+  }
+
+  // ---------------- teardown ----------------
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (*abort_flag != 0) {
+    // Give copies and MMAs still in flight time to land before the CTA's shared
+    // and tensor memory are handed back.
+    for (int i = 0; i < 200; ++i) __nanosleep(1000);
+  }
+  if (warp == kMmaWarp) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc(tmem, C::kTmemCols);
+  }
+}
+
+// Joins the partial rows of every (sequence, head) whose tiles went to more than one CTA, in the
+// order of the tiles.  One CTA per (sequence, head) and row.
+template <int D, int RP, int TERMS>
+__global__ void __launch_bounds__(D)
+kv_decode_join_kernel(const AttentionArgs a, int grid) {
+  using C = DecodeCfg<D, RP, TERMS>;
+  using T = typename std::conditional<TERMS == 2, __nv_bfloat16, __half>::type;
+  __shared__ int64_t sums[2 * 32];
+  const int b = blockIdx.x / a.cache.kv_heads, head = blockIdx.x % a.cache.kv_heads;
+  const int r = blockIdx.y;
+  ptx::grid_dependency_wait();
+  const KvSequence seq = kv_sequence(a, b);
+  if (seq.tiles == 0 || r >= seq.rows * a.group) return;
+  int64_t before = 0, total = 0;  // tiles of the sequences before b, of all
+  for (int i = threadIdx.x; i < a.batch.batch; i += D) {
+    const int tiles = kv_sequence(a, i).tiles;
+    total += tiles;
+    if (i < b) before += tiles;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    before += __shfl_xor_sync(0xffffffffu, before, o);
+    total += __shfl_xor_sync(0xffffffffu, total, o);
+  }
+  if ((threadIdx.x & 31) == 0) {
+    sums[2 * (threadIdx.x >> 5)] = before;
+    sums[2 * (threadIdx.x >> 5) + 1] = total;
+  }
+  __syncthreads();
+  before = total = 0;
+  for (int w = 0; w < D / 32; ++w) {
+    before += sums[2 * w];
+    total += sums[2 * w + 1];
+  }
+  const Share s = share_of(total * a.cache.kv_heads, grid);
+  const int64_t t0 = before * a.cache.kv_heads + (int64_t)head * seq.tiles;
+  const int64_t t1 = t0 + seq.tiles - 1;
+  // CTA of tile t: the last one whose share begins at or before it.
+  const int c0 = (int)(((t0 + 1) * s.ctas - 1) / s.total);
+  const int c1 = (int)(((t1 + 1) * s.ctas - 1) / s.total);
+  if (c0 == c1) return;  // one CTA had all of it and wrote the row
+  float top = -INFINITY;
+  auto part_of = [&](int cta) {
+    // The first CTA's share may begin here exactly, or earlier with other work.
+    const bool begins_inside = share_begin(s, cta) > t0;
+    return a.partials + (int64_t)(2 * cta + (begins_inside ? 0 : 1)) * C::kPartialFloats;
+  };
+  for (int cta = c0; cta <= c1; ++cta) top = fmaxf(top, part_of(cta)[RP * D + 2 * r]);
+  const float base = top == -INFINITY ? 0.0f : top;
+  float l = 0.0f, o = 0.0f;
+#pragma unroll 4
+  for (int cta = c0; cta <= c1; ++cta) {
+    const float* part = part_of(cta);
+    const float f = exp2f(part[RP * D + 2 * r] - base);
+    l += f * part[RP * D + 2 * r + 1];
+    o += f * part[r * D + threadIdx.x];
+  }
+  o = l == 0.0f ? 0.0f : o / l;
+  int64_t at;
+  output_row<RP>(a, seq, head, r, &at);
+  T* out = static_cast<T*>(a.out) + at + threadIdx.x;
+  if constexpr (TERMS == 2) *out = __float2bfloat16_rn(o);
+  else *out = __float2half_rn(o);
+}
+
+constexpr int kSms = 148;
+
+bool use_pdl() {
+  static const bool enabled = []() {
+    const char* env = std::getenv("MXFP6_B200_PDL");
+    return env == nullptr || env[0] != '0';
+  }();
+  return enabled;
+}
+
+template <int D, int RP, int TERMS>
+int launch(const CUtensorMap& tm_k, const CUtensorMap& tm_v, const AttentionArgs& a, int grid,
+           cudaStream_t stream) {
+  using C = DecodeCfg<D, RP, TERMS>;
+  static bool configured[64] = {};
+  int device = 0;
+  MX_CUDA(cudaGetDevice(&device));
+  if (device >= 64 || !configured[device]) {
+    MX_CUDA(cudaFuncSetAttribute(kv_decode_kernel<D, RP, TERMS>,
+                                 cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes));
+    if (device < 64) configured[device] = true;
+  }
+  cudaLaunchAttribute attribute[1];
+  attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3((unsigned)grid);
+  config.blockDim = dim3(kThreads);
+  config.dynamicSmemBytes = C::kSmemBytes;
+  config.stream = stream;
+  config.attrs = attribute;
+  config.numAttrs = use_pdl() ? 1 : 0;
+  MX_CUDA(cudaLaunchKernelEx(&config, kv_decode_kernel<D, RP, TERMS>, tm_k, tm_v, a));
+  if (grid == 1) return kOk;  // nothing was split
+  config.gridDim = dim3((unsigned)(a.batch.batch * a.cache.kv_heads), (unsigned)a.max_rows);
+  config.blockDim = dim3(D);
+  config.dynamicSmemBytes = 0;
+  MX_CUDA(cudaLaunchKernelEx(&config, kv_decode_join_kernel<D, RP, TERMS>, a, grid));
+  return kOk;
+}
+
+template <int D, int TERMS>
+int launch_rows(const CUtensorMap& tm_k, const CUtensorMap& tm_v, const AttentionArgs& a, int grid,
+                cudaStream_t stream) {
+  if (a.max_rows <= 8) return launch<D, 8, TERMS>(tm_k, tm_v, a, grid, stream);
+  if (a.max_rows <= 16) return launch<D, 16, TERMS>(tm_k, tm_v, a, grid, stream);
+  return launch<D, 32, TERMS>(tm_k, tm_v, a, grid, stream);
+}
+
+int padded_rows(int rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : 32; }
+
+}  // namespace
+
+// CTAs of a decode launch: at most one per SM, at most one per two tiles that there can be.
+int kv_decode_grid(int64_t batch, int kv_heads, int64_t max_context) {
+  const int64_t tiles = batch * kv_heads * ceil_div64(max_context < 1 ? 1 : max_context, kKvTile);
+  const int64_t want = ceil_div64(tiles, kMinTiles);
+  return (int)(want < kSms ? want : kSms);
+}
+
+int64_t kv_decode_workspace(int64_t batch, int kv_heads, int head_dim, int rows, int64_t max_context) {
+  const int grid = kv_decode_grid(batch, kv_heads, max_context);
+  if (grid == 1) return 0;
+  const int rp = padded_rows(rows);
+  return (int64_t)grid * 2 * (rp * head_dim + 2 * rp) * 4;
+}
+
+// Sequences with at most a.max_rows <= 32 rows (tokens x group); others are left alone.
+int launch_kv_decode(const AttentionArgs& a, int dtype, cudaStream_t stream) {
+  CUtensorMap tm_k, tm_v;
+  if (int rc = make_kv_map(&tm_k, a.cache.k_values, a.cache)) return rc;
+  if (int rc = make_kv_map(&tm_v, a.cache.v_values, a.cache)) return rc;
+  const int grid = kv_decode_grid(a.batch.batch, a.cache.kv_heads,
+                                  (int64_t)a.batch.table_width * a.cache.page_size);
+  const int d = a.cache.head_dim;
+  if (dtype == kBF16) {
+    if (d == 64) return launch_rows<64, 2>(tm_k, tm_v, a, grid, stream);
+    if (d == 128) return launch_rows<128, 2>(tm_k, tm_v, a, grid, stream);
+    return launch_rows<256, 2>(tm_k, tm_v, a, grid, stream);
+  }
+  if (d == 64) return launch_rows<64, 3>(tm_k, tm_v, a, grid, stream);
+  if (d == 128) return launch_rows<128, 3>(tm_k, tm_v, a, grid, stream);
+  return launch_rows<256, 3>(tm_k, tm_v, a, grid, stream);
+}
+
+}  // namespace mx

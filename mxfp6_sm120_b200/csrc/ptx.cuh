@@ -51,6 +51,13 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
   return ok != 0;
 }
 
+// Largest value over the warp, NaN ignored.
+__device__ __forceinline__ float warp_max(float v) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+
 // ---- programmatic dependent launch -------------------------------------------------
 // Blocks until every grid this one depends on has completed and its writes are
 // visible (returns at once when the launch carried no programmatic dependency).
@@ -243,6 +250,24 @@ __device__ __forceinline__ void tmem_ld_x32(uint32_t taddr, uint32_t (&r)[32]) {
       : "r"(taddr)
       : "memory");
 }
+// 32 lanes x 8 consecutive 32-bit columns <-> 8 registers per thread.
+__device__ __forceinline__ void tmem_ld_x8(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_x8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
 template <int kCols>
 __device__ __forceinline__ void tmem_ld_chunk(uint32_t taddr, uint32_t (&r)[kCols]) {
   static_assert(kCols == 16 || kCols == 32, "chunk is 16 or 32 columns");
@@ -306,6 +331,20 @@ __device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t saddr) {
   d |= static_cast<uint64_t>(1024u >> 4) << 32;             // stride between 8-row groups
   d |= 1ull << 46;                                          // descriptor version (sm_100)
   d |= 2ull << 61;                                          // 128-byte swizzle
+  return d;
+}
+// General form.  K-major operands: `group_bytes` between groups of eight rows (`leading_bytes`
+// unused).  MN-major operands: `group_bytes` between groups of eight K values, `leading_bytes`
+// between swizzle rows (128 or 64 values) along M / N.
+enum : uint64_t { kSwizzle128 = 2, kSwizzle64 = 4 };
+__device__ __forceinline__ uint64_t smem_desc(uint32_t saddr, uint32_t leading_bytes,
+                                              uint32_t group_bytes, uint64_t swizzle) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((saddr & 0x3ffffu) >> 4);
+  d |= static_cast<uint64_t>(leading_bytes >> 4) << 16;
+  d |= static_cast<uint64_t>(group_bytes >> 4) << 32;
+  d |= 1ull << 46;
+  d |= swizzle << 61;
   return d;
 }
 // Descriptor of one 512-byte scale atom: 32 rows x 16 bytes, no swizzle,
