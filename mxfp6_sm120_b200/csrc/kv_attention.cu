@@ -11,7 +11,9 @@
 namespace mx {
 
 int launch_kv_decode(const AttentionArgs& a, int dtype, cudaStream_t stream);
-int64_t kv_decode_workspace(int64_t batch, int kv_heads, int head_dim, int rows, int64_t max_context);
+int kv_decode_rows(int head_dim, int dtype);
+int64_t kv_decode_workspace(int64_t batch, int kv_heads, int head_dim, int dtype, int rows,
+                            int64_t max_context);
 int* device_status_word(int device);
 
 namespace {
@@ -145,8 +147,6 @@ void launch_rows(const AttentionArgs& a, cudaStream_t stream) {
   if (a.cache.head_dim == 256) kv_attention_rows_kernel<T, 256><<<grid, kWarps * 32, 0, stream>>>(a);
 }
 
-constexpr int kDecodeRows = 32;  // rows (tokens x group) of a sequence that the decode kernel takes
-
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
@@ -198,14 +198,13 @@ int64_t kv_cache_attention_workspace(int64_t batch, int64_t tokens, int64_t max_
                                      int q_heads, int kv_heads, int head_dim, int dtype,
                                      int64_t max_context) {
   (void)tokens;
-  (void)dtype;
   if (batch < 1 || max_query_len < 1 || q_heads < 1 || kv_heads < 1 || q_heads % kv_heads != 0 ||
       (head_dim != 64 && head_dim != 128 && head_dim != 256) || max_context < 1) {
     return -1;
   }
   const int64_t rows = max_query_len * (q_heads / kv_heads);
-  if (rows > kDecodeRows) return 0;
-  return kv_decode_workspace(batch, kv_heads, head_dim, (int)rows, max_context);
+  if (rows > kv_decode_rows(head_dim, dtype)) return 0;
+  return kv_decode_workspace(batch, kv_heads, head_dim, dtype, (int)rows, max_context);
 }
 
 int kv_cache_attention(const KvCache& cache, const KvBatch& batch, const void* q, void* out,
@@ -245,7 +244,7 @@ int kv_cache_attention(const KvCache& cache, const KvBatch& batch, const void* q
   a.causal = causal;
   a.vector = aligned16(q) && strides[0] % 8 == 0 && strides[1] % 8 == 0;
   const int64_t rows = max_query_len * a.group;
-  if (rows <= kDecodeRows) {
+  if (rows <= kv_decode_rows(cache.head_dim, dtype)) {
     a.max_rows = (int)rows;
     return launch_kv_decode(a, dtype, stream);
   }

@@ -11,8 +11,10 @@
 //  * Queries and weights are E4M3 terms (kv_attention.cuh).  The terms lie side by side along N,
 //    so that one pass of the K or V tile serves all of them, and are added in 32 bits afterwards.
 //    With at most 96 columns an MMA costs what its 128-row operand costs (about 33 ns).
-//  * Warps: 0-3 softmax (one lane per token), 4 TMA, 5 MMA, 6-7 quantise queries.  K(j+1) is
-//    multiplied before V(j), so the softmax of a tile overlaps the next tile's scores.
+//  * Warps: 0-3 and 4-7 softmax (one lane per token; the two groups take alternate tiles, each
+//    with its own running maximum and output accumulator, because one group needs about as long
+//    for a tile as HBM does), 8 TMA, 9 MMA, 10-11 quantise queries.  K(j+1) is multiplied before
+//    V(j), so the softmax of a tile overlaps the next tile's scores.
 //  * The list of (sequence, key head, tile of 128 tokens) is cut into equal shares, one per CTA
 //    (one per SM), whatever the lengths are: the cut follows the lengths on the device.  A CTA
 //    whose share covers all tiles of a (sequence, head) writes its rows; otherwise it leaves
@@ -33,9 +35,9 @@ int* device_status_word(int device);
 
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kSoftmaxWarps = 4;
-constexpr int kTmaWarp = 4, kMmaWarp = 5, kQueryWarp = 6, kQueryWarps = 2;
+constexpr int kThreads = 384;
+constexpr int kGroupWarps = 4;  // warps of a softmax group, one per 32 lanes of tensor memory
+constexpr int kTmaWarp = 8, kMmaWarp = 9, kQueryWarp = 10, kQueryWarps = 2;
 constexpr float kWeightScale = 128.0f;  // weights 0..1 become 0..128 before rounding
 constexpr float kSlackLog2 = 1.5f;      // and may reach 2^1.5 times that before the maximum moves
 constexpr int kMinTiles = 2;           // tiles a CTA takes at least, see the plan
@@ -49,7 +51,7 @@ struct DecodeCfg {
   static constexpr int kSlotBytes = kKvTile * D;     // a K or V tile
   static constexpr int kQBytes = (kN * D + 1023) / 1024 * 1024;
   static constexpr int kPBytes = kN * kKvTile;
-  static constexpr int kFixedBytes = 4096;
+  static constexpr int kFixedBytes = 5120;
   static constexpr int kBudget = 227 * 1024 - 1024;
   static constexpr int kFit =
       (kBudget - kFixedBytes - 2 * kQBytes - 2 * kPBytes) / (kSlotBytes + 512);
@@ -57,11 +59,11 @@ struct DecodeCfg {
   static_assert(kSlots >= 4, "the ring needs two tiles of K and V");
   static constexpr int kSmemBytes =
       1024 + kSlots * (kSlotBytes + 512) + 2 * kQBytes + 2 * kPBytes + kFixedBytes;
-  // Tensor memory columns: two score tiles, the output halves, scales.
+  // Tensor memory columns: two score tiles, two outputs of one or two halves, scales.
   static constexpr int kHalves = D > 128 ? 2 : 1;
   static constexpr int kOCol = 2 * kN;
-  static constexpr int kSfCol = kOCol + kHalves * kN;
-  static constexpr int kColsUsed = (kSfCol + 3) / 4 * 4 + 20;
+  static constexpr int kSfCol = kOCol + 2 * kHalves * kN;
+  static constexpr int kColsUsed = kSfCol + 20;
   static constexpr int kTmemCols = kColsUsed <= 64 ? 64 : kColsUsed <= 128 ? 128 : kColsUsed <= 256 ? 256 : 512;
   static_assert(kColsUsed <= 512, "tensor memory");
   static constexpr uint64_t kSwizzle = kRowBytes == 128 ? ptx::kSwizzle128 : ptx::kSwizzle64;
@@ -69,6 +71,10 @@ struct DecodeCfg {
   // Partial rows of one CTA end: RP rows of D values, then RP pairs (maximum, sum).
   static constexpr int kPartialFloats = RP * D + 2 * RP;
 };
+
+// Rows (new tokens x query heads) of the widest variant: two accumulators of two halves and
+// three terms each leave tensor memory for 24 rows, the others take 32.
+constexpr int most_rows(int d, int terms) { return d == 256 && terms == 3 ? 24 : 32; }
 
 // Share of the work list of one CTA, the same arithmetic in both kernels.
 struct Share {
@@ -175,13 +181,14 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   uint64_t* bars = reinterpret_cast<uint64_t*>(fixed);
   uint8_t* ones = fixed + 512;                                 // scale atom of factors of one
   float* row_scale = reinterpret_cast<float*>(fixed + 1024);   // [2][RP]
-  float* red_max = row_scale + 2 * RP;                         // [2][4][RP]
-  float* red_sum = red_max + 8 * RP;                           // [4][RP]
-  Cursor* start = reinterpret_cast<Cursor*>(red_sum + 4 * RP);
+  float* red_max = row_scale + 2 * RP;                         // [group][2][warp][RP]
+  float* red_sum = red_max + 16 * RP;                          // [group][warp][RP]
+  float* red_top = red_sum + 8 * RP;                           // [group][RP]
+  Cursor* start = reinterpret_cast<Cursor*>(red_top + 2 * RP);
   int64_t* share_smem = reinterpret_cast<int64_t*>(start + 1);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(share_smem + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  static_assert(1024 + 14 * RP * 4 + sizeof(Cursor) + 64 <= C::kFixedBytes, "fixed area");
+  static_assert(1024 + 28 * RP * 4 + sizeof(Cursor) + 64 <= C::kFixedBytes, "fixed area");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t full0 = ptx::smem_u32(bars);
@@ -191,23 +198,21 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   const uint32_t pvdone0 = pfull0 + 16;
   const uint32_t qfull0 = pvdone0 + 16;
   const uint32_t qempty0 = qfull0 + 16;
-  const uint32_t wsync = qempty0 + 16;             // among the softmax warps
-  static_assert(8 * (2 * 16 + 11) <= 512, "barriers");
+  static_assert(8 * (2 * 16 + 10) <= 512, "barriers");
 
   if (threadIdx.x == 0) {
     *abort_flag = 0;
     for (int s = 0; s < C::kSlots; ++s) {
-      ptx::mbar_init(full0 + 8 * s, 33);  // expected bytes, and one arrival per lane for the scales
+      ptx::mbar_init(full0 + 8 * s, 2);  // the copies' bytes, and the scales
       ptx::mbar_init(empty0 + 8 * s, 1);
     }
     for (int i = 0; i < 2; ++i) {
       ptx::mbar_init(sfull0 + 8 * i, 1);
-      ptx::mbar_init(pfull0 + 8 * i, kSoftmaxWarps);
+      ptx::mbar_init(pfull0 + 8 * i, kGroupWarps);
       ptx::mbar_init(pvdone0 + 8 * i, 1);
       ptx::mbar_init(qfull0 + 8 * i, kQueryWarps);
-      ptx::mbar_init(qempty0 + 8 * i, 1 + kSoftmaxWarps);
+      ptx::mbar_init(qempty0 + 8 * i, 1 + 2 * kGroupWarps);
     }
-    ptx::mbar_init(wsync, kSoftmaxWarps);
     ptx::fence_mbar_init();
     ptx::prefetch_tensormap(&tm_k);
     ptx::prefetch_tensormap(&tm_v);
@@ -242,11 +247,11 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   if (count > 0 && warp == kTmaWarp) {
     // ---------------- TMA producer ----------------
     // Tiles are fetched in the order of their use: K0, K1, V0, K2, V1, ...  Lane l looks up block
-    // l % 4 of tile l / 4 of a group of eight tiles; the next group's lookups are in flight while
-    // this group is copied.
+    // l % 4 of tile l / 4 of a group of eight tiles and later issues that block's copies itself;
+    // the next group's lookups are in flight while this group is copied.
     Cursor mine = *start;
     for (int i = 0; i < (lane >> 2); ++i) mine.next(a);
-    int64_t page = -1, next_page = -1;  // first scale / value block of this lane's block, or -1
+    int64_t page = -1, next_page = -1;  // scale block of this lane's block of tokens, or -1
     uint32_t k_sf = 127, v_sf = 127, next_k = 127, next_v = 127;
     auto lookup_page = [&]() -> int64_t {
       const int block = mine.tile * kKvTileBlocks + (lane & 3);
@@ -265,44 +270,39 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
     int slot = 0;
     uint32_t phase = 0;
     bool ok = true;
+    const bool leads = (lane & 3) % per_page == 0;  // first block of a page in its tile
+    const uint32_t page_bytes = (uint32_t)(a.cache.page_size * D);
+    const uint32_t slots_s = ptx::smem_u32(slots) + (lane & 3) * kKvBlock * C::kRowBytes;
     // Copies one tile whose four blocks are known to lanes src .. src + 3.
     auto copy = [&](bool is_v, int64_t lane_page, uint32_t lane_sf, int src) {
       ok = ok && __all_sync(0xffffffffu, bounded_wait(empty0 + 8 * slot, phase ^ 1u, abort_flag,
                                                       a.status, 401));
-      int64_t at[kKvTileBlocks];
-      uint32_t sf[kKvTileBlocks];
-#pragma unroll
-      for (int i = 0; i < kKvTileBlocks; ++i) {
-        at[i] = __shfl_sync(0xffffffffu, lane_page, src + i);
-        sf[i] = __shfl_sync(0xffffffffu, lane_sf, src + i);
-      }
       if (!ok) return;
       const uint32_t bar = full0 + 8 * slot;
+      // One copy per page and 128 columns; blocks of no page are left as they are.
+      const bool issue = (lane & ~3) == src && leads && lane_page >= 0;
+      const uint32_t pages = __popc(__ballot_sync(0xffffffffu, issue));
+      if (lane == src) ptx::mbar_arrive_expect_tx(bar, pages * page_bytes);
+      __syncwarp();
+      if (issue) {
+#pragma unroll
+        for (int s = 0; s < C::kSubs; ++s)
+          ptx::tma_load_2d(slots_s + slot * C::kSlotBytes + s * C::kSubBytes, is_v ? &tm_v : &tm_k,
+                           s * 128, (int)(lane_page * kKvBlock), bar);
+      }
       // Scale atom: lane = row % 32.  Keys: row block c of 32 tokens has one factor for all of
       // head_dim; values: every row has the factors of the four 32-token steps along K.
-      const uint4 word = is_v ? make_uint4(sf[0] | sf[1] << 8 | sf[2] << 16 | sf[3] << 24, 0, 0, 0)
-                              : make_uint4(sf[0] * 0x01010101u, sf[1] * 0x01010101u,
-                                           sf[2] * 0x01010101u, sf[3] * 0x01010101u);
-      uint4* atom = reinterpret_cast<uint4*>(sf_tiles + slot * 512);
-      atom[lane] = is_v ? make_uint4(word.x, word.x, word.x, word.x) : word;
-      ptx::fence_proxy_async();
-      ptx::mbar_arrive(bar);
-      if (ptx::elect_one()) {
-        // One copy per page and 128 columns; blocks of no page are left as they are.
-        uint32_t bytes = 0;
-        for (int i = 0; i < kKvTileBlocks; i += per_page)
-          if (at[i] >= 0) bytes += (uint32_t)(a.cache.page_size * D);
-        ptx::mbar_arrive_expect_tx(bar, bytes);
-        const uint32_t dst = ptx::smem_u32(slots + slot * C::kSlotBytes);
-        for (int i = 0; i < kKvTileBlocks; i += per_page) {
-          if (at[i] < 0) continue;
+      uint32_t sf[kKvTileBlocks];
 #pragma unroll
-          for (int s = 0; s < C::kSubs; ++s)
-            ptx::tma_load_2d(dst + s * C::kSubBytes + i * kKvBlock * C::kRowBytes,
-                             is_v ? &tm_v : &tm_k, s * 128, (int)(at[i] * kKvBlock), bar);
-        }
-      }
+      for (int i = 0; i < kKvTileBlocks; ++i) sf[i] = __shfl_sync(0xffffffffu, lane_sf, src + i);
+      const uint32_t all = sf[0] | sf[1] << 8 | sf[2] << 16 | sf[3] << 24;
+      reinterpret_cast<uint4*>(sf_tiles + slot * 512)[lane] =
+          is_v ? make_uint4(all, all, all, all)
+               : make_uint4(sf[0] * 0x01010101u, sf[1] * 0x01010101u, sf[2] * 0x01010101u,
+                            sf[3] * 0x01010101u);
+      ptx::fence_proxy_async();
       __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(bar);
       if (++slot == C::kSlots) {
         slot = 0;
         phase ^= 1u;
@@ -333,20 +333,20 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   } else if (count > 0 && warp == kMmaWarp) {
     // ---------------- MMA issuer ----------------
     constexpr uint32_t kIdesc = ((uint32_t)(C::kN >> 3) << 17) | (1u << 23) | ((128u >> 4) << 24);
-    const uint32_t sf0 = tmem + (C::kSfCol + 3) / 4 * 4;  // K and V scales by tile parity, ones
+    const uint32_t sf0 = tmem + C::kSfCol;  // K and V scales by tile parity, then ones
     const uint32_t ones_t = sf0 + 16;
     if (ptx::elect_one()) ptx::tc_cp_32x128b_warpx4(ones_t, ptx::smem_desc_scale_atom(ptx::smem_u32(ones)));
     __syncwarp();
-    Cursor scored = *start, summed = scored;  // tile of the last QK and PV issued
-    int segment = 0;                          // of `scored`
+    Cursor scored = *start;        // tile of the last scores issued
+    int segment = 0, in_segment = 0;  // its segment, and its number there
+    int summed = 0;                // number of the last V tile within its segment
     bool ok = true;
     // Slot of K(i) is 2i - 1 (0 for the first), of V(i) 2i + 2 (2i + 1 for the last).
     auto scores = [&](int i) {
-      const bool first = i == 0 || scored.tile == 0;
       const bool last = i + 1 == count || scored.tile + 1 == scored.seq.tiles;
       const int at = i == 0 ? 0 : 2 * i - 1;
       const int slot = at % C::kSlots;
-      if (first)
+      if (in_segment == 0)
         ok = ok && __all_sync(0xffffffffu, bounded_wait(qfull0 + 8 * (segment & 1),
                                                         (uint32_t)(segment >> 1) & 1u, abort_flag,
                                                         a.status, 402));
@@ -369,15 +369,22 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
             ptx::tc_mma_mxf8f6f4(tmem + (i & 1) * C::kN, ad + 2 * ks, bd + 2 * ks, kIdesc, sf_t,
                                  ones_t, (s > 0 || ks > 0) ? 1u : 0u);
         }
-        ptx::tc_commit(empty0 + 8 * slot);
         ptx::tc_commit(sfull0 + 8 * (i & 1));
+        ptx::tc_commit(empty0 + 8 * slot);
         if (last) ptx::tc_commit(qempty0 + 8 * (segment & 1));
       }
       __syncwarp();
-      if (last) ++segment;
+      ++in_segment;
+      if (last) {
+        ++segment;
+        in_segment = 0;
+      }
     };
     scores(0);
     for (int i = 0; ok && i < count; ++i) {
+      // Number of tile i within its segment: the scores of tile i + 1 tell whether one ended.
+      const int number = summed;
+      summed = in_segment == 0 ? 0 : summed + 1;
       if (i + 1 < count) {
         scored.next(a);
         scores(i + 1);
@@ -391,7 +398,6 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
                                          abort_flag, a.status, 405));
       if (!ok) break;
       ptx::tc_fence_after();
-      const bool first = i == 0 || summed.tile == 0;
       if (ptx::elect_one()) {
         const uint32_t sf_t = sf0 + 8 * (i & 1) + 4;
         ptx::tc_cp_32x128b_warpx4(sf_t, ptx::smem_desc_scale_atom(ptx::smem_u32(sf_tiles + slot * 512)));
@@ -406,15 +412,15 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
 #pragma unroll
           for (int ks = 0; ks < kKvTileBlocks; ++ks) {
             const uint32_t idesc = kIdesc | (1u << 15) | ((uint32_t)ks << 29);
-            ptx::tc_mma_mxf8f6f4(tmem + C::kOCol + h * C::kN, ad + ks * (kKvBlock * C::kRowBytes / 16),
-                                 bd + 2 * ks, idesc, sf_t, ones_t, (!first || ks > 0) ? 1u : 0u);
+            ptx::tc_mma_mxf8f6f4(tmem + C::kOCol + ((i & 1) * C::kHalves + h) * C::kN,
+                                 ad + ks * (kKvBlock * C::kRowBytes / 16), bd + 2 * ks, idesc, sf_t,
+                                 ones_t, (number >= 2 || ks > 0) ? 1u : 0u);
           }
         }
-        ptx::tc_commit(empty0 + 8 * slot);
         ptx::tc_commit(pvdone0 + 8 * (i & 1));
+        ptx::tc_commit(empty0 + 8 * slot);
       }
       __syncwarp();
-      if (i + 1 < count) summed.next(a);
     }
   } else if (count > 0 && warp >= kQueryWarp) {
     // ---------------- query terms ----------------
@@ -498,245 +504,258 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       c.tile = c.seq.tiles - 1;
       if (left > 0) c.next(a);
     }
-  } else if (count > 0 && warp < kSoftmaxWarps) {
+  } else if (count > 0 && warp < 2 * kGroupWarps) {
     // ---------------- softmax: lane = token of the tile ----------------
-    const int token = warp * 32 + lane;  // within the tile; warp = its scale block
-    const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
+    // Two groups of four warps take alternate tiles, each with its own maximum, sum and output
+    // accumulator; they meet at the end of a segment (the tiles of one (sequence, head)).
+    // A wait that runs out makes `failed` true; the votes below end both groups together.
+    const int group = warp / kGroupWarps, quarter = warp % kGroupWarps;
+    const int token = quarter * 32 + lane;  // within the tile; quarter = its scale block
+    const uint32_t lane_t = tmem + ((uint32_t)(quarter * 32) << 16);
+    const uint32_t s_t = lane_t + group * C::kN;
+    const uint32_t sfull = sfull0 + 8 * group, pfull = pfull0 + 8 * group;
+    const uint32_t pvdone = pvdone0 + 8 * group;
+    uint8_t* p_s = p_tiles + group * C::kPBytes + (token & 15);
+    float* my_max = red_max + group * 8 * RP;
     Cursor c = *start;
-    float top[RP], sum[RP], factor[RP];  // top: the same in all lanes
-    int segment = 0;
-    int segment_tile0 = c.tile;          // first tile of this CTA in the segment
-    bool ok = true;
-    // Barrier among the four warps; bounded like every other wait.
-    uint32_t wphase = 0;
-    auto warps_sync = [&]() -> bool {
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(wsync);
-      const bool done = bounded_wait(wsync, wphase, abort_flag, a.status, 413);
-      wphase ^= 1u;
-      return __all_sync(0xffffffffu, done);
-    };
-    auto block_named = [&](const Cursor& at) -> bool {
-      const int block = at.tile * kKvTileBlocks + warp;
-      return block * kKvBlock < at.seq.length && kv_page(a.batch, a.cache, at.b, block) >= 0;
-    };
-    bool named = block_named(c);
-    for (int i = 0; i < count; ++i) {
-      const bool first = i == 0 || c.tile == 0;
-      const bool last = i + 1 == count || c.tile + 1 == c.seq.tiles;
-      // The next tile's page lookup is in flight during this tile.
-      Cursor ahead = c;
-      bool named_ahead = false;
-      if (i + 1 < count) {
-        ahead.next(a);
-        named_ahead = block_named(ahead);
+    bool failed = false;
+    int i0 = 0;            // first tile of the segment in the CTA's list
+    uint32_t done = 0;     // tiles this group has taken
+    for (int segment = 0; i0 < count; ++segment) {
+      const int tiles = min(count - i0, c.seq.tiles - c.tile);
+      const int32_t* table = a.batch.block_table + (int64_t)c.b * a.batch.table_stride;
+      // Entry of the block table for this warp's block of a tile, -1 where there is no token.
+      auto entry = [&](int j) -> int32_t {
+        const int block = (c.tile + j) * kKvTileBlocks + quarter;
+        return j < tiles && block * kKvBlock < c.seq.length ? table[block / per_page] : -1;
+      };
+      const int j0 = (group ^ i0) & 1;
+      int32_t page = entry(j0), page_next = entry(j0 + 2);
+      failed |= !bounded_wait(qfull0 + 8 * (segment & 1), (uint32_t)(segment >> 1) & 1u, abort_flag,
+                              a.status, 407);
+      float top[RP], sum[RP], factor[RP];  // top: the same in all lanes of the group
+#pragma unroll
+      for (int r = 0; r < RP; ++r) {
+        factor[r] = row_scale[(segment & 1) * RP + r] * a.scale_log2;
+        top[r] = -INFINITY;
+        sum[r] = 0.0f;
       }
-      if (first) {
-        segment_tile0 = c.tile;
-        ok = bounded_wait(qfull0 + 8 * (segment & 1), (uint32_t)(segment >> 1) & 1u, abort_flag,
-                          a.status, 407);
-        if (!__all_sync(0xffffffffu, ok)) break;
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(qempty0 + 8 * (segment & 1));
+#pragma unroll 1
+      for (int j = j0; j < tiles; j += 2, ++done) {
+        const int i = i0 + j;
+        const bool named = page >= 0 && page < a.cache.pages;
+        page = page_next;
+        page_next = entry(j + 4);
+        // Tokens of this tile that exist.
+        const int t0 = (c.tile + j) * kKvTile;
+        const int held = min(kKvTile, c.seq.length - t0);
+        if (!(named && (quarter + 1) * 32 <= held)) {
+          // Rows of V without a token may hold anything, NaN among them, and 0 * NaN is NaN: clear
+          // them once the tile has landed.
+          const int at = i + 1 < count ? 2 * i + 2 : 2 * i + 1;
+          const int slot = at % C::kSlots;
+          failed |= !bounded_wait(full0 + 8 * slot, (uint32_t)(at / C::kSlots) & 1u, abort_flag,
+                                  a.status, 408);
+          uint8_t* v_s = slots + slot * C::kSlotBytes;
+          const int from = named ? max(0, held - quarter * 32) : 0;
+          for (int at16 = from * (D / 16) + lane; at16 < 32 * (D / 16); at16 += 32) {
+            const int t = at16 / (D / 16), piece = at16 % (D / 16);
+            const int s = piece / (C::kRowBytes / 16), in_row = piece % (C::kRowBytes / 16);
+            *reinterpret_cast<uint4*>(v_s + s * C::kSubBytes + (quarter * 32 + t) * C::kRowBytes +
+                                      in_row * 16) = make_uint4(0, 0, 0, 0);
+          }
+          ptx::fence_proxy_async();
+        }
+        const bool here = named && token < held;
+        failed |= !bounded_wait(sfull, done & 1u, abort_flag, a.status, 409);
+        __syncwarp();
+        ptx::tc_fence_after();
+        float s[RP];
+#pragma unroll
+        for (int r0 = 0; r0 < RP; r0 += 8) {
+          uint32_t raw[TERMS][8];
+#pragma unroll
+          for (int k = 0; k < TERMS; ++k) ptx::tmem_ld_x8(s_t + k * RP + r0, raw[k]);
+          ptx::tmem_ld_wait();
+#pragma unroll
+          for (int n = 0; n < 8; ++n) {
+            float v = __uint_as_float(raw[TERMS - 1][n]);
+#pragma unroll
+            for (int k = TERMS - 2; k >= 0; --k) v = v * 0.0625f + __uint_as_float(raw[k][n]);
+            s[r0 + n] = here ? v * factor[r0 + n] : -INFINITY;
+          }
+        }
+        ptx::tc_fence_before();
+        if (a.causal && t0 + held - 1 > c.seq.last - c.seq.rows + 1) {
+#pragma unroll
+          for (int r = 0; r < RP; ++r)
+            if (t0 + token > c.seq.last - c.seq.rows + 1 + r / a.group) s[r] = -INFINITY;
+        }
+        // Largest score of the tile per row, over the four warps.
+        float* mine = my_max + (done & 1u) * 4 * RP;
 #pragma unroll
         for (int r = 0; r < RP; ++r) {
-          factor[r] = row_scale[(segment & 1) * RP + r] * a.scale_log2;
-          top[r] = -INFINITY;
-          sum[r] = 0.0f;
+          const float m = ptx::warp_max(s[r]);
+          if (lane == (r & 31)) mine[quarter * RP + r] = m;
         }
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(qempty0 + 8 * (segment & 1));
-      }
-      // Tokens of this tile that exist, and how far the rows see.
-      const int64_t t0 = (int64_t)c.tile * kKvTile;
-      const int held = (int)min((int64_t)kKvTile, c.seq.length - t0);
-      const bool here = named && token < held;
-      if (!__all_sync(0xffffffffu, named && (warp + 1) * 32 <= held)) {
-        // Rows of V without a token may hold anything, NaN among them, and 0 * NaN is NaN: clear
-        // them once the tile has landed.
-        const int at = i + 1 < count ? 2 * i + 2 : 2 * i + 1;
-        const int slot = at % C::kSlots;
-        ok = bounded_wait(full0 + 8 * slot, (uint32_t)(at / C::kSlots) & 1u, abort_flag, a.status, 408);
-        if (!__all_sync(0xffffffffu, ok)) break;
-        uint8_t* v_s = slots + slot * C::kSlotBytes;
-        for (int t = 0; t < 32; ++t) {
-          if (named && warp * 32 + t < held) continue;
-          for (int at16 = lane; at16 < D / 16; at16 += 32) {
-            const int s = at16 * 16 / C::kRowBytes, in_row = at16 % (C::kRowBytes / 16);
-            *reinterpret_cast<uint4*>(v_s + s * C::kSubBytes + (warp * 32 + t) * C::kRowBytes +
-                                      in_row * 16) = make_uint4(0, 0, 0, 0);
+        failed = ptx::barrier_any(1 + group, kGroupWarps * 32, failed);
+        if (failed) break;
+        bool raise = false;
+        float next[RP];
+#pragma unroll
+        for (int r = 0; r < RP; ++r) {
+          const float m = fmaxf(fmaxf(mine[r], mine[RP + r]), fmaxf(mine[2 * RP + r], mine[3 * RP + r]));
+          next[r] = m > top[r] + kSlackLog2 || (top[r] == -INFINITY && m > top[r]) ? m : top[r];
+          raise = raise || next[r] != top[r];
+        }
+        // PV of this group's last tile has read the weights that this tile's replace.
+        if (done > 0) failed |= !bounded_wait(pvdone, (done - 1) & 1u, abort_flag, a.status, 410);
+        if (raise) {  // the same in all threads of the group
+          if (j != j0) {
+            __syncwarp();
+            ptx::tc_fence_after();
+#pragma unroll
+            for (int h = 0; h < C::kHalves; ++h) {
+#pragma unroll
+              for (int c0 = 0; c0 < C::kN; c0 += 8) {
+                uint32_t o[8];
+                const uint32_t at = lane_t + C::kOCol + (group * C::kHalves + h) * C::kN + c0;
+                ptx::tmem_ld_x8(at, o);
+                ptx::tmem_ld_wait();
+#pragma unroll
+                for (int n = 0; n < 8; ++n) {
+                  const int r = (c0 + n) % RP;
+                  const float f = next[r] == top[r] ? 1.0f : exp2f(top[r] - next[r]);
+                  o[n] = __float_as_uint(__uint_as_float(o[n]) * f);
+                }
+                ptx::tmem_st_x8(at, o);
+              }
+            }
+            ptx::tmem_st_wait();
+          }
+#pragma unroll
+          for (int r = 0; r < RP; ++r) {
+            if (next[r] != top[r]) sum[r] *= exp2f(top[r] - next[r]);
+            top[r] = next[r];
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < RP; r += 2) {
+          float p[2];
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            p[n] = exp2f(s[r + n] - (top[r + n] == -INFINITY ? 0.0f : top[r + n]));
+            sum[r + n] += p[n];
+          }
+          uint32_t codes[TERMS];
+          e4m3_terms<TERMS>(p[0] * kWeightScale, p[1] * kWeightScale, codes);
+#pragma unroll
+          for (int k = 0; k < TERMS; ++k) {
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+              const int col = k * RP + r + n;
+              p_s[col * 128 + (((token >> 4) ^ (col & 7)) << 4)] = (uint8_t)(codes[k] >> (8 * n));
+            }
           }
         }
         ptx::fence_proxy_async();
-      }
-      ok = bounded_wait(sfull0 + 8 * (i & 1), (uint32_t)(i >> 1) & 1u, abort_flag, a.status, 409);
-      if (!__all_sync(0xffffffffu, ok)) break;
-      ptx::tc_fence_after();
-      float s[RP];
-#pragma unroll
-      for (int r0 = 0; r0 < RP; r0 += 8) {
-        uint32_t raw[TERMS][8];
-#pragma unroll
-        for (int k = 0; k < TERMS; ++k)
-          ptx::tmem_ld_x8(tmem + lane_base + (i & 1) * C::kN + k * RP + r0, raw[k]);
-        ptx::tmem_ld_wait();
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          float v = __uint_as_float(raw[TERMS - 1][j]);
-#pragma unroll
-          for (int k = TERMS - 2; k >= 0; --k) v = v * 0.0625f + __uint_as_float(raw[k][j]);
-          s[r0 + j] = here ? v * factor[r0 + j] : -INFINITY;
-        }
-      }
-      ptx::tc_fence_before();
-      if (a.causal && t0 + held > c.seq.last - c.seq.rows + 1) {
-#pragma unroll
-        for (int r = 0; r < RP; ++r)
-          if (t0 + token > c.seq.last - c.seq.rows + 1 + r / a.group) s[r] = -INFINITY;
-      }
-      // Largest score of the tile per row, over the four warps.
-      float* mine = red_max + (i & 1) * 4 * RP;
-#pragma unroll
-      for (int r = 0; r < RP; ++r) {
-        const float m = ptx::warp_max(s[r]);
-        if (lane == (r & 31)) mine[warp * RP + r] = m;
-      }
-      if (!warps_sync()) break;
-      bool raise = false;
-      float next[RP];
-#pragma unroll
-      for (int r = 0; r < RP; ++r) {
-        const float m = fmaxf(fmaxf(mine[r], mine[RP + r]), fmaxf(mine[2 * RP + r], mine[3 * RP + r]));
-        next[r] = m > top[r] + kSlackLog2 || (top[r] == -INFINITY && m > top[r]) ? m : top[r];
-        raise = raise || next[r] != top[r];
-      }
-      if (raise) {  // the same in all threads of the four warps
-        if (c.tile != segment_tile0) {
-          // The output so far shrinks; the last PV of this segment has to be done.
-          ok = bounded_wait(pvdone0 + 8 * ((i - 1) & 1), (uint32_t)((i - 1) >> 1) & 1u, abort_flag,
-                            a.status, 410);
-          if (!__all_sync(0xffffffffu, ok)) break;
-          ptx::tc_fence_after();
-#pragma unroll
-          for (int h = 0; h < C::kHalves; ++h) {
-#pragma unroll
-            for (int c0 = 0; c0 < C::kN; c0 += 8) {
-              uint32_t o[8];
-              const uint32_t at = tmem + lane_base + C::kOCol + h * C::kN + c0;
-              ptx::tmem_ld_x8(at, o);
-              ptx::tmem_ld_wait();
-#pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                const int r = (c0 + j) % RP;
-                const float f = next[r] == top[r] ? 1.0f : exp2f(top[r] - next[r]);
-                o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-              }
-              ptx::tmem_st_x8(at, o);
-            }
-          }
-          ptx::tmem_st_wait();
-          ptx::tc_fence_before();
-        }
-#pragma unroll
-        for (int r = 0; r < RP; ++r) {
-          if (next[r] != top[r]) sum[r] *= exp2f(top[r] - next[r]);
-          top[r] = next[r];
-        }
-      }
-      if (i >= 2) {  // PV(i - 2) has read the buffer that this tile's weights go to
-        ok = bounded_wait(pvdone0 + 8 * (i & 1), (uint32_t)((i - 2) >> 1) & 1u, abort_flag, a.status, 411);
-        if (!__all_sync(0xffffffffu, ok)) break;
-      }
-      uint8_t* p_s = p_tiles + (i & 1) * C::kPBytes + (token & 15);
-#pragma unroll
-      for (int r = 0; r < RP; r += 2) {
-        float p[2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          p[j] = exp2f(s[r + j] - (top[r + j] == -INFINITY ? 0.0f : top[r + j]));
-          sum[r + j] += p[j];
-        }
-        uint32_t codes[TERMS];
-        e4m3_terms<TERMS>(p[0] * kWeightScale, p[1] * kWeightScale, codes);
-#pragma unroll
-        for (int k = 0; k < TERMS; ++k) {
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int col = k * RP + r + j;
-            p_s[col * 128 + (((token >> 4) ^ (col & 7)) << 4)] = (uint8_t)(codes[k] >> (8 * j));
-          }
-        }
-      }
-      ptx::fence_proxy_async();
-      ptx::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(pfull0 + 8 * (i & 1));
-      if (last) {
-        // ---- the segment's rows: sums over the tokens, then the output of this CTA's tiles ----
-#pragma unroll
-        for (int r = 0; r < RP; ++r) {
-          float v = sum[r];
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-          if (lane == (r & 31)) red_sum[warp * RP + r] = v;
-        }
-        if (!warps_sync()) break;
-        ok = bounded_wait(pvdone0 + 8 * (i & 1), (uint32_t)(i >> 1) & 1u, abort_flag, a.status, 412);
-        if (!__all_sync(0xffffffffu, ok)) break;
-        ptx::tc_fence_after();
-        const int rows = c.seq.rows * a.group;
-        const bool whole = segment_tile0 == 0 && c.tile + 1 == c.seq.tiles;
-        // A share that begins inside a (sequence, head) uses the CTA's first partial slot for it,
-        // one that ends inside the second.
-        float* part = a.partials + (int64_t)(2 * blockIdx.x + (segment_tile0 != 0 ? 0 : 1)) *
-                                       C::kPartialFloats;
-#pragma unroll 1
-        for (int r0 = 0; r0 < RP; r0 += 8) {
-#pragma unroll
-          for (int h = 0; h < C::kHalves; ++h) {
-            uint32_t raw[TERMS][8];
-#pragma unroll
-            for (int k = 0; k < TERMS; ++k)
-              ptx::tmem_ld_x8(tmem + lane_base + C::kOCol + h * C::kN + k * RP + r0, raw[k]);
-            ptx::tmem_ld_wait();
-            const int d = h * 128 + token;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const int r = r0 + j;
-              float v = __uint_as_float(raw[TERMS - 1][j]);
-#pragma unroll
-              for (int k = TERMS - 2; k >= 0; --k) v = v * 0.0625f + __uint_as_float(raw[k][j]);
-              v *= 1.0f / kWeightScale;
-              if (r < rows && d < D) {
-                if (whole) {
-                  const float l = red_sum[r] + red_sum[RP + r] + red_sum[2 * RP + r] + red_sum[3 * RP + r];
-                  int64_t at;
-                  output_row<RP>(a, c.seq, c.head, r, &at);
-                  v = l == 0.0f ? 0.0f : v / l;
-                  T* out = static_cast<T*>(a.out) + at + d;
-                  if constexpr (TERMS == 2) *out = __float2bfloat16_rn(v);
-                  else *out = __float2half_rn(v);
-                } else {
-                  part[r * D + d] = v;
-                }
-              }
-            }
-          }
-        }
-        if (!whole) {
-#pragma unroll
-          for (int r = 0; r < RP; ++r)
-            if (token == r) {
-              part[RP * D + 2 * r] = top[r];
-              part[RP * D + 2 * r + 1] =
-                  red_sum[r] + red_sum[RP + r] + red_sum[2 * RP + r] + red_sum[3 * RP + r];
-            }
-        }
         ptx::tc_fence_before();
-        // red_sum is written again by the next segment.
-        if (!warps_sync()) break;
-        ++segment;
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(pfull);
       }
-      c = ahead;
-      named = named_ahead;
+      // ---- the segment's rows: sums over the tokens, then the output of this CTA's tiles ----
+#pragma unroll
+      for (int r = 0; r < RP; ++r) {
+        float v = sum[r];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        if (lane == (r & 31)) {
+          red_sum[(group * 4 + quarter) * RP + r] = v;
+          if (quarter == 0) red_top[group * RP + r] = top[r];
+        }
+      }
+      if (j0 < tiles && !failed)
+        failed |= !bounded_wait(pvdone, (done - 1) & 1u, abort_flag, a.status, 411);
+      failed = ptx::barrier_any(3, 2 * kGroupWarps * 32, failed);
+      if (failed) break;
+      ptx::tc_fence_after();
+      const int rows = c.seq.rows * a.group;
+      const bool whole = c.tile == 0 && tiles == c.seq.tiles;
+      // A share that begins inside a (sequence, head) uses the CTA's first partial slot for it,
+      // one that ends inside the second.
+      float* part = a.partials +
+                    (int64_t)(2 * blockIdx.x + (c.tile != 0 ? 0 : 1)) * C::kPartialFloats;
+      // The groups share the output by halves of head_dim, or by eight rows.
+#pragma unroll 1
+      for (int unit = group; unit < C::kHalves * (RP / 8); unit += 2) {
+        const int h = unit % C::kHalves, r0 = unit / C::kHalves * 8;
+        float v[8];
+#pragma unroll
+        for (int n = 0; n < 8; ++n) v[n] = 0.0f;
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          if (g == 1 && tiles < 2) break;  // only one group had a tile
+          const int owner = (g ^ i0) & 1;  // group of the segment's tile g
+          uint32_t raw[TERMS][8];
+#pragma unroll
+          for (int k = 0; k < TERMS; ++k)
+            ptx::tmem_ld_x8(lane_t + C::kOCol + (owner * C::kHalves + h) * C::kN + k * RP + r0, raw[k]);
+          ptx::tmem_ld_wait();
+#pragma unroll
+          for (int n = 0; n < 8; ++n) {
+            float x = __uint_as_float(raw[TERMS - 1][n]);
+#pragma unroll
+            for (int k = TERMS - 2; k >= 0; --k) x = x * 0.0625f + __uint_as_float(raw[k][n]);
+            const float ta = red_top[owner * RP + r0 + n], tb = red_top[(owner ^ 1) * RP + r0 + n];
+            const float most = fmaxf(ta, tb);
+            // Maxima are -inf where a row saw nothing, NaN scores leave them there too.
+            v[n] += x * (ta == most ? 1.0f : exp2f(ta - most)) * (1.0f / kWeightScale);
+          }
+        }
+        const int d = h * 128 + token;
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+          const int r = r0 + n;
+          if (r < rows && d < D) {
+            if (whole) {
+              const float ta = red_top[r], tb = red_top[RP + r], most = fmaxf(ta, tb);
+              const float la = red_sum[r] + red_sum[RP + r] + red_sum[2 * RP + r] + red_sum[3 * RP + r];
+              const float lb = red_sum[4 * RP + r] + red_sum[5 * RP + r] + red_sum[6 * RP + r] +
+                               red_sum[7 * RP + r];
+              const float l = la * (ta == most ? 1.0f : exp2f(ta - most)) +
+                              lb * (tb == most ? 1.0f : exp2f(tb - most));
+              int64_t at;
+              output_row<RP>(a, c.seq, c.head, r, &at);
+              const float o = l == 0.0f ? 0.0f : v[n] / l;
+              T* out = static_cast<T*>(a.out) + at + d;
+              if constexpr (TERMS == 2) *out = __float2bfloat16_rn(o);
+              else *out = __float2half_rn(o);
+            } else {
+              part[r * D + d] = v[n];
+            }
+          }
+        }
+      }
+      if (!whole && threadIdx.x < RP) {
+        const int r = threadIdx.x;
+        const float ta = red_top[r], tb = red_top[RP + r], most = fmaxf(ta, tb);
+        const float la = red_sum[r] + red_sum[RP + r] + red_sum[2 * RP + r] + red_sum[3 * RP + r];
+        const float lb = red_sum[4 * RP + r] + red_sum[5 * RP + r] + red_sum[6 * RP + r] +
+                         red_sum[7 * RP + r];
+        part[RP * D + 2 * r] = most;
+        part[RP * D + 2 * r + 1] = la * (ta == most ? 1.0f : exp2f(ta - most)) +
+                                   lb * (tb == most ? 1.0f : exp2f(tb - most));
+      }
+      ptx::tc_fence_before();
+      i0 += tiles;
+      if (i0 < count) {
+        // The accumulators and sums of this segment have been read.
+        if (ptx::barrier_any(3, 2 * kGroupWarps * 32, false)) break;
+        c.tile = c.seq.tiles - 1;
+        c.next(a);
+      }
     }
   }
 
@@ -865,10 +884,8 @@ int launch_rows(const CUtensorMap& tm_k, const CUtensorMap& tm_v, const Attentio
                 cudaStream_t stream) {
   if (a.max_rows <= 8) return launch<D, 8, TERMS>(tm_k, tm_v, a, grid, stream);
   if (a.max_rows <= 16) return launch<D, 16, TERMS>(tm_k, tm_v, a, grid, stream);
-  return launch<D, 32, TERMS>(tm_k, tm_v, a, grid, stream);
+  return launch<D, most_rows(D, TERMS), TERMS>(tm_k, tm_v, a, grid, stream);
 }
-
-int padded_rows(int rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : 32; }
 
 }  // namespace
 
@@ -879,14 +896,18 @@ int kv_decode_grid(int64_t batch, int kv_heads, int64_t max_context) {
   return (int)(want < kSms ? want : kSms);
 }
 
-int64_t kv_decode_workspace(int64_t batch, int kv_heads, int head_dim, int rows, int64_t max_context) {
+int kv_decode_rows(int head_dim, int dtype) { return most_rows(head_dim, dtype == kBF16 ? 2 : 3); }
+
+int64_t kv_decode_workspace(int64_t batch, int kv_heads, int head_dim, int dtype, int rows,
+                            int64_t max_context) {
   const int grid = kv_decode_grid(batch, kv_heads, max_context);
   if (grid == 1) return 0;
-  const int rp = padded_rows(rows);
+  const int rp = rows <= 8 ? 8 : rows <= 16 ? 16 : kv_decode_rows(head_dim, dtype);
   return (int64_t)grid * 2 * (rp * head_dim + 2 * rp) * 4;
 }
 
-// Sequences with at most a.max_rows <= 32 rows (tokens x group); others are left alone.
+// Sequences with at most a.max_rows <= kv_decode_rows() rows (tokens x group); others are left
+// alone.
 int launch_kv_decode(const AttentionArgs& a, int dtype, cudaStream_t stream) {
   CUtensorMap tm_k, tm_v;
   if (int rc = make_kv_map(&tm_k, a.cache.k_values, a.cache)) return rc;

@@ -57,6 +57,19 @@ __device__ __forceinline__ float warp_max(float v) {
   asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
   return r;
 }
+// Barrier `id` (1..15) among `threads` threads of the CTA; true in all of them when `v` is in any.
+__device__ __forceinline__ bool barrier_any(int id, int threads, bool v) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 q, %3, 0;\n\t"
+      "bar.red.or.pred p, %1, %2, q;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r)
+      : "r"(id), "r"(threads), "r"((uint32_t)v)
+      : "memory");
+  return r != 0;
+}
 
 // ---- programmatic dependent launch -------------------------------------------------
 // Blocks until every grid this one depends on has completed and its writes are
