@@ -63,6 +63,23 @@ __device__ __forceinline__ void e4m3_terms(float a, float b, uint32_t (&codes)[k
   }
 }
 
+// The same of two FP16 numbers; returns what the terms add up to (exact in FP16: two terms have
+// at most nine bits, three hold all eleven).
+template <int kTerms>
+__device__ __forceinline__ __half2 e4m3_terms_half(__half2 x, uint32_t (&codes)[kTerms]) {
+  __half2 whole = x;
+#pragma unroll
+  for (int t = 0; t < kTerms; ++t) {
+    codes[t] = __nv_cvt_halfraw2_to_fp8x2(static_cast<__half2_raw>(x), __NV_SATFINITE, __NV_E4M3);
+    if (t + 1 < kTerms || kTerms == 2) {
+      const __half2 v(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)codes[t], __NV_E4M3));
+      if (kTerms == 2) whole = t == 0 ? v : __hfma2(v, __float2half2_rn(0.0625f), whole);
+      if (t + 1 < kTerms) x = __hmul2(__hsub2(x, v), __float2half2_rn(16.0f));
+    }
+  }
+  return whole;
+}
+
 __device__ __forceinline__ float pow2_int(int e) {  // 2^e, -126 <= e <= 127
   return __uint_as_float((uint32_t)(e + 127) << 23);
 }

@@ -21,10 +21,14 @@
 //    unnormalised rows with their maximum and sum, and a second kernel (launched as a
 //    programmatic dependent) joins them in the order of the tiles, so the result does not depend
 //    on timing.
-//  * Weights are scaled by 128 before they become E4M3 terms, so that small ones stay clear of
-//    E4M3's smallest step (the last of two terms ends at 2^-21 of the largest weight; at a scale
-//    of 16 a row whose softmax one token dominates was off by more than 2^-8 of its weights).
-//    E4M3 ends at 448, so the running maximum is raised when a tile exceeds it by 2^1.5.
+//  * Online softmax without touching the output.  The weights of a row are taken relative to the
+//    largest score among the warp's own 32 tokens, rounded up to a power of two, and that power
+//    (relative to a reference fixed by the first tile) is the hardware block scale of the
+//    weights: 32 tokens is one scale block of the second product.  So no maximum crosses warps
+//    and no accumulator is rescaled from tile to tile.  Only where a tile exceeds the reference
+//    by more than 2^16 the four warps move it and shrink the accumulator.  It is also the more
+//    exact way: each block's largest weight is in (128, 256], so E4M3's smallest step never
+//    reaches a weight that counts.
 #include "kv_attention.cuh"
 
 #include <cstdlib>
@@ -38,8 +42,9 @@ namespace {
 constexpr int kThreads = 384;
 constexpr int kGroupWarps = 4;  // warps of a softmax group, one per 32 lanes of tensor memory
 constexpr int kTmaWarp = 8, kMmaWarp = 9, kQueryWarp = 10, kQueryWarps = 2;
-constexpr float kWeightScale = 128.0f;  // weights 0..1 become 0..128 before rounding
-constexpr float kSlackLog2 = 1.5f;      // and may reach 2^1.5 times that before the maximum moves
+constexpr float kWeightScale = 256.0f;  // weights 0..1 become 0..256 before they become E4M3 terms
+constexpr float kMostLog2 = 16.0f;      // a tile may exceed the reference by 2^16
+constexpr int kSms = 148;
 constexpr int kMinTiles = 2;           // tiles a CTA takes at least, see the plan
 
 template <int D, int RP, int TERMS>
@@ -63,7 +68,8 @@ struct DecodeCfg {
   static constexpr int kHalves = D > 128 ? 2 : 1;
   static constexpr int kOCol = 2 * kN;
   static constexpr int kSfCol = kOCol + 2 * kHalves * kN;
-  static constexpr int kColsUsed = kSfCol + 20;
+  static constexpr int kColsUsed = kSfCol + 28;
+  static constexpr int kChunk = RP % 16 == 0 ? 16 : 8;  // rows of a score tile held at a time
   static constexpr int kTmemCols = kColsUsed <= 64 ? 64 : kColsUsed <= 128 ? 128 : kColsUsed <= 256 ? 256 : 512;
   static_assert(kColsUsed <= 512, "tensor memory");
   static constexpr uint64_t kSwizzle = kRowBytes == 128 ? ptx::kSwizzle128 : ptx::kSwizzle64;
@@ -180,15 +186,16 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   uint8_t* fixed = sf_tiles + C::kSlots * 512;
   uint64_t* bars = reinterpret_cast<uint64_t*>(fixed);
   uint8_t* ones = fixed + 512;                                 // scale atom of factors of one
-  float* row_scale = reinterpret_cast<float*>(fixed + 1024);   // [2][RP]
-  float* red_max = row_scale + 2 * RP;                         // [group][2][warp][RP]
-  float* red_sum = red_max + 16 * RP;                          // [group][warp][RP]
+  uint8_t* p_sf = fixed + 1024;                                // scale atom of each group's weights
+  float* row_scale = reinterpret_cast<float*>(fixed + 2048);   // [2][RP]
+  float* red_max = row_scale + 2 * RP;                         // [group][warp][RP]
+  float* red_sum = red_max + 8 * RP;                           // [group][warp][RP]
   float* red_top = red_sum + 8 * RP;                           // [group][RP]
   Cursor* start = reinterpret_cast<Cursor*>(red_top + 2 * RP);
   int64_t* share_smem = reinterpret_cast<int64_t*>(start + 1);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(share_smem + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  static_assert(1024 + 28 * RP * 4 + sizeof(Cursor) + 64 <= C::kFixedBytes, "fixed area");
+  static_assert(2048 + 20 * RP * 4 + sizeof(Cursor) + 64 <= C::kFixedBytes, "fixed area");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t full0 = ptx::smem_u32(bars);
@@ -333,8 +340,8 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   } else if (count > 0 && warp == kMmaWarp) {
     // ---------------- MMA issuer ----------------
     constexpr uint32_t kIdesc = ((uint32_t)(C::kN >> 3) << 17) | (1u << 23) | ((128u >> 4) << 24);
-    const uint32_t sf0 = tmem + C::kSfCol;  // K and V scales by tile parity, then ones
-    const uint32_t ones_t = sf0 + 16;
+    const uint32_t sf0 = tmem + C::kSfCol;  // keys, values, weights by tile parity, then ones
+    const uint32_t ones_t = sf0 + 24;
     if (ptx::elect_one()) ptx::tc_cp_32x128b_warpx4(ones_t, ptx::smem_desc_scale_atom(ptx::smem_u32(ones)));
     __syncwarp();
     Cursor scored = *start;        // tile of the last scores issued
@@ -356,7 +363,7 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       if (!ok) return;
       ptx::tc_fence_after();
       if (ptx::elect_one()) {
-        const uint32_t sf_t = sf0 + 8 * (i & 1);
+        const uint32_t sf_t = sf0 + 12 * (i & 1);
         ptx::tc_cp_32x128b_warpx4(sf_t, ptx::smem_desc_scale_atom(ptx::smem_u32(sf_tiles + slot * 512)));
         const uint32_t k_s = ptx::smem_u32(slots + slot * C::kSlotBytes);
         const uint32_t q_s = ptx::smem_u32(q_tiles + (segment & 1) * C::kQBytes);
@@ -399,8 +406,9 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       if (!ok) break;
       ptx::tc_fence_after();
       if (ptx::elect_one()) {
-        const uint32_t sf_t = sf0 + 8 * (i & 1) + 4;
+        const uint32_t sf_t = sf0 + 12 * (i & 1) + 4, weight_t = sf_t + 4;
         ptx::tc_cp_32x128b_warpx4(sf_t, ptx::smem_desc_scale_atom(ptx::smem_u32(sf_tiles + slot * 512)));
+        ptx::tc_cp_32x128b_warpx4(weight_t, ptx::smem_desc_scale_atom(ptx::smem_u32(p_sf + (i & 1) * 512)));
         const uint32_t v_s = ptx::smem_u32(slots + slot * C::kSlotBytes);
         const uint64_t bd =
             ptx::smem_desc(ptx::smem_u32(p_tiles + (i & 1) * C::kPBytes), 0, 1024, ptx::kSwizzle128);
@@ -411,10 +419,10 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
           const uint64_t ad = ptx::smem_desc(v_s + h * C::kSubBytes, C::kGroup, C::kGroup, C::kSwizzle);
 #pragma unroll
           for (int ks = 0; ks < kKvTileBlocks; ++ks) {
-            const uint32_t idesc = kIdesc | (1u << 15) | ((uint32_t)ks << 29);
+            const uint32_t idesc = kIdesc | (1u << 15) | ((uint32_t)ks << 29) | ((uint32_t)ks << 4);
             ptx::tc_mma_mxf8f6f4(tmem + C::kOCol + ((i & 1) * C::kHalves + h) * C::kN,
                                  ad + ks * (kKvBlock * C::kRowBytes / 16), bd + 2 * ks, idesc, sf_t,
-                                 ones_t, (number >= 2 || ks > 0) ? 1u : 0u);
+                                 weight_t, (number >= 2 || ks > 0) ? 1u : 0u);
           }
         }
         ptx::tc_commit(pvdone0 + 8 * (i & 1));
@@ -516,7 +524,7 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
     const uint32_t sfull = sfull0 + 8 * group, pfull = pfull0 + 8 * group;
     const uint32_t pvdone = pvdone0 + 8 * group;
     uint8_t* p_s = p_tiles + group * C::kPBytes + (token & 15);
-    float* my_max = red_max + group * 8 * RP;
+    float* my_max = red_max + group * 4 * RP;
     Cursor c = *start;
     bool failed = false;
     int i0 = 0;            // first tile of the segment in the CTA's list
@@ -533,15 +541,13 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       int32_t page = entry(j0), page_next = entry(j0 + 2);
       failed |= !bounded_wait(qfull0 + 8 * (segment & 1), (uint32_t)(segment >> 1) & 1u, abort_flag,
                               a.status, 407);
-      float top[RP], sum[RP], factor[RP];  // top: the same in all lanes of the group
+      const float* scales = row_scale + (segment & 1) * RP;
+      float ref[RP], sum[RP];  // ref: the same in all lanes of the group
 #pragma unroll
       for (int r = 0; r < RP; ++r) {
-        factor[r] = row_scale[(segment & 1) * RP + r] * a.scale_log2;
-        top[r] = -INFINITY;
+        ref[r] = -INFINITY;
         sum[r] = 0.0f;
       }
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(qempty0 + 8 * (segment & 1));
 #pragma unroll 1
       for (int j = j0; j < tiles; j += 2, ++done) {
         const int i = i0 + j;
@@ -562,109 +568,145 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
           const int from = named ? max(0, held - quarter * 32) : 0;
           for (int at16 = from * (D / 16) + lane; at16 < 32 * (D / 16); at16 += 32) {
             const int t = at16 / (D / 16), piece = at16 % (D / 16);
-            const int s = piece / (C::kRowBytes / 16), in_row = piece % (C::kRowBytes / 16);
-            *reinterpret_cast<uint4*>(v_s + s * C::kSubBytes + (quarter * 32 + t) * C::kRowBytes +
+            const int sub = piece / (C::kRowBytes / 16), in_row = piece % (C::kRowBytes / 16);
+            *reinterpret_cast<uint4*>(v_s + sub * C::kSubBytes + (quarter * 32 + t) * C::kRowBytes +
                                       in_row * 16) = make_uint4(0, 0, 0, 0);
           }
           ptx::fence_proxy_async();
         }
         const bool here = named && token < held;
+        const bool bounded = a.causal && t0 + held - 1 > c.seq.last - c.seq.rows + 1;
         failed |= !bounded_wait(sfull, done & 1u, abort_flag, a.status, 409);
         __syncwarp();
         ptx::tc_fence_after();
-        float s[RP];
+        uint32_t my_code = 127;  // weight scale of row lane % RP in this warp's 32 tokens
+        bool ended = false;
 #pragma unroll
-        for (int r0 = 0; r0 < RP; r0 += 8) {
-          uint32_t raw[TERMS][8];
+        for (int c0 = 0; c0 < RP; c0 += C::kChunk) {
+          if (ended) continue;
+          float s[C::kChunk], top[C::kChunk];
+          bool raise = failed;
 #pragma unroll
-          for (int k = 0; k < TERMS; ++k) ptx::tmem_ld_x8(s_t + k * RP + r0, raw[k]);
-          ptx::tmem_ld_wait();
+          for (int r0 = 0; r0 < C::kChunk; r0 += 8) {
+            uint32_t raw[TERMS][8];
 #pragma unroll
-          for (int n = 0; n < 8; ++n) {
-            float v = __uint_as_float(raw[TERMS - 1][n]);
+            for (int k = 0; k < TERMS; ++k) ptx::tmem_ld_x8(s_t + k * RP + c0 + r0, raw[k]);
+            ptx::tmem_ld_wait();
 #pragma unroll
-            for (int k = TERMS - 2; k >= 0; --k) v = v * 0.0625f + __uint_as_float(raw[k][n]);
-            s[r0 + n] = here ? v * factor[r0 + n] : -INFINITY;
+            for (int n = 0; n < 8; ++n) {
+              float v = __uint_as_float(raw[TERMS - 1][n]);
+#pragma unroll
+              for (int k = TERMS - 2; k >= 0; --k) v = v * 0.0625f + __uint_as_float(raw[k][n]);
+              s[r0 + n] = here ? v * (scales[c0 + r0 + n] * a.scale_log2) : -INFINITY;
+            }
           }
-        }
-        ptx::tc_fence_before();
-        if (a.causal && t0 + held - 1 > c.seq.last - c.seq.rows + 1) {
+          if (bounded) {
 #pragma unroll
-          for (int r = 0; r < RP; ++r)
-            if (t0 + token > c.seq.last - c.seq.rows + 1 + r / a.group) s[r] = -INFINITY;
-        }
-        // Largest score of the tile per row, over the four warps.
-        float* mine = my_max + (done & 1u) * 4 * RP;
+            for (int r = 0; r < C::kChunk; ++r)
+              if (t0 + token > c.seq.last - c.seq.rows + 1 + (c0 + r) / a.group) s[r] = -INFINITY;
+          }
 #pragma unroll
-        for (int r = 0; r < RP; ++r) {
-          const float m = ptx::warp_max(s[r]);
-          if (lane == (r & 31)) mine[quarter * RP + r] = m;
-        }
-        failed = ptx::barrier_any(1 + group, kGroupWarps * 32, failed);
-        if (failed) break;
-        bool raise = false;
-        float next[RP];
+          for (int r = 0; r < C::kChunk; ++r) {
+            top[r] = ceilf(ptx::warp_max(s[r]));
+            raise = raise || top[r] > ref[c0 + r] + kMostLog2;
+          }
+          if (ptx::barrier_any(1 + group, kGroupWarps * 32, raise)) {
+            // The first tokens that a row sees, a later maximum far above its reference, or a wait
+            // that ran out: the four warps agree on the reference.
 #pragma unroll
-        for (int r = 0; r < RP; ++r) {
-          const float m = fmaxf(fmaxf(mine[r], mine[RP + r]), fmaxf(mine[2 * RP + r], mine[3 * RP + r]));
-          next[r] = m > top[r] + kSlackLog2 || (top[r] == -INFINITY && m > top[r]) ? m : top[r];
-          raise = raise || next[r] != top[r];
-        }
-        // PV of this group's last tile has read the weights that this tile's replace.
-        if (done > 0) failed |= !bounded_wait(pvdone, (done - 1) & 1u, abort_flag, a.status, 410);
-        if (raise) {  // the same in all threads of the group
-          if (j != j0) {
-            __syncwarp();
-            ptx::tc_fence_after();
+            for (int r = 0; r < C::kChunk; ++r)
+              if (lane == (r & 31)) my_max[quarter * RP + r] = top[r];
+            failed = ptx::barrier_any(1 + group, kGroupWarps * 32, failed);
+            if (failed) {
+              ended = true;
+              continue;
+            }
+            const bool shrink = j != j0;
+            if (shrink) {
+              failed |= !bounded_wait(pvdone, (done - 1) & 1u, abort_flag, a.status, 412);
+              __syncwarp();
+              ptx::tc_fence_after();
+            }
 #pragma unroll
-            for (int h = 0; h < C::kHalves; ++h) {
+            for (int r0 = 0; r0 < C::kChunk; r0 += 8) {
+              float f[8];
 #pragma unroll
-              for (int c0 = 0; c0 < C::kN; c0 += 8) {
-                uint32_t o[8];
-                const uint32_t at = lane_t + C::kOCol + (group * C::kHalves + h) * C::kN + c0;
-                ptx::tmem_ld_x8(at, o);
-                ptx::tmem_ld_wait();
+              for (int n = 0; n < 8; ++n) {
+                const int r = r0 + n;
+                const float m = fmaxf(fmaxf(my_max[r], my_max[RP + r]),
+                                      fmaxf(my_max[2 * RP + r], my_max[3 * RP + r]));
+                const float old = ref[c0 + r];
+                const bool up = m > old + kMostLog2;
+                f[n] = up ? exp2f(old - m) : 1.0f;
+                sum[c0 + r] *= f[n];
+                ref[c0 + r] = up ? m : old;
+              }
+              if (shrink) {
 #pragma unroll
-                for (int n = 0; n < 8; ++n) {
-                  const int r = (c0 + n) % RP;
-                  const float f = next[r] == top[r] ? 1.0f : exp2f(top[r] - next[r]);
-                  o[n] = __float_as_uint(__uint_as_float(o[n]) * f);
+                for (int h = 0; h < C::kHalves; ++h) {
+#pragma unroll
+                  for (int k = 0; k < TERMS; ++k) {
+                    uint32_t o[8];
+                    const uint32_t at = lane_t + C::kOCol + (group * C::kHalves + h) * C::kN + k * RP + c0 + r0;
+                    ptx::tmem_ld_x8(at, o);
+                    ptx::tmem_ld_wait();
+#pragma unroll
+                    for (int n = 0; n < 8; ++n)
+                      o[n] = __float_as_uint(__uint_as_float(o[n]) * f[n]);
+                    ptx::tmem_st_x8(at, o);
+                  }
                 }
-                ptx::tmem_st_x8(at, o);
               }
             }
-            ptx::tmem_st_wait();
+            if (shrink) ptx::tmem_st_wait();
           }
+          // PV of this group's last tile has read the weights that this tile's replace.
+          if (c0 == 0 && done > 0)
+            failed |= !bounded_wait(pvdone, (done - 1) & 1u, abort_flag, a.status, 410);
 #pragma unroll
-          for (int r = 0; r < RP; ++r) {
-            if (next[r] != top[r]) sum[r] *= exp2f(top[r] - next[r]);
-            top[r] = next[r];
-          }
-        }
-#pragma unroll
-        for (int r = 0; r < RP; r += 2) {
-          float p[2];
-#pragma unroll
-          for (int n = 0; n < 2; ++n) {
-            p[n] = exp2f(s[r + n] - (top[r + n] == -INFINITY ? 0.0f : top[r + n]));
-            sum[r + n] += p[n];
-          }
-          uint32_t codes[TERMS];
-          e4m3_terms<TERMS>(p[0] * kWeightScale, p[1] * kWeightScale, codes);
-#pragma unroll
-          for (int k = 0; k < TERMS; ++k) {
+          for (int r = 0; r < C::kChunk; r += 2) {
+            float p[2], power[2];
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
-              const int col = k * RP + r + n;
-              p_s[col * 128 + (((token >> 4) ^ (col & 7)) << 4)] = (uint8_t)(codes[k] >> (8 * n));
+              const float m = top[r + n];
+              p[n] = exp2f(s[r + n] - (m == -INFINITY ? 0.0f : m));
+              int up = (int)(m - ref[c0 + r + n]);  // -inf - -inf: 0
+              up = m == -INFINITY ? 0 : max(up, -126);
+              power[n] = pow2_int(up);
+              if (lane % RP == c0 + r + n) my_code = (uint32_t)(127 + up);
+            }
+            uint32_t codes[TERMS];
+            const float2 held2 = __half22float2(e4m3_terms_half<TERMS>(
+                __floats2half2_rn(p[0] * kWeightScale, p[1] * kWeightScale), codes));
+            // The sum takes the weights as they were rounded, so that they add up to one.
+            sum[c0 + r] += held2.x * power[0];
+            sum[c0 + r + 1] += held2.y * power[1];
+#pragma unroll
+            for (int k = 0; k < TERMS; ++k) {
+#pragma unroll
+              for (int n = 0; n < 2; ++n) {
+                const int col = k * RP + c0 + r + n;
+                p_s[col * 128 + ((token & 0x70) ^ ((col & 7) << 4))] = (uint8_t)(codes[k] >> (8 * n));
+              }
             }
           }
+        }
+        if (ended) break;
+        // Scale atom of the weights: column col is row col % 32 of the atom, word col / 32, and
+        // this warp's tokens are byte `quarter` of the word.
+#pragma unroll
+        for (int col0 = 0; col0 < C::kN; col0 += 32) {
+          const int col = col0 + lane;
+          uint32_t code = my_code;
+          if constexpr (RP == 24) code = __shfl_sync(0xffffffffu, my_code, col % RP);
+          if (col < C::kN) p_sf[group * 512 + lane * 16 + (col0 / 32) * 4 + quarter] = (uint8_t)code;
         }
         ptx::fence_proxy_async();
         ptx::tc_fence_before();
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(pfull);
       }
+      if (lane == 0) ptx::mbar_arrive(qempty0 + 8 * (segment & 1));
       // ---- the segment's rows: sums over the tokens, then the output of this CTA's tiles ----
 #pragma unroll
       for (int r = 0; r < RP; ++r) {
@@ -673,7 +715,7 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
         if (lane == (r & 31)) {
           red_sum[(group * 4 + quarter) * RP + r] = v;
-          if (quarter == 0) red_top[group * RP + r] = top[r];
+          if (quarter == 0) red_top[group * RP + r] = ref[r];
         }
       }
       if (j0 < tiles && !failed)
@@ -711,7 +753,7 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
             const float ta = red_top[owner * RP + r0 + n], tb = red_top[(owner ^ 1) * RP + r0 + n];
             const float most = fmaxf(ta, tb);
             // Maxima are -inf where a row saw nothing, NaN scores leave them there too.
-            v[n] += x * (ta == most ? 1.0f : exp2f(ta - most)) * (1.0f / kWeightScale);
+            v[n] += x * (ta == most ? 1.0f : exp2f(ta - most));
           }
         }
         const int d = h * 128 + token;
@@ -781,6 +823,7 @@ kv_decode_join_kernel(const AttentionArgs a, int grid) {
   using C = DecodeCfg<D, RP, TERMS>;
   using T = typename std::conditional<TERMS == 2, __nv_bfloat16, __half>::type;
   __shared__ int64_t sums[2 * 32];
+  __shared__ float tops[kSms], lsum[kSms];
   const int b = blockIdx.x / a.cache.kv_heads, head = blockIdx.x % a.cache.kv_heads;
   const int r = blockIdx.y;
   ptx::grid_dependency_wait();
@@ -814,22 +857,32 @@ kv_decode_join_kernel(const AttentionArgs a, int grid) {
   const int c0 = (int)(((t0 + 1) * s.ctas - 1) / s.total);
   const int c1 = (int)(((t1 + 1) * s.ctas - 1) / s.total);
   if (c0 == c1) return;  // one CTA had all of it and wrote the row
-  float top = -INFINITY;
-  auto part_of = [&](int cta) {
-    // The first CTA's share may begin here exactly, or earlier with other work.
-    const bool begins_inside = share_begin(s, cta) > t0;
-    return a.partials + (int64_t)(2 * cta + (begins_inside ? 0 : 1)) * C::kPartialFloats;
+  // The first CTA began before this (sequence, head) or with it, the others inside it.
+  const int parts = c1 - c0 + 1;
+  const int64_t first = 2 * c0 + 1, later = 2 * c0;  // slot of part p: p == 0 ? first : later + 2 p
+  auto part_of = [&](int p) {
+    return a.partials + (p == 0 ? first : later + 2 * p) * C::kPartialFloats;
   };
-  for (int cta = c0; cta <= c1; ++cta) top = fmaxf(top, part_of(cta)[RP * D + 2 * r]);
-  const float base = top == -INFINITY ? 0.0f : top;
-  float l = 0.0f, o = 0.0f;
-#pragma unroll 4
-  for (int cta = c0; cta <= c1; ++cta) {
-    const float* part = part_of(cta);
-    const float f = exp2f(part[RP * D + 2 * r] - base);
-    l += f * part[RP * D + 2 * r + 1];
-    o += f * part[r * D + threadIdx.x];
+  for (int p = threadIdx.x; p < parts; p += D) {
+    const float2 v = *reinterpret_cast<const float2*>(part_of(p) + RP * D + 2 * r);
+    tops[p] = v.x;
+    lsum[p] = v.y;
   }
+  __syncthreads();
+  const int lane = threadIdx.x & 31;
+  float top = -INFINITY;
+  for (int p = lane; p < parts; p += 32) top = fmaxf(top, tops[p]);
+  top = ptx::warp_max(top);
+  const float base = top == -INFINITY ? 0.0f : top;
+  float l = 0.0f;  // every warp the same sum in the same order
+  for (int p = lane; p < parts; p += 32) l += exp2f(tops[p] - base) * lsum[p];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+  float o = 0.0f;
+  const float* column = a.partials + r * D + threadIdx.x;
+#pragma unroll 8
+  for (int p = 0; p < parts; ++p)
+    o += exp2f(tops[p] - base) * column[(p == 0 ? first : later + 2 * p) * C::kPartialFloats];
   o = l == 0.0f ? 0.0f : o / l;
   int64_t at;
   output_row<RP>(a, seq, head, r, &at);
@@ -837,8 +890,6 @@ kv_decode_join_kernel(const AttentionArgs a, int grid) {
   if constexpr (TERMS == 2) *out = __float2bfloat16_rn(o);
   else *out = __float2half_rn(o);
 }
-
-constexpr int kSms = 148;
 
 bool use_pdl() {
   static const bool enabled = []() {
