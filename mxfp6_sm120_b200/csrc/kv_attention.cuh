@@ -36,6 +36,7 @@ struct AttentionArgs {
   int causal;
   int max_rows;     // rows (tokens x group) a sequence may have to be this kernel's
   int vector;       // q rows can be read sixteen bytes at a time
+  int whole_items;  // a (sequence, head) is not cut between CTAs
 };
 
 int make_kv_map(CUtensorMap* map, const uint8_t* values, const KvCache& cache);
@@ -80,8 +81,10 @@ __device__ __forceinline__ __half2 e4m3_terms_half(__half2 x, uint32_t (&codes)[
   return whole;
 }
 
-__device__ __forceinline__ float pow2_int(int e) {  // 2^e, -126 <= e <= 127
-  return __uint_as_float((uint32_t)(e + 127) << 23);
+// 2^v of a whole v up to 127 (below -126: 2^-126): adding 1.5 * 2^23 leaves v in the low bits.
+__device__ __forceinline__ float pow2_whole(float v) {
+  const uint32_t bits = __float_as_uint(fmaxf(v, -126.0f) + 12582912.0f);
+  return __uint_as_float((bits + 127u) << 23);
 }
 
 // A sequence as this kernel sees it: `tiles` is 0 when it has no rows or is another kernel's.

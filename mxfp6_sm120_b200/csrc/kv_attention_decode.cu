@@ -45,7 +45,9 @@ constexpr int kTmaWarp = 8, kMmaWarp = 9, kQueryWarp = 10, kQueryWarps = 2;
 constexpr float kWeightScale = 256.0f;  // weights 0..1 become 0..256 before they become E4M3 terms
 constexpr float kMostLog2 = 16.0f;      // a tile may exceed the reference by 2^16
 constexpr int kSms = 148;
-constexpr int kMinTiles = 2;           // tiles a CTA takes at least, see the plan
+constexpr int kSegmentUnits = 1;  // what an item costs beside its tiles
+constexpr int kWholeTiles = 4;    // items of at most this many tiles are not cut (and not joined)
+constexpr int kMinUnits = 3;      // units that a CTA takes at least
 
 template <int D, int RP, int TERMS>
 struct DecodeCfg {
@@ -56,7 +58,7 @@ struct DecodeCfg {
   static constexpr int kSlotBytes = kKvTile * D;     // a K or V tile
   static constexpr int kQBytes = (kN * D + 1023) / 1024 * 1024;
   static constexpr int kPBytes = kN * kKvTile;
-  static constexpr int kFixedBytes = 5120;
+  static constexpr int kFixedBytes = 6144;
   static constexpr int kBudget = 227 * 1024 - 1024;
   static constexpr int kFit =
       (kBudget - kFixedBytes - 2 * kQBytes - 2 * kPBytes) / (kSlotBytes + 512);
@@ -82,9 +84,12 @@ struct DecodeCfg {
 // three terms each leave tensor memory for 24 rows, the others take 32.
 constexpr int most_rows(int d, int terms) { return d == 256 && terms == 3 ? 24 : 32; }
 
-// Share of the work list of one CTA, the same arithmetic in both kernels.
+// The work list and its cut, the same arithmetic in both kernels.  An item is a (sequence, key
+// head); it counts its tiles and kSegmentUnits more for the rows' start and end (a CTA that takes
+// seven short items was 60 % later than one that takes 27 tiles of one).  A CTA gets the tiles
+// whose units lie in its share.
 struct Share {
-  int64_t total;  // tiles in all
+  int64_t total;  // units in all
   int ctas;
 };
 __host__ __device__ __forceinline__ int64_t share_begin(const Share& s, int cta) {
@@ -94,15 +99,16 @@ __device__ __forceinline__ Share share_of(int64_t total, int grid) {
   Share s;
   s.total = total;
   // Fewer, larger shares while the list is short: joining costs more than a second tile.
-  const int64_t want = (total + kMinTiles - 1) / kMinTiles;
+  const int64_t want = (total + kMinUnits - 1) / kMinUnits;
   s.ctas = (int)(want < grid ? (want < 1 ? 1 : want) : grid);
   return s;
 }
+__device__ __forceinline__ int units_of(int tiles) { return tiles == 0 ? 0 : tiles + kSegmentUnits; }
 
-// Sum of tiles over all sequences (one key head), by a full warp.
-__device__ __forceinline__ int64_t warp_total_tiles(const AttentionArgs& a, int lane) {
+// Units of all sequences (one key head), by a full warp.
+__device__ __forceinline__ int64_t warp_total_units(const AttentionArgs& a, int lane) {
   int64_t mine = 0;
-  for (int b = lane; b < a.batch.batch; b += 32) mine += kv_sequence(a, b).tiles;
+  for (int b = lane; b < a.batch.batch; b += 32) mine += units_of(kv_sequence(a, b).tiles);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
   return mine;
@@ -130,45 +136,67 @@ struct Cursor {
   }
 };
 
-// The cursor at flattened tile `at` (< total), by a full warp; all lanes get it.
-__device__ __forceinline__ Cursor warp_locate(const AttentionArgs& a, int64_t at, int lane) {
-  Cursor c;
-  c.b = a.batch.batch - 1;
-  c.head = 0;
-  c.tile = 0;
-  int64_t before = 0;  // tiles of all heads of the sequences before this group of 32
+// The first tile at or behind unit `at`, by a full warp: returns its number in the list of all
+// tiles and, in all lanes, the place.  `whole`: items are not cut, the place is the first item that
+// begins at or behind `at`.
+__device__ __forceinline__ int64_t warp_locate(const AttentionArgs& a, int64_t at, bool whole,
+                                               int lane, Cursor* place) {
+  const int heads = a.cache.kv_heads;
+  int64_t units = 0, tiles = 0;  // of all heads of the sequences before this group of 32
+  place->b = a.batch.batch - 1;
+  place->head = place->tile = 0;
   for (int b0 = 0; b0 < a.batch.batch; b0 += 32) {
     const int b = b0 + lane;
-    const int tiles = b < a.batch.batch ? kv_sequence(a, b).tiles : 0;
-    int64_t upto = (int64_t)tiles * a.cache.kv_heads;
+    const int mine = b < a.batch.batch ? kv_sequence(a, b).tiles : 0;
+    int64_t upto = (int64_t)units_of(mine) * heads, tiles_upto = (int64_t)mine * heads;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t other = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += other;
+      const int64_t u = __shfl_up_sync(0xffffffffu, upto, o);
+      const int64_t t = __shfl_up_sync(0xffffffffu, tiles_upto, o);
+      if (lane >= o) {
+        upto += u;
+        tiles_upto += t;
+      }
     }
-    const unsigned reached = __ballot_sync(0xffffffffu, before + upto > at);
+    // The sequence whose last item's last tile is not before `at`.
+    const int64_t reach = units + upto - (whole ? units_of(mine) - 1 : 0);
+    const unsigned reached = __ballot_sync(0xffffffffu, mine > 0 && reach > at);
     if (reached != 0) {
       const int l = __ffs(reached) - 1;
-      const int64_t first = before + __shfl_sync(0xffffffffu, upto, l) -
-                            (int64_t)__shfl_sync(0xffffffffu, tiles, l) * a.cache.kv_heads;
-      const int count = __shfl_sync(0xffffffffu, tiles, l);
-      c.b = b0 + l;
-      c.head = (int)((at - first) / count);
-      c.tile = (int)((at - first) % count);
-      break;
+      const int count = __shfl_sync(0xffffffffu, mine, l);
+      const int64_t per_item = units_of(count);
+      const int64_t first = units + __shfl_sync(0xffffffffu, upto, l) - per_item * heads;
+      const int64_t into = at > first ? at - first : 0;
+      place->b = b0 + l;
+      if (whole) {
+        place->head = (int)((into + per_item - 1) / per_item);
+      } else {
+        place->head = (int)(into / per_item);
+        const int64_t in_item = into % per_item - kSegmentUnits;
+        place->tile = in_item > 0 ? (int)in_item : 0;
+      }
+      return tiles + __shfl_sync(0xffffffffu, tiles_upto, l) - (int64_t)count * heads +
+             (int64_t)place->head * count + place->tile;
     }
-    before += __shfl_sync(0xffffffffu, upto, 31);
+    units += __shfl_sync(0xffffffffu, upto, 31);
+    tiles += __shfl_sync(0xffffffffu, tiles_upto, 31);
   }
-  c.load(a);
-  return c;
+  return tiles;
 }
 
+// A segment: the tiles of one item that a CTA takes, and where its rows go.  Filled by the query
+// warps, one segment ahead.
 template <int RP>
-__device__ __forceinline__ void output_row(const AttentionArgs& a, const KvSequence& seq, int head,
-                                           int r, int64_t* offset) {
-  *offset = (seq.row + r / a.group) * a.out_token_stride +
-            (int64_t)(head * a.group + r % a.group) * a.out_head_stride;
-}
+struct Segment {
+  int64_t out[RP];  // offset of each output row
+  float scale[RP];  // of the quantised query rows, times the softmax scale and log2(e)
+  int64_t first_position;  // of the first row; rows see cached tokens up to their own
+  int length;       // cached tokens
+  int rows;         // query rows: new tokens x group
+  int tile;         // first tile
+  int tiles;
+  int whole;        // all tiles of the item are here
+};
 
 template <int D, int RP, int TERMS>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -187,15 +215,19 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   uint64_t* bars = reinterpret_cast<uint64_t*>(fixed);
   uint8_t* ones = fixed + 512;                                 // scale atom of factors of one
   uint8_t* p_sf = fixed + 1024;                                // scale atom of each group's weights
-  float* row_scale = reinterpret_cast<float*>(fixed + 2048);   // [2][RP]
-  float* red_max = row_scale + 2 * RP;                         // [group][warp][RP]
+  Segment<RP>* segments = reinterpret_cast<Segment<RP>*>(fixed + 2048);  // two
+  float* red_max = reinterpret_cast<float*>(segments + 2);     // [group][warp][RP]
   float* red_sum = red_max + 8 * RP;                           // [group][warp][RP]
   float* red_top = red_sum + 8 * RP;                           // [group][RP]
   Cursor* start = reinterpret_cast<Cursor*>(red_top + 2 * RP);
   int64_t* share_smem = reinterpret_cast<int64_t*>(start + 1);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(share_smem + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  static_assert(2048 + 20 * RP * 4 + sizeof(Cursor) + 64 <= C::kFixedBytes, "fixed area");
+  volatile int* ask_flag = abort_flag + 1;                     // [group][2]
+  volatile uint32_t* slot_named = reinterpret_cast<volatile uint32_t*>(ask_flag + 4);  // [slot]
+  static_assert(2048 + 2 * sizeof(Segment<RP>) + 18 * RP * 4 + sizeof(Cursor) + 16 + 8 + 16 + 64 <=
+                    C::kFixedBytes,
+                "fixed area");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t full0 = ptx::smem_u32(bars);
@@ -205,10 +237,12 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   const uint32_t pvdone0 = pfull0 + 16;
   const uint32_t qfull0 = pvdone0 + 16;
   const uint32_t qempty0 = qfull0 + 16;
-  static_assert(8 * (2 * 16 + 10) <= 512, "barriers");
+  const uint32_t vsync0 = qempty0 + 16;
+  static_assert(8 * (2 * 16 + 12) <= 512, "barriers");
 
   if (threadIdx.x == 0) {
     *abort_flag = 0;
+    for (int i = 0; i < 4; ++i) ask_flag[i] = 0;
     for (int s = 0; s < C::kSlots; ++s) {
       ptx::mbar_init(full0 + 8 * s, 2);  // the copies' bytes, and the scales
       ptx::mbar_init(empty0 + 8 * s, 1);
@@ -219,6 +253,7 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       ptx::mbar_init(pvdone0 + 8 * i, 1);
       ptx::mbar_init(qfull0 + 8 * i, kQueryWarps);
       ptx::mbar_init(qempty0 + 8 * i, 1 + 2 * kGroupWarps);
+      ptx::mbar_init(vsync0 + 8 * i, kGroupWarps);
     }
     ptx::fence_mbar_init();
     ptx::prefetch_tensormap(&tm_k);
@@ -232,23 +267,23 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   }
   ptx::grid_launch_dependents();
   ptx::grid_dependency_wait();
-  if (warp == 0) {
-    const Share s = share_of(warp_total_tiles(a, lane) * a.cache.kv_heads, (int)gridDim.x);
-    const int cta = (int)blockIdx.x;
-    const int64_t t0 = cta < s.ctas ? share_begin(s, cta) : 0;
-    const int64_t t1 = cta < s.ctas ? share_begin(s, cta + 1) : 0;
+  if (warp < 2) {
+    // Warp 0 finds the first tile of this CTA, warp 1 the first of the next.
+    const Share s = share_of(warp_total_units(a, lane) * a.cache.kv_heads, (int)gridDim.x);
+    const int cta = (int)blockIdx.x + warp;
     Cursor c;
-    if (t1 > t0) c = warp_locate(a, t0, lane);
+    int64_t tile = 0;
+    if ((int)blockIdx.x < s.ctas) tile = warp_locate(a, share_begin(s, cta), a.whole_items != 0, lane, &c);
     if (lane == 0) {
-      share_smem[0] = t1 - t0;
-      if (t1 > t0) *start = c;
+      share_smem[warp] = tile;
+      if (warp == 0) *start = c;
     }
   }
   ptx::tc_fence_before();
   __syncthreads();
   ptx::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const int count = (int)share_smem[0];  // tiles of this CTA
+  const int count = (int)(share_smem[1] - share_smem[0]);  // tiles of this CTA
   const int per_page = a.cache.page_size / kKvBlock;
 
   if (count > 0 && warp == kTmaWarp) {
@@ -257,6 +292,7 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
     // l % 4 of tile l / 4 of a group of eight tiles and later issues that block's copies itself;
     // the next group's lookups are in flight while this group is copied.
     Cursor mine = *start;
+    mine.load(a);
     for (int i = 0; i < (lane >> 2); ++i) mine.next(a);
     int64_t page = -1, next_page = -1;  // scale block of this lane's block of tokens, or -1
     uint32_t k_sf = 127, v_sf = 127, next_k = 127, next_v = 127;
@@ -307,6 +343,8 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
           is_v ? make_uint4(all, all, all, all)
                : make_uint4(sf[0] * 0x01010101u, sf[1] * 0x01010101u, sf[2] * 0x01010101u,
                             sf[3] * 0x01010101u);
+      const uint32_t named = __ballot_sync(0xffffffffu, lane_page >= 0) >> src & 15u;
+      if (lane == 0) slot_named[slot] = named;
       ptx::fence_proxy_async();
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(bar);
@@ -344,19 +382,20 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
     const uint32_t ones_t = sf0 + 24;
     if (ptx::elect_one()) ptx::tc_cp_32x128b_warpx4(ones_t, ptx::smem_desc_scale_atom(ptx::smem_u32(ones)));
     __syncwarp();
-    Cursor scored = *start;        // tile of the last scores issued
-    int segment = 0, in_segment = 0;  // its segment, and its number there
-    int summed = 0;                // number of the last V tile within its segment
+    int segment = 0, in_segment = 0, of_segment = 0;  // of the next scores: segment, tile, tiles
+    int summed = 0;                // number of the next V tile within its segment
     bool ok = true;
     // Slot of K(i) is 2i - 1 (0 for the first), of V(i) 2i + 2 (2i + 1 for the last).
     auto scores = [&](int i) {
-      const bool last = i + 1 == count || scored.tile + 1 == scored.seq.tiles;
       const int at = i == 0 ? 0 : 2 * i - 1;
       const int slot = at % C::kSlots;
-      if (in_segment == 0)
+      if (in_segment == 0) {
         ok = ok && __all_sync(0xffffffffu, bounded_wait(qfull0 + 8 * (segment & 1),
                                                         (uint32_t)(segment >> 1) & 1u, abort_flag,
                                                         a.status, 402));
+        of_segment = segments[segment & 1].tiles;
+      }
+      const bool last = in_segment + 1 == of_segment;
       ok = ok && __all_sync(0xffffffffu,
                             bounded_wait(full0 + 8 * slot, (uint32_t)(at / C::kSlots) & 1u,
                                          abort_flag, a.status, 403));
@@ -392,10 +431,7 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       // Number of tile i within its segment: the scores of tile i + 1 tell whether one ended.
       const int number = summed;
       summed = in_segment == 0 ? 0 : summed + 1;
-      if (i + 1 < count) {
-        scored.next(a);
-        scores(i + 1);
-      }
+      if (i + 1 < count) scores(i + 1);
       const int at = i + 1 < count ? 2 * i + 2 : 2 * i + 1;
       const int slot = at % C::kSlots;
       ok = ok && __all_sync(0xffffffffu, bounded_wait(pfull0 + 8 * (i & 1), (uint32_t)(i >> 1) & 1u,
@@ -433,6 +469,7 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   } else if (count > 0 && warp >= kQueryWarp) {
     // ---------------- query terms ----------------
     Cursor c = *start;
+    c.load(a);
     int left = count;
     bool ok = true;
     for (int segment = 0; ok && left > 0; ++segment) {
@@ -440,130 +477,149 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       ok = __all_sync(0xffffffffu, bounded_wait(qempty0 + 8 * buffer, ((uint32_t)(segment >> 1) & 1u) ^ 1u,
                                                 abort_flag, a.status, 406));
       if (!ok) break;
+      Segment<RP>& seg = segments[buffer];
       uint8_t* q_s = q_tiles + buffer * C::kQBytes;
       const int rows = c.seq.rows * a.group;
-      constexpr int kPer = D / 32;  // values per lane
+      const int tiles = min(left, c.seq.tiles - c.tile);
+      if (warp == kQueryWarp) {
+        if (lane < RP) {
+          const int r = lane < rows ? lane : 0;
+          seg.out[lane] = (c.seq.row + r / a.group) * a.out_token_stride +
+                          (int64_t)(c.head * a.group + r % a.group) * a.out_head_stride;
+        }
+        if (lane == 0) {
+          seg.first_position = c.seq.last - c.seq.rows + 1;
+          seg.length = c.seq.length;
+          seg.rows = rows;
+          seg.tile = c.tile;
+          seg.tiles = tiles;
+          seg.whole = c.tile == 0 && tiles == c.seq.tiles;
+        }
+      }
+      constexpr int kPer = D / 32;   // values per lane
+      constexpr int kBatch = RP / kQueryWarps < 4 ? RP / kQueryWarps : 4;  // rows in flight
 #pragma unroll 1
-      for (int r = warp - kQueryWarp; r < RP; r += kQueryWarps) {
-        float v[kPer];
-        uint32_t top = 0;
-        constexpr uint32_t kInf = TERMS == 2 ? 0x7f80u : 0x7c00u;
-        const T* src = static_cast<const T*>(a.q) + (c.seq.row + r / a.group) * a.q_token_stride +
-                       (int64_t)(c.head * a.group + r % a.group) * a.q_head_stride + lane * kPer;
-        __align__(16) uint16_t raw[kPer];
-        if (r < rows) {
-          if (a.vector && kPer == 8) {
-            *reinterpret_cast<uint4*>(raw) = *reinterpret_cast<const uint4*>(src);
-          } else if (a.vector && kPer == 4) {
-            *reinterpret_cast<uint2*>(raw) = *reinterpret_cast<const uint2*>(src);
+      for (int r0 = warp - kQueryWarp; r0 < RP; r0 += kQueryWarps * kBatch) {
+        __align__(16) uint16_t raw[kBatch][kPer];
+#pragma unroll
+        for (int n = 0; n < kBatch; ++n) {
+          const int r = r0 + n * kQueryWarps;
+          const T* src = static_cast<const T*>(a.q) + (c.seq.row + r / a.group) * a.q_token_stride +
+                         (int64_t)(c.head * a.group + r % a.group) * a.q_head_stride + lane * kPer;
+          if (r < rows) {
+            if (a.vector && kPer == 8) {
+              *reinterpret_cast<uint4*>(raw[n]) = *reinterpret_cast<const uint4*>(src);
+            } else if (a.vector && kPer == 4) {
+              *reinterpret_cast<uint2*>(raw[n]) = *reinterpret_cast<const uint2*>(src);
+            } else {
+#pragma unroll
+              for (int i = 0; i < kPer; ++i) raw[n][i] = reinterpret_cast<const uint16_t*>(src)[i];
+            }
           } else {
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) raw[i] = reinterpret_cast<const uint16_t*>(src)[i];
+            for (int i = 0; i < kPer; ++i) raw[n][i] = 0;
           }
-        } else {
-#pragma unroll
-          for (int i = 0; i < kPer; ++i) raw[i] = 0;
         }
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-          top = max(top, (uint32_t)(raw[i] & 0x7fffu));
-          if constexpr (TERMS == 2) v[i] = __uint_as_float((uint32_t)raw[i] << 16);
-          else v[i] = __half2float(__ushort_as_half(raw[i]));
-        }
-        top = __reduce_max_sync(0xffffffffu, top);
-        const float most = TERMS == 2 ? __uint_as_float(top << 16)
-                                      : __half2float(__ushort_as_half((unsigned short)top));
-        // A row with an infinity or NaN has no scale: its scores become NaN.
-        const uint32_t bits = ue8m0_scale_bits_shift<8>(top < kInf ? most : 1.0f);
-        const float inverse = ue8m0_inverse(bits);
-        if (lane == 0) row_scale[buffer * RP + r] = top < kInf ? __uint_as_float(bits) : NAN;
-        uint32_t codes[TERMS][kPer / 2];
+        for (int n = 0; n < kBatch; ++n) {
+          const int r = r0 + n * kQueryWarps;
+          float v[kPer];
+          uint32_t top = 0;
+          constexpr uint32_t kInf = TERMS == 2 ? 0x7f80u : 0x7c00u;
 #pragma unroll
-        for (int i = 0; i < kPer / 2; ++i) {
-          uint32_t t[TERMS];
-          e4m3_terms<TERMS>(v[2 * i] * inverse, v[2 * i + 1] * inverse, t);
+          for (int i = 0; i < kPer; ++i) {
+            top = max(top, (uint32_t)(raw[n][i] & 0x7fffu));
+            if constexpr (TERMS == 2) v[i] = __uint_as_float((uint32_t)raw[n][i] << 16);
+            else v[i] = __half2float(__ushort_as_half(raw[n][i]));
+          }
+          top = __reduce_max_sync(0xffffffffu, top);
+          const float most = TERMS == 2 ? __uint_as_float(top << 16)
+                                        : __half2float(__ushort_as_half((unsigned short)top));
+          // A row with an infinity or NaN has no scale: its scores become NaN.
+          const uint32_t bits = ue8m0_scale_bits_shift<8>(top < kInf ? most : 1.0f);
+          const float inverse = ue8m0_inverse(bits);
+          if (lane == 0) seg.scale[r] = top < kInf ? __uint_as_float(bits) * a.scale_log2 : NAN;
+          uint32_t codes[TERMS][kPer / 2];
 #pragma unroll
-          for (int k = 0; k < TERMS; ++k) codes[k][i] = t[k];
-        }
-        const int d0 = lane * kPer;
+          for (int i = 0; i < kPer / 2; ++i) {
+            uint32_t t[TERMS];
+            e4m3_terms<TERMS>(v[2 * i] * inverse, v[2 * i + 1] * inverse, t);
 #pragma unroll
-        for (int k = 0; k < TERMS; ++k) {
-          const int col = k * RP + r;
-          const int in_row = d0 % C::kRowBytes;
-          const int swizzle = C::kRowBytes == 128 ? (col & 7) : ((col >> 1) & 3);
-          uint8_t* dst = q_s + (d0 / C::kRowBytes) * C::kN * C::kRowBytes + col * C::kRowBytes +
-                         (((in_row >> 4) ^ swizzle) << 4) + (in_row & 15);
-          if constexpr (kPer == 8) {
-            *reinterpret_cast<uint2*>(dst) = make_uint2(codes[k][0] | codes[k][1] << 16,
-                                                        codes[k][2] | codes[k][3] << 16);
-          } else if constexpr (kPer == 4) {
-            *reinterpret_cast<uint32_t*>(dst) = codes[k][0] | codes[k][1] << 16;
-          } else {
-            *reinterpret_cast<uint16_t*>(dst) = (uint16_t)codes[k][0];
+            for (int k = 0; k < TERMS; ++k) codes[k][i] = t[k];
+          }
+          const int d0 = lane * kPer;
+#pragma unroll
+          for (int k = 0; k < TERMS; ++k) {
+            const int col = k * RP + r;
+            const int in_row = d0 % C::kRowBytes;
+            const int swizzle = C::kRowBytes == 128 ? (col & 7) : ((col >> 1) & 3);
+            uint8_t* dst = q_s + (d0 / C::kRowBytes) * C::kN * C::kRowBytes + col * C::kRowBytes +
+                           (((in_row >> 4) ^ swizzle) << 4) + (in_row & 15);
+            if constexpr (kPer == 8) {
+              *reinterpret_cast<uint2*>(dst) = make_uint2(codes[k][0] | codes[k][1] << 16,
+                                                          codes[k][2] | codes[k][3] << 16);
+            } else if constexpr (kPer == 4) {
+              *reinterpret_cast<uint32_t*>(dst) = codes[k][0] | codes[k][1] << 16;
+            } else {
+              *reinterpret_cast<uint16_t*>(dst) = (uint16_t)codes[k][0];
+            }
           }
         }
       }
       ptx::fence_proxy_async();
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(qfull0 + 8 * buffer);
-      // On to the first tile of the next (sequence, head) of this share.
-      const int rest = min(left, c.seq.tiles - c.tile);
-      left -= rest;
+      // On to the first tile of the next item of this share.
+      left -= tiles;
       c.tile = c.seq.tiles - 1;
       if (left > 0) c.next(a);
     }
   } else if (count > 0 && warp < 2 * kGroupWarps) {
     // ---------------- softmax: lane = token of the tile ----------------
-    // Two groups of four warps take alternate tiles, each with its own maximum, sum and output
-    // accumulator; they meet at the end of a segment (the tiles of one (sequence, head)).
-    // A wait that runs out makes `failed` true; the votes below end both groups together.
+    // Two groups of four warps take alternate tiles, each with its own reference, sum and output
+    // accumulator; they meet at the end of a segment.  A wait that runs out ends the warp's tiles,
+    // and the vote at the end of the segment ends both groups together.
     const int group = warp / kGroupWarps, quarter = warp % kGroupWarps;
     const int token = quarter * 32 + lane;  // within the tile; quarter = its scale block
     const uint32_t lane_t = tmem + ((uint32_t)(quarter * 32) << 16);
     const uint32_t s_t = lane_t + group * C::kN;
     const uint32_t sfull = sfull0 + 8 * group, pfull = pfull0 + 8 * group;
-    const uint32_t pvdone = pvdone0 + 8 * group;
+    const uint32_t pvdone = pvdone0 + 8 * group, vsync = vsync0 + 8 * group;
     uint8_t* p_s = p_tiles + group * C::kPBytes + (token & 15);
     float* my_max = red_max + group * 4 * RP;
-    Cursor c = *start;
     bool failed = false;
-    int i0 = 0;            // first tile of the segment in the CTA's list
     uint32_t done = 0;     // tiles this group has taken
-    for (int segment = 0; i0 < count; ++segment) {
-      const int tiles = min(count - i0, c.seq.tiles - c.tile);
-      const int32_t* table = a.batch.block_table + (int64_t)c.b * a.batch.table_stride;
-      // Entry of the block table for this warp's block of a tile, -1 where there is no token.
-      auto entry = [&](int j) -> int32_t {
-        const int block = (c.tile + j) * kKvTileBlocks + quarter;
-        return j < tiles && block * kKvBlock < c.seq.length ? table[block / per_page] : -1;
-      };
-      const int j0 = (group ^ i0) & 1;
-      int32_t page = entry(j0), page_next = entry(j0 + 2);
-      failed |= !bounded_wait(qfull0 + 8 * (segment & 1), (uint32_t)(segment >> 1) & 1u, abort_flag,
-                              a.status, 407);
-      const float* scales = row_scale + (segment & 1) * RP;
+    uint32_t syncs = 0;    // times the four warps of the group have met
+    uint32_t votes = 0;    // of them, to ask for another reference
+    auto wait = [&](uint32_t bar, uint32_t parity, int code) {
+      if (!failed) failed = !__all_sync(0xffffffffu, bounded_wait(bar, parity, abort_flag, a.status, code));
+    };
+    for (int segment = 0, i0 = 0; i0 < count; ++segment) {
+      wait(qfull0 + 8 * (segment & 1), (uint32_t)(segment >> 1) & 1u, 407);
+      const Segment<RP>& seg = segments[segment & 1];
+      const int tiles = failed ? 0 : seg.tiles, length = seg.length;
+      const int64_t first_position = seg.first_position;
       float ref[RP], sum[RP];  // ref: the same in all lanes of the group
 #pragma unroll
       for (int r = 0; r < RP; ++r) {
         ref[r] = -INFINITY;
         sum[r] = 0.0f;
       }
+      const int j0 = (group ^ i0) & 1;
 #pragma unroll 1
       for (int j = j0; j < tiles; j += 2, ++done) {
         const int i = i0 + j;
-        const bool named = page >= 0 && page < a.cache.pages;
-        page = page_next;
-        page_next = entry(j + 4);
-        // Tokens of this tile that exist.
-        const int t0 = (c.tile + j) * kKvTile;
-        const int held = min(kKvTile, c.seq.length - t0);
-        if (!(named && (quarter + 1) * 32 <= held)) {
-          // Rows of V without a token may hold anything, NaN among them, and 0 * NaN is NaN: clear
-          // them once the tile has landed.
-          const int at = i + 1 < count ? 2 * i + 2 : 2 * i + 1;
-          const int slot = at % C::kSlots;
-          failed |= !bounded_wait(full0 + 8 * slot, (uint32_t)(at / C::kSlots) & 1u, abort_flag,
-                                  a.status, 408);
+        const int t0 = (seg.tile + j) * kKvTile;
+        const int held = min(kKvTile, length - t0);  // tokens of this tile that exist
+        wait(sfull, done & 1u, 409);
+        const int at = i + 1 < count ? 2 * i + 2 : 2 * i + 1;
+        const int slot = at % C::kSlots;
+        wait(full0 + 8 * slot, (uint32_t)(at / C::kSlots) & 1u, 408);
+        if (failed) break;
+        ptx::tc_fence_after();
+        const bool named = (slot_named[slot] >> quarter & 1u) != 0;
+        if (!named || (quarter + 1) * 32 > held) {
+          // Rows of V without a token may hold anything, NaN among them, and 0 * NaN is NaN.
           uint8_t* v_s = slots + slot * C::kSlotBytes;
           const int from = named ? max(0, held - quarter * 32) : 0;
           for (int at16 = from * (D / 16) + lane; at16 < 32 * (D / 16); at16 += 32) {
@@ -572,20 +628,14 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
             *reinterpret_cast<uint4*>(v_s + sub * C::kSubBytes + (quarter * 32 + t) * C::kRowBytes +
                                       in_row * 16) = make_uint4(0, 0, 0, 0);
           }
-          ptx::fence_proxy_async();
         }
         const bool here = named && token < held;
-        const bool bounded = a.causal && t0 + held - 1 > c.seq.last - c.seq.rows + 1;
-        failed |= !bounded_wait(sfull, done & 1u, abort_flag, a.status, 409);
-        __syncwarp();
-        ptx::tc_fence_after();
+        const bool bounded = a.causal && t0 + held - 1 > first_position;
         uint32_t my_code = 127;  // weight scale of row lane % RP in this warp's 32 tokens
-        bool ended = false;
 #pragma unroll
         for (int c0 = 0; c0 < RP; c0 += C::kChunk) {
-          if (ended) continue;
           float s[C::kChunk], top[C::kChunk];
-          bool raise = failed;
+          bool ask = false;
 #pragma unroll
           for (int r0 = 0; r0 < C::kChunk; r0 += 8) {
             uint32_t raw[TERMS][8];
@@ -597,36 +647,64 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
               float v = __uint_as_float(raw[TERMS - 1][n]);
 #pragma unroll
               for (int k = TERMS - 2; k >= 0; --k) v = v * 0.0625f + __uint_as_float(raw[k][n]);
-              s[r0 + n] = here ? v * (scales[c0 + r0 + n] * a.scale_log2) : -INFINITY;
+              s[r0 + n] = here ? v * seg.scale[c0 + r0 + n] : -INFINITY;
             }
           }
           if (bounded) {
 #pragma unroll
             for (int r = 0; r < C::kChunk; ++r)
-              if (t0 + token > c.seq.last - c.seq.rows + 1 + (c0 + r) / a.group) s[r] = -INFINITY;
+              if (t0 + token > first_position + (c0 + r) / a.group) s[r] = -INFINITY;
           }
 #pragma unroll
           for (int r = 0; r < C::kChunk; ++r) {
             top[r] = ceilf(ptx::warp_max(s[r]));
-            raise = raise || top[r] > ref[c0 + r] + kMostLog2;
+            ask = ask || top[r] > ref[c0 + r] + kMostLog2;
           }
-          if (ptx::barrier_any(1 + group, kGroupWarps * 32, raise)) {
-            // The first tokens that a row sees, a later maximum far above its reference, or a wait
-            // that ran out: the four warps agree on the reference.
+          // Does any of the four warps ask for another reference?  The answer is only needed
+          // after the weights, which do not depend on it.
+          volatile int* asked = ask_flag + group * 2 + (votes++ & 1u);
+          if (lane == 0) {
+            if (ask) *asked = 1;
+            ptx::mbar_arrive(vsync);
+          }
+          // PV of this group's last tile has read the weights that this tile's replace.
+          if (c0 == 0 && done > 0) wait(pvdone, (done - 1) & 1u, 410);
+          float kept[C::kChunk];
+#pragma unroll
+          for (int r = 0; r < C::kChunk; r += 2) {
+            float p[2];
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+              p[n] = ptx::exp2_approx(s[r + n] - (top[r + n] == -INFINITY ? 0.0f : top[r + n]));
+            uint32_t codes[TERMS];
+            const float2 held2 = __half22float2(e4m3_terms_half<TERMS>(
+                __floats2half2_rn(p[0] * kWeightScale, p[1] * kWeightScale), codes));
+            kept[r] = held2.x;
+            kept[r + 1] = held2.y;
+#pragma unroll
+            for (int k = 0; k < TERMS; ++k) {
+#pragma unroll
+              for (int n = 0; n < 2; ++n) {
+                const int col = k * RP + c0 + r + n;
+                p_s[col * 128 + ((token & 0x70) ^ ((col & 7) << 4))] = (uint8_t)(codes[k] >> (8 * n));
+              }
+            }
+          }
+          wait(vsync, syncs & 1u, 413);
+          ++syncs;
+          if (!failed && *asked != 0) {
+            // The first tokens that a row sees, or a maximum far above its reference: the four
+            // warps agree on a new one.
 #pragma unroll
             for (int r = 0; r < C::kChunk; ++r)
               if (lane == (r & 31)) my_max[quarter * RP + r] = top[r];
-            failed = ptx::barrier_any(1 + group, kGroupWarps * 32, failed);
-            if (failed) {
-              ended = true;
-              continue;
-            }
-            const bool shrink = j != j0;
-            if (shrink) {
-              failed |= !bounded_wait(pvdone, (done - 1) & 1u, abort_flag, a.status, 412);
-              __syncwarp();
-              ptx::tc_fence_after();
-            }
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(vsync);
+            wait(vsync, syncs & 1u, 414);
+            ++syncs;
+            if (quarter == 0 && lane == 0) *asked = 0;  // not used by the next vote, but the one after
+            const bool shrink = j != j0 && !failed;
+            if (shrink) ptx::tc_fence_after();
 #pragma unroll
             for (int r0 = 0; r0 < C::kChunk; r0 += 8) {
               float f[8];
@@ -637,7 +715,7 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
                                       fmaxf(my_max[2 * RP + r], my_max[3 * RP + r]));
                 const float old = ref[c0 + r];
                 const bool up = m > old + kMostLog2;
-                f[n] = up ? exp2f(old - m) : 1.0f;
+                f[n] = up ? pow2_whole(old - m) : 1.0f;
                 sum[c0 + r] *= f[n];
                 ref[c0 + r] = up ? m : old;
               }
@@ -647,51 +725,30 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
 #pragma unroll
                   for (int k = 0; k < TERMS; ++k) {
                     uint32_t o[8];
-                    const uint32_t at = lane_t + C::kOCol + (group * C::kHalves + h) * C::kN + k * RP + c0 + r0;
-                    ptx::tmem_ld_x8(at, o);
+                    const uint32_t at_o = lane_t + C::kOCol + (group * C::kHalves + h) * C::kN + k * RP + c0 + r0;
+                    ptx::tmem_ld_x8(at_o, o);
                     ptx::tmem_ld_wait();
 #pragma unroll
                     for (int n = 0; n < 8; ++n)
                       o[n] = __float_as_uint(__uint_as_float(o[n]) * f[n]);
-                    ptx::tmem_st_x8(at, o);
+                    ptx::tmem_st_x8(at_o, o);
                   }
                 }
               }
             }
             if (shrink) ptx::tmem_st_wait();
           }
-          // PV of this group's last tile has read the weights that this tile's replace.
-          if (c0 == 0 && done > 0)
-            failed |= !bounded_wait(pvdone, (done - 1) & 1u, abort_flag, a.status, 410);
 #pragma unroll
-          for (int r = 0; r < C::kChunk; r += 2) {
-            float p[2], power[2];
-#pragma unroll
-            for (int n = 0; n < 2; ++n) {
-              const float m = top[r + n];
-              p[n] = exp2f(s[r + n] - (m == -INFINITY ? 0.0f : m));
-              int up = (int)(m - ref[c0 + r + n]);  // -inf - -inf: 0
-              up = m == -INFINITY ? 0 : max(up, -126);
-              power[n] = pow2_int(up);
-              if (lane % RP == c0 + r + n) my_code = (uint32_t)(127 + up);
-            }
-            uint32_t codes[TERMS];
-            const float2 held2 = __half22float2(e4m3_terms_half<TERMS>(
-                __floats2half2_rn(p[0] * kWeightScale, p[1] * kWeightScale), codes));
-            // The sum takes the weights as they were rounded, so that they add up to one.
-            sum[c0 + r] += held2.x * power[0];
-            sum[c0 + r + 1] += held2.y * power[1];
-#pragma unroll
-            for (int k = 0; k < TERMS; ++k) {
-#pragma unroll
-              for (int n = 0; n < 2; ++n) {
-                const int col = k * RP + c0 + r + n;
-                p_s[col * 128 + ((token & 0x70) ^ ((col & 7) << 4))] = (uint8_t)(codes[k] >> (8 * n));
-              }
-            }
+          for (int r = 0; r < C::kChunk; ++r) {
+            // 2^(top - ref), a power of two between 2^-126 and 2^16; its exponent field is the
+            // UE8M0 code.  The sum takes the weights as they were rounded, so that they add up
+            // to one.
+            const float power = pow2_whole(top[r] == -INFINITY ? 0.0f : top[r] - ref[c0 + r]);
+            sum[c0 + r] += kept[r] * power;
+            if (lane % RP == c0 + r) my_code = __float_as_uint(power) >> 23;
           }
         }
-        if (ended) break;
+        if (failed) break;
         // Scale atom of the weights: column col is row col % 32 of the atom, word col / 32, and
         // this warp's tokens are byte `quarter` of the word.
 #pragma unroll
@@ -706,33 +763,68 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(pfull);
       }
-      if (lane == 0) ptx::mbar_arrive(qempty0 + 8 * (segment & 1));
       // ---- the segment's rows: sums over the tokens, then the output of this CTA's tiles ----
+      // Sums over the warp: pairs of rows are folded into one value per lane, so that eight rows
+      // take nine exchanges.
 #pragma unroll
-      for (int r = 0; r < RP; ++r) {
-        float v = sum[r];
+      for (int r0 = 0; r0 < RP; r0 += 8) {
+        float v[8];
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        if (lane == (r & 31)) {
-          red_sum[(group * 4 + quarter) * RP + r] = v;
-          if (quarter == 0) red_top[group * RP + r] = ref[r];
+        for (int n = 0; n < 8; ++n) v[n] = sum[r0 + n];
+#pragma unroll
+        for (int width = 4; width >= 1; width >>= 1) {
+          const bool high = (lane & width) != 0;
+#pragma unroll
+          for (int n = 0; n < width; ++n) {
+            const float mine = high ? v[n + width] : v[n];
+            const float other = __shfl_xor_sync(0xffffffffu, high ? v[n] : v[n + width], width);
+            v[n] = mine + other;
+          }
+        }
+        v[0] += __shfl_xor_sync(0xffffffffu, v[0], 8);
+        v[0] += __shfl_xor_sync(0xffffffffu, v[0], 16);
+        if (lane < 8) red_sum[(group * 4 + quarter) * RP + r0 + lane] = v[0];
+        if (quarter == 0) {
+#pragma unroll
+          for (int n = 0; n < 8; ++n)
+            if (lane == n) red_top[group * RP + r0 + n] = ref[r0 + n];
         }
       }
-      if (j0 < tiles && !failed)
-        failed |= !bounded_wait(pvdone, (done - 1) & 1u, abort_flag, a.status, 411);
+      if (j0 < tiles) wait(pvdone, (done - 1) & 1u, 411);
       failed = ptx::barrier_any(3, 2 * kGroupWarps * 32, failed);
       if (failed) break;
       ptx::tc_fence_after();
-      const int rows = c.seq.rows * a.group;
-      const bool whole = c.tile == 0 && tiles == c.seq.tiles;
-      // A share that begins inside a (sequence, head) uses the CTA's first partial slot for it,
-      // one that ends inside the second.
+      // Lane r: what row r's two accumulators are multiplied by (RP <= 32).
+      float factor_a = 0.0f, factor_b = 0.0f;
+      // A share that begins inside an item uses the CTA's first partial slot for it, one that ends
+      // inside the second.
       float* part = a.partials +
-                    (int64_t)(2 * blockIdx.x + (c.tile != 0 ? 0 : 1)) * C::kPartialFloats;
+                    (int64_t)(2 * blockIdx.x + (seg.tile != 0 ? 0 : 1)) * C::kPartialFloats;
+      if (lane < RP) {
+        const float ta = red_top[lane], tb = red_top[RP + lane], most = fmaxf(ta, tb);
+        // A reference is -inf where the row saw nothing (NaN scores leave it there too).
+        factor_a = ta == most ? 1.0f : pow2_whole(ta - most);
+        factor_b = tb == most ? 1.0f : pow2_whole(tb - most);
+        float l = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+          l += red_sum[w * RP + lane] * factor_a + red_sum[(4 + w) * RP + lane] * factor_b;
+        if (seg.whole) {
+          const float scale = l == 0.0f ? 0.0f : 1.0f / l;
+          factor_a *= scale;
+          factor_b *= scale;
+        } else if (warp == 0) {
+          part[RP * D + 2 * lane] = most;
+          part[RP * D + 2 * lane + 1] = l;
+        }
+      }
+      const int rows = seg.rows;
+      const bool whole = seg.whole != 0;
       // The groups share the output by halves of head_dim, or by eight rows.
 #pragma unroll 1
       for (int unit = group; unit < C::kHalves * (RP / 8); unit += 2) {
         const int h = unit % C::kHalves, r0 = unit / C::kHalves * 8;
+        if (r0 >= rows) continue;
         float v[8];
 #pragma unroll
         for (int n = 0; n < 8; ++n) v[n] = 0.0f;
@@ -750,10 +842,7 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
             float x = __uint_as_float(raw[TERMS - 1][n]);
 #pragma unroll
             for (int k = TERMS - 2; k >= 0; --k) x = x * 0.0625f + __uint_as_float(raw[k][n]);
-            const float ta = red_top[owner * RP + r0 + n], tb = red_top[(owner ^ 1) * RP + r0 + n];
-            const float most = fmaxf(ta, tb);
-            // Maxima are -inf where a row saw nothing, NaN scores leave them there too.
-            v[n] += x * (ta == most ? 1.0f : exp2f(ta - most));
+            v[n] += x * __shfl_sync(0xffffffffu, owner ? factor_b : factor_a, r0 + n);
           }
         }
         const int d = h * 128 + token;
@@ -762,42 +851,20 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
           const int r = r0 + n;
           if (r < rows && d < D) {
             if (whole) {
-              const float ta = red_top[r], tb = red_top[RP + r], most = fmaxf(ta, tb);
-              const float la = red_sum[r] + red_sum[RP + r] + red_sum[2 * RP + r] + red_sum[3 * RP + r];
-              const float lb = red_sum[4 * RP + r] + red_sum[5 * RP + r] + red_sum[6 * RP + r] +
-                               red_sum[7 * RP + r];
-              const float l = la * (ta == most ? 1.0f : exp2f(ta - most)) +
-                              lb * (tb == most ? 1.0f : exp2f(tb - most));
-              int64_t at;
-              output_row<RP>(a, c.seq, c.head, r, &at);
-              const float o = l == 0.0f ? 0.0f : v[n] / l;
-              T* out = static_cast<T*>(a.out) + at + d;
-              if constexpr (TERMS == 2) *out = __float2bfloat16_rn(o);
-              else *out = __float2half_rn(o);
+              T* out = static_cast<T*>(a.out) + seg.out[r] + d;
+              if constexpr (TERMS == 2) *out = __float2bfloat16_rn(v[n]);
+              else *out = __float2half_rn(v[n]);
             } else {
               part[r * D + d] = v[n];
             }
           }
         }
       }
-      if (!whole && threadIdx.x < RP) {
-        const int r = threadIdx.x;
-        const float ta = red_top[r], tb = red_top[RP + r], most = fmaxf(ta, tb);
-        const float la = red_sum[r] + red_sum[RP + r] + red_sum[2 * RP + r] + red_sum[3 * RP + r];
-        const float lb = red_sum[4 * RP + r] + red_sum[5 * RP + r] + red_sum[6 * RP + r] +
-                         red_sum[7 * RP + r];
-        part[RP * D + 2 * r] = most;
-        part[RP * D + 2 * r + 1] = la * (ta == most ? 1.0f : exp2f(ta - most)) +
-                                   lb * (tb == most ? 1.0f : exp2f(tb - most));
-      }
       ptx::tc_fence_before();
       i0 += tiles;
-      if (i0 < count) {
-        // The accumulators and sums of this segment have been read.
-        if (ptx::barrier_any(3, 2 * kGroupWarps * 32, false)) break;
-        c.tile = c.seq.tiles - 1;
-        c.next(a);
-      }
+      // The accumulators, sums and the segment's description have been read.
+      if (i0 < count && ptx::barrier_any(3, 2 * kGroupWarps * 32, false)) break;
+      if (lane == 0) ptx::mbar_arrive(qempty0 + 8 * (segment & 1));
     }
   }
 
@@ -829,11 +896,11 @@ kv_decode_join_kernel(const AttentionArgs a, int grid) {
   ptx::grid_dependency_wait();
   const KvSequence seq = kv_sequence(a, b);
   if (seq.tiles == 0 || r >= seq.rows * a.group) return;
-  int64_t before = 0, total = 0;  // tiles of the sequences before b, of all
+  int64_t before = 0, total = 0;  // units of the sequences before b, of all
   for (int i = threadIdx.x; i < a.batch.batch; i += D) {
-    const int tiles = kv_sequence(a, i).tiles;
-    total += tiles;
-    if (i < b) before += tiles;
+    const int units = units_of(kv_sequence(a, i).tiles);
+    total += units;
+    if (i < b) before += units;
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
@@ -851,11 +918,11 @@ kv_decode_join_kernel(const AttentionArgs a, int grid) {
     total += sums[2 * w + 1];
   }
   const Share s = share_of(total * a.cache.kv_heads, grid);
-  const int64_t t0 = before * a.cache.kv_heads + (int64_t)head * seq.tiles;
-  const int64_t t1 = t0 + seq.tiles - 1;
-  // CTA of tile t: the last one whose share begins at or before it.
-  const int c0 = (int)(((t0 + 1) * s.ctas - 1) / s.total);
-  const int c1 = (int)(((t1 + 1) * s.ctas - 1) / s.total);
+  const int64_t u0 = before * a.cache.kv_heads + (int64_t)head * units_of(seq.tiles) + kSegmentUnits;
+  const int64_t u1 = u0 + seq.tiles - 1;
+  // CTA of a unit: the last one whose share begins at or before it.
+  const int c0 = (int)(((u0 + 1) * s.ctas - 1) / s.total);
+  const int c1 = (int)(((u1 + 1) * s.ctas - 1) / s.total);
   if (c0 == c1) return;  // one CTA had all of it and wrote the row
   // The first CTA began before this (sequence, head) or with it, the others inside it.
   const int parts = c1 - c0 + 1;
@@ -884,9 +951,8 @@ kv_decode_join_kernel(const AttentionArgs a, int grid) {
   for (int p = 0; p < parts; ++p)
     o += exp2f(tops[p] - base) * column[(p == 0 ? first : later + 2 * p) * C::kPartialFloats];
   o = l == 0.0f ? 0.0f : o / l;
-  int64_t at;
-  output_row<RP>(a, seq, head, r, &at);
-  T* out = static_cast<T*>(a.out) + at + threadIdx.x;
+  T* out = static_cast<T*>(a.out) + (seq.row + r / a.group) * a.out_token_stride +
+           (int64_t)(head * a.group + r % a.group) * a.out_head_stride + threadIdx.x;
   if constexpr (TERMS == 2) *out = __float2bfloat16_rn(o);
   else *out = __float2half_rn(o);
 }
@@ -922,7 +988,7 @@ int launch(const CUtensorMap& tm_k, const CUtensorMap& tm_v, const AttentionArgs
   config.attrs = attribute;
   config.numAttrs = use_pdl() ? 1 : 0;
   MX_CUDA(cudaLaunchKernelEx(&config, kv_decode_kernel<D, RP, TERMS>, tm_k, tm_v, a));
-  if (grid == 1) return kOk;  // nothing was split
+  if (a.whole_items != 0 || grid == 1) return kOk;  // nothing was cut
   config.gridDim = dim3((unsigned)(a.batch.batch * a.cache.kv_heads), (unsigned)a.max_rows);
   config.blockDim = dim3(D);
   config.dynamicSmemBytes = 0;
@@ -940,10 +1006,12 @@ int launch_rows(const CUtensorMap& tm_k, const CUtensorMap& tm_v, const Attentio
 
 }  // namespace
 
-// CTAs of a decode launch: at most one per SM, at most one per two tiles that there can be.
+// CTAs of a decode launch: at most one per SM and no more than there can be work for.
 int kv_decode_grid(int64_t batch, int kv_heads, int64_t max_context) {
-  const int64_t tiles = batch * kv_heads * ceil_div64(max_context < 1 ? 1 : max_context, kKvTile);
-  const int64_t want = ceil_div64(tiles, kMinTiles);
+  const int64_t tiles = ceil_div64(max_context < 1 ? 1 : max_context, kKvTile);
+  const int64_t items = batch * kv_heads;
+  const int64_t want =
+      tiles <= kWholeTiles ? items : ceil_div64(items * (tiles + kSegmentUnits), kMinUnits);
   return (int)(want < kSms ? want : kSms);
 }
 
@@ -952,14 +1020,16 @@ int kv_decode_rows(int head_dim, int dtype) { return most_rows(head_dim, dtype =
 int64_t kv_decode_workspace(int64_t batch, int kv_heads, int head_dim, int dtype, int rows,
                             int64_t max_context) {
   const int grid = kv_decode_grid(batch, kv_heads, max_context);
-  if (grid == 1) return 0;
+  if (grid == 1 || max_context <= kWholeTiles * kKvTile) return 0;
   const int rp = rows <= 8 ? 8 : rows <= 16 ? 16 : kv_decode_rows(head_dim, dtype);
   return (int64_t)grid * 2 * (rp * head_dim + 2 * rp) * 4;
 }
 
 // Sequences with at most a.max_rows <= kv_decode_rows() rows (tokens x group); others are left
 // alone.
-int launch_kv_decode(const AttentionArgs& a, int dtype, cudaStream_t stream) {
+int launch_kv_decode(const AttentionArgs& args, int dtype, cudaStream_t stream) {
+  AttentionArgs a = args;
+  a.whole_items = (int64_t)a.batch.table_width * a.cache.page_size <= kWholeTiles * kKvTile;
   CUtensorMap tm_k, tm_v;
   if (int rc = make_kv_map(&tm_k, a.cache.k_values, a.cache)) return rc;
   if (int rc = make_kv_map(&tm_v, a.cache.v_values, a.cache)) return rc;

@@ -51,6 +51,12 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
   return ok != 0;
 }
 
+// 2^v by the special-function unit (results below 2^-126 become 0).
+__device__ __forceinline__ float exp2_approx(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
 // Largest value over the warp, NaN ignored.
 __device__ __forceinline__ float warp_max(float v) {
   float r;
