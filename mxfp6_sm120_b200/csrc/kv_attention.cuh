@@ -64,21 +64,17 @@ __device__ __forceinline__ void e4m3_terms(float a, float b, uint32_t (&codes)[k
   }
 }
 
-// The same of two FP16 numbers; returns what the terms add up to (exact in FP16: two terms have
-// at most nine bits, three hold all eleven).
+// The same of two FP16 numbers (their remainders are exact in FP16).
 template <int kTerms>
-__device__ __forceinline__ __half2 e4m3_terms_half(__half2 x, uint32_t (&codes)[kTerms]) {
-  __half2 whole = x;
+__device__ __forceinline__ void e4m3_terms_half(__half2 x, uint32_t (&codes)[kTerms]) {
 #pragma unroll
   for (int t = 0; t < kTerms; ++t) {
     codes[t] = __nv_cvt_halfraw2_to_fp8x2(static_cast<__half2_raw>(x), __NV_SATFINITE, __NV_E4M3);
-    if (t + 1 < kTerms || kTerms == 2) {
+    if (t + 1 < kTerms) {
       const __half2 v(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)codes[t], __NV_E4M3));
-      if (kTerms == 2) whole = t == 0 ? v : __hfma2(v, __float2half2_rn(0.0625f), whole);
-      if (t + 1 < kTerms) x = __hmul2(__hsub2(x, v), __float2half2_rn(16.0f));
+      x = __hmul2(__hsub2(x, v), __float2half2_rn(16.0f));
     }
   }
-  return whole;
 }
 
 // 2^v of a whole v up to 127 (below -126: 2^-126): adding 1.5 * 2^23 leaves v in the low bits.

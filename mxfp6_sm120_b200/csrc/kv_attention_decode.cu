@@ -13,8 +13,8 @@
 //    With at most 96 columns an MMA costs what its 128-row operand costs (about 33 ns).
 //  * Warps: 0-3 and 4-7 softmax (one lane per token; the two groups take alternate tiles, each
 //    with its own running maximum and output accumulator, because one group needs about as long
-//    for a tile as HBM does), 8 TMA, 9 MMA, 10-11 quantise queries.  K(j+1) is multiplied before
-//    V(j), so the softmax of a tile overlaps the next tile's scores.
+//    for a tile as HBM does), 8 TMA, 9 MMA, 10-11 quantise queries.  The scores of tile j + 2 are
+//    issued as soon as those of tile j have been read, before the output of tile j.
 //  * The list of (sequence, key head, tile of 128 tokens) is cut into equal shares, one per CTA
 //    (one per SM), whatever the lengths are: the cut follows the lengths on the device.  A CTA
 //    whose share covers all tiles of a (sequence, head) writes its rows; otherwise it leaves
@@ -22,13 +22,13 @@
 //    programmatic dependent) joins them in the order of the tiles, so the result does not depend
 //    on timing.
 //  * Online softmax without touching the output.  The weights of a row are taken relative to the
-//    largest score among the warp's own 32 tokens, rounded up to a power of two, and that power
+//    largest score among the warp's own 32 tokens, rounded to a power of two, and that power
 //    (relative to a reference fixed by the first tile) is the hardware block scale of the
 //    weights: 32 tokens is one scale block of the second product.  So no maximum crosses warps
 //    and no accumulator is rescaled from tile to tile.  Only where a tile exceeds the reference
 //    by more than 2^16 the four warps move it and shrink the accumulator.  It is also the more
-//    exact way: each block's largest weight is in (128, 256], so E4M3's smallest step never
-//    reaches a weight that counts.
+//    exact way: each block's largest weight is in (181, 363), so E4M3's smallest step never
+//    reaches a weight that counts.  The sums of the weights are a product with ones.
 #include "kv_attention.cuh"
 
 #include <cstdlib>
@@ -42,7 +42,10 @@ namespace {
 constexpr int kThreads = 384;
 constexpr int kGroupWarps = 4;  // warps of a softmax group, one per 32 lanes of tensor memory
 constexpr int kTmaWarp = 8, kMmaWarp = 9, kQueryWarp = 10, kQueryWarps = 2;
-constexpr float kWeightScale = 256.0f;  // weights 0..1 become 0..256 before they become E4M3 terms
+// Query buffers.  Scores run two tiles ahead of the outputs, so a tile of one segment may be
+// waiting for its output while the scores of the second segment behind it are due.
+constexpr int kQueries = 3;
+constexpr float kWeightLog2 = 8.0f;     // weights are scaled by 256 before they become E4M3 terms
 constexpr float kMostLog2 = 16.0f;      // a tile may exceed the reference by 2^16
 constexpr int kSms = 148;
 constexpr int kSegmentUnits = 1;  // what an item costs beside its tiles
@@ -58,18 +61,20 @@ struct DecodeCfg {
   static constexpr int kSlotBytes = kKvTile * D;     // a K or V tile
   static constexpr int kQBytes = (kN * D + 1023) / 1024 * 1024;
   static constexpr int kPBytes = kN * kKvTile;
-  static constexpr int kFixedBytes = 6144;
+  static constexpr int kFixedBytes = 7168;
   static constexpr int kBudget = 227 * 1024 - 1024;
   static constexpr int kFit =
-      (kBudget - kFixedBytes - 2 * kQBytes - 2 * kPBytes) / (kSlotBytes + 512);
+      (kBudget - kFixedBytes - kQueries * kQBytes - 2 * kPBytes) / (kSlotBytes + 512);
   static constexpr int kSlots = kFit > 16 ? 16 : kFit;
   static_assert(kSlots >= 4, "the ring needs two tiles of K and V");
   static constexpr int kSmemBytes =
-      1024 + kSlots * (kSlotBytes + 512) + 2 * kQBytes + 2 * kPBytes + kFixedBytes;
-  // Tensor memory columns: two score tiles, two outputs of one or two halves, scales.
+      1024 + kSlots * (kSlotBytes + 512) + kQueries * kQBytes + 2 * kPBytes + kFixedBytes;
+  // Tensor memory columns: two score tiles; per softmax group an output of one or two halves
+  // and the sums of the weights; scales.
   static constexpr int kHalves = D > 128 ? 2 : 1;
   static constexpr int kOCol = 2 * kN;
-  static constexpr int kSfCol = kOCol + 2 * kHalves * kN;
+  static constexpr int kLCol = kOCol + 2 * kHalves * kN;  // sums of the weights, per group
+  static constexpr int kSfCol = kLCol + 2 * kN;
   static constexpr int kColsUsed = kSfCol + 28;
   static constexpr int kChunk = RP % 16 == 0 ? 16 : 8;  // rows of a score tile held at a time
   static constexpr int kTmemCols = kColsUsed <= 64 ? 64 : kColsUsed <= 128 ? 128 : kColsUsed <= 256 ? 256 : 512;
@@ -80,9 +85,11 @@ struct DecodeCfg {
   static constexpr int kPartialFloats = RP * D + 2 * RP;
 };
 
-// Rows (new tokens x query heads) of the widest variant: two accumulators of two halves and
-// three terms each leave tensor memory for 24 rows, the others take 32.
-constexpr int most_rows(int d, int terms) { return d == 256 && terms == 3 ? 24 : 32; }
+// Rows (new tokens x query heads) of the widest variant: tensor memory holds, for two groups,
+// scores, sums and one or two output halves of rows x terms columns.
+constexpr int most_rows(int d, int terms) {
+  return d == 256 ? (terms == 3 ? 16 : 24) : (terms == 3 ? 24 : 32);
+}
 
 // The work list and its cut, the same arithmetic in both kernels.  An item is a (sequence, key
 // head); it counts its tiles and kSegmentUnits more for the rows' start and end (a CTA that takes
@@ -198,6 +205,12 @@ struct Segment {
   int whole;        // all tiles of the item are here
 };
 
+// Place of tile i's K and V (of `count` tiles) in the order of the copies: K0, K1, K2, V0, K3, V1, ...
+__device__ __forceinline__ int slot_of_k(int i) { return i < 2 ? i : 2 * i - 2; }
+__device__ __forceinline__ int slot_of_v(int i, int count) {
+  return i + 2 < count ? 2 * i + 3 : count + i;
+}
+
 template <int D, int RP, int TERMS>
 __global__ void __launch_bounds__(kThreads, 1)
 kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
@@ -208,37 +221,38 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* slots = smem;
-  uint8_t* q_tiles = slots + C::kSlots * C::kSlotBytes;        // two, [sub][column][row bytes]
-  uint8_t* p_tiles = q_tiles + 2 * C::kQBytes;                 // two, [column][128 tokens]
+  uint8_t* q_tiles = slots + C::kSlots * C::kSlotBytes;        // [buffer][sub][column][row bytes]
+  uint8_t* p_tiles = q_tiles + kQueries * C::kQBytes;                 // two, [column][128 tokens]
   uint8_t* sf_tiles = p_tiles + 2 * C::kPBytes;                // scale atom of every slot
   uint8_t* fixed = sf_tiles + C::kSlots * 512;
   uint64_t* bars = reinterpret_cast<uint64_t*>(fixed);
   uint8_t* ones = fixed + 512;                                 // scale atom of factors of one
   uint8_t* p_sf = fixed + 1024;                                // scale atom of each group's weights
-  Segment<RP>* segments = reinterpret_cast<Segment<RP>*>(fixed + 2048);  // two
-  float* red_max = reinterpret_cast<float*>(segments + 2);     // [group][warp][RP]
-  float* red_sum = red_max + 8 * RP;                           // [group][warp][RP]
-  float* red_top = red_sum + 8 * RP;                           // [group][RP]
+  uint8_t* one_values = fixed + 1024 + 1024;                   // E4M3 ones, see the sums
+  Segment<RP>* segments = reinterpret_cast<Segment<RP>*>(fixed + 4096);  // [buffer]
+  float* red_max = reinterpret_cast<float*>(segments + kQueries);     // [group][warp][RP]
+  float* red_top = red_max + 8 * RP;                           // [group][RP]
   Cursor* start = reinterpret_cast<Cursor*>(red_top + 2 * RP);
   int64_t* share_smem = reinterpret_cast<int64_t*>(start + 1);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(share_smem + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* ask_flag = abort_flag + 1;                     // [group][2]
   volatile uint32_t* slot_named = reinterpret_cast<volatile uint32_t*>(ask_flag + 4);  // [slot]
-  static_assert(2048 + 2 * sizeof(Segment<RP>) + 18 * RP * 4 + sizeof(Cursor) + 16 + 8 + 16 + 64 <=
+  static_assert(4096 + kQueries * sizeof(Segment<RP>) + 10 * RP * 4 + sizeof(Cursor) + 16 + 8 + 16 + 64 <=
                     C::kFixedBytes,
                 "fixed area");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t full0 = ptx::smem_u32(bars);
   const uint32_t empty0 = full0 + 8 * C::kSlots;
-  const uint32_t sfull0 = empty0 + 8 * C::kSlots;  // two of each from here on
+  const uint32_t sfull0 = empty0 + 8 * C::kSlots;  // two of each but the query barriers
   const uint32_t pfull0 = sfull0 + 16;
   const uint32_t pvdone0 = pfull0 + 16;
   const uint32_t qfull0 = pvdone0 + 16;
-  const uint32_t qempty0 = qfull0 + 16;
-  const uint32_t vsync0 = qempty0 + 16;
-  static_assert(8 * (2 * 16 + 12) <= 512, "barriers");
+  const uint32_t qempty0 = qfull0 + 8 * kQueries;
+  const uint32_t vsync0 = qempty0 + 8 * kQueries;
+  const uint32_t sread0 = vsync0 + 16;
+  static_assert(8 * (2 * 16 + 10 + 2 * kQueries) <= 512, "barriers");
 
   if (threadIdx.x == 0) {
     *abort_flag = 0;
@@ -251,15 +265,20 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       ptx::mbar_init(sfull0 + 8 * i, 1);
       ptx::mbar_init(pfull0 + 8 * i, kGroupWarps);
       ptx::mbar_init(pvdone0 + 8 * i, 1);
+      ptx::mbar_init(vsync0 + 8 * i, kGroupWarps);
+      ptx::mbar_init(sread0 + 8 * i, kGroupWarps);
+    }
+    for (int i = 0; i < kQueries; ++i) {
       ptx::mbar_init(qfull0 + 8 * i, kQueryWarps);
       ptx::mbar_init(qempty0 + 8 * i, 1 + 2 * kGroupWarps);
-      ptx::mbar_init(vsync0 + 8 * i, kGroupWarps);
     }
     ptx::fence_mbar_init();
     ptx::prefetch_tensormap(&tm_k);
     ptx::prefetch_tensormap(&tm_v);
   }
   if (threadIdx.x < 128) reinterpret_cast<uint32_t*>(ones)[threadIdx.x] = 0x7f7f7f7fu;
+  for (int i = threadIdx.x; i < 512; i += kThreads)
+    reinterpret_cast<uint32_t*>(one_values)[i] = 0x38383838u;
   ptx::fence_proxy_async();
   if (warp == kMmaWarp) {
     ptx::tmem_alloc(ptx::smem_u32(tmem_slot), C::kTmemCols);
@@ -288,7 +307,7 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
 
   if (count > 0 && warp == kTmaWarp) {
     // ---------------- TMA producer ----------------
-    // Tiles are fetched in the order of their use: K0, K1, V0, K2, V1, ...  Lane l looks up block
+    // Tiles are fetched in the order of their use: K0, K1, K2, V0, K3, V1, ...  Lane l looks up block
     // l % 4 of tile l / 4 of a group of eight tiles and later issues that block's copies itself;
     // the next group's lookups are in flight while this group is copied.
     Cursor mine = *start;
@@ -307,7 +326,7 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       k_sf = a.cache.k_scales[page];
       v_sf = a.cache.v_scales[page];
     }
-    // The V tile of a group's last tile is copied after the next group's first K tile.
+    // The V tiles of a group's last two tiles are copied after the next group's first K tiles.
     int64_t last_page = -1;
     uint32_t last_v = 127;
     int slot = 0;
@@ -361,20 +380,26 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       }
       for (int j = 0; ok && j < 8 && i0 + j < count; ++j) {
         copy(false, page, k_sf, 4 * j);
-        if (j > 0) copy(true, page, v_sf, 4 * (j - 1));
-        else if (i0 > 0) copy(true, last_page, last_v, 28);
+        if (j > 1) copy(true, page, v_sf, 4 * (j - 2));
+        else if (i0 > 0) copy(true, last_page, last_v, 4 * (j + 6));
         if (j == 3 && more) {
           next_k = next_page >= 0 ? a.cache.k_scales[next_page] : 127u;
           next_v = next_page >= 0 ? a.cache.v_scales[next_page] : 127u;
         }
       }
+      if (!more) break;
       last_page = page;
       last_v = v_sf;
       page = next_page;
       k_sf = next_k;
       v_sf = next_v;
     }
-    if (ok) copy(true, last_page, last_v, 4 * ((count - 1) & 7));
+    if (count > 1) {
+      // The tile before the last one may have been the last of the group before.
+      const bool before = ((count - 1) & 7) == 0;
+      copy(true, before ? last_page : page, before ? last_v : v_sf, 4 * ((count - 2) & 7));
+    }
+    copy(true, page, v_sf, 4 * ((count - 1) & 7));
   } else if (count > 0 && warp == kMmaWarp) {
     // ---------------- MMA issuer ----------------
     constexpr uint32_t kIdesc = ((uint32_t)(C::kN >> 3) << 17) | (1u << 23) | ((128u >> 4) << 24);
@@ -383,17 +408,16 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
     if (ptx::elect_one()) ptx::tc_cp_32x128b_warpx4(ones_t, ptx::smem_desc_scale_atom(ptx::smem_u32(ones)));
     __syncwarp();
     int segment = 0, in_segment = 0, of_segment = 0;  // of the next scores: segment, tile, tiles
-    int summed = 0;                // number of the next V tile within its segment
+    uint32_t fresh = 0;  // bit i % 32: tile i is one of the first two of its segment
     bool ok = true;
-    // Slot of K(i) is 2i - 1 (0 for the first), of V(i) 2i + 2 (2i + 1 for the last).
     auto scores = [&](int i) {
-      const int at = i == 0 ? 0 : 2 * i - 1;
+      const int at = slot_of_k(i);
       const int slot = at % C::kSlots;
       if (in_segment == 0) {
-        ok = ok && __all_sync(0xffffffffu, bounded_wait(qfull0 + 8 * (segment & 1),
-                                                        (uint32_t)(segment >> 1) & 1u, abort_flag,
-                                                        a.status, 402));
-        of_segment = segments[segment & 1].tiles;
+        ok = ok && __all_sync(0xffffffffu, bounded_wait(qfull0 + 8 * (segment % kQueries),
+                                                        (uint32_t)(segment / kQueries) & 1u,
+                                                        abort_flag, a.status, 402));
+        of_segment = segments[segment % kQueries].tiles;
       }
       const bool last = in_segment + 1 == of_segment;
       ok = ok && __all_sync(0xffffffffu,
@@ -405,7 +429,7 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         const uint32_t sf_t = sf0 + 12 * (i & 1);
         ptx::tc_cp_32x128b_warpx4(sf_t, ptx::smem_desc_scale_atom(ptx::smem_u32(sf_tiles + slot * 512)));
         const uint32_t k_s = ptx::smem_u32(slots + slot * C::kSlotBytes);
-        const uint32_t q_s = ptx::smem_u32(q_tiles + (segment & 1) * C::kQBytes);
+        const uint32_t q_s = ptx::smem_u32(q_tiles + (segment % kQueries) * C::kQBytes);
 #pragma unroll
         for (int s = 0; s < C::kSubs; ++s) {
           const uint64_t ad = ptx::smem_desc(k_s + s * C::kSubBytes, 0, C::kGroup, C::kSwizzle);
@@ -417,9 +441,10 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         }
         ptx::tc_commit(sfull0 + 8 * (i & 1));
         ptx::tc_commit(empty0 + 8 * slot);
-        if (last) ptx::tc_commit(qempty0 + 8 * (segment & 1));
+        if (last) ptx::tc_commit(qempty0 + 8 * (segment % kQueries));
       }
       __syncwarp();
+      fresh = (fresh & ~(1u << (i & 31))) | (uint32_t)(in_segment < 2) << (i & 31);
       ++in_segment;
       if (last) {
         ++segment;
@@ -427,12 +452,16 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       }
     };
     scores(0);
+    if (count > 1) scores(1);
     for (int i = 0; ok && i < count; ++i) {
-      // Number of tile i within its segment: the scores of tile i + 1 tell whether one ended.
-      const int number = summed;
-      summed = in_segment == 0 ? 0 : summed + 1;
-      if (i + 1 < count) scores(i + 1);
-      const int at = i + 1 < count ? 2 * i + 2 : 2 * i + 1;
+      // Scores of tile i + 2 as soon as those of tile i have been read.
+      if (i + 2 < count) {
+        ok = __all_sync(0xffffffffu, bounded_wait(sread0 + 8 * (i & 1), (uint32_t)(i >> 1) & 1u,
+                                                  abort_flag, a.status, 415));
+        if (!ok) break;
+        scores(i + 2);
+      }
+      const int at = slot_of_v(i, count);
       const int slot = at % C::kSlots;
       ok = ok && __all_sync(0xffffffffu, bounded_wait(pfull0 + 8 * (i & 1), (uint32_t)(i >> 1) & 1u,
                                                       abort_flag, a.status, 404));
@@ -448,6 +477,15 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         const uint32_t v_s = ptx::smem_u32(slots + slot * C::kSlotBytes);
         const uint64_t bd =
             ptx::smem_desc(ptx::smem_u32(p_tiles + (i & 1) * C::kPBytes), 0, 1024, ptx::kSwizzle128);
+        const bool first = (fresh >> (i & 31) & 1u) != 0;  // of its group in the segment
+        // Sums of the weights as they were rounded and scaled, so that they add up to one: a
+        // product with ones (eight rows of shared memory serve all 128).
+        const uint64_t ones_d = ptx::smem_desc(ptx::smem_u32(one_values), 0, 0, ptx::kSwizzle128);
+#pragma unroll
+        for (int ks = 0; ks < kKvTileBlocks; ++ks)
+          ptx::tc_mma_mxf8f6f4(tmem + C::kLCol + (i & 1) * C::kN, ones_d, bd + 2 * ks,
+                               kIdesc | ((uint32_t)ks << 4), ones_t, weight_t,
+                               (!first || ks > 0) ? 1u : 0u);
 #pragma unroll
         for (int h = 0; h < C::kHalves; ++h) {
           // V^T: 128 values of head_dim along M (MN-major), 32 tokens per step.  With a head of
@@ -458,7 +496,7 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
             const uint32_t idesc = kIdesc | (1u << 15) | ((uint32_t)ks << 29) | ((uint32_t)ks << 4);
             ptx::tc_mma_mxf8f6f4(tmem + C::kOCol + ((i & 1) * C::kHalves + h) * C::kN,
                                  ad + ks * (kKvBlock * C::kRowBytes / 16), bd + 2 * ks, idesc, sf_t,
-                                 weight_t, (number >= 2 || ks > 0) ? 1u : 0u);
+                                 weight_t, (!first || ks > 0) ? 1u : 0u);
           }
         }
         ptx::tc_commit(pvdone0 + 8 * (i & 1));
@@ -473,8 +511,8 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
     int left = count;
     bool ok = true;
     for (int segment = 0; ok && left > 0; ++segment) {
-      const int buffer = segment & 1;
-      ok = __all_sync(0xffffffffu, bounded_wait(qempty0 + 8 * buffer, ((uint32_t)(segment >> 1) & 1u) ^ 1u,
+      const int buffer = segment % kQueries;
+      ok = __all_sync(0xffffffffu, bounded_wait(qempty0 + 8 * buffer, ((uint32_t)(segment / kQueries) & 1u) ^ 1u,
                                                 abort_flag, a.status, 406));
       if (!ok) break;
       Segment<RP>& seg = segments[buffer];
@@ -585,6 +623,7 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
     const uint32_t s_t = lane_t + group * C::kN;
     const uint32_t sfull = sfull0 + 8 * group, pfull = pfull0 + 8 * group;
     const uint32_t pvdone = pvdone0 + 8 * group, vsync = vsync0 + 8 * group;
+    const uint32_t sread = sread0 + 8 * group;
     uint8_t* p_s = p_tiles + group * C::kPBytes + (token & 15);
     float* my_max = red_max + group * 4 * RP;
     bool failed = false;
@@ -595,16 +634,11 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       if (!failed) failed = !__all_sync(0xffffffffu, bounded_wait(bar, parity, abort_flag, a.status, code));
     };
     for (int segment = 0, i0 = 0; i0 < count; ++segment) {
-      wait(qfull0 + 8 * (segment & 1), (uint32_t)(segment >> 1) & 1u, 407);
-      const Segment<RP>& seg = segments[segment & 1];
+      wait(qfull0 + 8 * (segment % kQueries), (uint32_t)(segment / kQueries) & 1u, 407);
+      const Segment<RP>& seg = segments[segment % kQueries];
       const int tiles = failed ? 0 : seg.tiles, length = seg.length;
       const int64_t first_position = seg.first_position;
-      float ref[RP], sum[RP];  // ref: the same in all lanes of the group
-#pragma unroll
-      for (int r = 0; r < RP; ++r) {
-        ref[r] = -INFINITY;
-        sum[r] = 0.0f;
-      }
+      float ref = -INFINITY;  // of row lane % RP, the same in the four warps
       const int j0 = (group ^ i0) & 1;
 #pragma unroll 1
       for (int j = j0; j < tiles; j += 2, ++done) {
@@ -612,13 +646,14 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         const int t0 = (seg.tile + j) * kKvTile;
         const int held = min(kKvTile, length - t0);  // tokens of this tile that exist
         wait(sfull, done & 1u, 409);
-        const int at = i + 1 < count ? 2 * i + 2 : 2 * i + 1;
+        const int at = slot_of_v(i, count);
         const int slot = at % C::kSlots;
         wait(full0 + 8 * slot, (uint32_t)(at / C::kSlots) & 1u, 408);
         if (failed) break;
         ptx::tc_fence_after();
         const bool named = (slot_named[slot] >> quarter & 1u) != 0;
-        if (!named || (quarter + 1) * 32 > held) {
+        const bool here = named && token < held, full = named && (quarter + 1) * 32 <= held;
+        if (!full) {
           // Rows of V without a token may hold anything, NaN among them, and 0 * NaN is NaN.
           uint8_t* v_s = slots + slot * C::kSlotBytes;
           const int from = named ? max(0, held - quarter * 32) : 0;
@@ -629,13 +664,11 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
                                       in_row * 16) = make_uint4(0, 0, 0, 0);
           }
         }
-        const bool here = named && token < held;
         const bool bounded = a.causal && t0 + held - 1 > first_position;
-        uint32_t my_code = 127;  // weight scale of row lane % RP in this warp's 32 tokens
+        float my_top = -INFINITY;  // of row lane % RP in this warp's 32 tokens
 #pragma unroll
         for (int c0 = 0; c0 < RP; c0 += C::kChunk) {
-          float s[C::kChunk], top[C::kChunk];
-          bool ask = false;
+          float s[C::kChunk];
 #pragma unroll
           for (int r0 = 0; r0 < C::kChunk; r0 += 8) {
             uint32_t raw[TERMS][8];
@@ -647,40 +680,38 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
               float v = __uint_as_float(raw[TERMS - 1][n]);
 #pragma unroll
               for (int k = TERMS - 2; k >= 0; --k) v = v * 0.0625f + __uint_as_float(raw[k][n]);
-              s[r0 + n] = here ? v * seg.scale[c0 + r0 + n] : -INFINITY;
+              s[r0 + n] = v * seg.scale[c0 + r0 + n];
             }
+          }
+          if (c0 + C::kChunk == RP) {
+            ptx::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(sread);
+          }
+          if (!full) {
+#pragma unroll
+            for (int r = 0; r < C::kChunk; ++r)
+              if (!here) s[r] = -INFINITY;
           }
           if (bounded) {
 #pragma unroll
             for (int r = 0; r < C::kChunk; ++r)
               if (t0 + token > first_position + (c0 + r) / a.group) s[r] = -INFINITY;
           }
-#pragma unroll
-          for (int r = 0; r < C::kChunk; ++r) {
-            top[r] = ceilf(ptx::warp_max(s[r]));
-            ask = ask || top[r] > ref[c0 + r] + kMostLog2;
-          }
-          // Does any of the four warps ask for another reference?  The answer is only needed
-          // after the weights, which do not depend on it.
-          volatile int* asked = ask_flag + group * 2 + (votes++ & 1u);
-          if (lane == 0) {
-            if (ask) *asked = 1;
-            ptx::mbar_arrive(vsync);
-          }
           // PV of this group's last tile has read the weights that this tile's replace.
           if (c0 == 0 && done > 0) wait(pvdone, (done - 1) & 1u, 410);
-          float kept[C::kChunk];
 #pragma unroll
           for (int r = 0; r < C::kChunk; r += 2) {
             float p[2];
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
-              p[n] = ptx::exp2_approx(s[r + n] - (top[r + n] == -INFINITY ? 0.0f : top[r + n]));
+            for (int n = 0; n < 2; ++n) {
+              // To the nearest power of two: the largest weight is in (181, 363).
+              const float top = rintf(ptx::warp_max(s[r + n]));
+              if (lane % RP == c0 + r + n) my_top = top;
+              p[n] = ptx::exp2_approx(s[r + n] - (fmaxf(top, -1e30f) - kWeightLog2));
+            }
             uint32_t codes[TERMS];
-            const float2 held2 = __half22float2(e4m3_terms_half<TERMS>(
-                __floats2half2_rn(p[0] * kWeightScale, p[1] * kWeightScale), codes));
-            kept[r] = held2.x;
-            kept[r + 1] = held2.y;
+            e4m3_terms_half<TERMS>(__floats2half2_rn(p[0], p[1]), codes);
 #pragma unroll
             for (int k = 0; k < TERMS; ++k) {
 #pragma unroll
@@ -690,64 +721,58 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
               }
             }
           }
-          wait(vsync, syncs & 1u, 413);
+        }
+        // Does any row of the four warps need another reference?
+        volatile int* asked = ask_flag + group * 2 + (votes++ & 1u);
+        const bool ask = __any_sync(0xffffffffu, my_top > ref + kMostLog2);
+        if (lane == 0) {
+          if (ask) *asked = 1;
+          ptx::mbar_arrive(vsync);
+        }
+        wait(vsync, syncs & 1u, 413);
+        ++syncs;
+        if (!failed && *asked != 0) {
+          // The first tokens that a row sees, or a maximum far above its reference: the four
+          // warps agree on a new one.
+          if (lane < RP) my_max[quarter * RP + lane] = my_top;
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(vsync);
+          wait(vsync, syncs & 1u, 414);
           ++syncs;
-          if (!failed && *asked != 0) {
-            // The first tokens that a row sees, or a maximum far above its reference: the four
-            // warps agree on a new one.
+          if (quarter == 0 && lane == 0) *asked = 0;  // not used by the next vote, but the one after
+          const int r = lane % RP;
+          const float m = fmaxf(fmaxf(my_max[r], my_max[RP + r]),
+                                fmaxf(my_max[2 * RP + r], my_max[3 * RP + r]));
+          const bool up = m > ref + kMostLog2;
+          const float f = up ? pow2_whole(ref - m) : 1.0f;
+          if (up) ref = m;
+          if (j != j0 && !failed) {
+            // What has been added up so far shrinks (PV of this group's last tile is done).
+            ptx::tc_fence_after();
+#pragma unroll 1
+            for (int c0 = 0; c0 < C::kN; c0 += 8) {
+              float g[8];
 #pragma unroll
-            for (int r = 0; r < C::kChunk; ++r)
-              if (lane == (r & 31)) my_max[quarter * RP + r] = top[r];
-            __syncwarp();
-            if (lane == 0) ptx::mbar_arrive(vsync);
-            wait(vsync, syncs & 1u, 414);
-            ++syncs;
-            if (quarter == 0 && lane == 0) *asked = 0;  // not used by the next vote, but the one after
-            const bool shrink = j != j0 && !failed;
-            if (shrink) ptx::tc_fence_after();
+              for (int n = 0; n < 8; ++n) g[n] = __shfl_sync(0xffffffffu, f, (c0 + n) % RP);
 #pragma unroll
-            for (int r0 = 0; r0 < C::kChunk; r0 += 8) {
-              float f[8];
+              for (int h = 0; h <= C::kHalves; ++h) {
+                uint32_t o[8];
+                const uint32_t at_o = lane_t + c0 + (h < C::kHalves
+                                                         ? C::kOCol + (group * C::kHalves + h) * C::kN
+                                                         : C::kLCol + group * C::kN);
+                ptx::tmem_ld_x8(at_o, o);
+                ptx::tmem_ld_wait();
 #pragma unroll
-              for (int n = 0; n < 8; ++n) {
-                const int r = r0 + n;
-                const float m = fmaxf(fmaxf(my_max[r], my_max[RP + r]),
-                                      fmaxf(my_max[2 * RP + r], my_max[3 * RP + r]));
-                const float old = ref[c0 + r];
-                const bool up = m > old + kMostLog2;
-                f[n] = up ? pow2_whole(old - m) : 1.0f;
-                sum[c0 + r] *= f[n];
-                ref[c0 + r] = up ? m : old;
-              }
-              if (shrink) {
-#pragma unroll
-                for (int h = 0; h < C::kHalves; ++h) {
-#pragma unroll
-                  for (int k = 0; k < TERMS; ++k) {
-                    uint32_t o[8];
-                    const uint32_t at_o = lane_t + C::kOCol + (group * C::kHalves + h) * C::kN + k * RP + c0 + r0;
-                    ptx::tmem_ld_x8(at_o, o);
-                    ptx::tmem_ld_wait();
-#pragma unroll
-                    for (int n = 0; n < 8; ++n)
-                      o[n] = __float_as_uint(__uint_as_float(o[n]) * f[n]);
-                    ptx::tmem_st_x8(at_o, o);
-                  }
-                }
+                for (int n = 0; n < 8; ++n) o[n] = __float_as_uint(__uint_as_float(o[n]) * g[n]);
+                ptx::tmem_st_x8(at_o, o);
               }
             }
-            if (shrink) ptx::tmem_st_wait();
-          }
-#pragma unroll
-          for (int r = 0; r < C::kChunk; ++r) {
-            // 2^(top - ref), a power of two between 2^-126 and 2^16; its exponent field is the
-            // UE8M0 code.  The sum takes the weights as they were rounded, so that they add up
-            // to one.
-            const float power = pow2_whole(top[r] == -INFINITY ? 0.0f : top[r] - ref[c0 + r]);
-            sum[c0 + r] += kept[r] * power;
-            if (lane % RP == c0 + r) my_code = __float_as_uint(power) >> 23;
+            ptx::tmem_st_wait();
           }
         }
+        // 2^(top - ref), between 2^-126 and 2^16: its exponent field is the UE8M0 code.
+        const uint32_t my_code =
+            my_top == -INFINITY ? 127u : __float_as_uint(pow2_whole(my_top - ref)) >> 23;
         if (failed) break;
         // Scale atom of the weights: column col is row col % 32 of the atom, word col / 32, and
         // this warp's tokens are byte `quarter` of the word.
@@ -763,61 +788,24 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(pfull);
       }
-      // ---- the segment's rows: sums over the tokens, then the output of this CTA's tiles ----
-      // Sums over the warp: pairs of rows are folded into one value per lane, so that eight rows
-      // take nine exchanges.
-#pragma unroll
-      for (int r0 = 0; r0 < RP; r0 += 8) {
-        float v[8];
-#pragma unroll
-        for (int n = 0; n < 8; ++n) v[n] = sum[r0 + n];
-#pragma unroll
-        for (int width = 4; width >= 1; width >>= 1) {
-          const bool high = (lane & width) != 0;
-#pragma unroll
-          for (int n = 0; n < width; ++n) {
-            const float mine = high ? v[n + width] : v[n];
-            const float other = __shfl_xor_sync(0xffffffffu, high ? v[n] : v[n + width], width);
-            v[n] = mine + other;
-          }
-        }
-        v[0] += __shfl_xor_sync(0xffffffffu, v[0], 8);
-        v[0] += __shfl_xor_sync(0xffffffffu, v[0], 16);
-        if (lane < 8) red_sum[(group * 4 + quarter) * RP + r0 + lane] = v[0];
-        if (quarter == 0) {
-#pragma unroll
-          for (int n = 0; n < 8; ++n)
-            if (lane == n) red_top[group * RP + r0 + n] = ref[r0 + n];
-        }
-      }
+      // ---- the output of this CTA's tiles of the item ----
+      if (quarter == 0 && lane < RP) red_top[group * RP + lane] = ref;
       if (j0 < tiles) wait(pvdone, (done - 1) & 1u, 411);
       failed = ptx::barrier_any(3, 2 * kGroupWarps * 32, failed);
       if (failed) break;
       ptx::tc_fence_after();
       // Lane r: what row r's two accumulators are multiplied by (RP <= 32).
       float factor_a = 0.0f, factor_b = 0.0f;
-      // A share that begins inside an item uses the CTA's first partial slot for it, one that ends
-      // inside the second.
-      float* part = a.partials +
-                    (int64_t)(2 * blockIdx.x + (seg.tile != 0 ? 0 : 1)) * C::kPartialFloats;
       if (lane < RP) {
         const float ta = red_top[lane], tb = red_top[RP + lane], most = fmaxf(ta, tb);
         // A reference is -inf where the row saw nothing (NaN scores leave it there too).
         factor_a = ta == most ? 1.0f : pow2_whole(ta - most);
         factor_b = tb == most ? 1.0f : pow2_whole(tb - most);
-        float l = 0.0f;
-#pragma unroll
-        for (int w = 0; w < 4; ++w)
-          l += red_sum[w * RP + lane] * factor_a + red_sum[(4 + w) * RP + lane] * factor_b;
-        if (seg.whole) {
-          const float scale = l == 0.0f ? 0.0f : 1.0f / l;
-          factor_a *= scale;
-          factor_b *= scale;
-        } else if (warp == 0) {
-          part[RP * D + 2 * lane] = most;
-          part[RP * D + 2 * lane + 1] = l;
-        }
       }
+      // A share that begins inside an item uses the CTA's first partial slot for it, one that ends
+      // inside the second.
+      float* part = a.partials +
+                    (int64_t)(2 * blockIdx.x + (seg.tile != 0 ? 0 : 1)) * C::kPartialFloats;
       const int rows = seg.rows;
       const bool whole = seg.whole != 0;
       // The groups share the output by halves of head_dim, or by eight rows.
@@ -825,24 +813,40 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       for (int unit = group; unit < C::kHalves * (RP / 8); unit += 2) {
         const int h = unit % C::kHalves, r0 = unit / C::kHalves * 8;
         if (r0 >= rows) continue;
-        float v[8];
+        float v[8], l[8];
 #pragma unroll
-        for (int n = 0; n < 8; ++n) v[n] = 0.0f;
+        for (int n = 0; n < 8; ++n) v[n] = l[n] = 0.0f;
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
           if (g == 1 && tiles < 2) break;  // only one group had a tile
           const int owner = (g ^ i0) & 1;  // group of the segment's tile g
-          uint32_t raw[TERMS][8];
+          uint32_t raw[TERMS][8], sums[TERMS][8];
 #pragma unroll
-          for (int k = 0; k < TERMS; ++k)
+          for (int k = 0; k < TERMS; ++k) {
             ptx::tmem_ld_x8(lane_t + C::kOCol + (owner * C::kHalves + h) * C::kN + k * RP + r0, raw[k]);
+            ptx::tmem_ld_x8(lane_t + C::kLCol + owner * C::kN + k * RP + r0, sums[k]);
+          }
           ptx::tmem_ld_wait();
 #pragma unroll
           for (int n = 0; n < 8; ++n) {
-            float x = __uint_as_float(raw[TERMS - 1][n]);
+            float x = __uint_as_float(raw[TERMS - 1][n]), y = __uint_as_float(sums[TERMS - 1][n]);
 #pragma unroll
-            for (int k = TERMS - 2; k >= 0; --k) x = x * 0.0625f + __uint_as_float(raw[k][n]);
-            v[n] += x * __shfl_sync(0xffffffffu, owner ? factor_b : factor_a, r0 + n);
+            for (int k = TERMS - 2; k >= 0; --k) {
+              x = x * 0.0625f + __uint_as_float(raw[k][n]);
+              y = y * 0.0625f + __uint_as_float(sums[k][n]);
+            }
+            const float f = __shfl_sync(0xffffffffu, owner ? factor_b : factor_a, r0 + n);
+            v[n] += x * f;
+            l[n] += y * f;
+          }
+        }
+        if (!whole && h == 0 && quarter == 0) {
+#pragma unroll
+          for (int n = 0; n < 8; ++n) {
+            if (lane != n) continue;
+            const int r = r0 + n;
+            part[RP * D + 2 * r] = fmaxf(red_top[r], red_top[RP + r]);
+            part[RP * D + 2 * r + 1] = l[n];
           }
         }
         const int d = h * 128 + token;
@@ -852,8 +856,9 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
           if (r < rows && d < D) {
             if (whole) {
               T* out = static_cast<T*>(a.out) + seg.out[r] + d;
-              if constexpr (TERMS == 2) *out = __float2bfloat16_rn(v[n]);
-              else *out = __float2half_rn(v[n]);
+              const float o = l[n] == 0.0f ? 0.0f : __fdividef(v[n], l[n]);
+              if constexpr (TERMS == 2) *out = __float2bfloat16_rn(o);
+              else *out = __float2half_rn(o);
             } else {
               part[r * D + d] = v[n];
             }
@@ -864,7 +869,7 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       i0 += tiles;
       // The accumulators, sums and the segment's description have been read.
       if (i0 < count && ptx::barrier_any(3, 2 * kGroupWarps * 32, false)) break;
-      if (lane == 0) ptx::mbar_arrive(qempty0 + 8 * (segment & 1));
+      if (lane == 0) ptx::mbar_arrive(qempty0 + 8 * (segment % kQueries));
     }
   }
 
