@@ -36,6 +36,7 @@ struct AttentionArgs {
   int causal;
   int max_rows;     // rows (tokens x group) a sequence may have to be this kernel's
   int vector;       // q rows can be read sixteen bytes at a time
+  int item_units;   // what a (sequence, head) costs beside its tiles, in tiles
   int whole_items;  // a (sequence, head) is not cut between CTAs
 };
 
