@@ -146,10 +146,10 @@ struct Cursor {
 };
 
 // The first tile at or behind unit `at`, by a full warp: returns its number in the list of all
-// tiles and, in all lanes, the place.  `whole`: items are not cut, the place is the first item that
+// tiles and, in all lanes, the place and the first unit of its item.  `whole`: items are not cut, the place is the first item that
 // begins at or behind `at`.
 __device__ __forceinline__ int64_t warp_locate(const AttentionArgs& a, int64_t at, bool whole,
-                                               int lane, Cursor* place) {
+                                               int lane, Cursor* place, int64_t* item_begin) {
   const int heads = a.cache.kv_heads;
   int64_t units = 0, tiles = 0;  // of all heads of the sequences before this group of 32
   place->b = a.batch.batch - 1;
@@ -177,6 +177,7 @@ __device__ __forceinline__ int64_t warp_locate(const AttentionArgs& a, int64_t a
       const int64_t first = units + __shfl_sync(0xffffffffu, upto, l) - per_item * heads;
       const int64_t into = at > first ? at - first : 0;
       place->b = b0 + l;
+      *item_begin = first + into / per_item * per_item;
       if (whole) {
         place->head = (int)((into + per_item - 1) / per_item);
       } else {
@@ -296,7 +297,9 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
     const int cta = (int)blockIdx.x + warp;
     Cursor c;
     int64_t tile = 0;
-    if ((int)blockIdx.x < s.ctas) tile = warp_locate(a, share_begin(s, cta), a.whole_items != 0, lane, &c);
+    int64_t begin;
+    if ((int)blockIdx.x < s.ctas)
+      tile = warp_locate(a, share_begin(s, cta), a.whole_items != 0, lane, &c, &begin);
     if (lane == 0) {
       share_smem[warp] = tile;
       if (warp == 0) *start = c;
@@ -891,8 +894,8 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   }
 }
 
-// Joins the partial rows of every (sequence, head) whose tiles went to more than one CTA, in the
-// order of the tiles.  One CTA per (sequence, head) and row.
+// Joins the partial rows of every item whose tiles went to more than one CTA, in the order of the
+// tiles.  One CTA per row and border between two shares; the first border inside an item has it.
 template <int D, int RP, int TERMS>
 __global__ void __launch_bounds__(kJoinThreads)
 kv_decode_join_kernel(const AttentionArgs a, int grid) {
@@ -900,48 +903,36 @@ kv_decode_join_kernel(const AttentionArgs a, int grid) {
   using T = typename std::conditional<TERMS == 2, __nv_bfloat16, __half>::type;
   constexpr int kColumns = D / 4;                     // four values a thread
   constexpr int kShares = kJoinThreads / kColumns;    // threads that share a column's parts
-  __shared__ int64_t sums[2 * kJoinThreads / 32];
+  __shared__ Cursor item;
+  __shared__ int item_parts;
   __shared__ float factor[kSms];
   __shared__ float4 acc[kJoinThreads];
-  const int b = blockIdx.x / a.cache.kv_heads, head = blockIdx.x % a.cache.kv_heads;
-  const int r = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
-  // Which CTAs had the item's tiles; the lengths are final before the main kernel starts.
-  const KvSequence seq = kv_sequence(a, b);
-  int64_t before = 0, total = 0;  // units of the sequences before b, of all
-  if (seq.tiles > 0 && r < seq.rows * a.group) {
-    for (int i = tid; i < a.batch.batch; i += kJoinThreads) {
-      const int units = units_of(a, kv_sequence(a, i).tiles);
-      total += units;
-      if (i < b) before += units;
+  const int c0 = (int)blockIdx.x, r = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
+  // The item in which the share of CTA c0 + 1 begins, if its first tile is CTA c0's.  The lengths
+  // are final before the main kernel starts.
+  if (tid < 32) {
+    const Share s = share_of(warp_total_units(a, lane) * a.cache.kv_heads, grid);
+    int parts = 1;
+    Cursor c;
+    if (c0 + 1 < s.ctas) {
+      int64_t begin = 0;
+      warp_locate(a, share_begin(s, c0 + 1), false, lane, &c, &begin);
+      c.load(a);
+      const int64_t u0 = begin + a.item_units, u1 = u0 + c.seq.tiles - 1;
+      // CTA of a unit: the last one whose share begins at or before it.
+      if (c.seq.tiles > 0 && (int)(((u0 + 1) * s.ctas - 1) / s.total) == c0)
+        parts = (int)(((u1 + 1) * s.ctas - 1) / s.total) - c0 + 1;
+    }
+    if (lane == 0) {
+      item = c;
+      item_parts = parts;
     }
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    before += __shfl_xor_sync(0xffffffffu, before, o);
-    total += __shfl_xor_sync(0xffffffffu, total, o);
-  }
-  if (lane == 0) {
-    sums[2 * (tid >> 5)] = before;
-    sums[2 * (tid >> 5) + 1] = total;
-  }
   __syncthreads();
-  before = total = 0;
-#pragma unroll
-  for (int w = 0; w < kJoinThreads / 32; ++w) {
-    before += sums[2 * w];
-    total += sums[2 * w + 1];
-  }
-  int parts = 1, c0 = 0;
-  if (total > 0) {
-    const Share s = share_of(total * a.cache.kv_heads, grid);
-    const int64_t u0 = before * a.cache.kv_heads + (int64_t)head * units_of(a, seq.tiles) + a.item_units;
-    const int64_t u1 = u0 + seq.tiles - 1;
-    // CTA of a unit: the last one whose share begins at or before it.
-    c0 = (int)(((u0 + 1) * s.ctas - 1) / s.total);
-    parts = (int)(((u1 + 1) * s.ctas - 1) / s.total) - c0 + 1;
-  }
+  const int parts = item_parts, head = item.head;
+  const KvSequence seq = item.seq;
   ptx::grid_dependency_wait();
-  if (parts == 1) return;  // one CTA had all of it and wrote the row, or there is no such row
+  if (parts == 1 || r >= seq.rows * a.group) return;
   // The first CTA began before this item or with it, the others inside it.
   const int64_t first = 2 * c0 + 1, later = 2 * c0;  // slot of part p: p == 0 ? first : later + 2 p
   auto part_of = [&](int p) {
@@ -1033,7 +1024,7 @@ int launch(const CUtensorMap& tm_k, const CUtensorMap& tm_v, const AttentionArgs
   config.numAttrs = use_pdl() ? 1 : 0;
   MX_CUDA(cudaLaunchKernelEx(&config, kv_decode_kernel<D, RP, TERMS>, tm_k, tm_v, a));
   if (a.whole_items != 0 || grid == 1) return kOk;  // nothing was cut
-  config.gridDim = dim3((unsigned)(a.batch.batch * a.cache.kv_heads), (unsigned)a.max_rows);
+  config.gridDim = dim3((unsigned)(grid - 1), (unsigned)a.max_rows);
   config.blockDim = dim3(kJoinThreads);
   config.dynamicSmemBytes = 0;
   MX_CUDA(cudaLaunchKernelEx(&config, kv_decode_join_kernel<D, RP, TERMS>, a, grid));
