@@ -13,8 +13,8 @@
 //    With at most 96 columns an MMA costs what its 128-row operand costs (about 33 ns).
 //  * Warps: 0-3 and 4-7 softmax (one lane per token; the two groups take alternate tiles, each
 //    with its own running maximum and output accumulator, because one group needs about as long
-//    for a tile as HBM does), 8 TMA, 9 MMA, 10-11 quantise queries.  The scores of tile j + 2 are
-//    issued as soon as those of tile j have been read, before the output of tile j.
+//    for a tile as HBM does), 8 TMA, 9 MMAs of the scores (two tiles ahead), 10 MMAs of the
+//    outputs, 11 quantises queries and describes the segments.
 //  * The list of (sequence, key head, tile of 128 tokens) is cut into equal shares, one per CTA
 //    (one per SM), whatever the lengths are: the cut follows the lengths on the device.  A CTA
 //    whose share covers all tiles of a (sequence, head) writes its rows; otherwise it leaves
@@ -39,9 +39,9 @@ int* device_status_word(int device);
 
 namespace {
 
-constexpr int kThreads = 384;
+constexpr int kThreads = 416;
 constexpr int kGroupWarps = 4;  // warps of a softmax group, one per 32 lanes of tensor memory
-constexpr int kTmaWarp = 8, kMmaWarp = 9, kQueryWarp = 10, kQueryWarps = 2;
+constexpr int kTmaWarp = 8, kScoreWarp = 9, kOutputWarp = 10, kQueryWarp = 11, kQueryWarps = 2;
 // Query buffers.  Scores run two tiles ahead of the outputs, so a tile of one segment may be
 // waiting for its output while the scores of the second segment behind it are due.
 constexpr int kQueries = 3;
@@ -283,7 +283,7 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   for (int i = threadIdx.x; i < 512; i += kThreads)
     reinterpret_cast<uint32_t*>(one_values)[i] = 0x38383838u;
   ptx::fence_proxy_async();
-  if (warp == kMmaWarp) {
+  if (warp == kScoreWarp) {
     ptx::tmem_alloc(ptx::smem_u32(tmem_slot), C::kTmemCols);
     ptx::tmem_relinquish();
   }
@@ -311,6 +311,8 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   const uint32_t tmem = *tmem_slot;
   const int count = (int)(share_smem[1] - share_smem[0]);  // tiles of this CTA
   const int per_page = a.cache.page_size / kKvBlock;
+  // E4M3 x E4M3, UE8M0 scales, M = 128, N = kN; K-major unless bit 15 says otherwise for A.
+  constexpr uint32_t kIdesc = ((uint32_t)(C::kN >> 3) << 17) | (1u << 23) | ((128u >> 4) << 24);
 
   if (count > 0 && warp == kTmaWarp) {
     // ---------------- TMA producer ----------------
@@ -407,30 +409,35 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       copy(true, before ? last_page : page, before ? last_v : v_sf, 4 * ((count - 2) & 7));
     }
     copy(true, page, v_sf, 4 * ((count - 1) & 7));
-  } else if (count > 0 && warp == kMmaWarp) {
-    // ---------------- MMA issuer ----------------
-    constexpr uint32_t kIdesc = ((uint32_t)(C::kN >> 3) << 17) | (1u << 23) | ((128u >> 4) << 24);
+  } else if (count > 0 && warp == kScoreWarp) {
+    // ---------------- scores ----------------
+    // Two warps issue MMAs: with one, the scores of a tile waited behind the outputs of the tile
+    // before it, whose weights are not there yet.
     const uint32_t sf0 = tmem + C::kSfCol;  // keys, values, weights by tile parity, then ones
     const uint32_t ones_t = sf0 + 24;
     if (ptx::elect_one()) ptx::tc_cp_32x128b_warpx4(ones_t, ptx::smem_desc_scale_atom(ptx::smem_u32(ones)));
     __syncwarp();
-    int segment = 0, in_segment = 0, of_segment = 0;  // of the next scores: segment, tile, tiles
-    uint32_t fresh = 0;  // bit i % 32: tile i is one of the first two of its segment
     bool ok = true;
-    auto scores = [&](int i) {
+    int left = 0;  // tiles of the segment that are still to come
+    for (int i = 0, segment = -1; ok && i < count; ++i) {
+      if (left == 0) {
+        ++segment;
+        ok = __all_sync(0xffffffffu, bounded_wait(qfull0 + 8 * (segment % kQueries),
+                                                  (uint32_t)(segment / kQueries) & 1u, abort_flag,
+                                                  a.status, 402));
+        left = segments[segment % kQueries].tiles;
+      }
+      --left;
       const int at = slot_of_k(i);
       const int slot = at % C::kSlots;
-      if (in_segment == 0) {
-        ok = ok && __all_sync(0xffffffffu, bounded_wait(qfull0 + 8 * (segment % kQueries),
-                                                        (uint32_t)(segment / kQueries) & 1u,
-                                                        abort_flag, a.status, 402));
-        of_segment = segments[segment % kQueries].tiles;
-      }
-      const bool last = in_segment + 1 == of_segment;
+      // The score tile of two tiles ago has been read.
+      if (i >= 2)
+        ok = ok && __all_sync(0xffffffffu, bounded_wait(sread0 + 8 * (i & 1), (uint32_t)((i - 2) >> 1) & 1u,
+                                                        abort_flag, a.status, 415));
       ok = ok && __all_sync(0xffffffffu,
                             bounded_wait(full0 + 8 * slot, (uint32_t)(at / C::kSlots) & 1u,
                                          abort_flag, a.status, 403));
-      if (!ok) return;
+      if (!ok) break;
       ptx::tc_fence_after();
       if (ptx::elect_one()) {
         const uint32_t sf_t = sf0 + 12 * (i & 1);
@@ -448,26 +455,17 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         }
         ptx::tc_commit(sfull0 + 8 * (i & 1));
         ptx::tc_commit(empty0 + 8 * slot);
-        if (last) ptx::tc_commit(qempty0 + 8 * (segment % kQueries));
+        if (left == 0) ptx::tc_commit(qempty0 + 8 * (segment % kQueries));
       }
       __syncwarp();
-      fresh = (fresh & ~(1u << (i & 31))) | (uint32_t)(in_segment < 2) << (i & 31);
-      ++in_segment;
-      if (last) {
-        ++segment;
-        in_segment = 0;
-      }
-    };
-    scores(0);
-    if (count > 1) scores(1);
-    for (int i = 0; ok && i < count; ++i) {
-      // Scores of tile i + 2 as soon as those of tile i have been read.
-      if (i + 2 < count) {
-        ok = __all_sync(0xffffffffu, bounded_wait(sread0 + 8 * (i & 1), (uint32_t)(i >> 1) & 1u,
-                                                  abort_flag, a.status, 415));
-        if (!ok) break;
-        scores(i + 2);
-      }
+    }
+  } else if (count > 0 && warp == kOutputWarp) {
+    // ---------------- outputs and sums ----------------
+    const uint32_t sf0 = tmem + C::kSfCol;
+    const uint32_t ones_t = sf0 + 24;  // written before the first scores, which the weights follow
+    bool ok = true;
+    int left = 0, number = 0;  // tiles of the segment that are still to come, that were
+    for (int i = 0, segment = -1; i < count; ++i) {
       const int at = slot_of_v(i, count);
       const int slot = at % C::kSlots;
       ok = ok && __all_sync(0xffffffffu, bounded_wait(pfull0 + 8 * (i & 1), (uint32_t)(i >> 1) & 1u,
@@ -476,6 +474,11 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
                             bounded_wait(full0 + 8 * slot, (uint32_t)(at / C::kSlots) & 1u,
                                          abort_flag, a.status, 405));
       if (!ok) break;
+      if (left == 0) {
+        ++segment;
+        left = segments[segment % kQueries].tiles;
+        number = 0;
+      }
       ptx::tc_fence_after();
       if (ptx::elect_one()) {
         const uint32_t sf_t = sf0 + 12 * (i & 1) + 4, weight_t = sf_t + 4;
@@ -484,15 +487,7 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         const uint32_t v_s = ptx::smem_u32(slots + slot * C::kSlotBytes);
         const uint64_t bd =
             ptx::smem_desc(ptx::smem_u32(p_tiles + (i & 1) * C::kPBytes), 0, 1024, ptx::kSwizzle128);
-        const bool first = (fresh >> (i & 31) & 1u) != 0;  // of its group in the segment
-        // Sums of the weights as they were rounded and scaled, so that they add up to one: a
-        // product with ones (eight rows of shared memory serve all 128).
-        const uint64_t ones_d = ptx::smem_desc(ptx::smem_u32(one_values), 0, 0, ptx::kSwizzle128);
-#pragma unroll
-        for (int ks = 0; ks < kKvTileBlocks; ++ks)
-          ptx::tc_mma_mxf8f6f4(tmem + C::kLCol + (i & 1) * C::kN, ones_d, bd + 2 * ks,
-                               kIdesc | ((uint32_t)ks << 4), ones_t, weight_t,
-                               (!first || ks > 0) ? 1u : 0u);
+        const bool first = number < 2;  // of its group in the segment
 #pragma unroll
         for (int h = 0; h < C::kHalves; ++h) {
           // V^T: 128 values of head_dim along M (MN-major), 32 tokens per step.  With a head of
@@ -506,10 +501,20 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
                                  weight_t, (!first || ks > 0) ? 1u : 0u);
           }
         }
+        // Sums of the weights as they were rounded and scaled, so that they add up to one: a
+        // product with ones (eight rows of shared memory serve all 128).
+        const uint64_t ones_d = ptx::smem_desc(ptx::smem_u32(one_values), 0, 0, ptx::kSwizzle128);
+#pragma unroll
+        for (int ks = 0; ks < kKvTileBlocks; ++ks)
+          ptx::tc_mma_mxf8f6f4(tmem + C::kLCol + (i & 1) * C::kN, ones_d, bd + 2 * ks,
+                               kIdesc | ((uint32_t)ks << 4), ones_t, weight_t,
+                               (!first || ks > 0) ? 1u : 0u);
         ptx::tc_commit(pvdone0 + 8 * (i & 1));
         ptx::tc_commit(empty0 + 8 * slot);
       }
       __syncwarp();
+      --left;
+      ++number;
     }
   } else if (count > 0 && warp >= kQueryWarp) {
     // ---------------- query terms ----------------
@@ -526,12 +531,13 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       uint8_t* q_s = q_tiles + buffer * C::kQBytes;
       const int rows = c.seq.rows * a.group;
       const int tiles = min(left, c.seq.tiles - c.tile);
+      // Lane r: where row r is read (padding rows: row 0, unused) and where it goes.
+      const int own = lane < rows ? lane : 0;
+      const int64_t own_token = c.seq.row + own / a.group;
+      const int64_t own_head = c.head * a.group + own % a.group;
+      const int64_t own_q = own_token * a.q_token_stride + own_head * a.q_head_stride;
       if (warp == kQueryWarp) {
-        if (lane < RP) {
-          const int r = lane < rows ? lane : 0;
-          seg.out[lane] = (c.seq.row + r / a.group) * a.out_token_stride +
-                          (int64_t)(c.head * a.group + r % a.group) * a.out_head_stride;
-        }
+        if (lane < RP) seg.out[lane] = own_token * a.out_token_stride + own_head * a.out_head_stride;
         if (lane == 0) {
           seg.first_position = c.seq.last - c.seq.rows + 1;
           seg.length = c.seq.length;
@@ -542,15 +548,14 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         }
       }
       constexpr int kPer = D / 32;   // values per lane
-      constexpr int kBatch = RP / kQueryWarps < 4 ? RP / kQueryWarps : 4;  // rows in flight
+      constexpr int kBatch = 4;      // rows in flight
 #pragma unroll 1
-      for (int r0 = warp - kQueryWarp; r0 < RP; r0 += kQueryWarps * kBatch) {
+      for (int r0 = warp - kQueryWarp; r0 < RP; r0 += kBatch * kQueryWarps) {
         __align__(16) uint16_t raw[kBatch][kPer];
 #pragma unroll
         for (int n = 0; n < kBatch; ++n) {
           const int r = r0 + n * kQueryWarps;
-          const T* src = static_cast<const T*>(a.q) + (c.seq.row + r / a.group) * a.q_token_stride +
-                         (int64_t)(c.head * a.group + r % a.group) * a.q_head_stride + lane * kPer;
+          const T* src = static_cast<const T*>(a.q) + __shfl_sync(0xffffffffu, own_q, r) + lane * kPer;
           if (r < rows) {
             if (a.vector && kPer == 8) {
               *reinterpret_cast<uint4*>(raw[n]) = *reinterpret_cast<const uint4*>(src);
@@ -631,7 +636,11 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
     const uint32_t sfull = sfull0 + 8 * group, pfull = pfull0 + 8 * group;
     const uint32_t pvdone = pvdone0 + 8 * group, vsync = vsync0 + 8 * group;
     const uint32_t sread = sread0 + 8 * group;
-    uint8_t* p_s = p_tiles + group * C::kPBytes + (token & 15);
+    // Weights are stored four tokens at a time: the lane's are tokens lane & ~3 .. | 3 of row
+    // lane % 4 of every four.
+    uint8_t* p_s = p_tiles + group * C::kPBytes + (lane & 3) * 128 + (token & 12);
+    const uint32_t p_chunk = (token & 0x70) ^ ((lane & 3) << 4);
+    const uint32_t turn1 = lane & 1 ? 0x3715 : 0x6240, turn2 = lane & 2 ? 0x3276 : 0x5410;
     float* my_max = red_max + group * 4 * RP;
     bool failed = false;
     uint32_t done = 0;     // tiles this group has taken
@@ -708,24 +717,26 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
           // PV of this group's last tile has read the weights that this tile's replace.
           if (c0 == 0 && done > 0) wait(pvdone, (done - 1) & 1u, 410);
 #pragma unroll
-          for (int r = 0; r < C::kChunk; r += 2) {
-            float p[2];
+          for (int r = 0; r < C::kChunk; r += 4) {
+            float p[4];
 #pragma unroll
-            for (int n = 0; n < 2; ++n) {
+            for (int n = 0; n < 4; ++n) {
               // To the nearest power of two: the largest weight is in (181, 363).
               const float top = rintf(ptx::warp_max(s[r + n]));
               if (lane % RP == c0 + r + n) my_top = top;
               p[n] = ptx::exp2_approx(s[r + n] - (fmaxf(top, -1e30f) - kWeightLog2));
             }
-            uint32_t codes[TERMS];
-            e4m3_terms_half<TERMS>(__floats2half2_rn(p[0], p[1]), codes);
+            uint32_t lo[TERMS], hi[TERMS];
+            e4m3_terms_half<TERMS>(__floats2half2_rn(p[0], p[1]), lo);
+            e4m3_terms_half<TERMS>(__floats2half2_rn(p[2], p[3]), hi);
 #pragma unroll
             for (int k = 0; k < TERMS; ++k) {
-#pragma unroll
-              for (int n = 0; n < 2; ++n) {
-                const int col = k * RP + c0 + r + n;
-                p_s[col * 128 + ((token & 0x70) ^ ((col & 7) << 4))] = (uint8_t)(codes[k] >> (8 * n));
-              }
+              // This token's bytes of four rows become four tokens' bytes of row lane % 4.
+              uint32_t w = __byte_perm(lo[k], hi[k], 0x5410);
+              w = __byte_perm(w, __shfl_xor_sync(0xffffffffu, w, 1), turn1);
+              w = __byte_perm(w, __shfl_xor_sync(0xffffffffu, w, 2), turn2);
+              const int col = k * RP + c0 + r;  // a multiple of four; the lane's is col + lane % 4
+              *reinterpret_cast<uint32_t*>(p_s + col * 128 + (p_chunk ^ ((col & 7) << 4))) = w;
             }
           }
         }
@@ -888,7 +899,7 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
     // and tensor memory are handed back.
     for (int i = 0; i < 200; ++i) __nanosleep(1000);
   }
-  if (warp == kMmaWarp) {
+  if (warp == kScoreWarp) {
     ptx::tc_fence_after();
     ptx::tmem_dealloc(tmem, C::kTmemCols);
   }
