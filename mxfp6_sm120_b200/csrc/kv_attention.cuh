@@ -34,8 +34,10 @@ struct AttentionArgs {
   int group;        // query heads per key head
   float scale_log2; // softmax scale * log2(e)
   int causal;
-  int max_rows;     // rows (tokens x group) a sequence may have to be this kernel's
+  int max_rows;     // rows (tokens x group) a sequence may have to be the decode kernel's
+  int min_rows;     // and has more of to be the prefill kernel's
   int vector;       // q rows can be read sixteen bytes at a time
+  int vector_out;   // and output rows written so
   int item_units;   // what a (sequence, head) costs beside its tiles, in tiles
   int whole_items;  // a (sequence, head) is not cut between CTAs
 };

@@ -1,0 +1,1032 @@
+// Attention of many new rows per sequence over the paged 8-bit cache (prompts, prompt chunks).
+//
+// S = Q K^T and O = P V on 128 rows (new tokens x query heads of a key head, flattened) by 128
+// cached tokens.  K and V are read by tcgen05.mma as they lie in the pages (TMA tiles, block
+// scales in hardware, V as an MN-major operand); Q and P are E4M3 terms (kv_attention.cuh): a
+// product is two passes (BF16; three for FP16) at the 8-bit rate, so the tensor cores bound it at
+// what they give 16-bit operands, with half the bytes per cached token and no conversion of a
+// cached value anywhere.
+//
+//  * The terms of a product accumulate into the same tensor memory: their factors 1, 1/16, 1/256
+//    are block scales of the A operand.
+//  * Online softmax as in the decode kernel: a row's weights are taken relative to the largest
+//    score of each block of 32 tokens, rounded to a power of two, and that power relative to the
+//    row's reference is the block scale of P.  No maximum crosses threads and the output is not
+//    rescaled, except where a block exceeds the reference by more than 2^16.
+//  * Warps: 0-7 softmax (a thread holds 64 scores of one row, two scale blocks), 8 TMA, 9 MMA,
+//    10-13 turn the next rows into E4M3 terms as soon as the last scores of the rows before are
+//    out.  Scores of tile j + 1 are issued before the output of tile j.
+//  * Work: the list of (sequence, row tile, key head) with its tiles of cached tokens is cut into
+//    equal shares, one per SM; an item that is cut leaves partial rows, which a second kernel
+//    joins in the order of the tiles.
+#include "kv_attention.cuh"
+
+#include <cstdlib>
+
+namespace mx {
+namespace {
+
+constexpr int kThreads = 448;
+constexpr int kSoftmaxWarps = 8;
+constexpr int kTmaWarp = 8, kMmaWarp = 9, kQueryWarp = 10, kQueryWarps = 4;
+constexpr int kRows = 128;            // rows of an item
+constexpr float kWeightLog2 = 8.0f;   // weights are scaled by 256 before they become E4M3 terms
+constexpr float kMostLog2 = 16.0f;    // a block may exceed the reference by 2^16
+constexpr int kSms = 148;
+constexpr int kItemUnits = 2;         // what an item costs beside its tiles
+constexpr int kMinUnits = 4;          // units a CTA takes at least
+
+template <int D, int TERMS>
+struct PrefillCfg {
+  static constexpr int kRowBytes = D < 128 ? D : 128;
+  static constexpr int kSubs = D / kRowBytes;
+  static constexpr int kSubBytes = kKvTile * kRowBytes;  // also of a Q sub-tile: 128 rows
+  static constexpr int kSlotBytes = kKvTile * D;
+  static constexpr int kQBytes = TERMS * kRows * D;
+  static constexpr int kPBytes = TERMS * kRows * kKvTile;
+  // A head of 256 leaves room for one score tile in tensor memory and one P in shared memory.
+  static constexpr int kBuffers = D == 256 ? 1 : 2;
+  static constexpr int kFixedBytes = 10240;
+  static constexpr int kBudget = 227 * 1024 - 1024;
+  static constexpr int kFit = (kBudget - kFixedBytes - kQBytes - kBuffers * kPBytes) / (kSlotBytes + 512);
+  static constexpr int kSlots = kFit > 8 ? 8 : kFit;
+  static_assert(kSlots >= 2, "a K and a V tile");
+  static constexpr int kSmemBytes =
+      1024 + kSlots * (kSlotBytes + 512) + kQBytes + kBuffers * kPBytes + kFixedBytes;
+  static constexpr int kOCol = kBuffers * kKvTile;
+  static constexpr int kSfCol = kOCol + D;
+  // Scales: constants per term; per buffer (what an MMA may still read is not overwritten) keys,
+  // values (8 for 256 rows of B), weights per term.
+  static constexpr int kSfTerm = kSfCol, kSfSets = kSfTerm + 4 * TERMS;
+  static constexpr int kSfV = 4, kSfP = 12, kSfSet = 12 + 4 * TERMS;
+  static_assert(kSfSets + kBuffers * kSfSet <= 512, "tensor memory");
+  static constexpr uint64_t kSwizzle = kRowBytes == 128 ? ptx::kSwizzle128 : ptx::kSwizzle64;
+  static constexpr int kGroup = 8 * kRowBytes;
+  static constexpr int kPartialFloats = kRows * D + 2 * kRows;
+};
+
+struct Share {
+  int64_t total;
+  int ctas;
+};
+__device__ __forceinline__ int64_t share_begin(const Share& s, int cta) {
+  return s.total * cta / s.ctas;
+}
+__device__ __forceinline__ Share share_of(int64_t total, int grid) {
+  Share s;
+  s.total = total;
+  const int64_t want = (total + kMinUnits - 1) / kMinUnits;
+  s.ctas = (int)(want < grid ? (want < 1 ? 1 : want) : grid);
+  return s;
+}
+
+// A sequence: rows of q are new tokens x group, in tiles of 128.
+struct Sequence {
+  int64_t row;             // first token row
+  int64_t first_position;  // of its first new token
+  int rows;                // new tokens x group
+  int length;              // cached tokens
+};
+__device__ __forceinline__ Sequence load_sequence(const AttentionArgs& a, int b) {
+  const KvSpan s = kv_span(a.batch, a.cache.page_size, b);
+  Sequence q;
+  q.row = s.row;
+  q.first_position = (int64_t)a.batch.seq_lens[b] - s.rows;
+  const int64_t rows = (int64_t)s.rows * a.group;
+  q.rows = rows > a.min_rows ? (int)rows : 0;  // shorter ones are the decode kernel's
+  q.length = s.length;
+  return q;
+}
+// Tiles of cached tokens that row tile t sees (one even if it sees none: it writes zeros).
+__device__ __forceinline__ int tiles_of(const AttentionArgs& a, const Sequence& q, int t) {
+  int64_t see = q.length;
+  if (a.causal) {
+    const int last = min(q.rows - 1, kRows * t + kRows - 1) / a.group;
+    const int64_t upto = q.first_position + last + 1;
+    see = upto < see ? upto : see;
+  }
+  return see <= 0 ? 1 : (int)((see + kKvTile - 1) / kKvTile);
+}
+
+// An item and a tile of it.
+struct Place {
+  int b, t, head, tile;
+};
+
+// Walks the items in the order sequence, row tile, head.  Returns the units of all items when
+// `at` is negative; else the number of the first tile at or behind unit `at`, its place and the
+// first unit of its item.  By a full warp.
+__device__ __forceinline__ int64_t warp_walk(const AttentionArgs& a, int64_t at, int lane,
+                                             Place* place, int64_t* item_begin) {
+  int64_t units = 0, tiles = 0;
+  const int heads = a.cache.kv_heads;
+  for (int b0 = 0; b0 < a.batch.batch; b0 += 32) {
+    Sequence mine{};
+    if (b0 + lane < a.batch.batch) mine = load_sequence(a, b0 + lane);
+    unsigned todo = __ballot_sync(0xffffffffu, mine.rows > 0);
+    while (todo != 0) {
+      const int l = __ffs(todo) - 1;
+      todo &= todo - 1;
+      Sequence q;
+      q.row = 0;
+      q.first_position = __shfl_sync(0xffffffffu, mine.first_position, l);
+      q.rows = __shfl_sync(0xffffffffu, mine.rows, l);
+      q.length = __shfl_sync(0xffffffffu, mine.length, l);
+      const int row_tiles = (q.rows + kRows - 1) / kRows;
+      for (int t0 = 0; t0 < row_tiles; t0 += 32) {
+        const int t = t0 + lane;
+        const int n = t < row_tiles ? tiles_of(a, q, t) : 0;
+        int64_t upto = n > 0 ? (int64_t)(n + kItemUnits) * heads : 0, tiles_upto = (int64_t)n * heads;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int64_t u = __shfl_up_sync(0xffffffffu, upto, o);
+          const int64_t v = __shfl_up_sync(0xffffffffu, tiles_upto, o);
+          if (lane >= o) {
+            upto += u;
+            tiles_upto += v;
+          }
+        }
+        const unsigned reached = __ballot_sync(0xffffffffu, at >= 0 && n > 0 && units + upto > at);
+        if (reached != 0) {
+          const int k = __ffs(reached) - 1;
+          const int count = __shfl_sync(0xffffffffu, n, k);
+          const int64_t per_item = count + kItemUnits;
+          const int64_t first = units + __shfl_sync(0xffffffffu, upto, k) - per_item * heads;
+          const int64_t into = at > first ? at - first : 0;
+          place->b = b0 + l;
+          place->t = t0 + k;
+          place->head = (int)(into / per_item);
+          const int64_t in_item = into % per_item - kItemUnits;
+          place->tile = in_item > 0 ? (int)in_item : 0;
+          *item_begin = first + into / per_item * per_item;
+          return tiles + __shfl_sync(0xffffffffu, tiles_upto, k) - (int64_t)count * heads +
+                 (int64_t)place->head * count + place->tile;
+        }
+        units += __shfl_sync(0xffffffffu, upto, 31);
+        tiles += __shfl_sync(0xffffffffu, tiles_upto, 31);
+      }
+    }
+  }
+  return at < 0 ? units : tiles;
+}
+
+// A place with its sequence, stepped from item to item.
+struct Cursor {
+  Place at;
+  Sequence seq;
+  int tiles;  // of the item
+  __device__ __forceinline__ void load(const AttentionArgs& a) {
+    seq = load_sequence(a, at.b);
+    tiles = tiles_of(a, seq, at.t);
+  }
+  __device__ __forceinline__ void next_item(const AttentionArgs& a) {
+    at.tile = 0;
+    if (++at.head < a.cache.kv_heads) return;
+    at.head = 0;
+    if (kRows * ++at.t < seq.rows) {
+      tiles = tiles_of(a, seq, at.t);
+      return;
+    }
+    at.t = 0;
+    do {
+      if (++at.b >= a.batch.batch) {
+        at.b = a.batch.batch - 1;
+        break;
+      }
+      seq = load_sequence(a, at.b);
+    } while (seq.rows == 0);
+    tiles = tiles_of(a, seq, 0);
+  }
+};
+
+// The tiles of one item that a CTA takes.
+struct Segment {
+  float scale[kRows];      // of the quantised rows, times the softmax scale and log2(e)
+  int64_t row;             // first token row of the sequence
+  int64_t first_position;  // of the sequence's first new token
+  int rows;                // rows of the sequence
+  int row0;                // first row of the item
+  int length;
+  int head;
+  int tile;
+  int tiles;
+  int whole;
+  int b;
+  int all_named;           // every page of its tiles is in the block table
+};
+
+template <int D, int TERMS>
+__global__ void __launch_bounds__(kThreads, 1)
+kv_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                  const AttentionArgs a) {
+  using C = PrefillCfg<D, TERMS>;
+  using T = typename std::conditional<TERMS == 2, __nv_bfloat16, __half>::type;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* slots = smem;
+  uint8_t* q_tiles = slots + C::kSlots * C::kSlotBytes;  // [term][sub][row][row bytes]
+  uint8_t* p_tiles = q_tiles + C::kQBytes;               // [buffer][term][row][128 tokens]
+  uint8_t* sf_tiles = p_tiles + C::kBuffers * C::kPBytes;
+  uint8_t* fixed = sf_tiles + C::kSlots * 512;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(fixed);
+  uint8_t* term_sf = fixed + 512;                        // [term] atoms of 1, 1/16, 1/256
+  uint8_t* p_sf = term_sf + 3 * 512;                     // [buffer][term]
+  Segment* segments = reinterpret_cast<Segment*>(p_sf + 6 * 512);  // two
+  float* row_sum = reinterpret_cast<float*>(segments + 2);         // [half][row]
+  float* row_top = row_sum + 2 * kRows;                            // [half][row]
+  Cursor* start = reinterpret_cast<Cursor*>(row_top + 2 * kRows);
+  int64_t* share_smem = reinterpret_cast<int64_t*>(start + 1);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(share_smem + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* ask_flag = abort_flag + 1;               // [quarter][2]
+  static_assert(512 + 9 * 512 + 2 * sizeof(Segment) + 4 * kRows * 4 + sizeof(Cursor) + 16 + 8 + 32 <=
+                    C::kFixedBytes,
+                "fixed area");
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t full0 = ptx::smem_u32(bars);
+  const uint32_t empty0 = full0 + 8 * C::kSlots;
+  const uint32_t sfull0 = empty0 + 8 * C::kSlots;
+  const uint32_t sread0 = sfull0 + 16;
+  const uint32_t pfull0 = sread0 + 16;
+  const uint32_t pvdone0 = pfull0 + 16;
+  const uint32_t sdone0 = pvdone0 + 16;  // softmax has left a segment (by its parity)
+  const uint32_t qfull = sdone0 + 16, qfree = qfull + 8;
+  const uint32_t vsync0 = qfree + 8;     // four: the two warps of a lane quarter
+  static_assert(8 * (2 * 8 + 10 + 2 + 4) <= 512, "barriers");
+
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    for (int i = 0; i < 8; ++i) ask_flag[i] = 0;
+    for (int s = 0; s < C::kSlots; ++s) {
+      ptx::mbar_init(full0 + 8 * s, 2);  // the copies' bytes, and the scales
+      ptx::mbar_init(empty0 + 8 * s, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      ptx::mbar_init(sfull0 + 8 * i, 1);
+      ptx::mbar_init(sread0 + 8 * i, kSoftmaxWarps);
+      ptx::mbar_init(pfull0 + 8 * i, kSoftmaxWarps);
+      ptx::mbar_init(pvdone0 + 8 * i, 1);
+      ptx::mbar_init(sdone0 + 8 * i, kSoftmaxWarps);
+    }
+    ptx::mbar_init(qfull, kQueryWarps);
+    ptx::mbar_init(qfree, 1);
+    for (int i = 0; i < 4; ++i) ptx::mbar_init(vsync0 + 8 * i, 2);
+    ptx::fence_mbar_init();
+    ptx::prefetch_tensormap(&tm_k);
+    ptx::prefetch_tensormap(&tm_v);
+  }
+  if (threadIdx.x < 3 * 128)
+    reinterpret_cast<uint32_t*>(term_sf)[threadIdx.x] =
+        threadIdx.x < 128 ? 0x7f7f7f7fu : threadIdx.x < 256 ? 0x7b7b7b7bu : 0x77777777u;
+  ptx::fence_proxy_async();
+  if (warp == kMmaWarp) {
+    ptx::tmem_alloc(ptx::smem_u32(tmem_slot), 512);
+    ptx::tmem_relinquish();
+  }
+  ptx::grid_dependency_wait();
+  // From here on everything before this kernel has completed, also for the joining kernel, which
+  // reads the same lengths before it waits for this one.
+  ptx::grid_launch_dependents();
+  if (warp < 2) {
+    // Warp 0 finds the first tile of this CTA, warp 1 the first of the next.
+    Place p{};
+    int64_t begin;
+    const Share s = share_of(warp_walk(a, -1, lane, &p, &begin), (int)gridDim.x);
+    const int cta = (int)blockIdx.x + warp;
+    int64_t tile = 0;
+    if ((int)blockIdx.x < s.ctas && s.total > 0) tile = warp_walk(a, share_begin(s, cta), lane, &p, &begin);
+    if (lane == 0) {
+      share_smem[warp] = tile;
+      if (warp == 0) start->at = p;
+    }
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int count = (int)(share_smem[1] - share_smem[0]);  // tiles of this CTA
+  const int per_page = a.cache.page_size / kKvBlock;
+
+  if (count > 0 && warp == kTmaWarp) {
+    // ---------------- TMA producer: K0, K1, V0, K2, V1, ... per segment ----------------
+    Cursor c = *start;
+    c.load(a);
+    int slot = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    const bool leads = (lane & 3) % per_page == 0;  // first block of a page in its tile
+    const uint32_t page_bytes = (uint32_t)(a.cache.page_size * D);
+    const uint32_t slots_s = ptx::smem_u32(slots) + (lane & 3) * kKvBlock * C::kRowBytes;
+    auto copy = [&](bool is_v, int64_t lane_page, uint32_t lane_sf, int src) {
+      ok = ok && __all_sync(0xffffffffu, bounded_wait(empty0 + 8 * slot, phase ^ 1u, abort_flag,
+                                                      a.status, 501));
+      if (!ok) return;
+      const uint32_t bar = full0 + 8 * slot;
+      const bool issue = (lane & ~3) == src && leads && lane_page >= 0;
+      const uint32_t pages = __popc(__ballot_sync(0xffffffffu, issue));
+      if (lane == src) ptx::mbar_arrive_expect_tx(bar, pages * page_bytes);
+      __syncwarp();
+      if (issue) {
+#pragma unroll
+        for (int s = 0; s < C::kSubs; ++s)
+          ptx::tma_load_2d(slots_s + slot * C::kSlotBytes + s * C::kSubBytes, is_v ? &tm_v : &tm_k,
+                           s * 128, (int)(lane_page * kKvBlock), bar);
+      }
+      // Scale atom: lane = row % 32.  Keys: 32 tokens are a word of rows; values: every row has
+      // the factors of the four 32-token steps along K.
+      uint32_t sf[kKvTileBlocks];
+#pragma unroll
+      for (int i = 0; i < kKvTileBlocks; ++i) sf[i] = __shfl_sync(0xffffffffu, lane_sf, src + i);
+      const uint32_t all = sf[0] | sf[1] << 8 | sf[2] << 16 | sf[3] << 24;
+      reinterpret_cast<uint4*>(sf_tiles + slot * 512)[lane] =
+          is_v ? make_uint4(all, all, all, all)
+               : make_uint4(sf[0] * 0x01010101u, sf[1] * 0x01010101u, sf[2] * 0x01010101u,
+                            sf[3] * 0x01010101u);
+      ptx::fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(bar);
+      if (++slot == C::kSlots) {
+        slot = 0;
+        phase ^= 1u;
+      }
+    };
+    for (int left = count; ok && left > 0;) {
+      const int tiles = min(left, c.tiles - c.at.tile);
+      // Lane l looks up block l % 4 of tile l / 4 of a group of eight tiles.
+      auto lookup_page = [&](int j) -> int64_t {
+        const int block = (c.at.tile + j + (lane >> 2)) * kKvTileBlocks + (lane & 3);
+        if (j + (lane >> 2) >= tiles || block * kKvBlock >= c.seq.length) return -1;
+        const int64_t p = kv_page(a.batch, a.cache, c.at.b, block);
+        return p < 0 ? -1 : (p * a.cache.kv_heads + c.at.head) * per_page + block % per_page;
+      };
+      int64_t page = lookup_page(0), next_page = -1, last_page = -1;
+      uint32_t k_sf = 127, v_sf = 127, next_k = 127, next_v = 127, last_v = 127;
+      if (page >= 0) {
+        k_sf = a.cache.k_scales[page];
+        v_sf = a.cache.v_scales[page];
+      }
+      for (int j0 = 0; ok && j0 < tiles; j0 += 8) {
+        if (j0 + 8 < tiles) next_page = lookup_page(j0 + 8);
+        for (int j = 0; ok && j < 8 && j0 + j < tiles; ++j) {
+          copy(false, page, k_sf, 4 * j);
+          if (j > 0) copy(true, page, v_sf, 4 * (j - 1));
+          else if (j0 > 0) copy(true, last_page, last_v, 28);
+          if (j == 3 && j0 + 8 < tiles) {
+            next_k = next_page >= 0 ? a.cache.k_scales[next_page] : 127u;
+            next_v = next_page >= 0 ? a.cache.v_scales[next_page] : 127u;
+          }
+        }
+        last_page = page;
+        last_v = v_sf;
+        page = next_page;
+        k_sf = next_k;
+        v_sf = next_v;
+      }
+      copy(true, last_page, last_v, 4 * ((tiles - 1) & 7));
+      left -= tiles;
+      if (left > 0) c.next_item(a);
+    }
+  } else if (count > 0 && warp == kMmaWarp) {
+    // ---------------- MMA issuer ----------------
+    constexpr uint32_t kIdescS = ((uint32_t)(kKvTile >> 3) << 17) | (1u << 23) | ((128u >> 4) << 24);
+    constexpr uint32_t kIdescO =
+        (1u << 16) | ((uint32_t)(D >> 3) << 17) | (1u << 23) | ((128u >> 4) << 24);
+    if (ptx::elect_one()) {
+#pragma unroll
+      for (int k = 0; k < TERMS; ++k)
+        ptx::tc_cp_32x128b_warpx4(tmem + C::kSfTerm + 4 * k,
+                                  ptx::smem_desc_scale_atom(ptx::smem_u32(term_sf + k * 512)));
+    }
+    __syncwarp();
+    bool ok = true;
+    int at = 0;  // place in the order of the copies
+    auto scores = [&](int i, bool last) {
+      const int slot = at % C::kSlots, buffer = i % C::kBuffers;
+      // The tile that these scores replace has been read.
+      if (i >= C::kBuffers)
+        ok = ok && __all_sync(0xffffffffu, bounded_wait(sread0 + 8 * buffer,
+                                                        (uint32_t)(i / C::kBuffers - 1) & 1u, abort_flag,
+                                                        a.status, 502));
+      ok = ok && __all_sync(0xffffffffu,
+                            bounded_wait(full0 + 8 * slot, (uint32_t)(at / C::kSlots) & 1u,
+                                         abort_flag, a.status, 503));
+      if (!ok) return;
+      ptx::tc_fence_after();
+      if (ptx::elect_one()) {
+        const uint32_t sf_t = tmem + C::kSfSets + buffer * C::kSfSet;
+        ptx::tc_cp_32x128b_warpx4(sf_t, ptx::smem_desc_scale_atom(ptx::smem_u32(sf_tiles + slot * 512)));
+        const uint32_t k_s = ptx::smem_u32(slots + slot * C::kSlotBytes);
+        const uint32_t q_s = ptx::smem_u32(q_tiles);
+#pragma unroll
+        for (int k = 0; k < TERMS; ++k) {
+#pragma unroll
+          for (int s = 0; s < C::kSubs; ++s) {
+            const uint64_t ad = ptx::smem_desc(q_s + (k * C::kSubs + s) * C::kSubBytes, 0, C::kGroup, C::kSwizzle);
+            const uint64_t bd = ptx::smem_desc(k_s + s * C::kSubBytes, 0, C::kGroup, C::kSwizzle);
+#pragma unroll
+            for (int ks = 0; ks < C::kRowBytes / 32; ++ks)
+              ptx::tc_mma_mxf8f6f4(tmem + buffer * kKvTile, ad + 2 * ks, bd + 2 * ks, kIdescS,
+                                   tmem + C::kSfTerm + 4 * k, sf_t,
+                                   (k > 0 || s > 0 || ks > 0) ? 1u : 0u);
+          }
+        }
+        ptx::tc_commit(sfull0 + 8 * buffer);
+        ptx::tc_commit(empty0 + 8 * slot);
+        if (last) ptx::tc_commit(qfree);
+      }
+      __syncwarp();
+      ++at;
+    };
+    for (int i0 = 0, segment = 0; ok && i0 < count; ++segment) {
+      ok = __all_sync(0xffffffffu, bounded_wait(qfull, (uint32_t)segment & 1u, abort_flag, a.status, 504));
+      if (!ok) break;
+      const int tiles = segments[segment & 1].tiles;
+      scores(i0, tiles == 1);
+      for (int j = 0; ok && j < tiles; ++j) {
+        const int i = i0 + j, buffer = i % C::kBuffers;
+        if (j + 1 < tiles) scores(i + 1, j + 2 == tiles);
+        const int slot = at % C::kSlots;
+        ok = ok && __all_sync(0xffffffffu, bounded_wait(pfull0 + 8 * buffer, (uint32_t)(i / C::kBuffers) & 1u,
+                                                        abort_flag, a.status, 505));
+        ok = ok && __all_sync(0xffffffffu,
+                              bounded_wait(full0 + 8 * slot, (uint32_t)(at / C::kSlots) & 1u,
+                                           abort_flag, a.status, 506));
+        if (!ok) break;
+        ptx::tc_fence_after();
+        if (ptx::elect_one()) {
+          const uint64_t v_atom = ptx::smem_desc_scale_atom(ptx::smem_u32(sf_tiles + slot * 512));
+          const uint32_t sf_t = tmem + C::kSfSets + buffer * C::kSfSet;
+          ptx::tc_cp_32x128b_warpx4(sf_t + C::kSfV, v_atom);
+          if (D > 128) ptx::tc_cp_32x128b_warpx4(sf_t + C::kSfV + 4, v_atom);
+#pragma unroll
+          for (int k = 0; k < TERMS; ++k)
+            ptx::tc_cp_32x128b_warpx4(sf_t + C::kSfP + 4 * k,
+                                      ptx::smem_desc_scale_atom(ptx::smem_u32(p_sf + (buffer * TERMS + k) * 512)));
+          // V: head_dim along N (MN-major), 32 tokens per step.
+          const uint64_t bd = ptx::smem_desc(ptx::smem_u32(slots + slot * C::kSlotBytes), C::kSubBytes,
+                                             C::kGroup, C::kSwizzle);
+          const uint32_t p_s = ptx::smem_u32(p_tiles + buffer * C::kPBytes);
+#pragma unroll
+          for (int k = 0; k < TERMS; ++k) {
+            const uint64_t ad = ptx::smem_desc(p_s + k * kRows * kKvTile, 0, 1024, ptx::kSwizzle128);
+#pragma unroll
+            for (int ks = 0; ks < kKvTileBlocks; ++ks)
+              ptx::tc_mma_mxf8f6f4(tmem + C::kOCol, ad + 2 * ks, bd + ks * (kKvBlock * C::kRowBytes / 16),
+                                   kIdescO | ((uint32_t)ks << 29) | ((uint32_t)ks << 4),
+                                   sf_t + C::kSfP + 4 * k, sf_t + C::kSfV,
+                                   (j > 0 || k > 0 || ks > 0) ? 1u : 0u);
+          }
+          ptx::tc_commit(pvdone0 + 8 * buffer);
+          ptx::tc_commit(empty0 + 8 * slot);
+        }
+        __syncwarp();
+        ++at;
+      }
+      i0 += tiles;
+    }
+  } else if (count > 0 && warp >= kQueryWarp) {
+    // ---------------- query terms ----------------
+    Cursor c = *start;
+    c.load(a);
+    bool ok = true;
+    const float sign = a.scale_log2 < 0.0f ? -1.0f : 1.0f;  // the softmax takes a factor >= 0
+    const float magnitude = fabsf(a.scale_log2);
+    for (int left = count, segment = 0; ok && left > 0; ++segment) {
+      // The rows' buffer is free with the last scores of the segment before, the description with
+      // the end of the one before that.
+      if (segment > 0)
+        ok = __all_sync(0xffffffffu, bounded_wait(qfree, (uint32_t)(segment - 1) & 1u, abort_flag, a.status, 507));
+      if (segment > 1)
+        ok = ok && __all_sync(0xffffffffu, bounded_wait(sdone0 + 8 * (segment & 1),
+                                                        (uint32_t)(segment / 2 - 1) & 1u, abort_flag,
+                                                        a.status, 508));
+      if (!ok) break;
+      Segment& seg = segments[segment & 1];
+      const int tiles = min(left, c.tiles - c.at.tile);
+      const int row0 = c.at.t * kRows;
+      if (warp == kQueryWarp) {
+        bool named = true;
+        const int64_t end = min((int64_t)c.seq.length, (int64_t)(c.at.tile + tiles) * kKvTile);
+        for (int64_t block = (int64_t)c.at.tile * kKvTileBlocks + lane * per_page; block * kKvBlock < end;
+             block += 32 * per_page)
+          named = named && kv_page(a.batch, a.cache, c.at.b, (int)block) >= 0;
+        named = __all_sync(0xffffffffu, named);
+        if (lane == 0) {
+          seg.row = c.seq.row;
+          seg.first_position = c.seq.first_position;
+          seg.rows = c.seq.rows;
+          seg.row0 = row0;
+          seg.length = c.seq.length;
+          seg.head = c.at.head;
+          seg.tile = c.at.tile;
+          seg.tiles = tiles;
+          seg.whole = c.at.tile == 0 && tiles == c.tiles;
+          seg.b = c.at.b;
+          seg.all_named = named;
+        }
+      }
+      constexpr int kPer = D / 32;  // values per lane
+      constexpr int kBatch = 8;     // rows in flight
+      // Lane l: where row 32 * (warp - kQueryWarp) + l is read.
+      const int first_row = (warp - kQueryWarp) * 32;
+      const int own = min(row0 + first_row + lane, c.seq.rows - 1);
+      const int64_t own_q = (c.seq.row + own / a.group) * a.q_token_stride +
+                            (int64_t)(c.at.head * a.group + own % a.group) * a.q_head_stride;
+      constexpr uint32_t kInf = TERMS == 2 ? 0x7f80u : 0x7c00u;
+#pragma unroll 1
+      for (int r0 = 0; r0 < 32; r0 += kBatch) {
+        __align__(16) uint16_t raw[kBatch][kPer];
+#pragma unroll
+        for (int n = 0; n < kBatch; ++n) {
+          const T* src = static_cast<const T*>(a.q) + __shfl_sync(0xffffffffu, own_q, r0 + n) + lane * kPer;
+          if (row0 + first_row + r0 + n < c.seq.rows) {
+            if (a.vector && kPer == 8) {
+              *reinterpret_cast<uint4*>(raw[n]) = *reinterpret_cast<const uint4*>(src);
+            } else if (a.vector && kPer == 4) {
+              *reinterpret_cast<uint2*>(raw[n]) = *reinterpret_cast<const uint2*>(src);
+            } else {
+#pragma unroll
+              for (int i = 0; i < kPer; ++i) raw[n][i] = reinterpret_cast<const uint16_t*>(src)[i];
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) raw[n][i] = 0;
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < kBatch; ++n) {
+          const int r = first_row + r0 + n;
+          uint32_t top = 0;
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) top = max(top, (uint32_t)(raw[n][i] & 0x7fffu));
+          top = __reduce_max_sync(0xffffffffu, top);
+          const float most = TERMS == 2 ? __uint_as_float(top << 16)
+                                        : __half2float(__ushort_as_half((unsigned short)top));
+          // A row with an infinity or NaN has no scale: its scores become NaN.
+          const uint32_t bits = ue8m0_scale_bits_shift<8>(top < kInf ? most : 1.0f);
+          const float inverse = ue8m0_inverse(bits) * sign;
+          if (lane == 0) seg.scale[r] = top < kInf ? __uint_as_float(bits) * magnitude : NAN;
+          uint32_t codes[TERMS][kPer / 2];
+#pragma unroll
+          for (int i = 0; i < kPer / 2; ++i) {
+            float v[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              if constexpr (TERMS == 2) v[e] = __uint_as_float((uint32_t)raw[n][2 * i + e] << 16);
+              else v[e] = __half2float(__ushort_as_half(raw[n][2 * i + e]));
+            }
+            uint32_t t[TERMS];
+            e4m3_terms<TERMS>(v[0] * inverse, v[1] * inverse, t);
+#pragma unroll
+            for (int k = 0; k < TERMS; ++k) codes[k][i] = t[k];
+          }
+          const int d0 = lane * kPer, in_row = d0 % C::kRowBytes;
+          const int swizzle = C::kRowBytes == 128 ? (r & 7) : ((r >> 1) & 3);
+#pragma unroll
+          for (int k = 0; k < TERMS; ++k) {
+            uint8_t* dst = q_tiles + (k * C::kSubs + d0 / C::kRowBytes) * C::kSubBytes + r * C::kRowBytes +
+                           (((in_row >> 4) ^ swizzle) << 4) + (in_row & 15);
+            if constexpr (kPer == 8) {
+              *reinterpret_cast<uint2*>(dst) = make_uint2(codes[k][0] | codes[k][1] << 16,
+                                                          codes[k][2] | codes[k][3] << 16);
+            } else if constexpr (kPer == 4) {
+              *reinterpret_cast<uint32_t*>(dst) = codes[k][0] | codes[k][1] << 16;
+            } else {
+              *reinterpret_cast<uint16_t*>(dst) = (uint16_t)codes[k][0];
+            }
+          }
+        }
+      }
+      ptx::fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(qfull);
+      left -= tiles;
+      if (left > 0) c.next_item(a);
+    }
+  } else if (count > 0 && warp < kSoftmaxWarps) {
+    // ---------------- softmax: a thread has 64 tokens of one row ----------------
+    // A wait that runs out ends the warp's tiles, and the vote at the end of the segment ends all.
+    const int quarter = warp & 3, half = warp >> 2;
+    const int row = quarter * 32 + lane;  // of the item
+    const uint32_t lane_t = tmem + ((uint32_t)(quarter * 32) << 16);
+    const uint32_t vsync = vsync0 + 8 * quarter;
+    uint8_t* p_row = p_tiles + row * kKvTile;
+    uint8_t* p_sf_row = p_sf + lane * 16 + quarter * 4 + half * 2;  // two bytes: this thread's blocks
+    bool failed = false;
+    uint32_t syncs = 0, votes = 0;
+    auto wait = [&](uint32_t bar, uint32_t parity, int code) {
+      if (!failed) failed = !__all_sync(0xffffffffu, bounded_wait(bar, parity, abort_flag, a.status, code));
+    };
+    int at0 = 0;  // place of the segment in the order of the copies
+    for (int i0 = 0, segment = 0; i0 < count; ++segment) {
+      wait(qfull, (uint32_t)segment & 1u, 510);
+      const Segment& seg = segments[segment & 1];
+      const int tiles = failed ? 0 : seg.tiles, length = seg.length;
+      // Above zero, so that a masked score (-inf) stays one where the scale is zero.
+      const float factor = seg.scale[row] < 1e-30f ? 1e-30f : seg.scale[row];
+      // Cached tokens that this row sees.
+      int64_t sees = length;
+      if (a.causal) sees = min(sees, seg.first_position + (seg.row0 + row) / a.group + 1);
+      const int visible = sees < 0 ? 0 : (int)sees;
+      float ref = -INFINITY, sum = 0.0f;
+#pragma unroll 1
+      for (int j = 0; j < tiles; ++j) {
+        const int i = i0 + j, buffer = i % C::kBuffers;
+        const int t0 = (seg.tile + j) * kKvTile + half * 64;  // this thread's first token
+        unsigned named = 3u;  // which of the thread's two blocks are on a page
+        if (!seg.all_named) {
+          named = 0;
+          for (int kb = 0; kb < 2; ++kb) {
+            const int block = (seg.tile + j) * kKvTileBlocks + half * 2 + kb;
+            if (block * kKvBlock < length && kv_page(a.batch, a.cache, seg.b, block) >= 0) named |= 1u << kb;
+          }
+        }
+        if (named != 3u || t0 + 64 > length) {
+          // Rows of V without a token may hold anything, NaN among them, and 0 * NaN is NaN: clear
+          // them once the tile has landed.  The four warps of a half clear sixteen rows each.
+          const int at = at0 + (j + 1 < tiles ? 2 * j + 2 : 2 * j + 1);
+          const int slot = at % C::kSlots;
+          wait(full0 + 8 * slot, (uint32_t)(at / C::kSlots) & 1u, 511);
+          uint8_t* v_s = slots + slot * C::kSlotBytes;
+          for (int t = quarter * 16; t < quarter * 16 + 16; ++t) {
+            if ((named >> (t >> 5) & 1u) != 0 && t0 + t < length) continue;
+            for (int piece = lane; piece < D / 16; piece += 32) {
+              const int sub = piece / (C::kRowBytes / 16), in_row = piece % (C::kRowBytes / 16);
+              *reinterpret_cast<uint4*>(v_s + sub * C::kSubBytes + (half * 64 + t) * C::kRowBytes +
+                                        in_row * 16) = make_uint4(0, 0, 0, 0);
+            }
+          }
+          ptx::fence_proxy_async();
+        }
+        wait(sfull0 + 8 * buffer, (uint32_t)(i / C::kBuffers) & 1u, 512);
+        if (failed) break;
+        ptx::tc_fence_after();
+        uint32_t raw[2][32];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+          ptx::tmem_ld_x32(lane_t + buffer * kKvTile + half * 64 + kb * 32, raw[kb]);
+        ptx::tmem_ld_wait();
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(sread0 + 8 * buffer);
+        if (named != 3u || !__all_sync(0xffffffffu, t0 + 64 <= visible)) {
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb) {
+            const int n = (named >> kb & 1u) != 0 ? visible - t0 - kb * 32 : 0;
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (e >= n) raw[kb][e] = 0xff800000u;  // -inf
+          }
+        }
+        uint32_t codes[2][TERMS][8];
+        float top[2], part[2];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+          float m = -INFINITY;
+#pragma unroll
+          for (int e = 0; e < 32; e += 2)
+            m = fmaxf(m, fmaxf(__uint_as_float(raw[kb][e]), __uint_as_float(raw[kb][e + 1])));
+          top[kb] = rintf(m * factor);  // nearest power of two: the largest weight is in (181, 363)
+          const float base = fmaxf(top[kb], -1e30f) - kWeightLog2;
+          float s0 = 0.0f, s1 = 0.0f;
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) {
+            float p[4];
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+              p[n] = ptx::exp2_approx(__uint_as_float(raw[kb][e + n]) * factor - base);
+            s0 += p[0] + p[2];
+            s1 += p[1] + p[3];
+            uint32_t lo[TERMS], hi[TERMS];
+            e4m3_terms_half<TERMS>(__floats2half2_rn(p[0], p[1]), lo);
+            e4m3_terms_half<TERMS>(__floats2half2_rn(p[2], p[3]), hi);
+#pragma unroll
+            for (int k = 0; k < TERMS; ++k) codes[kb][k][e / 4] = __byte_perm(lo[k], hi[k], 0x5410);
+          }
+          part[kb] = s0 + s1;
+        }
+        // The reference moves only where a block exceeds it by much, or was not set: the two
+        // warps that share the rows agree.
+        volatile int* asked = ask_flag + quarter * 2 + (votes++ & 1u);
+        const bool ask = __any_sync(0xffffffffu, fmaxf(top[0], top[1]) > ref + kMostLog2);
+        if (lane == 0) {
+          if (ask) *asked = 1;
+          ptx::mbar_arrive(vsync);
+        }
+        // P of the tile before last (or of the last one) has been read.
+        if (i >= C::kBuffers)
+          wait(pvdone0 + 8 * buffer, (uint32_t)(i / C::kBuffers - 1) & 1u, 513);
+        uint8_t* p_buffer = p_row + buffer * C::kPBytes;
+#pragma unroll
+        for (int k = 0; k < TERMS; ++k) {
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+            for (int c16 = 0; c16 < 2; ++c16) {
+              const int chunk = half * 4 + kb * 2 + c16;
+              *reinterpret_cast<uint4*>(p_buffer + k * kRows * kKvTile + ((chunk ^ (row & 7)) << 4)) =
+                  make_uint4(codes[kb][k][c16 * 4], codes[kb][k][c16 * 4 + 1], codes[kb][k][c16 * 4 + 2],
+                             codes[kb][k][c16 * 4 + 3]);
+            }
+          }
+        }
+        wait(vsync, syncs & 1u, 514);
+        ++syncs;
+        if (!failed && *asked != 0) {
+          row_top[half * kRows + row] = fmaxf(top[0], top[1]);
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(vsync);
+          wait(vsync, syncs & 1u, 515);
+          ++syncs;
+          if (half == 0 && lane == 0) *asked = 0;  // not used by the next vote, but the one after
+          const float m = fmaxf(row_top[row], row_top[kRows + row]);
+          const bool up = m > ref + kMostLog2;
+          const float f = up ? pow2_whole(ref - m) : 1.0f;
+          if (up) ref = m;
+          sum *= f;
+          if (j > 0) {
+            // What has been added up so far shrinks, once the last output has been added.
+            wait(pvdone0 + 8 * ((i - 1) % C::kBuffers), (uint32_t)((i - 1) / C::kBuffers) & 1u, 516);
+            if (failed) break;
+            ptx::tc_fence_after();
+#pragma unroll 1
+            for (int c0 = half * (D / 2); c0 < (half + 1) * (D / 2); c0 += 8) {
+              uint32_t o[8];
+              ptx::tmem_ld_x8(lane_t + C::kOCol + c0, o);
+              ptx::tmem_ld_wait();
+#pragma unroll
+              for (int n = 0; n < 8; ++n) o[n] = __float_as_uint(__uint_as_float(o[n]) * f);
+              ptx::tmem_st_x8(lane_t + C::kOCol + c0, o);
+            }
+            ptx::tmem_st_wait();
+          }
+          // The partner reads row_top of this meeting before the next one is written.
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(vsync);
+          wait(vsync, syncs & 1u, 517);
+          ++syncs;
+        }
+        if (failed) break;
+        // Block scales of P: 2^(top - ref), the further terms 2^-4 and 2^-8 of it.
+        uint32_t code[2];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+          const float power = pow2_whole(top[kb] == -INFINITY ? 0.0f : top[kb] - ref);
+          sum += part[kb] * power;
+          code[kb] = __float_as_uint(power) >> 23;
+        }
+#pragma unroll
+        for (int k = 0; k < TERMS; ++k) {
+          const uint32_t lo = code[0] > 4u * k ? code[0] - 4u * k : 0u;
+          const uint32_t hi = code[1] > 4u * k ? code[1] - 4u * k : 0u;
+          *reinterpret_cast<uint16_t*>(p_sf_row + (buffer * TERMS + k) * 512) = (uint16_t)(lo | hi << 8);
+        }
+        ptx::fence_proxy_async();
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(pfull0 + 8 * buffer);
+      }
+      // ---- the rows of this CTA's tiles of the item ----
+      row_sum[half * kRows + row] = sum;
+      const int i = i0 + tiles - 1;
+      if (tiles > 0) wait(pvdone0 + 8 * (i % C::kBuffers), (uint32_t)(i / C::kBuffers) & 1u, 518);
+      failed = ptx::barrier_any(1, kSoftmaxWarps * 32, failed);
+      if (failed) break;
+      ptx::tc_fence_after();
+      const float l = row_sum[row] + row_sum[kRows + row];
+      const int r = seg.row0 + row;
+      const bool mine = r < seg.rows;
+      if (seg.whole) {
+        const float scale = l == 0.0f ? 0.0f : 1.0f / l;
+        T* out = static_cast<T*>(a.out) + (seg.row + r / a.group) * a.out_token_stride +
+                 (int64_t)(seg.head * a.group + r % a.group) * a.out_head_stride;
+#pragma unroll 1
+        for (int c0 = half * (D / 2); c0 < (half + 1) * (D / 2); c0 += 32) {
+          uint32_t o[32];
+          ptx::tmem_ld_x32(lane_t + C::kOCol + c0, o);
+          ptx::tmem_ld_wait();
+          uint32_t w[16];
+#pragma unroll
+          for (int n = 0; n < 16; ++n) {
+            const float x = __uint_as_float(o[2 * n]) * scale, y = __uint_as_float(o[2 * n + 1]) * scale;
+            if constexpr (TERMS == 2) {
+              const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+              w[n] = *reinterpret_cast<const uint32_t*>(&v);
+            } else {
+              const __half2 v = __floats2half2_rn(x, y);
+              w[n] = *reinterpret_cast<const uint32_t*>(&v);
+            }
+          }
+          if (mine) {
+            if (a.vector_out) {
+#pragma unroll
+              for (int n = 0; n < 4; ++n)
+                *reinterpret_cast<uint4*>(out + c0 + n * 8) =
+                    make_uint4(w[4 * n], w[4 * n + 1], w[4 * n + 2], w[4 * n + 3]);
+            } else {
+              uint16_t* dst = reinterpret_cast<uint16_t*>(out + c0);
+#pragma unroll
+              for (int n = 0; n < 16; ++n) {
+                dst[2 * n] = (uint16_t)w[n];
+                dst[2 * n + 1] = (uint16_t)(w[n] >> 16);
+              }
+            }
+          }
+        }
+      } else {
+        // A share that begins inside an item uses the CTA's first partial slot for it, one that
+        // ends inside the second.
+        float* part = a.partials +
+                      (int64_t)(2 * blockIdx.x + (seg.tile != 0 ? 0 : 1)) * C::kPartialFloats;
+        if (half == 0) {
+          part[kRows * D + 2 * row] = ref;
+          part[kRows * D + 2 * row + 1] = l;
+        }
+#pragma unroll 1
+        for (int c0 = half * (D / 2); c0 < (half + 1) * (D / 2); c0 += 32) {
+          uint32_t o[32];
+          ptx::tmem_ld_x32(lane_t + C::kOCol + c0, o);
+          ptx::tmem_ld_wait();
+          if (mine) {
+#pragma unroll
+            for (int n = 0; n < 8; ++n)
+              *reinterpret_cast<uint4*>(part + row * D + c0 + n * 4) =
+                  make_uint4(o[4 * n], o[4 * n + 1], o[4 * n + 2], o[4 * n + 3]);
+          }
+        }
+      }
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(sdone0 + 8 * (segment & 1));
+      i0 += tiles;
+      at0 += 2 * tiles;
+    }
+  }
+
+  // ---------------- teardown ----------------
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (*abort_flag != 0) {
+    // Give copies and MMAs still in flight time to land before the CTA's shared
+    // and tensor memory are handed back.
+    for (int i = 0; i < 200; ++i) __nanosleep(1000);
+  }
+  if (warp == kMmaWarp) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc(tmem, 512);
+  }
+}
+
+// Joins the partial rows of every item whose tiles went to more than one CTA, in the order of the
+// tiles.  A border between two shares has kRows / kJoinRows CTAs; the first border inside an item
+// has it.
+constexpr int kJoinRows = 8;
+constexpr int kJoinThreads = 256;
+
+template <int D, int TERMS>
+__global__ void __launch_bounds__(kJoinThreads)
+kv_prefill_join_kernel(const AttentionArgs a, int grid) {
+  using C = PrefillCfg<D, TERMS>;
+  using T = typename std::conditional<TERMS == 2, __nv_bfloat16, __half>::type;
+  constexpr int kColumns = D / 4;                   // four values a thread
+  constexpr int kAtOnce = kJoinThreads / kColumns;  // rows
+  __shared__ Place item;
+  __shared__ int item_parts;
+  const int c0 = (int)blockIdx.x, tid = threadIdx.x, lane = tid & 31;
+  if (tid < 32) {
+    Place p{};
+    int64_t begin = 0;
+    const Share s = share_of(warp_walk(a, -1, lane, &p, &begin), grid);
+    int parts = 1;
+    if (c0 + 1 < s.ctas && s.total > 0) {
+      warp_walk(a, share_begin(s, c0 + 1), lane, &p, &begin);
+      Cursor c;
+      c.at = p;
+      c.load(a);
+      const int64_t u0 = begin + kItemUnits, u1 = u0 + c.tiles - 1;
+      // CTA of a unit: the last one whose share begins at or before it.
+      if ((int)(((u0 + 1) * s.ctas - 1) / s.total) == c0)
+        parts = (int)(((u1 + 1) * s.ctas - 1) / s.total) - c0 + 1;
+    }
+    if (lane == 0) {
+      item = p;
+      item_parts = parts;
+    }
+  }
+  __syncthreads();
+  const int parts = item_parts;
+  ptx::grid_dependency_wait();
+  if (parts == 1) return;
+  const Sequence seq = load_sequence(a, item.b);
+  const int column = tid % kColumns;
+  // The first CTA began before this item or with it, the others inside it.
+  const int64_t first = 2 * c0 + 1, later = 2 * c0;  // slot of part p: p == 0 ? first : later + 2 p
+  for (int k = tid / kColumns; k < kJoinRows; k += kAtOnce) {
+    const int row = (int)blockIdx.y * kJoinRows + k;
+    const int r = item.t * kRows + row;
+    if (r >= seq.rows) continue;
+    float top = -INFINITY;
+    for (int p = 0; p < parts; ++p)
+      top = fmaxf(top, a.partials[(p == 0 ? first : later + 2 * p) * C::kPartialFloats + kRows * D + 2 * row]);
+    float l = 0.0f;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+    for (int p = 0; p < parts; ++p) {
+      const float* part = a.partials + (p == 0 ? first : later + 2 * p) * C::kPartialFloats;
+      const float2 tl = *reinterpret_cast<const float2*>(part + kRows * D + 2 * row);
+      const float4 v = *reinterpret_cast<const float4*>(part + row * D + column * 4);
+      const float f = tl.x == top ? 1.0f : pow2_whole(tl.x - top);
+      l += f * tl.y;
+      o.x += f * v.x;
+      o.y += f * v.y;
+      o.z += f * v.z;
+      o.w += f * v.w;
+    }
+    const float scale = l == 0.0f ? 0.0f : 1.0f / l;
+    T* out = static_cast<T*>(a.out) + (seq.row + r / a.group) * a.out_token_stride +
+             (int64_t)(item.head * a.group + r % a.group) * a.out_head_stride + column * 4;
+    const float v[4] = {o.x * scale, o.y * scale, o.z * scale, o.w * scale};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (TERMS == 2) out[i] = __float2bfloat16_rn(v[i]);
+      else out[i] = __float2half_rn(v[i]);
+    }
+  }
+}
+
+bool use_pdl() {
+  static const bool enabled = []() {
+    const char* env = std::getenv("MXFP6_B200_PDL");
+    return env == nullptr || env[0] != '0';
+  }();
+  return enabled;
+}
+
+template <int D, int TERMS>
+int launch(const CUtensorMap& tm_k, const CUtensorMap& tm_v, const AttentionArgs& a, int grid,
+           cudaStream_t stream) {
+  using C = PrefillCfg<D, TERMS>;
+  static bool configured[64] = {};
+  int device = 0;
+  MX_CUDA(cudaGetDevice(&device));
+  if (device >= 64 || !configured[device]) {
+    MX_CUDA(cudaFuncSetAttribute(kv_prefill_kernel<D, TERMS>,
+                                 cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes));
+    if (device < 64) configured[device] = true;
+  }
+  cudaLaunchAttribute attribute[1];
+  attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3((unsigned)grid);
+  config.blockDim = dim3(kThreads);
+  config.dynamicSmemBytes = C::kSmemBytes;
+  config.stream = stream;
+  config.attrs = attribute;
+  config.numAttrs = use_pdl() ? 1 : 0;
+  MX_CUDA(cudaLaunchKernelEx(&config, kv_prefill_kernel<D, TERMS>, tm_k, tm_v, a));
+  if (grid == 1) return kOk;  // nothing was cut
+  config.gridDim = dim3((unsigned)(grid - 1), kRows / kJoinRows);
+  config.blockDim = dim3(kJoinThreads);
+  config.dynamicSmemBytes = 0;
+  MX_CUDA(cudaLaunchKernelEx(&config, kv_prefill_join_kernel<D, TERMS>, a, grid));
+  return kOk;
+}
+
+}  // namespace
+
+// CTAs of a prefill launch: at most one per SM and no more than there can be work for.
+int kv_prefill_grid(int64_t batch, int64_t tokens, int kv_heads, int group, int64_t max_context) {
+  const int64_t items = (tokens * group / kRows + batch) * kv_heads;
+  const int64_t units = items * (ceil_div64(max_context < 1 ? 1 : max_context, kKvTile) + kItemUnits);
+  const int64_t want = ceil_div64(units, kMinUnits);
+  return (int)(want < kSms ? want : kSms);
+}
+
+int64_t kv_prefill_workspace(int64_t batch, int64_t tokens, int kv_heads, int group, int head_dim,
+                             int64_t max_context) {
+  const int grid = kv_prefill_grid(batch, tokens, kv_heads, group, max_context);
+  return grid == 1 ? 0 : (int64_t)grid * 2 * (kRows * head_dim + 2 * kRows) * 4;
+}
+
+// Sequences with more than a.min_rows rows (tokens x group).
+int launch_kv_prefill(const AttentionArgs& a, int dtype, cudaStream_t stream) {
+  CUtensorMap tm_k, tm_v;
+  if (int rc = make_kv_map(&tm_k, a.cache.k_values, a.cache)) return rc;
+  if (int rc = make_kv_map(&tm_v, a.cache.v_values, a.cache)) return rc;
+  const int grid = kv_prefill_grid(a.batch.batch, a.batch.tokens, a.cache.kv_heads, a.group,
+                                   (int64_t)a.batch.table_width * a.cache.page_size);
+  const int d = a.cache.head_dim;
+  if (dtype == kBF16) {
+    if (d == 64) return launch<64, 2>(tm_k, tm_v, a, grid, stream);
+    if (d == 128) return launch<128, 2>(tm_k, tm_v, a, grid, stream);
+    return launch<256, 2>(tm_k, tm_v, a, grid, stream);
+  }
+  if (d == 64) return launch<64, 3>(tm_k, tm_v, a, grid, stream);
+  if (d == 128) return launch<128, 3>(tm_k, tm_v, a, grid, stream);
+  return launch<256, 3>(tm_k, tm_v, a, grid, stream);
+}
+
+}  // namespace mx
