@@ -25,39 +25,36 @@ from dataclasses import dataclass
 import torch
 
 from ._loader import check, library
-from .ops import SCALE_VECTOR_SIZE, _DTYPE_CODE, _ptr, _refuse, _require_sm100
+from .ops import SCALE_VECTOR_SIZE, _DTYPE_CODE, _refuse, _require_sm100
 
 KV_HEAD_DIMS = (64, 128, 256)
 KV_PAGE_SIZES = (32, 64, 128)
 
 
-class _on_device:
-    """``torch.cuda.device`` that costs nothing when the device is the current one already."""
-
-    __slots__ = ("index", "guard")
-
-    def __init__(self, device: torch.device):
-        self.index, self.guard = device.index, None
-
-    def __enter__(self) -> int:
-        if torch.cuda.current_device() != self.index:
-            self.guard = torch.cuda.device(self.index)
-            self.guard.__enter__()
-        return torch.cuda.current_stream().cuda_stream
-
-    def __exit__(self, *exc) -> None:
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
-
-
+_BF16, _F16 = torch.bfloat16, torch.float16
 _SM100_SEEN: set[int] = set()
 
 
-def _require_gpu(device: torch.device) -> None:
-    _refuse(device.type != "cuda", f"the tensors must be on a CUDA device; got {device}")
-    if device.index not in _SM100_SEEN:
+def _launch(device: torch.device, function, *args) -> None:
+    """Call a C entry on ``device`` and its current stream.
+
+    These operators run several times per decoder layer with microseconds of GPU work each, so the
+    argument rules above the call are plain comparisons whose messages are only built to be raised,
+    and the device is switched only when it is not the current one.
+    """
+    index = device.index
+    if index not in _SM100_SEEN:
+        if device.type != "cuda":
+            raise ValueError(f"the tensors must be on a CUDA device; got {device}")
         _require_sm100(device)
-        _SM100_SEEN.add(device.index)
+        _SM100_SEEN.add(index)
+    if torch.cuda.current_device() == index:
+        status = function(*args, torch.cuda.current_stream(index).cuda_stream)
+    else:
+        with torch.cuda.device(index):
+            status = function(*args, torch.cuda.current_stream(index).cuda_stream)
+    if status != 0:
+        check(status)
 
 
 @dataclass(frozen=True)
@@ -75,21 +72,34 @@ class PagedKVCache:
     v_scales: torch.Tensor
 
     def __post_init__(self) -> None:
-        values, scales = self.k_values, self.k_scales
-        _refuse(values.ndim != 4, f"k_values must be [pages, kv_heads, page_size, head_dim]; got "
-                                  f"{tuple(values.shape)}")
-        pages, heads, page, dim = values.shape
-        _refuse(page not in KV_PAGE_SIZES, f"page_size must be one of {KV_PAGE_SIZES}; got {page}")
-        _refuse(dim not in KV_HEAD_DIMS, f"head_dim must be one of {KV_HEAD_DIMS}; got {dim}")
-        _refuse(pages < 1 or heads < 1, "the cache needs at least one page and one head")
-        _refuse(self.v_values.shape != values.shape, "v_values must have the shape of k_values")
+        k, v, ks, vs = self.k_values, self.v_values, self.k_scales, self.v_scales
+        shape = k.shape
+        if len(shape) != 4:
+            raise ValueError(f"k_values must be [pages, kv_heads, page_size, head_dim]; got {tuple(shape)}")
+        pages, heads, page, dim = shape
+        if page not in KV_PAGE_SIZES:
+            raise ValueError(f"page_size must be one of {KV_PAGE_SIZES}; got {page}")
+        if dim not in KV_HEAD_DIMS:
+            raise ValueError(f"head_dim must be one of {KV_HEAD_DIMS}; got {dim}")
+        if pages < 1 or heads < 1:
+            raise ValueError("the cache needs at least one page and one head")
+        if v.shape != shape:
+            raise ValueError("v_values must have the shape of k_values")
         want = (pages, heads, page // SCALE_VECTOR_SIZE)
-        _refuse(scales.shape != want or self.v_scales.shape != want,
-                f"k_scales and v_scales must be {list(want)}")
-        for tensor in (values, self.v_values, scales, self.v_scales):
-            _refuse(tensor.dtype != torch.uint8, "cache tensors must be uint8", TypeError)
-            _refuse(tensor.device != values.device, "cache tensors must be on one device")
-            _refuse(not tensor.is_contiguous(), "cache tensors must be contiguous")
+        if ks.shape != want or vs.shape != want:
+            raise ValueError(f"k_scales and v_scales must be {list(want)}")
+        u8 = torch.uint8
+        if k.dtype != u8 or v.dtype != u8 or ks.dtype != u8 or vs.dtype != u8:
+            raise TypeError("cache tensors must be uint8")
+        device = k.device
+        if v.device != device or ks.device != device or vs.device != device:
+            raise ValueError("cache tensors must be on one device")
+        if not (k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
+            raise ValueError("cache tensors must be contiguous")
+        # What every call passes on.
+        object.__setattr__(self, "device", device)
+        object.__setattr__(self, "_arguments", (k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(),
+                                                pages, heads, page, dim))
 
     @classmethod
     def allocate(cls, pages: int, kv_heads: int, page_size: int, head_dim: int,
@@ -103,83 +113,94 @@ class PagedKVCache:
                    torch.full(blocks, 127, dtype=torch.uint8, device=device))
 
     @property
-    def device(self) -> torch.device:
-        return self.k_values.device
-
-    @property
     def pages(self) -> int:
-        return self.k_values.shape[0]
+        return self._arguments[4]
 
     @property
     def kv_heads(self) -> int:
-        return self.k_values.shape[1]
+        return self._arguments[5]
 
     @property
     def page_size(self) -> int:
-        return self.k_values.shape[2]
+        return self._arguments[6]
 
     @property
     def head_dim(self) -> int:
-        return self.k_values.shape[3]
+        return self._arguments[7]
 
     def nbytes(self) -> int:
         """Bytes of the values and scales."""
         return 2 * (self.k_values.numel() + self.k_scales.numel())
 
-    def _pointers(self) -> tuple:
-        return (self.k_values.data_ptr(), self.v_values.data_ptr(), self.k_scales.data_ptr(),
-                self.v_scales.data_ptr(), *self.k_values.shape)
-
 
 def _check_batch(cache: PagedKVCache, block_table: torch.Tensor, seq_lens: torch.Tensor,
                  cu_seqlens: torch.Tensor | None, tokens: int) -> tuple:
     """The batch description's argument rules; returns its C arguments."""
-    _refuse(not isinstance(cache, PagedKVCache), "cache must be a PagedKVCache instance", TypeError)
+    if not isinstance(cache, PagedKVCache):
+        raise TypeError("cache must be a PagedKVCache instance")
     device = cache.device
-    _refuse(block_table.dtype != torch.int32 or seq_lens.dtype != torch.int32,
-            "block_table and seq_lens must be int32", TypeError)
-    _refuse(block_table.ndim != 2 or block_table.shape[1] < 1
-            or (block_table.shape[1] > 1 and block_table.stride(1) != 1),
-            "block_table must be [batch, width] with contiguous rows")
-    batch = block_table.shape[0]
-    _refuse(batch < 1, "the batch must hold at least one sequence")
-    _refuse(seq_lens.shape != (batch,) or not seq_lens.is_contiguous(),
-            f"seq_lens must be contiguous [{batch}]")
-    _refuse(block_table.device != device or seq_lens.device != device,
-            "block_table and seq_lens must be on the cache's device")
+    if block_table.dtype != torch.int32 or seq_lens.dtype != torch.int32:
+        raise TypeError("block_table and seq_lens must be int32")
+    shape = block_table.shape
+    if len(shape) != 2 or shape[1] < 1 or (shape[1] > 1 and block_table.stride(1) != 1):
+        raise ValueError("block_table must be [batch, width] with contiguous rows")
+    batch, width = shape
+    if batch < 1:
+        raise ValueError("the batch must hold at least one sequence")
+    if seq_lens.shape != (batch,) or not seq_lens.is_contiguous():
+        raise ValueError(f"seq_lens must be contiguous [{batch}]")
+    if block_table.device != device or seq_lens.device != device:
+        raise ValueError("block_table and seq_lens must be on the cache's device")
+    offsets = None
     if cu_seqlens is None:
-        _refuse(tokens != batch, f"without cu_seqlens every sequence has one row; got {tokens} rows "
-                                 f"for {batch} sequences")
+        if tokens != batch:
+            raise ValueError(f"without cu_seqlens every sequence has one row; got {tokens} rows for "
+                             f"{batch} sequences")
     else:
-        _refuse(cu_seqlens.dtype != torch.int32, "cu_seqlens must be int32", TypeError)
-        _refuse(cu_seqlens.shape != (batch + 1,) or not cu_seqlens.is_contiguous(),
-                f"cu_seqlens must be contiguous [{batch + 1}]")
-        _refuse(cu_seqlens.device != device, "cu_seqlens must be on the cache's device")
-    return (block_table.data_ptr(), seq_lens.data_ptr(), _ptr(cu_seqlens), block_table.stride(0),
-            tokens, block_table.shape[1], batch)
+        if cu_seqlens.dtype != torch.int32:
+            raise TypeError("cu_seqlens must be int32")
+        if cu_seqlens.shape != (batch + 1,) or not cu_seqlens.is_contiguous():
+            raise ValueError(f"cu_seqlens must be contiguous [{batch + 1}]")
+        if cu_seqlens.device != device:
+            raise ValueError("cu_seqlens must be on the cache's device")
+        offsets = cu_seqlens.data_ptr()
+    return (block_table.data_ptr(), seq_lens.data_ptr(), offsets, block_table.stride(0), tokens, width,
+            batch)
 
 
 def _check_rows(tensor: torch.Tensor, name: str, heads: int | None, dim: int,
-                device: torch.device) -> None:
-    _refuse(tensor.dtype not in _DTYPE_CODE,
-            f"{name} must have dtype torch.float16 or torch.bfloat16; got {tensor.dtype}", TypeError)
-    _refuse(tensor.ndim != 3 or tensor.shape[2] != dim
-            or (heads is not None and tensor.shape[1] != heads),
-            f"{name} must be [tokens, {'heads' if heads is None else heads}, {dim}]; got "
-            f"{tuple(tensor.shape)}")
-    _refuse(tensor.stride(2) != 1, f"{name}'s last dimension must be contiguous")
-    _refuse(tensor.device != device, f"{name} must be on {device}; got {tensor.device}")
+                device: torch.device) -> tuple:
+    """Rules of ``[tokens, heads, dim]`` rows of 16-bit numbers; returns the strides."""
+    dtype = tensor.dtype
+    if dtype is not _BF16 and dtype is not _F16:
+        raise TypeError(f"{name} must have dtype torch.float16 or torch.bfloat16; got {dtype}")
+    shape = tensor.shape
+    if len(shape) != 3 or shape[2] != dim or (heads is not None and shape[1] != heads):
+        raise ValueError(f"{name} must be [tokens, {'heads' if heads is None else heads}, {dim}]; got "
+                         f"{tuple(shape)}")
+    strides = tensor.stride()
+    if strides[2] != 1:
+        raise ValueError(f"{name}'s last dimension must be contiguous")
+    if tensor.device != device:
+        raise ValueError(f"{name} must be on {device}; got {tensor.device}")
+    return strides
 
 
-def _no_overlap_within(tensor: torch.Tensor, name: str) -> None:
-    """Refuse outputs whose rows share memory (expanded views)."""
-    tokens, heads, dim = tensor.shape
-    token_stride, head_stride, _ = tensor.stride()
+def _check_output_rows(tensor: torch.Tensor, name: str, like: torch.Tensor,
+                       device: torch.device) -> tuple:
+    """Rules of an output of ``like``'s shape and dtype, whose rows share no memory."""
+    tokens, heads, dim = like.shape
+    strides = _check_rows(tensor, name, heads, dim, device)
+    if tensor.shape[0] != tokens or tensor.dtype != like.dtype:
+        raise ValueError(f"{name} must match its input's shape and dtype")
+    token_stride, head_stride, _ = strides
     bad = (heads > 1 and head_stride < dim) or (tokens > 1 and token_stride < dim)
     if not bad and tokens > 1 and heads > 1:
         inner, outer = sorted(((head_stride, heads), (token_stride, tokens)))
         bad = outer[0] < inner[0] * (inner[1] - 1) + dim
-    _refuse(bad, f"{name} must not overlap itself")
+    if bad:
+        raise ValueError(f"{name} must not overlap itself")
+    return strides
 
 
 def kv_cache_write(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor,
@@ -195,17 +216,17 @@ def kv_cache_write(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor,
     than the sequence's rows) and positions behind the block table are not written.  No page may
     be named by two sequences, or twice by one, for positions that the call writes.
     """
-    _refuse(k.ndim != 3, f"k must be [tokens, kv_heads, head_dim]; got {tuple(k.shape)}")
+    if k.ndim != 3:
+        raise ValueError(f"k must be [tokens, kv_heads, head_dim]; got {tuple(k.shape)}")
     batch = _check_batch(cache, block_table, seq_lens, cu_seqlens, k.shape[0])
-    device = cache.device
-    _check_rows(k, "k", cache.kv_heads, cache.head_dim, device)
-    _check_rows(v, "v", cache.kv_heads, cache.head_dim, device)
-    _refuse(v.shape != k.shape or v.dtype != k.dtype, "k and v must have one shape and dtype")
-    _require_gpu(device)
-    with _on_device(device) as stream:
-        check(library().mxfp6_kv_cache_write(
-            *cache._pointers(), *batch, k.data_ptr(), v.data_ptr(), _DTYPE_CODE[k.dtype],
-            k.stride(0), k.stride(1), v.stride(0), v.stride(1), stream))
+    device, arguments = cache.device, cache._arguments
+    heads, dim = arguments[5], arguments[7]
+    k_strides = _check_rows(k, "k", heads, dim, device)
+    v_strides = _check_rows(v, "v", heads, dim, device)
+    if v.shape != k.shape or v.dtype is not k.dtype:
+        raise ValueError("k and v must have one shape and dtype")
+    _launch(device, library().mxfp6_kv_cache_write, *arguments, *batch, k.data_ptr(), v.data_ptr(),
+            _DTYPE_CODE[k.dtype], k_strides[0], k_strides[1], v_strides[0], v_strides[1])
 
 
 def kv_cache_read(cache: PagedKVCache, block_table: torch.Tensor, seq_lens: torch.Tensor,
@@ -220,29 +241,35 @@ def kv_cache_read(cache: PagedKVCache, block_table: torch.Tensor, seq_lens: torc
     whose position is below zero or on no page are zero.  Every value is ``code * scale`` rounded
     once: exact in BF16.
     """
-    _refuse(not isinstance(cache, PagedKVCache), "cache must be a PagedKVCache instance", TypeError)
+    if not isinstance(cache, PagedKVCache):
+        raise TypeError("cache must be a PagedKVCache instance")
+    device, arguments = cache.device, cache._arguments
+    heads, dim = arguments[5], arguments[7]
     if out is None:
-        _refuse(dtype not in _DTYPE_CODE,
-                f"dtype must be torch.float16 or torch.bfloat16; got {dtype}", TypeError)
-        _refuse(tokens is None and cu_seqlens is not None,
-                "tokens (rows in all) is needed with cu_seqlens when out is not given")
+        if dtype not in _DTYPE_CODE:
+            raise TypeError(f"dtype must be torch.float16 or torch.bfloat16; got {dtype}")
+        if tokens is None and cu_seqlens is not None:
+            raise ValueError("tokens (rows in all) is needed with cu_seqlens when out is not given")
         rows = block_table.shape[0] if tokens is None else int(tokens)
-        _refuse(rows < 0, f"tokens must not be negative; got {rows}")
-        shape = (rows, cache.kv_heads, cache.head_dim)
-        out = (torch.empty(shape, dtype=dtype, device=cache.device),
-               torch.empty(shape, dtype=dtype, device=cache.device))
+        if rows < 0:
+            raise ValueError(f"tokens must not be negative; got {rows}")
+        out = (torch.empty((rows, heads, dim), dtype=dtype, device=device),
+               torch.empty((rows, heads, dim), dtype=dtype, device=device))
     k, v = out
-    _refuse(k.ndim != 3, "out must be two [tokens, kv_heads, head_dim] tensors")
-    _refuse(tokens is not None and k.shape[0] != tokens, "out must have `tokens` rows")
-    batch = _check_batch(cache, block_table, seq_lens, cu_seqlens, k.shape[0])
-    for tensor, name in ((k, "out[0]"), (v, "out[1]")):
-        _check_rows(tensor, name, cache.kv_heads, cache.head_dim, cache.device)
-        _refuse(not tensor.is_contiguous(), f"{name} must be contiguous")
-    _refuse(v.shape != k.shape or v.dtype != k.dtype, "the outputs must have one shape and dtype")
-    _require_gpu(cache.device)
-    with _on_device(cache.device) as stream:
-        check(library().mxfp6_kv_cache_read(
-            *cache._pointers(), *batch, k.data_ptr(), v.data_ptr(), _DTYPE_CODE[k.dtype], stream))
+    if k.ndim != 3:
+        raise ValueError("out must be two [tokens, kv_heads, head_dim] tensors")
+    rows = k.shape[0]
+    if tokens is not None and rows != tokens:
+        raise ValueError("out must have `tokens` rows")
+    batch = _check_batch(cache, block_table, seq_lens, cu_seqlens, rows)
+    _check_rows(k, "out[0]", heads, dim, device)
+    _check_rows(v, "out[1]", heads, dim, device)
+    if not (k.is_contiguous() and v.is_contiguous()):
+        raise ValueError("out's tensors must be contiguous")
+    if v.shape != k.shape or v.dtype is not k.dtype:
+        raise ValueError("the outputs must have one shape and dtype")
+    _launch(device, library().mxfp6_kv_cache_read, *arguments, *batch, k.data_ptr(), v.data_ptr(),
+            _DTYPE_CODE[k.dtype])
     return k, v
 
 
@@ -257,38 +284,41 @@ def kv_cache_attention(q: torch.Tensor, cache: PagedKVCache, block_table: torch.
     query head ``h`` reads key head ``h // (q_heads // kv_heads)``.  A row that sees no token is
     zero.  ``scale`` multiplies the scores (default ``head_dim ** -0.5``).  ``max_query_len``: an
     upper bound of the rows of any sequence (default: 1 without ``cu_seqlens``, else all rows); a
-    tight one picks the better kernel.  Write the rows' own keys and values first
-    (:func:`kv_cache_write` takes the same ``block_table``, ``seq_lens`` and ``cu_seqlens``).
+    tight one picks the better kernel, and rows of a sequence that has more are not written.
+    Write the rows' own keys and values first (:func:`kv_cache_write` takes the same
+    ``block_table``, ``seq_lens`` and ``cu_seqlens``).
     """
-    _refuse(q.ndim != 3, f"q must be [tokens, q_heads, head_dim]; got {tuple(q.shape)}")
+    if q.ndim != 3:
+        raise ValueError(f"q must be [tokens, q_heads, head_dim]; got {tuple(q.shape)}")
     tokens, q_heads, dim = q.shape
     batch = _check_batch(cache, block_table, seq_lens, cu_seqlens, tokens)
-    _check_rows(q, "q", None, cache.head_dim, cache.device)
-    _refuse(q_heads < 1 or q_heads % cache.kv_heads != 0,
-            f"q_heads ({q_heads}) must be a multiple of the cache's {cache.kv_heads} heads")
+    device, arguments = cache.device, cache._arguments
+    heads = arguments[5]
+    q_strides = _check_rows(q, "q", None, arguments[7], device)
+    if q_heads < 1 or q_heads % heads != 0:
+        raise ValueError(f"q_heads ({q_heads}) must be a multiple of the cache's {heads} heads")
     if max_query_len is None:
         max_query_len = 1 if cu_seqlens is None else max(1, tokens)
-    _refuse(max_query_len < 1, f"max_query_len must be positive; got {max_query_len}")
-    scale = dim ** -0.5 if scale is None else float(scale)
-    _refuse(not math.isfinite(scale), f"scale must be finite; got {scale}")
+    elif max_query_len < 1:
+        raise ValueError(f"max_query_len must be positive; got {max_query_len}")
+    if scale is None:
+        scale = dim ** -0.5
+    elif not math.isfinite(scale):
+        raise ValueError(f"scale must be finite; got {scale}")
     if out is None:
-        out = torch.empty((tokens, q_heads, dim), dtype=q.dtype, device=q.device)
+        out = torch.empty((tokens, q_heads, dim), dtype=q.dtype, device=device)
+        out_strides = (q_heads * dim, dim)
     else:
-        _check_rows(out, "out", q_heads, dim, cache.device)
-        _refuse(out.shape != q.shape or out.dtype != q.dtype, "out must match q's shape and dtype")
-        _no_overlap_within(out, "out")
-    _require_gpu(cache.device)
-    with _on_device(cache.device) as stream:
-        lib = library()
-        need = lib.mxfp6_kv_cache_attention_workspace(
-            batch[-1], tokens, max_query_len, q_heads, cache.kv_heads, dim, _DTYPE_CODE[q.dtype],
-            batch[-2] * cache.page_size)
-        # Scratch of this call alone: the allocator keeps it apart between streams and graphs.
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-        check(lib.mxfp6_kv_cache_attention(
-            *cache._pointers(), *batch, q.data_ptr(), out.data_ptr(), _DTYPE_CODE[q.dtype], q_heads,
-            q.stride(0), q.stride(1), out.stride(0), out.stride(1), max_query_len, scale,
-            1 if causal else 0, _ptr(workspace), need, stream))
+        out_strides = _check_output_rows(out, "out", q, device)
+    lib = library()
+    code = _DTYPE_CODE[q.dtype]
+    need = lib.mxfp6_kv_cache_attention_workspace(batch[6], tokens, max_query_len, q_heads, heads, dim,
+                                                  code, batch[5] * arguments[6])
+    # Scratch of this call alone: the allocator keeps it apart between streams and graphs.
+    workspace = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
+    _launch(device, lib.mxfp6_kv_cache_attention, *arguments, *batch, q.data_ptr(), out.data_ptr(), code,
+            q_heads, q_strides[0], q_strides[1], out_strides[0], out_strides[1], max_query_len, scale,
+            1 if causal else 0, None if workspace is None else workspace.data_ptr(), need)
     return out
 
 
@@ -306,16 +336,21 @@ class RotaryFrequencies:
     adjacent: bool = False
 
     def __post_init__(self) -> None:
-        half = self.inv_freq.shape[0] if self.inv_freq.ndim == 1 else -1
-        _refuse(half < 8 or half % 8 != 0 or half > 128,
-                "inv_freq must be [rotary_dim / 2] with rotary_dim a multiple of 16 up to 256; got "
-                f"{tuple(self.inv_freq.shape)}")
-        _refuse(self.inv_freq.dtype != torch.float64, "inv_freq must be float64", TypeError)
-        _refuse(self.axis.dtype != torch.int32, "axis must be int32", TypeError)
-        _refuse(self.axis.shape != (half,), "axis must have the shape of inv_freq")
-        _refuse(self.axis.device != self.inv_freq.device, "axis must be on inv_freq's device")
-        _refuse(not (self.inv_freq.is_contiguous() and self.axis.is_contiguous()),
-                "inv_freq and axis must be contiguous")
+        inv, axis = self.inv_freq, self.axis
+        half = inv.shape[0] if inv.ndim == 1 else -1
+        if half < 8 or half % 8 != 0 or half > 128:
+            raise ValueError("inv_freq must be [rotary_dim / 2] with rotary_dim a multiple of 16 up to "
+                             f"256; got {tuple(inv.shape)}")
+        if inv.dtype != torch.float64:
+            raise TypeError("inv_freq must be float64")
+        if axis.dtype != torch.int32:
+            raise TypeError("axis must be int32")
+        if axis.shape != (half,):
+            raise ValueError("axis must have the shape of inv_freq")
+        if axis.device != inv.device:
+            raise ValueError("axis must be on inv_freq's device")
+        if not (inv.is_contiguous() and axis.is_contiguous()):
+            raise ValueError("inv_freq and axis must be contiguous")
 
     @property
     def rotary_dim(self) -> int:
@@ -361,46 +396,46 @@ def rotary_multi_axis(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
     Values behind ``rotary_dim`` are copied.  ``q_out`` / ``k_out`` may be ``q`` / ``k``
     themselves (in place); other overlaps are not allowed.
     """
-    _refuse(not isinstance(frequencies, RotaryFrequencies),
-            "frequencies must be a RotaryFrequencies instance", TypeError)
+    if not isinstance(frequencies, RotaryFrequencies):
+        raise TypeError("frequencies must be a RotaryFrequencies instance")
     device = q.device
-    _refuse(q.ndim != 3, f"q must be [tokens, heads, head_dim]; got {tuple(q.shape)}")
-    tokens, _, dim = q.shape
-    _check_rows(q, "q", None, dim, device)
-    _check_rows(k, "k", None, dim, device)
-    _refuse(k.shape[0] != tokens or k.dtype != q.dtype, "q and k must have one token count and dtype")
-    rotary_dim = frequencies.rotary_dim
-    _refuse(dim % 8 != 0 or rotary_dim > dim,
-            f"head_dim must be a multiple of 8 and at least rotary_dim ({rotary_dim}); got {dim}")
-    _refuse(frequencies.inv_freq.device != device, "frequencies must be on q's device")
+    if q.ndim != 3:
+        raise ValueError(f"q must be [tokens, heads, head_dim]; got {tuple(q.shape)}")
+    tokens, q_heads, dim = q.shape
+    q_strides = _check_rows(q, "q", None, dim, device)
+    k_strides = _check_rows(k, "k", None, dim, device)
+    if k.shape[0] != tokens or k.dtype is not q.dtype:
+        raise ValueError("q and k must have one token count and dtype")
+    inv_freq = frequencies.inv_freq
+    half = inv_freq.shape[0]
+    if dim % 8 != 0 or 2 * half > dim:
+        raise ValueError(f"head_dim must be a multiple of 8 and at least rotary_dim ({2 * half}); got {dim}")
+    if inv_freq.device != device:
+        raise ValueError("frequencies must be on q's device")
     if positions.ndim == 1:
         positions = positions.unsqueeze(0)
-    _refuse(positions.dtype not in (torch.int32, torch.int64), "positions must be int32 or int64",
-            TypeError)
-    _refuse(positions.ndim != 2 or not 1 <= positions.shape[0] <= 8 or positions.shape[1] != tokens
-            or (tokens > 1 and positions.stride(1) != 1),
-            f"positions must be [axes, {tokens}] with contiguous rows, 1 to 8 axes")
-    _refuse(positions.device != device, "positions must be on q's device")
-    outs = []
-    for x, y, name in ((q, q_out, "q_out"), (k, k_out, "k_out")):
-        if y is None:
-            y = torch.empty(x.shape, dtype=x.dtype, device=device)
-        elif y is not x:
-            _check_rows(y, name, x.shape[1], dim, device)
-            _refuse(y.shape != x.shape or y.dtype != x.dtype,
-                    f"{name} must match its input's shape and dtype")
-        _no_overlap_within(y, name)
-        _refuse(tokens > 0 and y.data_ptr() == x.data_ptr() and y.stride() != x.stride(),
-                f"{name} overlaps its input with other strides")
-        outs.append(y)
-    q_out, k_out = outs
-    _require_gpu(device)
-    with _on_device(device) as stream:
-        check(library().mxfp6_rotary_multi_axis(
-            q.data_ptr(), q_out.data_ptr(), q.shape[1], q.stride(0), q.stride(1), q_out.stride(0),
-            q_out.stride(1), k.data_ptr(), k_out.data_ptr(), k.shape[1], k.stride(0), k.stride(1),
-            k_out.stride(0), k_out.stride(1), _DTYPE_CODE[q.dtype], tokens, dim,
-            positions.data_ptr(), positions.stride(0), positions.shape[0],
-            1 if positions.dtype == torch.int64 else 0, frequencies.inv_freq.data_ptr(),
-            frequencies.axis.data_ptr(), rotary_dim // 2, 1 if frequencies.adjacent else 0, stream))
+    wide = positions.dtype == torch.int64
+    if not wide and positions.dtype != torch.int32:
+        raise TypeError("positions must be int32 or int64")
+    shape = positions.shape
+    if len(shape) != 2 or not 1 <= shape[0] <= 8 or shape[1] != tokens or (
+            tokens > 1 and positions.stride(1) != 1):
+        raise ValueError(f"positions must be [axes, {tokens}] with contiguous rows, 1 to 8 axes")
+    if positions.device != device:
+        raise ValueError("positions must be on q's device")
+    if q_out is None:
+        q_out = torch.empty((tokens, q_heads, dim), dtype=q.dtype, device=device)
+    if k_out is None:
+        k_out = torch.empty(k.shape, dtype=k.dtype, device=device)
+    q_out_strides = _check_output_rows(q_out, "q_out", q, device)
+    k_out_strides = _check_output_rows(k_out, "k_out", k, device)
+    q_at, k_at, q_out_at, k_out_at = q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr()
+    if tokens > 0 and ((q_at == q_out_at and q_strides != q_out_strides)
+                       or (k_at == k_out_at and k_strides != k_out_strides)):
+        raise ValueError("an output overlaps its input with other strides")
+    _launch(device, library().mxfp6_rotary_multi_axis, q_at, q_out_at, q_heads, q_strides[0], q_strides[1],
+            q_out_strides[0], q_out_strides[1], k_at, k_out_at, k.shape[1], k_strides[0], k_strides[1],
+            k_out_strides[0], k_out_strides[1], _DTYPE_CODE[q.dtype], tokens, dim, positions.data_ptr(),
+            positions.stride(0), shape[0], 1 if wide else 0, inv_freq.data_ptr(),
+            frequencies.axis.data_ptr(), half, 1 if frequencies.adjacent else 0)
     return q_out, k_out
