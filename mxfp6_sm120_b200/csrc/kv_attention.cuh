@@ -86,6 +86,75 @@ __device__ __forceinline__ float pow2_whole(float v) {
   return __uint_as_float((bits + 127u) << 23);
 }
 
+// Words of kBatch query rows, kPer values a lane: row n is at `base` plus lane r0 + n's `offset`.
+// All loads are issued before anything waits for one.
+template <int kBatch, int kPer>
+__device__ __forceinline__ void load_query_rows(const uint16_t* base, int64_t offset, int r0, int vector,
+                                                uint32_t (&raw)[kBatch][kPer / 2]) {
+  const uint16_t* src[kBatch];
+#pragma unroll
+  for (int n = 0; n < kBatch; ++n) src[n] = base + __shfl_sync(0xffffffffu, offset, r0 + n);
+  if (vector) {
+#pragma unroll
+    for (int n = 0; n < kBatch; ++n) {
+      if constexpr (kPer == 8) {
+        const uint4 v = *reinterpret_cast<const uint4*>(src[n]);
+        raw[n][0] = v.x;
+        raw[n][1] = v.y;
+        raw[n][2] = v.z;
+        raw[n][3] = v.w;
+      } else if constexpr (kPer == 4) {
+        const uint2 v = *reinterpret_cast<const uint2*>(src[n]);
+        raw[n][0] = v.x;
+        raw[n][1] = v.y;
+      } else {
+        raw[n][0] = *reinterpret_cast<const uint32_t*>(src[n]);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int n = 0; n < kBatch; ++n)
+#pragma unroll
+      for (int i = 0; i < kPer / 2; ++i) raw[n][i] = (uint32_t)src[n][2 * i] | (uint32_t)src[n][2 * i + 1] << 16;
+  }
+}
+
+// E4M3 terms of one row (kPer values a lane, zeros where `real` is false), times `sign`; returns
+// the power of two that they are to be multiplied by, NaN where the row has an infinity or NaN
+// (it has no scale: its scores become NaN).  By a full warp.
+template <class T, int kTerms, int kPer>
+__device__ __forceinline__ float query_terms(const uint32_t (&words)[kPer / 2], bool real, float sign,
+                                             uint32_t (&codes)[kTerms][kPer / 2]) {
+  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  constexpr uint32_t kInf = kBf16 ? 0x7f80u : 0x7c00u;
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < kPer / 2; ++i)
+    top = max(top, max(words[i] & 0x7fffu, (words[i] >> 16) & 0x7fffu));
+  top = __reduce_max_sync(0xffffffffu, real ? top : 0u);
+  const float most = kBf16 ? __uint_as_float(top << 16)
+                           : __half2float(__ushort_as_half((unsigned short)top));
+  const uint32_t bits = ue8m0_scale_bits_shift<8>(top < kInf ? most : 1.0f);
+  const float inverse = ue8m0_inverse(bits) * sign;
+#pragma unroll
+  for (int i = 0; i < kPer / 2; ++i) {
+    const uint32_t w = real ? words[i] : 0u;
+    float lo, hi;
+    if constexpr (kBf16) {
+      lo = __uint_as_float(w << 16);
+      hi = __uint_as_float(w & 0xffff0000u);
+    } else {
+      lo = __half2float(__ushort_as_half((unsigned short)w));
+      hi = __half2float(__ushort_as_half((unsigned short)(w >> 16)));
+    }
+    uint32_t t[kTerms];
+    e4m3_terms<kTerms>(lo * inverse, hi * inverse, t);
+#pragma unroll
+    for (int k = 0; k < kTerms; ++k) codes[k][i] = t[k];
+  }
+  return top < kInf ? __uint_as_float(bits) : NAN;
+}
+
 // A sequence as this kernel sees it: `tiles` is 0 when it has no rows or is another kernel's.
 struct KvSequence {
   int64_t row;  // first token row

@@ -551,52 +551,16 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       constexpr int kBatch = 4;      // rows in flight
 #pragma unroll 1
       for (int r0 = warp - kQueryWarp; r0 < RP; r0 += kBatch * kQueryWarps) {
-        __align__(16) uint16_t raw[kBatch][kPer];
+        // Row r0 + n * kQueryWarps is batch entry n.
+        uint32_t raw[kBatch][kPer / 2];
+        const int64_t offset = __shfl_sync(0xffffffffu, own_q, (r0 + lane * kQueryWarps) % 32);
+        load_query_rows<kBatch, kPer>(static_cast<const uint16_t*>(a.q) + lane * kPer, offset, 0, a.vector, raw);
 #pragma unroll
         for (int n = 0; n < kBatch; ++n) {
           const int r = r0 + n * kQueryWarps;
-          const T* src = static_cast<const T*>(a.q) + __shfl_sync(0xffffffffu, own_q, r) + lane * kPer;
-          if (r < rows) {
-            if (a.vector && kPer == 8) {
-              *reinterpret_cast<uint4*>(raw[n]) = *reinterpret_cast<const uint4*>(src);
-            } else if (a.vector && kPer == 4) {
-              *reinterpret_cast<uint2*>(raw[n]) = *reinterpret_cast<const uint2*>(src);
-            } else {
-#pragma unroll
-              for (int i = 0; i < kPer; ++i) raw[n][i] = reinterpret_cast<const uint16_t*>(src)[i];
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) raw[n][i] = 0;
-          }
-        }
-#pragma unroll
-        for (int n = 0; n < kBatch; ++n) {
-          const int r = r0 + n * kQueryWarps;
-          float v[kPer];
-          uint32_t top = 0;
-          constexpr uint32_t kInf = TERMS == 2 ? 0x7f80u : 0x7c00u;
-#pragma unroll
-          for (int i = 0; i < kPer; ++i) {
-            top = max(top, (uint32_t)(raw[n][i] & 0x7fffu));
-            if constexpr (TERMS == 2) v[i] = __uint_as_float((uint32_t)raw[n][i] << 16);
-            else v[i] = __half2float(__ushort_as_half(raw[n][i]));
-          }
-          top = __reduce_max_sync(0xffffffffu, top);
-          const float most = TERMS == 2 ? __uint_as_float(top << 16)
-                                        : __half2float(__ushort_as_half((unsigned short)top));
-          // A row with an infinity or NaN has no scale: its scores become NaN.
-          const uint32_t bits = ue8m0_scale_bits_shift<8>(top < kInf ? most : 1.0f);
-          const float inverse = ue8m0_inverse(bits);
-          if (lane == 0) seg.scale[r] = top < kInf ? __uint_as_float(bits) * a.scale_log2 : NAN;
           uint32_t codes[TERMS][kPer / 2];
-#pragma unroll
-          for (int i = 0; i < kPer / 2; ++i) {
-            uint32_t t[TERMS];
-            e4m3_terms<TERMS>(v[2 * i] * inverse, v[2 * i + 1] * inverse, t);
-#pragma unroll
-            for (int k = 0; k < TERMS; ++k) codes[k][i] = t[k];
-          }
+          const float scale = query_terms<T, TERMS, kPer>(raw[n], r < rows, 1.0f, codes);
+          if (lane == 0) seg.scale[r] = scale * a.scale_log2;
           const int d0 = lane * kPer;
 #pragma unroll
           for (int k = 0; k < TERMS; ++k) {

@@ -113,12 +113,35 @@ struct Place {
   int b, t, head, tile;
 };
 
-// Walks the items in the order sequence, row tile, head.  Returns the units of all items when
-// `at` is negative; else the number of the first tile at or behind unit `at`, its place and the
-// first unit of its item.  By a full warp.
-__device__ __forceinline__ int64_t warp_walk(const AttentionArgs& a, int64_t at, int lane,
-                                             Place* place, int64_t* item_begin) {
-  int64_t units = 0, tiles = 0;
+// Units of all items, by a full warp.
+__device__ __forceinline__ int64_t warp_total_units(const AttentionArgs& a, int lane) {
+  int64_t units = 0;  // of this lane's row tiles, one key head
+  for (int b0 = 0; b0 < a.batch.batch; b0 += 32) {
+    Sequence mine{};
+    if (b0 + lane < a.batch.batch) mine = load_sequence(a, b0 + lane);
+    unsigned todo = __ballot_sync(0xffffffffu, mine.rows > 0);
+    while (todo != 0) {
+      const int l = __ffs(todo) - 1;
+      todo &= todo - 1;
+      Sequence q;
+      q.first_position = __shfl_sync(0xffffffffu, mine.first_position, l);
+      q.rows = __shfl_sync(0xffffffffu, mine.rows, l);
+      q.length = __shfl_sync(0xffffffffu, mine.length, l);
+      const int row_tiles = (q.rows + kRows - 1) / kRows;
+      for (int t = lane; t < row_tiles; t += 32) units += tiles_of(a, q, t) + kItemUnits;
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) units += __shfl_xor_sync(0xffffffffu, units, o);
+  return units * a.cache.kv_heads;
+}
+
+// The first tile at or behind unit `at`, in the order sequence, row tile, head, by a full warp:
+// returns its number in the list of all tiles and, in all lanes, its place and the first unit of
+// its item.
+__device__ __forceinline__ int64_t warp_locate(const AttentionArgs& a, int64_t at, int lane,
+                                               Place* place, int64_t* item_begin) {
+  int64_t units = 0, tiles = 0;  // of all heads before this group of 32 row tiles
   const int heads = a.cache.kv_heads;
   for (int b0 = 0; b0 < a.batch.batch; b0 += 32) {
     Sequence mine{};
@@ -128,7 +151,6 @@ __device__ __forceinline__ int64_t warp_walk(const AttentionArgs& a, int64_t at,
       const int l = __ffs(todo) - 1;
       todo &= todo - 1;
       Sequence q;
-      q.row = 0;
       q.first_position = __shfl_sync(0xffffffffu, mine.first_position, l);
       q.rows = __shfl_sync(0xffffffffu, mine.rows, l);
       q.length = __shfl_sync(0xffffffffu, mine.length, l);
@@ -136,22 +158,21 @@ __device__ __forceinline__ int64_t warp_walk(const AttentionArgs& a, int64_t at,
       for (int t0 = 0; t0 < row_tiles; t0 += 32) {
         const int t = t0 + lane;
         const int n = t < row_tiles ? tiles_of(a, q, t) : 0;
-        int64_t upto = n > 0 ? (int64_t)(n + kItemUnits) * heads : 0, tiles_upto = (int64_t)n * heads;
+        // A tile count is below 2^23 (2^30 tokens), so 32 of them fit 32 bits.
+        int upto = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-          const int64_t u = __shfl_up_sync(0xffffffffu, upto, o);
-          const int64_t v = __shfl_up_sync(0xffffffffu, tiles_upto, o);
-          if (lane >= o) {
-            upto += u;
-            tiles_upto += v;
-          }
+          const int other = __shfl_up_sync(0xffffffffu, upto, o);
+          if (lane >= o) upto += other;
         }
-        const unsigned reached = __ballot_sync(0xffffffffu, at >= 0 && n > 0 && units + upto > at);
+        const int items = min(lane + 1, row_tiles - t0);
+        const int64_t units_upto = ((int64_t)upto + (int64_t)items * kItemUnits) * heads;
+        const unsigned reached = __ballot_sync(0xffffffffu, n > 0 && units + units_upto > at);
         if (reached != 0) {
           const int k = __ffs(reached) - 1;
           const int count = __shfl_sync(0xffffffffu, n, k);
           const int64_t per_item = count + kItemUnits;
-          const int64_t first = units + __shfl_sync(0xffffffffu, upto, k) - per_item * heads;
+          const int64_t first = units + __shfl_sync(0xffffffffu, units_upto, k) - per_item * heads;
           const int64_t into = at > first ? at - first : 0;
           place->b = b0 + l;
           place->t = t0 + k;
@@ -159,15 +180,25 @@ __device__ __forceinline__ int64_t warp_walk(const AttentionArgs& a, int64_t at,
           const int64_t in_item = into % per_item - kItemUnits;
           place->tile = in_item > 0 ? (int)in_item : 0;
           *item_begin = first + into / per_item * per_item;
-          return tiles + __shfl_sync(0xffffffffu, tiles_upto, k) - (int64_t)count * heads +
+          return tiles + (int64_t)(__shfl_sync(0xffffffffu, upto, k) - count) * heads +
                  (int64_t)place->head * count + place->tile;
         }
-        units += __shfl_sync(0xffffffffu, upto, 31);
-        tiles += __shfl_sync(0xffffffffu, tiles_upto, 31);
+        units += __shfl_sync(0xffffffffu, units_upto, 31);
+        tiles += (int64_t)__shfl_sync(0xffffffffu, upto, 31) * heads;
       }
     }
   }
-  return at < 0 ? units : tiles;
+  return tiles;
+}
+
+// What the joining kernel is told about the border behind each CTA's share; in the workspace,
+// before the partial rows.
+struct Border {
+  int b, t, head;
+  int parts;  // CTAs over which the item goes, 1: nothing to join here
+};
+__device__ __forceinline__ Border* borders_of(const AttentionArgs& a) {
+  return reinterpret_cast<Border*>(a.partials) - kSms;
 }
 
 // A place with its sequence, stepped from item to item.
@@ -286,20 +317,31 @@ kv_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
     ptx::tmem_relinquish();
   }
   ptx::grid_dependency_wait();
-  // From here on everything before this kernel has completed, also for the joining kernel, which
-  // reads the same lengths before it waits for this one.
   ptx::grid_launch_dependents();
   if (warp < 2) {
     // Warp 0 finds the first tile of this CTA, warp 1 the first of the next.
     Place p{};
-    int64_t begin;
-    const Share s = share_of(warp_walk(a, -1, lane, &p, &begin), (int)gridDim.x);
+    int64_t begin = 0, tile = 0;
+    const Share s = share_of(warp_total_units(a, lane), (int)gridDim.x);
     const int cta = (int)blockIdx.x + warp;
-    int64_t tile = 0;
-    if ((int)blockIdx.x < s.ctas && s.total > 0) tile = warp_walk(a, share_begin(s, cta), lane, &p, &begin);
+    if ((int)blockIdx.x < s.ctas && s.total > 0) tile = warp_locate(a, share_begin(s, cta), lane, &p, &begin);
     if (lane == 0) {
       share_smem[warp] = tile;
       if (warp == 0) start->at = p;
+    }
+    if (warp == 1 && (int)gridDim.x > 1 && (int)blockIdx.x + 1 < (int)gridDim.x) {
+      // For the joining kernel: the item in which the next share begins, and over how many CTAs
+      // it goes if its first tile is this CTA's.
+      Border* border = borders_of(a) + blockIdx.x;
+      int parts = 1;
+      if (cta < s.ctas && s.total > 0) {
+        const Sequence q = load_sequence(a, p.b);
+        const int64_t u0 = begin + kItemUnits, u1 = u0 + tiles_of(a, q, p.t) - 1;
+        // CTA of a unit: the last one whose share begins at or before it.
+        if ((int)(((u0 + 1) * s.ctas - 1) / s.total) == (int)blockIdx.x)
+          parts = (int)(((u1 + 1) * s.ctas - 1) / s.total) - (int)blockIdx.x + 1;
+      }
+      if (lane == 0) *border = Border{p.b, p.t, p.head, parts};
     }
   }
   ptx::tc_fence_before();
@@ -507,11 +549,18 @@ kv_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       const int tiles = min(left, c.tiles - c.at.tile);
       const int row0 = c.at.t * kRows;
       if (warp == kQueryWarp) {
+        // Eight lookups in flight.
         bool named = true;
-        const int64_t end = min((int64_t)c.seq.length, (int64_t)(c.at.tile + tiles) * kKvTile);
-        for (int64_t block = (int64_t)c.at.tile * kKvTileBlocks + lane * per_page; block * kKvBlock < end;
-             block += 32 * per_page)
-          named = named && kv_page(a.batch, a.cache, c.at.b, (int)block) >= 0;
+        const int end = (int)min((int64_t)c.seq.length, (int64_t)(c.at.tile + tiles) * kKvTile);
+        const int pages = (end + a.cache.page_size - 1) / a.cache.page_size;
+        const int32_t* table = a.batch.block_table + (int64_t)c.at.b * a.batch.table_stride;
+        for (int p0 = c.at.tile * kKvTile / a.cache.page_size + lane; p0 < pages; p0 += 8 * 32) {
+          int32_t id[8];
+#pragma unroll
+          for (int n = 0; n < 8; ++n) id[n] = p0 + 32 * n < pages ? table[p0 + 32 * n] : 0;
+#pragma unroll
+          for (int n = 0; n < 8; ++n) named = named && id[n] >= 0 && id[n] < a.cache.pages;
+        }
         named = __all_sync(0xffffffffu, named);
         if (lane == 0) {
           seg.row = c.seq.row;
@@ -534,54 +583,16 @@ kv_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       const int own = min(row0 + first_row + lane, c.seq.rows - 1);
       const int64_t own_q = (c.seq.row + own / a.group) * a.q_token_stride +
                             (int64_t)(c.at.head * a.group + own % a.group) * a.q_head_stride;
-      constexpr uint32_t kInf = TERMS == 2 ? 0x7f80u : 0x7c00u;
 #pragma unroll 1
       for (int r0 = 0; r0 < 32; r0 += kBatch) {
-        __align__(16) uint16_t raw[kBatch][kPer];
-#pragma unroll
-        for (int n = 0; n < kBatch; ++n) {
-          const T* src = static_cast<const T*>(a.q) + __shfl_sync(0xffffffffu, own_q, r0 + n) + lane * kPer;
-          if (row0 + first_row + r0 + n < c.seq.rows) {
-            if (a.vector && kPer == 8) {
-              *reinterpret_cast<uint4*>(raw[n]) = *reinterpret_cast<const uint4*>(src);
-            } else if (a.vector && kPer == 4) {
-              *reinterpret_cast<uint2*>(raw[n]) = *reinterpret_cast<const uint2*>(src);
-            } else {
-#pragma unroll
-              for (int i = 0; i < kPer; ++i) raw[n][i] = reinterpret_cast<const uint16_t*>(src)[i];
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) raw[n][i] = 0;
-          }
-        }
+        uint32_t raw[kBatch][kPer / 2];
+        load_query_rows<kBatch, kPer>(static_cast<const uint16_t*>(a.q) + lane * kPer, own_q, r0, a.vector, raw);
 #pragma unroll
         for (int n = 0; n < kBatch; ++n) {
           const int r = first_row + r0 + n;
-          uint32_t top = 0;
-#pragma unroll
-          for (int i = 0; i < kPer; ++i) top = max(top, (uint32_t)(raw[n][i] & 0x7fffu));
-          top = __reduce_max_sync(0xffffffffu, top);
-          const float most = TERMS == 2 ? __uint_as_float(top << 16)
-                                        : __half2float(__ushort_as_half((unsigned short)top));
-          // A row with an infinity or NaN has no scale: its scores become NaN.
-          const uint32_t bits = ue8m0_scale_bits_shift<8>(top < kInf ? most : 1.0f);
-          const float inverse = ue8m0_inverse(bits) * sign;
-          if (lane == 0) seg.scale[r] = top < kInf ? __uint_as_float(bits) * magnitude : NAN;
           uint32_t codes[TERMS][kPer / 2];
-#pragma unroll
-          for (int i = 0; i < kPer / 2; ++i) {
-            float v[2];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              if constexpr (TERMS == 2) v[e] = __uint_as_float((uint32_t)raw[n][2 * i + e] << 16);
-              else v[e] = __half2float(__ushort_as_half(raw[n][2 * i + e]));
-            }
-            uint32_t t[TERMS];
-            e4m3_terms<TERMS>(v[0] * inverse, v[1] * inverse, t);
-#pragma unroll
-            for (int k = 0; k < TERMS; ++k) codes[k][i] = t[k];
-          }
+          const float scale = query_terms<T, TERMS, kPer>(raw[n], row0 + r < c.seq.rows, sign, codes);
+          if (lane == 0) seg.scale[r] = scale * magnitude;
           const int d0 = lane * kPer, in_row = d0 % C::kRowBytes;
           const int swizzle = C::kRowBytes == 128 ? (r & 7) : ((r >> 1) & 3);
 #pragma unroll
@@ -623,7 +634,8 @@ kv_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
     for (int i0 = 0, segment = 0; i0 < count; ++segment) {
       wait(qfull, (uint32_t)segment & 1u, 510);
       const Segment& seg = segments[segment & 1];
-      const int tiles = failed ? 0 : seg.tiles, length = seg.length;
+      const int tiles = failed ? 0 : seg.tiles, length = seg.length, tile0 = seg.tile;
+      const bool all_named = seg.all_named != 0;
       // Above zero, so that a masked score (-inf) stays one where the scale is zero.
       const float factor = seg.scale[row] < 1e-30f ? 1e-30f : seg.scale[row];
       // Cached tokens that this row sees.
@@ -634,12 +646,12 @@ kv_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
 #pragma unroll 1
       for (int j = 0; j < tiles; ++j) {
         const int i = i0 + j, buffer = i % C::kBuffers;
-        const int t0 = (seg.tile + j) * kKvTile + half * 64;  // this thread's first token
+        const int t0 = (tile0 + j) * kKvTile + half * 64;  // this thread's first token
         unsigned named = 3u;  // which of the thread's two blocks are on a page
-        if (!seg.all_named) {
+        if (!all_named) {
           named = 0;
           for (int kb = 0; kb < 2; ++kb) {
-            const int block = (seg.tile + j) * kKvTileBlocks + half * 2 + kb;
+            const int block = (tile0 + j) * kKvTileBlocks + half * 2 + kb;
             if (block * kKvBlock < length && kv_page(a.batch, a.cache, seg.b, block) >= 0) named |= 1u << kb;
           }
         }
@@ -680,15 +692,29 @@ kv_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
               if (e >= n) raw[kb][e] = 0xff800000u;  // -inf
           }
         }
-        uint32_t codes[2][TERMS][8];
         float top[2], part[2];
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
-          float m = -INFINITY;
+          float m0 = -INFINITY, m1 = -INFINITY;
 #pragma unroll
-          for (int e = 0; e < 32; e += 2)
-            m = fmaxf(m, fmaxf(__uint_as_float(raw[kb][e]), __uint_as_float(raw[kb][e + 1])));
-          top[kb] = rintf(m * factor);  // nearest power of two: the largest weight is in (181, 363)
+          for (int e = 0; e < 32; e += 4) {
+            m0 = fmaxf(m0, fmaxf(__uint_as_float(raw[kb][e]), __uint_as_float(raw[kb][e + 1])));
+            m1 = fmaxf(m1, fmaxf(__uint_as_float(raw[kb][e + 2]), __uint_as_float(raw[kb][e + 3])));
+          }
+          // To the nearest power of two: the largest weight is in (181, 363).
+          top[kb] = rintf(fmaxf(m0, m1) * factor);
+        }
+        // The reference moves only where a block exceeds it by much, or was not set: the two
+        // warps that share the rows agree.  The answer is not needed before the weights are done.
+        volatile int* asked = ask_flag + quarter * 2 + (votes++ & 1u);
+        const bool ask = __any_sync(0xffffffffu, fmaxf(top[0], top[1]) > ref + kMostLog2);
+        if (lane == 0) {
+          if (ask) *asked = 1;
+          ptx::mbar_arrive(vsync);
+        }
+        uint32_t codes[2][TERMS][8];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
           const float base = fmaxf(top[kb], -1e30f) - kWeightLog2;
           float s0 = 0.0f, s1 = 0.0f;
 #pragma unroll
@@ -706,14 +732,6 @@ kv_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
             for (int k = 0; k < TERMS; ++k) codes[kb][k][e / 4] = __byte_perm(lo[k], hi[k], 0x5410);
           }
           part[kb] = s0 + s1;
-        }
-        // The reference moves only where a block exceeds it by much, or was not set: the two
-        // warps that share the rows agree.
-        volatile int* asked = ask_flag + quarter * 2 + (votes++ & 1u);
-        const bool ask = __any_sync(0xffffffffu, fmaxf(top[0], top[1]) > ref + kMostLog2);
-        if (lane == 0) {
-          if (ask) *asked = 1;
-          ptx::mbar_arrive(vsync);
         }
         // P of the tile before last (or of the last one) has been read.
         if (i >= C::kBuffers)
@@ -887,37 +905,15 @@ constexpr int kJoinThreads = 256;
 
 template <int D, int TERMS>
 __global__ void __launch_bounds__(kJoinThreads)
-kv_prefill_join_kernel(const AttentionArgs a, int grid) {
+kv_prefill_join_kernel(const AttentionArgs a) {
   using C = PrefillCfg<D, TERMS>;
   using T = typename std::conditional<TERMS == 2, __nv_bfloat16, __half>::type;
   constexpr int kColumns = D / 4;                   // four values a thread
   constexpr int kAtOnce = kJoinThreads / kColumns;  // rows
-  __shared__ Place item;
-  __shared__ int item_parts;
-  const int c0 = (int)blockIdx.x, tid = threadIdx.x, lane = tid & 31;
-  if (tid < 32) {
-    Place p{};
-    int64_t begin = 0;
-    const Share s = share_of(warp_walk(a, -1, lane, &p, &begin), grid);
-    int parts = 1;
-    if (c0 + 1 < s.ctas && s.total > 0) {
-      warp_walk(a, share_begin(s, c0 + 1), lane, &p, &begin);
-      Cursor c;
-      c.at = p;
-      c.load(a);
-      const int64_t u0 = begin + kItemUnits, u1 = u0 + c.tiles - 1;
-      // CTA of a unit: the last one whose share begins at or before it.
-      if ((int)(((u0 + 1) * s.ctas - 1) / s.total) == c0)
-        parts = (int)(((u1 + 1) * s.ctas - 1) / s.total) - c0 + 1;
-    }
-    if (lane == 0) {
-      item = p;
-      item_parts = parts;
-    }
-  }
-  __syncthreads();
-  const int parts = item_parts;
+  const int c0 = (int)blockIdx.x, tid = threadIdx.x;
   ptx::grid_dependency_wait();
+  const Border item = borders_of(a)[c0];
+  const int parts = item.parts;
   if (parts == 1) return;
   const Sequence seq = load_sequence(a, item.b);
   const int column = tid % kColumns;
@@ -991,7 +987,7 @@ int launch(const CUtensorMap& tm_k, const CUtensorMap& tm_v, const AttentionArgs
   config.gridDim = dim3((unsigned)(grid - 1), kRows / kJoinRows);
   config.blockDim = dim3(kJoinThreads);
   config.dynamicSmemBytes = 0;
-  MX_CUDA(cudaLaunchKernelEx(&config, kv_prefill_join_kernel<D, TERMS>, a, grid));
+  MX_CUDA(cudaLaunchKernelEx(&config, kv_prefill_join_kernel<D, TERMS>, a));
   return kOk;
 }
 
@@ -1008,11 +1004,15 @@ int kv_prefill_grid(int64_t batch, int64_t tokens, int kv_heads, int group, int6
 int64_t kv_prefill_workspace(int64_t batch, int64_t tokens, int kv_heads, int group, int head_dim,
                              int64_t max_context) {
   const int grid = kv_prefill_grid(batch, tokens, kv_heads, group, max_context);
-  return grid == 1 ? 0 : (int64_t)grid * 2 * (kRows * head_dim + 2 * kRows) * 4;
+  return grid == 1 ? 0 : kSms * (int64_t)sizeof(Border) +
+                             (int64_t)grid * 2 * (kRows * head_dim + 2 * kRows) * 4;
 }
 
 // Sequences with more than a.min_rows rows (tokens x group).
-int launch_kv_prefill(const AttentionArgs& a, int dtype, cudaStream_t stream) {
+int launch_kv_prefill(const AttentionArgs& args, int dtype, cudaStream_t stream) {
+  AttentionArgs a = args;
+  static_assert(sizeof(Border) % 16 == 0, "partial rows stay aligned");
+  a.partials = reinterpret_cast<float*>(reinterpret_cast<Border*>(args.partials) + kSms);
   CUtensorMap tm_k, tm_v;
   if (int rc = make_kv_map(&tm_k, a.cache.k_values, a.cache)) return rc;
   if (int rc = make_kv_map(&tm_v, a.cache.v_values, a.cache)) return rc;
