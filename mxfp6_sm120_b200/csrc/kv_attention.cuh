@@ -45,29 +45,8 @@ struct AttentionArgs {
 int make_kv_map(CUtensorMap* map, const uint8_t* values, const KvCache& cache);
 
 #ifdef __CUDACC__
-__device__ __forceinline__ uint32_t e4m3x2(float a, float b) {  // a in the low byte
-  return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
-}
-__device__ __forceinline__ float2 e4m3x2_values(uint32_t codes) {
-  return __half22float2(__half2(
-      __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(codes & 0xffffu), __NV_E4M3)));
-}
-
-// E4M3 terms of two values: codes[t] holds both in its low sixteen bits.
-template <int kTerms>
-__device__ __forceinline__ void e4m3_terms(float a, float b, uint32_t (&codes)[kTerms]) {
-#pragma unroll
-  for (int t = 0; t < kTerms; ++t) {
-    codes[t] = e4m3x2(a, b);
-    if (t + 1 < kTerms) {
-      const float2 v = e4m3x2_values(codes[t]);
-      a = (a - v.x) * 16.0f;
-      b = (b - v.y) * 16.0f;
-    }
-  }
-}
-
-// The same of two FP16 numbers (their remainders are exact in FP16).
+// E4M3 terms of two FP16 numbers: codes[t] holds both in its low sixteen bits.  The remainders
+// are exact in FP16.
 template <int kTerms>
 __device__ __forceinline__ void e4m3_terms_half(__half2 x, uint32_t (&codes)[kTerms]) {
 #pragma unroll
@@ -119,12 +98,11 @@ __device__ __forceinline__ void load_query_rows(const uint16_t* base, int64_t of
   }
 }
 
-// E4M3 terms of one row (kPer values a lane, zeros where `real` is false), times `sign`; returns
-// the power of two that they are to be multiplied by, NaN where the row has an infinity or NaN
-// (it has no scale: its scores become NaN).  By a full warp.
-template <class T, int kTerms, int kPer>
-__device__ __forceinline__ float query_terms(const uint32_t (&words)[kPer / 2], bool real, float sign,
-                                             uint32_t (&codes)[kTerms][kPer / 2]) {
+// Power of two that takes a row's largest magnitude (kPer values a lane, a row of zeros where
+// `real` is false) to E4M3's largest; NaN where it has an infinity or NaN: it has no scale, and
+// its scores become NaN.  By a full warp.
+template <class T, int kPer>
+__device__ __forceinline__ float query_scale(const uint32_t (&words)[kPer / 2], bool real) {
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr uint32_t kInf = kBf16 ? 0x7f80u : 0x7c00u;
   uint32_t top = 0;
@@ -134,11 +112,19 @@ __device__ __forceinline__ float query_terms(const uint32_t (&words)[kPer / 2], 
   top = __reduce_max_sync(0xffffffffu, real ? top : 0u);
   const float most = kBf16 ? __uint_as_float(top << 16)
                            : __half2float(__ushort_as_half((unsigned short)top));
-  const uint32_t bits = ue8m0_scale_bits_shift<8>(top < kInf ? most : 1.0f);
-  const float inverse = ue8m0_inverse(bits) * sign;
+  return top < kInf ? __uint_as_float(ue8m0_scale_bits_shift<8>(most)) : NAN;
+}
+
+// E4M3 terms of the row over its scale, times `sign`.  The scaled values go through FP16, which
+// holds them exactly down to 2^-14 (2^-23 of the row's largest) and rounds what is below.
+template <class T, int kTerms, int kPer>
+__device__ __forceinline__ void query_terms(const uint32_t (&words)[kPer / 2], bool real, float scale,
+                                            float sign, uint32_t (&codes)[kTerms][kPer / 2]) {
+  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  const float inverse = real && scale == scale ? ue8m0_inverse(__float_as_uint(scale)) * sign : 0.0f;
 #pragma unroll
   for (int i = 0; i < kPer / 2; ++i) {
-    const uint32_t w = real ? words[i] : 0u;
+    const uint32_t w = words[i];
     float lo, hi;
     if constexpr (kBf16) {
       lo = __uint_as_float(w << 16);
@@ -148,11 +134,10 @@ __device__ __forceinline__ float query_terms(const uint32_t (&words)[kPer / 2], 
       hi = __half2float(__ushort_as_half((unsigned short)(w >> 16)));
     }
     uint32_t t[kTerms];
-    e4m3_terms<kTerms>(lo * inverse, hi * inverse, t);
+    e4m3_terms_half<kTerms>(__floats2half2_rn(lo * inverse, hi * inverse), t);
 #pragma unroll
     for (int k = 0; k < kTerms; ++k) codes[k][i] = t[k];
   }
-  return top < kInf ? __uint_as_float(bits) : NAN;
 }
 
 // A sequence as this kernel sees it: `tiles` is 0 when it has no rows or is another kernel's.

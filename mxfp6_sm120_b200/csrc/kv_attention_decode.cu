@@ -555,12 +555,20 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         uint32_t raw[kBatch][kPer / 2];
         const int64_t offset = __shfl_sync(0xffffffffu, own_q, (r0 + lane * kQueryWarps) % 32);
         load_query_rows<kBatch, kPer>(static_cast<const uint16_t*>(a.q) + lane * kPer, offset, 0, a.vector, raw);
+        // All maxima first: the rows' conversions then overlap.
+        float scale[kBatch];
+#pragma unroll
+        for (int n = 0; n < kBatch; ++n)
+          scale[n] = query_scale<T, kPer>(raw[n], r0 + n * kQueryWarps < rows);
+        float mine = scale[0];
+#pragma unroll
+        for (int n = 1; n < kBatch; ++n) mine = lane == n ? scale[n] : mine;
+        if (lane < kBatch) seg.scale[r0 + lane * kQueryWarps] = mine * a.scale_log2;
 #pragma unroll
         for (int n = 0; n < kBatch; ++n) {
           const int r = r0 + n * kQueryWarps;
           uint32_t codes[TERMS][kPer / 2];
-          const float scale = query_terms<T, TERMS, kPer>(raw[n], r < rows, 1.0f, codes);
-          if (lane == 0) seg.scale[r] = scale * a.scale_log2;
+          query_terms<T, TERMS, kPer>(raw[n], r < rows, scale[n], 1.0f, codes);
           const int d0 = lane * kPer;
 #pragma unroll
           for (int k = 0; k < TERMS; ++k) {

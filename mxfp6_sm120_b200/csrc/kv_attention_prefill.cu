@@ -13,9 +13,12 @@
 //    score of each block of 32 tokens, rounded to a power of two, and that power relative to the
 //    row's reference is the block scale of P.  No maximum crosses threads and the output is not
 //    rescaled, except where a block exceeds the reference by more than 2^16.
-//  * Warps: 0-7 softmax (a thread holds 64 scores of one row, two scale blocks), 8 TMA, 9 MMA,
-//    10-13 turn the next rows into E4M3 terms as soon as the last scores of the rows before are
-//    out.  Scores of tile j + 1 are issued before the output of tile j.
+//  * Warps: 0-15 softmax (a thread holds the 32 scores of one row and scale block; with eight warps
+//    of 64 scores the waits and loads of a tile did not overlap its exponentials), 16 TMA, 17 MMA,
+//    18 copies the next item's rows to where its terms will be, as soon as the last scores of the
+//    item before are out (bulk copies: loads into the registers of a few warps, at the latency that
+//    memory has under this kernel, took 10 us an item); the softmax warps turn them into terms.
+//    Scores of tile j + 1 are issued before the output of tile j.
 //  * Work: the list of (sequence, row tile, key head) with its tiles of cached tokens is cut into
 //    equal shares, one per SM; an item that is cut leaves partial rows, which a second kernel
 //    joins in the order of the tiles.
@@ -26,9 +29,9 @@
 namespace mx {
 namespace {
 
-constexpr int kThreads = 448;
-constexpr int kSoftmaxWarps = 8;
-constexpr int kTmaWarp = 8, kMmaWarp = 9, kQueryWarp = 10, kQueryWarps = 4;
+constexpr int kThreads = 608;
+constexpr int kSoftmaxWarps = 16;
+constexpr int kTmaWarp = 16, kMmaWarp = 17, kQueryWarp = 18;
 constexpr int kRows = 128;            // rows of an item
 constexpr float kWeightLog2 = 8.0f;   // weights are scaled by 256 before they become E4M3 terms
 constexpr float kMostLog2 = 16.0f;    // a block may exceed the reference by 2^16
@@ -46,7 +49,7 @@ struct PrefillCfg {
   static constexpr int kPBytes = TERMS * kRows * kKvTile;
   // A head of 256 leaves room for one score tile in tensor memory and one P in shared memory.
   static constexpr int kBuffers = D == 256 ? 1 : 2;
-  static constexpr int kFixedBytes = 10240;
+  static constexpr int kFixedBytes = 11264;
   static constexpr int kBudget = 227 * 1024 - 1024;
   static constexpr int kFit = (kBudget - kFixedBytes - kQBytes - kBuffers * kPBytes) / (kSlotBytes + 512);
   static constexpr int kSlots = kFit > 8 ? 8 : kFit;
@@ -264,14 +267,14 @@ kv_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   uint8_t* term_sf = fixed + 512;                        // [term] atoms of 1, 1/16, 1/256
   uint8_t* p_sf = term_sf + 3 * 512;                     // [buffer][term]
   Segment* segments = reinterpret_cast<Segment*>(p_sf + 6 * 512);  // two
-  float* row_sum = reinterpret_cast<float*>(segments + 2);         // [half][row]
-  float* row_top = row_sum + 2 * kRows;                            // [half][row]
-  Cursor* start = reinterpret_cast<Cursor*>(row_top + 2 * kRows);
+  float* row_sum = reinterpret_cast<float*>(segments + 2);         // [block][row]
+  float* row_top = row_sum + 4 * kRows;                            // [block][row]
+  Cursor* start = reinterpret_cast<Cursor*>(row_top + 4 * kRows);
   int64_t* share_smem = reinterpret_cast<int64_t*>(start + 1);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(share_smem + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* ask_flag = abort_flag + 1;               // [quarter][2]
-  static_assert(512 + 9 * 512 + 2 * sizeof(Segment) + 4 * kRows * 4 + sizeof(Cursor) + 16 + 8 + 32 <=
+  static_assert(512 + 9 * 512 + 2 * sizeof(Segment) + 8 * kRows * 4 + sizeof(Cursor) + 16 + 8 + 32 <=
                     C::kFixedBytes,
                 "fixed area");
 
@@ -283,9 +286,10 @@ kv_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   const uint32_t pfull0 = sread0 + 16;
   const uint32_t pvdone0 = pfull0 + 16;
   const uint32_t sdone0 = pvdone0 + 16;  // softmax has left a segment (by its parity)
-  const uint32_t qfull = sdone0 + 16, qfree = qfull + 8;
-  const uint32_t vsync0 = qfree + 8;     // four: the two warps of a lane quarter
-  static_assert(8 * (2 * 8 + 10 + 2 + 4) <= 512, "barriers");
+  const uint32_t qraw = sdone0 + 16;     // an item's rows have been copied
+  const uint32_t qfull = qraw + 8, qfree = qfull + 8;
+  const uint32_t vsync0 = qfree + 8;     // four: the four warps of a lane quarter
+  static_assert(8 * (2 * 8 + 10 + 3 + 4) <= 512, "barriers");
 
   if (threadIdx.x == 0) {
     *abort_flag = 0;
@@ -301,9 +305,10 @@ kv_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       ptx::mbar_init(pvdone0 + 8 * i, 1);
       ptx::mbar_init(sdone0 + 8 * i, kSoftmaxWarps);
     }
-    ptx::mbar_init(qfull, kQueryWarps);
+    ptx::mbar_init(qraw, 2);  // the copies' bytes, and the description
+    ptx::mbar_init(qfull, kSoftmaxWarps);
     ptx::mbar_init(qfree, 1);
-    for (int i = 0; i < 4; ++i) ptx::mbar_init(vsync0 + 8 * i, 2);
+    for (int i = 0; i < 4; ++i) ptx::mbar_init(vsync0 + 8 * i, 4);
     ptx::fence_mbar_init();
     ptx::prefetch_tensormap(&tm_k);
     ptx::prefetch_tensormap(&tm_v);
@@ -528,13 +533,11 @@ kv_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       }
       i0 += tiles;
     }
-  } else if (count > 0 && warp >= kQueryWarp) {
-    // ---------------- query terms ----------------
+  } else if (count > 0 && warp == kQueryWarp) {
+    // ---------------- rows and descriptions of the segments ----------------
     Cursor c = *start;
     c.load(a);
     bool ok = true;
-    const float sign = a.scale_log2 < 0.0f ? -1.0f : 1.0f;  // the softmax takes a factor >= 0
-    const float magnitude = fabsf(a.scale_log2);
     for (int left = count, segment = 0; ok && left > 0; ++segment) {
       // The rows' buffer is free with the last scores of the segment before, the description with
       // the end of the one before that.
@@ -547,53 +550,102 @@ kv_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       if (!ok) break;
       Segment& seg = segments[segment & 1];
       const int tiles = min(left, c.tiles - c.at.tile);
-      const int row0 = c.at.t * kRows;
-      if (warp == kQueryWarp) {
-        // Eight lookups in flight.
-        bool named = true;
-        const int end = (int)min((int64_t)c.seq.length, (int64_t)(c.at.tile + tiles) * kKvTile);
-        const int pages = (end + a.cache.page_size - 1) / a.cache.page_size;
-        const int32_t* table = a.batch.block_table + (int64_t)c.at.b * a.batch.table_stride;
-        for (int p0 = c.at.tile * kKvTile / a.cache.page_size + lane; p0 < pages; p0 += 8 * 32) {
-          int32_t id[8];
-#pragma unroll
-          for (int n = 0; n < 8; ++n) id[n] = p0 + 32 * n < pages ? table[p0 + 32 * n] : 0;
-#pragma unroll
-          for (int n = 0; n < 8; ++n) named = named && id[n] >= 0 && id[n] < a.cache.pages;
-        }
-        named = __all_sync(0xffffffffu, named);
-        if (lane == 0) {
-          seg.row = c.seq.row;
-          seg.first_position = c.seq.first_position;
-          seg.rows = c.seq.rows;
-          seg.row0 = row0;
-          seg.length = c.seq.length;
-          seg.head = c.at.head;
-          seg.tile = c.at.tile;
-          seg.tiles = tiles;
-          seg.whole = c.at.tile == 0 && tiles == c.tiles;
-          seg.b = c.at.b;
-          seg.all_named = named;
+      const int row0 = c.at.t * kRows, rows = min(kRows, c.seq.rows - row0);
+      if (lane == 0) ptx::mbar_arrive_expect_tx(qraw, a.vector ? (uint32_t)(rows * 2 * D) : 0u);
+      __syncwarp();
+      for (int n = lane; n < rows; n += 32) {
+        const int r = row0 + n;
+        const uint16_t* src = static_cast<const uint16_t*>(a.q) + (c.seq.row + r / a.group) * a.q_token_stride +
+                              (int64_t)(c.at.head * a.group + r % a.group) * a.q_head_stride;
+        if (a.vector) {
+          ptx::bulk_load(ptx::smem_u32(q_tiles + n * 2 * D), src, 2 * D, qraw);
+        } else {
+          for (int d = 0; d < D; ++d) reinterpret_cast<uint16_t*>(q_tiles)[n * D + d] = src[d];
         }
       }
-      constexpr int kPer = D / 32;  // values per lane
-      constexpr int kBatch = 8;     // rows in flight
-      // Lane l: where row 32 * (warp - kQueryWarp) + l is read.
-      const int first_row = (warp - kQueryWarp) * 32;
-      const int own = min(row0 + first_row + lane, c.seq.rows - 1);
-      const int64_t own_q = (c.seq.row + own / a.group) * a.q_token_stride +
-                            (int64_t)(c.at.head * a.group + own % a.group) * a.q_head_stride;
-#pragma unroll 1
-      for (int r0 = 0; r0 < 32; r0 += kBatch) {
-        uint32_t raw[kBatch][kPer / 2];
-        load_query_rows<kBatch, kPer>(static_cast<const uint16_t*>(a.q) + lane * kPer, own_q, r0, a.vector, raw);
+      // Are all pages named?  Eight lookups in flight.
+      bool named = true;
+      const int end = (int)min((int64_t)c.seq.length, (int64_t)(c.at.tile + tiles) * kKvTile);
+      const int pages = (end + a.cache.page_size - 1) / a.cache.page_size;
+      const int32_t* table = a.batch.block_table + (int64_t)c.at.b * a.batch.table_stride;
+      for (int p0 = c.at.tile * kKvTile / a.cache.page_size + lane; p0 < pages; p0 += 8 * 32) {
+        int32_t id[8];
+#pragma unroll
+        for (int n = 0; n < 8; ++n) id[n] = p0 + 32 * n < pages ? table[p0 + 32 * n] : 0;
+#pragma unroll
+        for (int n = 0; n < 8; ++n) named = named && id[n] >= 0 && id[n] < a.cache.pages;
+      }
+      named = __all_sync(0xffffffffu, named);
+      if (lane == 0) {
+        seg.row = c.seq.row;
+        seg.first_position = c.seq.first_position;
+        seg.rows = c.seq.rows;
+        seg.row0 = row0;
+        seg.length = c.seq.length;
+        seg.head = c.at.head;
+        seg.tile = c.at.tile;
+        seg.tiles = tiles;
+        seg.whole = c.at.tile == 0 && tiles == c.tiles;
+        seg.b = c.at.b;
+        seg.all_named = named;
+      }
+      __syncwarp();  // the rows and the description are complete
+      if (lane == 0) ptx::mbar_arrive(qraw);
+      left -= tiles;
+      if (left > 0) c.next_item(a);
+    }
+  } else if (count > 0 && warp < kSoftmaxWarps) {
+    // ---------------- softmax: a thread has 32 tokens of one row ----------------
+    // A wait that runs out ends the warp's tiles, and the vote at the end of the segment ends all.
+    const int quarter = warp & 3, block = warp >> 2;  // rows, and scale block of the tile
+    const int row = quarter * 32 + lane;              // of the item
+    const uint32_t lane_t = tmem + ((uint32_t)(quarter * 32) << 16);
+    const uint32_t vsync = vsync0 + 8 * quarter;
+    uint8_t* p_row = p_tiles + row * kKvTile;
+    uint8_t* p_sf_row = p_sf + lane * 16 + quarter * 4 + block;
+    bool failed = false;
+    uint32_t syncs = 0, votes = 0;
+    auto wait = [&](uint32_t bar, uint32_t parity, int code) {
+      if (!failed) failed = !__all_sync(0xffffffffu, bounded_wait(bar, parity, abort_flag, a.status, code));
+    };
+    // The four warps of a quarter meet.
+    auto meet = [&](int code) {
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(vsync);
+      wait(vsync, syncs & 1u, code);
+      ++syncs;
+    };
+    int at0 = 0;  // place of the segment in the order of the copies
+    for (int i0 = 0, segment = 0; i0 < count; ++segment) {
+      wait(qraw, (uint32_t)segment & 1u, 510);
+      Segment& seg = segments[segment & 1];
+      {
+        // Eight rows a warp: their words leave shared memory before any terms replace them.
+        constexpr int kPer = D / 32, kBatch = kRows / kSoftmaxWarps;
+        const int first_row = warp * kBatch, real = failed ? 0 : seg.rows - seg.row0;
+        uint32_t words[kBatch][kPer / 2];
+        float scale[kBatch];
 #pragma unroll
         for (int n = 0; n < kBatch; ++n) {
-          const int r = first_row + r0 + n;
+          const uint32_t* src = reinterpret_cast<const uint32_t*>(q_tiles + (first_row + n) * 2 * D) + lane * (kPer / 2);
+#pragma unroll
+          for (int w = 0; w < kPer / 2; ++w) words[n][w] = src[w];
+        }
+#pragma unroll
+        for (int n = 0; n < kBatch; ++n) scale[n] = query_scale<T, kPer>(words[n], first_row + n < real);
+        failed = ptx::barrier_any(1, kSoftmaxWarps * 32, failed);
+        if (failed) break;
+        float mine = scale[0];
+#pragma unroll
+        for (int n = 1; n < kBatch; ++n) mine = lane == n ? scale[n] : mine;
+        if (lane < kBatch) seg.scale[first_row + lane] = mine * fabsf(a.scale_log2);
+        const float sign = a.scale_log2 < 0.0f ? -1.0f : 1.0f;  // the softmax takes a factor >= 0
+        const int d0 = lane * kPer, in_row = d0 % C::kRowBytes;
+#pragma unroll
+        for (int n = 0; n < kBatch; ++n) {
+          const int r = first_row + n;
           uint32_t codes[TERMS][kPer / 2];
-          const float scale = query_terms<T, TERMS, kPer>(raw[n], row0 + r < c.seq.rows, sign, codes);
-          if (lane == 0) seg.scale[r] = scale * magnitude;
-          const int d0 = lane * kPer, in_row = d0 % C::kRowBytes;
+          query_terms<T, TERMS, kPer>(words[n], r < real, scale[n], sign, codes);
           const int swizzle = C::kRowBytes == 128 ? (r & 7) : ((r >> 1) & 3);
 #pragma unroll
           for (int k = 0; k < TERMS; ++k) {
@@ -609,31 +661,11 @@ kv_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
             }
           }
         }
+        ptx::fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(qfull);
+        wait(qfull, (uint32_t)segment & 1u, 520);  // the other warps' scales
       }
-      ptx::fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(qfull);
-      left -= tiles;
-      if (left > 0) c.next_item(a);
-    }
-  } else if (count > 0 && warp < kSoftmaxWarps) {
-    // ---------------- softmax: a thread has 64 tokens of one row ----------------
-    // A wait that runs out ends the warp's tiles, and the vote at the end of the segment ends all.
-    const int quarter = warp & 3, half = warp >> 2;
-    const int row = quarter * 32 + lane;  // of the item
-    const uint32_t lane_t = tmem + ((uint32_t)(quarter * 32) << 16);
-    const uint32_t vsync = vsync0 + 8 * quarter;
-    uint8_t* p_row = p_tiles + row * kKvTile;
-    uint8_t* p_sf_row = p_sf + lane * 16 + quarter * 4 + half * 2;  // two bytes: this thread's blocks
-    bool failed = false;
-    uint32_t syncs = 0, votes = 0;
-    auto wait = [&](uint32_t bar, uint32_t parity, int code) {
-      if (!failed) failed = !__all_sync(0xffffffffu, bounded_wait(bar, parity, abort_flag, a.status, code));
-    };
-    int at0 = 0;  // place of the segment in the order of the copies
-    for (int i0 = 0, segment = 0; i0 < count; ++segment) {
-      wait(qfull, (uint32_t)segment & 1u, 510);
-      const Segment& seg = segments[segment & 1];
       const int tiles = failed ? 0 : seg.tiles, length = seg.length, tile0 = seg.tile;
       const bool all_named = seg.all_named != 0;
       // Above zero, so that a masked score (-inf) stays one where the scale is zero.
@@ -646,27 +678,20 @@ kv_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
 #pragma unroll 1
       for (int j = 0; j < tiles; ++j) {
         const int i = i0 + j, buffer = i % C::kBuffers;
-        const int t0 = (tile0 + j) * kKvTile + half * 64;  // this thread's first token
-        unsigned named = 3u;  // which of the thread's two blocks are on a page
-        if (!all_named) {
-          named = 0;
-          for (int kb = 0; kb < 2; ++kb) {
-            const int block = (tile0 + j) * kKvTileBlocks + half * 2 + kb;
-            if (block * kKvBlock < length && kv_page(a.batch, a.cache, seg.b, block) >= 0) named |= 1u << kb;
-          }
-        }
-        if (named != 3u || t0 + 64 > length) {
+        const int t0 = (tile0 + j) * kKvTile + block * kKvBlock;  // this thread's first token
+        const bool named = all_named || (t0 < length && kv_page(a.batch, a.cache, seg.b, t0 / kKvBlock) >= 0);
+        if (!named || t0 + kKvBlock > length) {
           // Rows of V without a token may hold anything, NaN among them, and 0 * NaN is NaN: clear
-          // them once the tile has landed.  The four warps of a half clear sixteen rows each.
+          // them once the tile has landed.  The four warps of a block clear eight rows each.
           const int at = at0 + (j + 1 < tiles ? 2 * j + 2 : 2 * j + 1);
           const int slot = at % C::kSlots;
           wait(full0 + 8 * slot, (uint32_t)(at / C::kSlots) & 1u, 511);
           uint8_t* v_s = slots + slot * C::kSlotBytes;
-          for (int t = quarter * 16; t < quarter * 16 + 16; ++t) {
-            if ((named >> (t >> 5) & 1u) != 0 && t0 + t < length) continue;
+          for (int t = quarter * 8; t < quarter * 8 + 8; ++t) {
+            if (named && t0 + t < length) continue;
             for (int piece = lane; piece < D / 16; piece += 32) {
               const int sub = piece / (C::kRowBytes / 16), in_row = piece % (C::kRowBytes / 16);
-              *reinterpret_cast<uint4*>(v_s + sub * C::kSubBytes + (half * 64 + t) * C::kRowBytes +
+              *reinterpret_cast<uint4*>(v_s + sub * C::kSubBytes + (block * kKvBlock + t) * C::kRowBytes +
                                         in_row * 16) = make_uint4(0, 0, 0, 0);
             }
           }
@@ -675,63 +700,50 @@ kv_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         wait(sfull0 + 8 * buffer, (uint32_t)(i / C::kBuffers) & 1u, 512);
         if (failed) break;
         ptx::tc_fence_after();
-        uint32_t raw[2][32];
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-          ptx::tmem_ld_x32(lane_t + buffer * kKvTile + half * 64 + kb * 32, raw[kb]);
+        uint32_t raw[32];
+        ptx::tmem_ld_x32(lane_t + buffer * kKvTile + block * kKvBlock, raw);
         ptx::tmem_ld_wait();
         ptx::tc_fence_before();
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(sread0 + 8 * buffer);
-        if (named != 3u || !__all_sync(0xffffffffu, t0 + 64 <= visible)) {
+        if (!named || !__all_sync(0xffffffffu, t0 + kKvBlock <= visible)) {
+          const int n = named ? visible - t0 : 0;
 #pragma unroll
-          for (int kb = 0; kb < 2; ++kb) {
-            const int n = (named >> kb & 1u) != 0 ? visible - t0 - kb * 32 : 0;
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (e >= n) raw[kb][e] = 0xff800000u;  // -inf
-          }
+          for (int e = 0; e < 32; ++e)
+            if (e >= n) raw[e] = 0xff800000u;  // -inf
         }
-        float top[2], part[2];
+        float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-          float m0 = -INFINITY, m1 = -INFINITY;
+        for (int e = 0; e < 32; e += 8)
 #pragma unroll
-          for (int e = 0; e < 32; e += 4) {
-            m0 = fmaxf(m0, fmaxf(__uint_as_float(raw[kb][e]), __uint_as_float(raw[kb][e + 1])));
-            m1 = fmaxf(m1, fmaxf(__uint_as_float(raw[kb][e + 2]), __uint_as_float(raw[kb][e + 3])));
-          }
-          // To the nearest power of two: the largest weight is in (181, 363).
-          top[kb] = rintf(fmaxf(m0, m1) * factor);
-        }
-        // The reference moves only where a block exceeds it by much, or was not set: the two
+          for (int n = 0; n < 4; ++n)
+            m[n] = fmaxf(m[n], fmaxf(__uint_as_float(raw[e + n]), __uint_as_float(raw[e + 4 + n])));
+        // To the nearest power of two: the largest weight is in (181, 363).
+        const float top = rintf(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * factor);
+        // The reference moves only where a block exceeds it by much, or was not set: the four
         // warps that share the rows agree.  The answer is not needed before the weights are done.
         volatile int* asked = ask_flag + quarter * 2 + (votes++ & 1u);
-        const bool ask = __any_sync(0xffffffffu, fmaxf(top[0], top[1]) > ref + kMostLog2);
+        const bool ask = __any_sync(0xffffffffu, top > ref + kMostLog2);
         if (lane == 0) {
           if (ask) *asked = 1;
           ptx::mbar_arrive(vsync);
         }
-        uint32_t codes[2][TERMS][8];
+        const float base = fmaxf(top, -1e30f) - kWeightLog2;
+        uint32_t codes[TERMS][8];
+        float s0 = 0.0f, s1 = 0.0f;
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-          const float base = fmaxf(top[kb], -1e30f) - kWeightLog2;
-          float s0 = 0.0f, s1 = 0.0f;
+        for (int e = 0; e < 32; e += 4) {
+          float p[4];
 #pragma unroll
-          for (int e = 0; e < 32; e += 4) {
-            float p[4];
+          for (int n = 0; n < 4; ++n)
+            p[n] = ptx::exp2_approx(__uint_as_float(raw[e + n]) * factor - base);
+          s0 += p[0] + p[2];
+          s1 += p[1] + p[3];
+          uint32_t lo[TERMS], hi[TERMS];
+          e4m3_terms_half<TERMS>(__floats2half2_rn(p[0], p[1]), lo);
+          e4m3_terms_half<TERMS>(__floats2half2_rn(p[2], p[3]), hi);
 #pragma unroll
-            for (int n = 0; n < 4; ++n)
-              p[n] = ptx::exp2_approx(__uint_as_float(raw[kb][e + n]) * factor - base);
-            s0 += p[0] + p[2];
-            s1 += p[1] + p[3];
-            uint32_t lo[TERMS], hi[TERMS];
-            e4m3_terms_half<TERMS>(__floats2half2_rn(p[0], p[1]), lo);
-            e4m3_terms_half<TERMS>(__floats2half2_rn(p[2], p[3]), hi);
-#pragma unroll
-            for (int k = 0; k < TERMS; ++k) codes[kb][k][e / 4] = __byte_perm(lo[k], hi[k], 0x5410);
-          }
-          part[kb] = s0 + s1;
+          for (int k = 0; k < TERMS; ++k) codes[k][e / 4] = __byte_perm(lo[k], hi[k], 0x5410);
         }
         // P of the tile before last (or of the last one) has been read.
         if (i >= C::kBuffers)
@@ -740,29 +752,24 @@ kv_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
 #pragma unroll
         for (int k = 0; k < TERMS; ++k) {
 #pragma unroll
-          for (int kb = 0; kb < 2; ++kb) {
-#pragma unroll
-            for (int c16 = 0; c16 < 2; ++c16) {
-              const int chunk = half * 4 + kb * 2 + c16;
-              *reinterpret_cast<uint4*>(p_buffer + k * kRows * kKvTile + ((chunk ^ (row & 7)) << 4)) =
-                  make_uint4(codes[kb][k][c16 * 4], codes[kb][k][c16 * 4 + 1], codes[kb][k][c16 * 4 + 2],
-                             codes[kb][k][c16 * 4 + 3]);
-            }
+          for (int c16 = 0; c16 < 2; ++c16) {
+            const int chunk = block * 2 + c16;
+            *reinterpret_cast<uint4*>(p_buffer + k * kRows * kKvTile + ((chunk ^ (row & 7)) << 4)) =
+                make_uint4(codes[k][c16 * 4], codes[k][c16 * 4 + 1], codes[k][c16 * 4 + 2],
+                           codes[k][c16 * 4 + 3]);
           }
         }
         wait(vsync, syncs & 1u, 514);
         ++syncs;
         if (!failed && *asked != 0) {
-          row_top[half * kRows + row] = fmaxf(top[0], top[1]);
-          __syncwarp();
-          if (lane == 0) ptx::mbar_arrive(vsync);
-          wait(vsync, syncs & 1u, 515);
-          ++syncs;
-          if (half == 0 && lane == 0) *asked = 0;  // not used by the next vote, but the one after
-          const float m = fmaxf(row_top[row], row_top[kRows + row]);
-          const bool up = m > ref + kMostLog2;
-          const float f = up ? pow2_whole(ref - m) : 1.0f;
-          if (up) ref = m;
+          row_top[block * kRows + row] = top;
+          meet(515);
+          if (block == 0 && lane == 0) *asked = 0;  // not used by the next vote, but the one after
+          const float most = fmaxf(fmaxf(row_top[row], row_top[kRows + row]),
+                                   fmaxf(row_top[2 * kRows + row], row_top[3 * kRows + row]));
+          const bool up = most > ref + kMostLog2;
+          const float f = up ? pow2_whole(ref - most) : 1.0f;
+          if (up) ref = most;
           sum *= f;
           if (j > 0) {
             // What has been added up so far shrinks, once the last output has been added.
@@ -770,7 +777,7 @@ kv_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
             if (failed) break;
             ptx::tc_fence_after();
 #pragma unroll 1
-            for (int c0 = half * (D / 2); c0 < (half + 1) * (D / 2); c0 += 8) {
+            for (int c0 = block * (D / 4); c0 < (block + 1) * (D / 4); c0 += 8) {
               uint32_t o[8];
               ptx::tmem_ld_x8(lane_t + C::kOCol + c0, o);
               ptx::tmem_ld_wait();
@@ -780,54 +787,50 @@ kv_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
             }
             ptx::tmem_st_wait();
           }
-          // The partner reads row_top of this meeting before the next one is written.
-          __syncwarp();
-          if (lane == 0) ptx::mbar_arrive(vsync);
-          wait(vsync, syncs & 1u, 517);
-          ++syncs;
+          // The others read row_top of this meeting before the next one is written.
+          meet(517);
         }
         if (failed) break;
-        // Block scales of P: 2^(top - ref), the further terms 2^-4 and 2^-8 of it.
-        uint32_t code[2];
+        // Block scale of P: 2^(top - ref), the further terms 2^-4 and 2^-8 of it.
+        const float power = pow2_whole(top == -INFINITY ? 0.0f : top - ref);
+        sum += (s0 + s1) * power;
+        const uint32_t code = __float_as_uint(power) >> 23;
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-          const float power = pow2_whole(top[kb] == -INFINITY ? 0.0f : top[kb] - ref);
-          sum += part[kb] * power;
-          code[kb] = __float_as_uint(power) >> 23;
-        }
-#pragma unroll
-        for (int k = 0; k < TERMS; ++k) {
-          const uint32_t lo = code[0] > 4u * k ? code[0] - 4u * k : 0u;
-          const uint32_t hi = code[1] > 4u * k ? code[1] - 4u * k : 0u;
-          *reinterpret_cast<uint16_t*>(p_sf_row + (buffer * TERMS + k) * 512) = (uint16_t)(lo | hi << 8);
-        }
+        for (int k = 0; k < TERMS; ++k)
+          p_sf_row[(buffer * TERMS + k) * 512] = (uint8_t)(code > 4u * k ? code - 4u * k : 0u);
         ptx::fence_proxy_async();
         ptx::tc_fence_before();
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(pfull0 + 8 * buffer);
       }
       // ---- the rows of this CTA's tiles of the item ----
-      row_sum[half * kRows + row] = sum;
+      row_sum[block * kRows + row] = sum;
       const int i = i0 + tiles - 1;
       if (tiles > 0) wait(pvdone0 + 8 * (i % C::kBuffers), (uint32_t)(i / C::kBuffers) & 1u, 518);
       failed = ptx::barrier_any(1, kSoftmaxWarps * 32, failed);
       if (failed) break;
       ptx::tc_fence_after();
-      const float l = row_sum[row] + row_sum[kRows + row];
+      const float l = (row_sum[row] + row_sum[kRows + row]) + (row_sum[2 * kRows + row] + row_sum[3 * kRows + row]);
       const int r = seg.row0 + row;
       const bool mine = r < seg.rows;
+      constexpr int kCols = D / 4 < 32 ? D / 4 : 32, kPieces = kCols / 8;  // a pass; 16-byte pieces
       if (seg.whole) {
         const float scale = l == 0.0f ? 0.0f : 1.0f / l;
-        T* out = static_cast<T*>(a.out) + (seg.row + r / a.group) * a.out_token_stride +
-                 (int64_t)(seg.head * a.group + r % a.group) * a.out_head_stride;
+        const int64_t own = (seg.row + r / a.group) * a.out_token_stride +
+                            (int64_t)(seg.head * a.group + r % a.group) * a.out_head_stride;
+        T* out = static_cast<T*>(a.out);
+        // Through shared memory, so that a row's values leave together: each warp has 2 KB of its
+        // rows in the first two terms of P, which no product reads any more.
+        uint8_t* stage = p_tiles + (block >> 1) * kRows * kKvTile + quarter * 4096 + (block & 1) * 2048;
+        const unsigned real = __ballot_sync(0xffffffffu, mine);
 #pragma unroll 1
-        for (int c0 = half * (D / 2); c0 < (half + 1) * (D / 2); c0 += 32) {
-          uint32_t o[32];
-          ptx::tmem_ld_x32(lane_t + C::kOCol + c0, o);
+        for (int c0 = block * (D / 4); c0 < (block + 1) * (D / 4); c0 += kCols) {
+          uint32_t o[kCols];
+          ptx::tmem_ld_chunk<kCols>(lane_t + C::kOCol + c0, o);
           ptx::tmem_ld_wait();
-          uint32_t w[16];
+          uint32_t w[kCols / 2];
 #pragma unroll
-          for (int n = 0; n < 16; ++n) {
+          for (int n = 0; n < kCols / 2; ++n) {
             const float x = __uint_as_float(o[2 * n]) * scale, y = __uint_as_float(o[2 * n + 1]) * scale;
             if constexpr (TERMS == 2) {
               const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
@@ -837,39 +840,49 @@ kv_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
               w[n] = *reinterpret_cast<const uint32_t*>(&v);
             }
           }
-          if (mine) {
+#pragma unroll
+          for (int n = 0; n < kPieces; ++n)
+            *reinterpret_cast<uint4*>(stage + lane * kCols * 2 + ((n ^ (lane / 2 & (kPieces - 1))) << 4)) =
+                make_uint4(w[4 * n], w[4 * n + 1], w[4 * n + 2], w[4 * n + 3]);
+          __syncwarp();
+#pragma unroll
+          for (int n = 0; n < kPieces; ++n) {
+            const int from = (n * 32 + lane) / kPieces, piece = lane % kPieces;
+            const int64_t at = __shfl_sync(0xffffffffu, own, from);
+            const uint4 v = *reinterpret_cast<const uint4*>(stage + from * kCols * 2 +
+                                                            ((piece ^ (from / 2 & (kPieces - 1))) << 4));
+            if ((real >> from & 1u) == 0) continue;
+            T* dst = out + at + c0 + piece * 8;
             if (a.vector_out) {
-#pragma unroll
-              for (int n = 0; n < 4; ++n)
-                *reinterpret_cast<uint4*>(out + c0 + n * 8) =
-                    make_uint4(w[4 * n], w[4 * n + 1], w[4 * n + 2], w[4 * n + 3]);
+              *reinterpret_cast<uint4*>(dst) = v;
             } else {
-              uint16_t* dst = reinterpret_cast<uint16_t*>(out + c0);
+              const uint32_t x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-              for (int n = 0; n < 16; ++n) {
-                dst[2 * n] = (uint16_t)w[n];
-                dst[2 * n + 1] = (uint16_t)(w[n] >> 16);
+              for (int e = 0; e < 4; ++e) {
+                reinterpret_cast<uint16_t*>(dst)[2 * e] = (uint16_t)x[e];
+                reinterpret_cast<uint16_t*>(dst)[2 * e + 1] = (uint16_t)(x[e] >> 16);
               }
             }
           }
+          __syncwarp();
         }
       } else {
         // A share that begins inside an item uses the CTA's first partial slot for it, one that
         // ends inside the second.
         float* part = a.partials +
                       (int64_t)(2 * blockIdx.x + (seg.tile != 0 ? 0 : 1)) * C::kPartialFloats;
-        if (half == 0) {
+        if (block == 0) {
           part[kRows * D + 2 * row] = ref;
           part[kRows * D + 2 * row + 1] = l;
         }
 #pragma unroll 1
-        for (int c0 = half * (D / 2); c0 < (half + 1) * (D / 2); c0 += 32) {
-          uint32_t o[32];
-          ptx::tmem_ld_x32(lane_t + C::kOCol + c0, o);
+        for (int c0 = block * (D / 4); c0 < (block + 1) * (D / 4); c0 += kCols) {
+          uint32_t o[kCols];
+          ptx::tmem_ld_chunk<kCols>(lane_t + C::kOCol + c0, o);
           ptx::tmem_ld_wait();
           if (mine) {
 #pragma unroll
-            for (int n = 0; n < 8; ++n)
+            for (int n = 0; n < kCols / 4; ++n)
               *reinterpret_cast<uint4*>(part + row * D + c0 + n * 4) =
                   make_uint4(o[4 * n], o[4 * n + 1], o[4 * n + 2], o[4 * n + 3]);
           }
@@ -878,6 +891,8 @@ kv_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       ptx::tc_fence_before();
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(sdone0 + 8 * (segment & 1));
+      // The warps of a quarter write P where they have staged their rows.
+      meet(519);
       i0 += tiles;
       at0 += 2 * tiles;
     }
