@@ -36,7 +36,7 @@ constexpr int kRows = 128;            // rows of an item
 constexpr float kWeightLog2 = 8.0f;   // weights are scaled by 256 before they become E4M3 terms
 constexpr float kMostLog2 = 16.0f;    // a block may exceed the reference by 2^16
 constexpr int kSms = 148;
-constexpr int kItemUnits = 2;         // what an item costs beside its tiles
+constexpr int kItemUnits = 5;         // what an item costs beside its tiles: about 8 us, a tile 1.7 us
 constexpr int kMinUnits = 4;          // units a CTA takes at least
 
 template <int D, int TERMS>
@@ -46,23 +46,29 @@ struct PrefillCfg {
   static constexpr int kSubBytes = kKvTile * kRowBytes;  // also of a Q sub-tile: 128 rows
   static constexpr int kSlotBytes = kKvTile * D;
   static constexpr int kQBytes = TERMS * kRows * D;
-  static constexpr int kPBytes = TERMS * kRows * kKvTile;
-  // A head of 256 leaves room for one score tile in tensor memory and one P in shared memory.
+  // A head of 256 leaves room for one score tile in tensor memory and one P.  Two terms of P fit
+  // tensor memory beside it, which frees shared memory for a fourth tile of keys and values: with
+  // three, a tile came 0.4 us after the tensor cores wanted it.
   static constexpr int kBuffers = D == 256 ? 1 : 2;
+  static constexpr bool kTmemP = D == 256 && TERMS == 2;
+  static constexpr int kPBytes = kTmemP ? 0 : TERMS * kRows * kKvTile;
+  static constexpr int kStageWarp = kTmemP ? 1024 : 2048;  // bytes a warp stages outputs in
+  static constexpr int kStageBytes = kTmemP ? kSoftmaxWarps * kStageWarp : 0;  // else in P
   static constexpr int kFixedBytes = 11264;
   static constexpr int kBudget = 227 * 1024 - 1024;
-  static constexpr int kFit = (kBudget - kFixedBytes - kQBytes - kBuffers * kPBytes) / (kSlotBytes + 512);
+  static constexpr int kFit = (kBudget - kFixedBytes - kStageBytes - kQBytes - kBuffers * kPBytes) / (kSlotBytes + 512);
   static constexpr int kSlots = kFit > 8 ? 8 : kFit;
   static_assert(kSlots >= 2, "a K and a V tile");
   static constexpr int kSmemBytes =
-      1024 + kSlots * (kSlotBytes + 512) + kQBytes + kBuffers * kPBytes + kFixedBytes;
+      1024 + kSlots * (kSlotBytes + 512) + kQBytes + kBuffers * kPBytes + kStageBytes + kFixedBytes;
   static constexpr int kOCol = kBuffers * kKvTile;
   static constexpr int kSfCol = kOCol + D;
   // Scales: constants per term; per buffer (what an MMA may still read is not overwritten) keys,
   // values (8 for 256 rows of B), weights per term.
   static constexpr int kSfTerm = kSfCol, kSfSets = kSfTerm + 4 * TERMS;
   static constexpr int kSfV = 4, kSfP = 12, kSfSet = 12 + 4 * TERMS;
-  static_assert(kSfSets + kBuffers * kSfSet <= 512, "tensor memory");
+  static constexpr int kPCol = (kSfSets + kBuffers * kSfSet + 15) / 16 * 16;  // [term][32 columns]
+  static_assert(kPCol + (kTmemP ? TERMS * 32 : 0) <= 512, "tensor memory");
   static constexpr uint64_t kSwizzle = kRowBytes == 128 ? ptx::kSwizzle128 : ptx::kSwizzle64;
   static constexpr int kGroup = 8 * kRowBytes;
   static constexpr int kPartialFloats = kRows * D + 2 * kRows;
@@ -261,7 +267,8 @@ kv_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   uint8_t* slots = smem;
   uint8_t* q_tiles = slots + C::kSlots * C::kSlotBytes;  // [term][sub][row][row bytes]
   uint8_t* p_tiles = q_tiles + C::kQBytes;               // [buffer][term][row][128 tokens]
-  uint8_t* sf_tiles = p_tiles + C::kBuffers * C::kPBytes;
+  uint8_t* stages = p_tiles + C::kBuffers * C::kPBytes;  // where P is in tensor memory
+  uint8_t* sf_tiles = stages + C::kStageBytes;
   uint8_t* fixed = sf_tiles + C::kSlots * 512;
   uint64_t* bars = reinterpret_cast<uint64_t*>(fixed);
   uint8_t* term_sf = fixed + 512;                        // [term] atoms of 1, 1/16, 1/256
@@ -519,11 +526,17 @@ kv_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
           for (int k = 0; k < TERMS; ++k) {
             const uint64_t ad = ptx::smem_desc(p_s + k * kRows * kKvTile, 0, 1024, ptx::kSwizzle128);
 #pragma unroll
-            for (int ks = 0; ks < kKvTileBlocks; ++ks)
-              ptx::tc_mma_mxf8f6f4(tmem + C::kOCol, ad + 2 * ks, bd + ks * (kKvBlock * C::kRowBytes / 16),
-                                   kIdescO | ((uint32_t)ks << 29) | ((uint32_t)ks << 4),
-                                   sf_t + C::kSfP + 4 * k, sf_t + C::kSfV,
-                                   (j > 0 || k > 0 || ks > 0) ? 1u : 0u);
+            for (int ks = 0; ks < kKvTileBlocks; ++ks) {
+              const uint32_t idesc = kIdescO | ((uint32_t)ks << 29) | ((uint32_t)ks << 4);
+              const uint64_t b_ks = bd + ks * (kKvBlock * C::kRowBytes / 16);
+              const uint32_t add = (j > 0 || k > 0 || ks > 0) ? 1u : 0u;
+              if constexpr (C::kTmemP)
+                ptx::tc_mma_mxf8f6f4_ts(tmem + C::kOCol, tmem + C::kPCol + 32 * k + 8 * ks, b_ks, idesc,
+                                        sf_t + C::kSfP + 4 * k, sf_t + C::kSfV, add);
+              else
+                ptx::tc_mma_mxf8f6f4(tmem + C::kOCol, ad + 2 * ks, b_ks, idesc, sf_t + C::kSfP + 4 * k,
+                                     sf_t + C::kSfV, add);
+            }
           }
           ptx::tc_commit(pvdone0 + 8 * buffer);
           ptx::tc_commit(empty0 + 8 * slot);
@@ -592,7 +605,19 @@ kv_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       __syncwarp();  // the rows and the description are complete
       if (lane == 0) ptx::mbar_arrive(qraw);
       left -= tiles;
-      if (left > 0) c.next_item(a);
+      if (left > 0) {
+        c.next_item(a);
+        if (a.vector) {
+          // The next rows will come from the L2.
+          const int next0 = c.at.t * kRows, next_rows = min(kRows, c.seq.rows - next0);
+          for (int n = lane; n < next_rows; n += 32) {
+            const int r = next0 + n;
+            ptx::bulk_prefetch_l2(static_cast<const uint16_t*>(a.q) + (c.seq.row + r / a.group) * a.q_token_stride +
+                                      (int64_t)(c.at.head * a.group + r % a.group) * a.q_head_stride,
+                                  2 * D);
+          }
+        }
+      }
     }
   } else if (count > 0 && warp < kSoftmaxWarps) {
     // ---------------- softmax: a thread has 32 tokens of one row ----------------
@@ -615,57 +640,60 @@ kv_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       wait(vsync, syncs & 1u, code);
       ++syncs;
     };
-    int at0 = 0;  // place of the segment in the order of the copies
-    for (int i0 = 0, segment = 0; i0 < count; ++segment) {
+    // Turns a segment's rows into terms, in place.
+    auto turn_rows = [&](int segment) {
       wait(qraw, (uint32_t)segment & 1u, 510);
       Segment& seg = segments[segment & 1];
-      {
-        // Eight rows a warp: their words leave shared memory before any terms replace them.
-        constexpr int kPer = D / 32, kBatch = kRows / kSoftmaxWarps;
-        const int first_row = warp * kBatch, real = failed ? 0 : seg.rows - seg.row0;
-        uint32_t words[kBatch][kPer / 2];
-        float scale[kBatch];
+      // Eight rows a warp: their words leave shared memory before any terms replace them.
+      constexpr int kPer = D / 32, kBatch = kRows / kSoftmaxWarps;
+      const int first_row = warp * kBatch, real = failed ? 0 : seg.rows - seg.row0;
+      uint32_t words[kBatch][kPer / 2];
+      float scale[kBatch];
 #pragma unroll
-        for (int n = 0; n < kBatch; ++n) {
-          const uint32_t* src = reinterpret_cast<const uint32_t*>(q_tiles + (first_row + n) * 2 * D) + lane * (kPer / 2);
+      for (int n = 0; n < kBatch; ++n) {
+        const uint32_t* src = reinterpret_cast<const uint32_t*>(q_tiles + (first_row + n) * 2 * D) + lane * (kPer / 2);
 #pragma unroll
-          for (int w = 0; w < kPer / 2; ++w) words[n][w] = src[w];
-        }
+        for (int w = 0; w < kPer / 2; ++w) words[n][w] = src[w];
+      }
 #pragma unroll
-        for (int n = 0; n < kBatch; ++n) scale[n] = query_scale<T, kPer>(words[n], first_row + n < real);
-        failed = ptx::barrier_any(1, kSoftmaxWarps * 32, failed);
-        if (failed) break;
-        float mine = scale[0];
+      for (int n = 0; n < kBatch; ++n) scale[n] = query_scale<T, kPer>(words[n], first_row + n < real);
+      failed = ptx::barrier_any(1, kSoftmaxWarps * 32, failed);
+      if (failed) return;
+      float mine = scale[0];
 #pragma unroll
-        for (int n = 1; n < kBatch; ++n) mine = lane == n ? scale[n] : mine;
-        if (lane < kBatch) seg.scale[first_row + lane] = mine * fabsf(a.scale_log2);
-        const float sign = a.scale_log2 < 0.0f ? -1.0f : 1.0f;  // the softmax takes a factor >= 0
-        const int d0 = lane * kPer, in_row = d0 % C::kRowBytes;
+      for (int n = 1; n < kBatch; ++n) mine = lane == n ? scale[n] : mine;
+      if (lane < kBatch) seg.scale[first_row + lane] = mine * fabsf(a.scale_log2);
+      const float sign = a.scale_log2 < 0.0f ? -1.0f : 1.0f;  // the softmax takes a factor >= 0
+      const int d0 = lane * kPer, in_row = d0 % C::kRowBytes;
 #pragma unroll
-        for (int n = 0; n < kBatch; ++n) {
-          const int r = first_row + n;
-          uint32_t codes[TERMS][kPer / 2];
-          query_terms<T, TERMS, kPer>(words[n], r < real, scale[n], sign, codes);
-          const int swizzle = C::kRowBytes == 128 ? (r & 7) : ((r >> 1) & 3);
+      for (int n = 0; n < kBatch; ++n) {
+        const int r = first_row + n;
+        uint32_t codes[TERMS][kPer / 2];
+        query_terms<T, TERMS, kPer>(words[n], r < real, scale[n], sign, codes);
+        const int swizzle = C::kRowBytes == 128 ? (r & 7) : ((r >> 1) & 3);
 #pragma unroll
-          for (int k = 0; k < TERMS; ++k) {
-            uint8_t* dst = q_tiles + (k * C::kSubs + d0 / C::kRowBytes) * C::kSubBytes + r * C::kRowBytes +
-                           (((in_row >> 4) ^ swizzle) << 4) + (in_row & 15);
-            if constexpr (kPer == 8) {
-              *reinterpret_cast<uint2*>(dst) = make_uint2(codes[k][0] | codes[k][1] << 16,
-                                                          codes[k][2] | codes[k][3] << 16);
-            } else if constexpr (kPer == 4) {
-              *reinterpret_cast<uint32_t*>(dst) = codes[k][0] | codes[k][1] << 16;
-            } else {
-              *reinterpret_cast<uint16_t*>(dst) = (uint16_t)codes[k][0];
-            }
+        for (int k = 0; k < TERMS; ++k) {
+          uint8_t* dst = q_tiles + (k * C::kSubs + d0 / C::kRowBytes) * C::kSubBytes + r * C::kRowBytes +
+                         (((in_row >> 4) ^ swizzle) << 4) + (in_row & 15);
+          if constexpr (kPer == 8) {
+            *reinterpret_cast<uint2*>(dst) = make_uint2(codes[k][0] | codes[k][1] << 16,
+                                                        codes[k][2] | codes[k][3] << 16);
+          } else if constexpr (kPer == 4) {
+            *reinterpret_cast<uint32_t*>(dst) = codes[k][0] | codes[k][1] << 16;
+          } else {
+            *reinterpret_cast<uint16_t*>(dst) = (uint16_t)codes[k][0];
           }
         }
-        ptx::fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(qfull);
-        wait(qfull, (uint32_t)segment & 1u, 520);  // the other warps' scales
       }
+      ptx::fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(qfull);
+    };
+    turn_rows(0);
+    int at0 = 0;  // place of the segment in the order of the copies
+    for (int i0 = 0, segment = 0; i0 < count; ++segment) {
+      const Segment& seg = segments[segment & 1];
+      wait(qfull, (uint32_t)segment & 1u, 520);  // the other warps' scales
       const int tiles = failed ? 0 : seg.tiles, length = seg.length, tile0 = seg.tile;
       const bool all_named = seg.all_named != 0;
       // Above zero, so that a masked score (-inf) stays one where the scale is zero.
@@ -748,15 +776,21 @@ kv_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         // P of the tile before last (or of the last one) has been read.
         if (i >= C::kBuffers)
           wait(pvdone0 + 8 * buffer, (uint32_t)(i / C::kBuffers - 1) & 1u, 513);
-        uint8_t* p_buffer = p_row + buffer * C::kPBytes;
+        if constexpr (C::kTmemP) {
 #pragma unroll
-        for (int k = 0; k < TERMS; ++k) {
+          for (int k = 0; k < TERMS; ++k)
+            ptx::tmem_st_x8(lane_t + C::kPCol + 32 * k + 8 * block, codes[k]);
+        } else {
+          uint8_t* p_buffer = p_row + buffer * C::kPBytes;
 #pragma unroll
-          for (int c16 = 0; c16 < 2; ++c16) {
-            const int chunk = block * 2 + c16;
-            *reinterpret_cast<uint4*>(p_buffer + k * kRows * kKvTile + ((chunk ^ (row & 7)) << 4)) =
-                make_uint4(codes[k][c16 * 4], codes[k][c16 * 4 + 1], codes[k][c16 * 4 + 2],
-                           codes[k][c16 * 4 + 3]);
+          for (int k = 0; k < TERMS; ++k) {
+#pragma unroll
+            for (int c16 = 0; c16 < 2; ++c16) {
+              const int chunk = block * 2 + c16;
+              *reinterpret_cast<uint4*>(p_buffer + k * kRows * kKvTile + ((chunk ^ (row & 7)) << 4)) =
+                  make_uint4(codes[k][c16 * 4], codes[k][c16 * 4 + 1], codes[k][c16 * 4 + 2],
+                             codes[k][c16 * 4 + 3]);
+            }
           }
         }
         wait(vsync, syncs & 1u, 514);
@@ -798,6 +832,7 @@ kv_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
 #pragma unroll
         for (int k = 0; k < TERMS; ++k)
           p_sf_row[(buffer * TERMS + k) * 512] = (uint8_t)(code > 4u * k ? code - 4u * k : 0u);
+        if constexpr (C::kTmemP) ptx::tmem_st_wait();
         ptx::fence_proxy_async();
         ptx::tc_fence_before();
         __syncwarp();
@@ -813,15 +848,18 @@ kv_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       const float l = (row_sum[row] + row_sum[kRows + row]) + (row_sum[2 * kRows + row] + row_sum[3 * kRows + row]);
       const int r = seg.row0 + row;
       const bool mine = r < seg.rows;
-      constexpr int kCols = D / 4 < 32 ? D / 4 : 32, kPieces = kCols / 8;  // a pass; 16-byte pieces
+      // Through shared memory, so that a row's values leave together: each warp has 2 KB of its
+      // rows in the first two terms of P, which no product reads any more, or 1 KB apart.
+      constexpr int kMost = C::kStageWarp / 64;                 // 16-bit columns that fit
+      constexpr int kCols = D / 4 < kMost ? D / 4 : kMost, kPieces = kCols / 8;  // a pass; 16-byte pieces
+      constexpr int kPartCols = kMost / 2, kPartPieces = kPartCols / 4;          // of 32-bit columns
+      uint8_t* stage = C::kTmemP ? stages + warp * C::kStageWarp
+                                 : p_tiles + (block >> 1) * kRows * kKvTile + quarter * 4096 + (block & 1) * 2048;
       if (seg.whole) {
         const float scale = l == 0.0f ? 0.0f : 1.0f / l;
         const int64_t own = (seg.row + r / a.group) * a.out_token_stride +
                             (int64_t)(seg.head * a.group + r % a.group) * a.out_head_stride;
         T* out = static_cast<T*>(a.out);
-        // Through shared memory, so that a row's values leave together: each warp has 2 KB of its
-        // rows in the first two terms of P, which no product reads any more.
-        uint8_t* stage = p_tiles + (block >> 1) * kRows * kKvTile + quarter * 4096 + (block & 1) * 2048;
         const unsigned real = __ballot_sync(0xffffffffu, mine);
 #pragma unroll 1
         for (int c0 = block * (D / 4); c0 < (block + 1) * (D / 4); c0 += kCols) {
@@ -842,7 +880,7 @@ kv_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
           }
 #pragma unroll
           for (int n = 0; n < kPieces; ++n)
-            *reinterpret_cast<uint4*>(stage + lane * kCols * 2 + ((n ^ (lane / 2 & (kPieces - 1))) << 4)) =
+            *reinterpret_cast<uint4*>(stage + lane * kCols * 2 + ((n ^ (lane * kPieces / 8 & (kPieces - 1))) << 4)) =
                 make_uint4(w[4 * n], w[4 * n + 1], w[4 * n + 2], w[4 * n + 3]);
           __syncwarp();
 #pragma unroll
@@ -850,7 +888,7 @@ kv_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
             const int from = (n * 32 + lane) / kPieces, piece = lane % kPieces;
             const int64_t at = __shfl_sync(0xffffffffu, own, from);
             const uint4 v = *reinterpret_cast<const uint4*>(stage + from * kCols * 2 +
-                                                            ((piece ^ (from / 2 & (kPieces - 1))) << 4));
+                                                            ((piece ^ (from * kPieces / 8 & (kPieces - 1))) << 4));
             if ((real >> from & 1u) == 0) continue;
             T* dst = out + at + c0 + piece * 8;
             if (a.vector_out) {
@@ -876,16 +914,24 @@ kv_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
           part[kRows * D + 2 * row + 1] = l;
         }
 #pragma unroll 1
-        for (int c0 = block * (D / 4); c0 < (block + 1) * (D / 4); c0 += kCols) {
-          uint32_t o[kCols];
-          ptx::tmem_ld_chunk<kCols>(lane_t + C::kOCol + c0, o);
+        for (int c0 = block * (D / 4); c0 < (block + 1) * (D / 4); c0 += kPartCols) {
+          uint32_t o[kPartCols];
+          ptx::tmem_ld_chunk<kPartCols>(lane_t + C::kOCol + c0, o);
           ptx::tmem_ld_wait();
-          if (mine) {
 #pragma unroll
-            for (int n = 0; n < kCols / 4; ++n)
-              *reinterpret_cast<uint4*>(part + row * D + c0 + n * 4) =
-                  make_uint4(o[4 * n], o[4 * n + 1], o[4 * n + 2], o[4 * n + 3]);
+          for (int n = 0; n < kPartPieces; ++n)
+            *reinterpret_cast<uint4*>(stage + lane * kPartCols * 4 +
+                                      ((n ^ (lane * kPartPieces / 8 & (kPartPieces - 1))) << 4)) =
+                make_uint4(o[4 * n], o[4 * n + 1], o[4 * n + 2], o[4 * n + 3]);
+          __syncwarp();
+#pragma unroll
+          for (int n = 0; n < kPartPieces; ++n) {
+            const int from = (n * 32 + lane) / kPartPieces, piece = lane % kPartPieces;
+            const uint4 v = *reinterpret_cast<const uint4*>(
+                stage + from * kPartCols * 4 + ((piece ^ (from * kPartPieces / 8 & (kPartPieces - 1))) << 4));
+            *reinterpret_cast<uint4*>(part + (quarter * 32 + from) * D + c0 + piece * 4) = v;
           }
+          __syncwarp();
         }
       }
       ptx::tc_fence_before();
@@ -895,6 +941,8 @@ kv_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       meet(519);
       i0 += tiles;
       at0 += 2 * tiles;
+      if (i0 < count) turn_rows(segment + 1);
+      if (failed) break;
     }
   }
 
