@@ -15,8 +15,12 @@ side of those shapes: per layer
 with every buffer preallocated so that the whole step captures into one CUDA graph.
 Tensor parallelism splits attention heads and the MLP intermediate over the ranks of
 one node (column-parallel QKV and gate/up, row-parallel output and down projections).
-No rotary embedding is applied: attention is the plain BF16 kernel the benchmark
-configuration asks for.
+
+:meth:`DenseDecoder.decode_step` and :meth:`DenseDecoder.prefill` apply no rotary embedding:
+their attention is the plain BF16 kernel the benchmark configuration asks for.
+:meth:`DenseDecoder.paged_step` is the serving form: ragged batches of single tokens, drafted
+tokens or prompt chunks over a paged 8-bit KV cache, with rotary positions
+(:mod:`mxfp6_sm120_b200.kv_cache`).
 """
 
 from __future__ import annotations
@@ -27,6 +31,13 @@ import torch
 import torch.distributed as dist
 import torch.nn.functional as F
 
+from .kv_cache import (
+    PagedKVCache,
+    RotaryFrequencies,
+    kv_cache_attention,
+    kv_cache_write,
+    rotary_multi_axis,
+)
 from .moe_ops import dense_w1_silu_mxfp8_out, silu_and_mul_mxfp8_packed_out
 from .ops import (
     MXFP8Tensor,
@@ -249,6 +260,12 @@ class DenseDecoder:
             cache.append((k, v))
         return cache
 
+    def new_paged_cache(self, pages: int, page_size: int = 64) -> list[PagedKVCache]:
+        """Per layer an empty 8-bit cache of ``pages`` pages (:class:`PagedKVCache`) of this rank's
+        heads; the layers of a model share one block table."""
+        return [PagedKVCache.allocate(pages, self.shape.kv_heads, page_size, self.cfg.head_dim,
+                                      self.device) for _ in self.layers]
+
     # ------------------------------------------------------------------ one layer
     def _all_reduce(self, tensor: torch.Tensor) -> None:
         if self.world > 1:
@@ -343,6 +360,40 @@ class DenseDecoder:
                     q.transpose(0, 1).unsqueeze(0), k.transpose(0, 1).unsqueeze(0),
                     v.transpose(0, 1).unsqueeze(0), is_causal=True, enable_gqa=True)
                 out.view(q.shape[0], q.shape[1], q.shape[2]).copy_(o.squeeze(0).transpose(0, 1))
+
+            return attention
+
+        return self._run(ws, attention_of_layer)
+
+    def paged_step(self, ws: DecoderWorkspace, caches: list[PagedKVCache], block_table: torch.Tensor,
+                   seq_lens: torch.Tensor, cu_seqlens: torch.Tensor | None = None, *,
+                   max_query_len: int | None = None, rotary: RotaryFrequencies | None = None,
+                   positions: torch.Tensor | None = None) -> torch.Tensor:
+        """New tokens of a batch of sequences over the paged 8-bit cache: ``ws.x`` holds their hidden
+        states, sequence after sequence, and is updated in place.
+
+        ``seq_lens`` counts the new tokens; ``cu_seqlens`` says which rows are whose (None: one
+        token per sequence), ``max_query_len`` how many a sequence has at most; see
+        :mod:`mxfp6_sm120_b200.kv_cache`.  With ``rotary`` the query and key heads are turned by
+        ``positions`` (``[axes, tokens]``) first.  Rows of ``ws.x`` behind ``cu_seqlens[-1]``
+        attend to nothing and carry no meaning.
+        """
+        if len(caches) != len(self.layers):
+            raise ValueError(f"{len(self.layers)} caches are needed, one per layer; got {len(caches)}")
+        if (rotary is None) != (positions is None):
+            raise ValueError("rotary and positions go together")
+        if cu_seqlens is not None:
+            ws.attn.zero_()  # rows of no sequence keep what is there
+
+        def attention_of_layer(index: int):
+            cache = caches[index]
+
+            def attention(q, k, v, out):
+                if rotary is not None:
+                    rotary_multi_axis(q, k, positions, rotary, q_out=q, k_out=k)
+                kv_cache_write(cache, k, v, block_table, seq_lens, cu_seqlens)
+                kv_cache_attention(q, cache, block_table, seq_lens, cu_seqlens,
+                                   max_query_len=max_query_len, out=out.view(q.shape))
 
             return attention
 
