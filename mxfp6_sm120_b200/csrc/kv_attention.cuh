@@ -140,6 +140,37 @@ __device__ __forceinline__ void query_terms(const uint32_t (&words)[kPer / 2], b
   }
 }
 
+// NaN among cached values.  A row's weight for a token that it does not see is zero, and the
+// tensor cores would make 0 * NaN a NaN.  So where some rows do not see all of a tile, its NaN
+// codes are cleared and `nan_from` remembers, per value of head_dim, the first such token: rows
+// that see it get NaN there when they are written.  Tokens t0 .. t0 + count of a V tile in shared
+// memory (sub-tiles of kRowBytes a token), by a full warp; `first` is the tile's first token.
+template <int D>
+__device__ __forceinline__ void clear_nan(uint8_t* tile, int t0, int count, int first, int* nan_from,
+                                          volatile int* nan_seen, int lane) {
+  constexpr int kRowBytes = D < 128 ? D : 128, kPieces = D / 16;
+  for (int n = lane; n < count * kPieces; n += 32) {
+    const int t = t0 + n / kPieces, piece = n % kPieces;
+    const int sub = piece / (kRowBytes / 16), place = piece % (kRowBytes / 16);
+    uint4* at = reinterpret_cast<uint4*>(tile + sub * kKvTile * kRowBytes + t * kRowBytes + place * 16);
+    uint4 v = *at;
+    // A byte of 0x7f or 0xff carries into bit 7.
+    const uint32_t found = ((v.x & 0x7f7f7f7fu) + 0x01010101u) | ((v.y & 0x7f7f7f7fu) + 0x01010101u) |
+                           ((v.z & 0x7f7f7f7fu) + 0x01010101u) | ((v.w & 0x7f7f7f7fu) + 0x01010101u);
+    if ((found & 0x80808080u) == 0) continue;
+    const int logical = place ^ (kRowBytes == 128 ? (t & 7) : ((t >> 1) & 3));
+    uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      if ((w[i / 4] >> (8 * (i % 4)) & 0x7fu) != 0x7fu) continue;
+      atomicMin(nan_from + sub * kRowBytes + logical * 16 + i, first + t);
+      w[i / 4] &= ~(0xffu << (8 * (i % 4)));
+    }
+    *at = make_uint4(w[0], w[1], w[2], w[3]);
+    *nan_seen = 1;
+  }
+}
+
 // A sequence as this kernel sees it: `tiles` is 0 when it has no rows or is another kernel's.
 struct KvSequence {
   int64_t row;  // first token row

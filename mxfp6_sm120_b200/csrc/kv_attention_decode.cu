@@ -31,6 +31,7 @@
 //    reaches a weight that counts.  The sums of the weights are a product with ones.
 #include "kv_attention.cuh"
 
+#include <climits>
 #include <cstdlib>
 
 namespace mx {
@@ -61,7 +62,7 @@ struct DecodeCfg {
   static constexpr int kSlotBytes = kKvTile * D;     // a K or V tile
   static constexpr int kQBytes = (kN * D + 1023) / 1024 * 1024;
   static constexpr int kPBytes = kN * kKvTile;
-  static constexpr int kFixedBytes = 7168;
+  static constexpr int kFixedBytes = 7168 + 2 * D * 4;
   static constexpr int kBudget = 227 * 1024 - 1024;
   static constexpr int kFit =
       (kBudget - kFixedBytes - kQueries * kQBytes - 2 * kPBytes) / (kSlotBytes + 512);
@@ -235,13 +236,15 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   Segment<RP>* segments = reinterpret_cast<Segment<RP>*>(fixed + 4096);  // [buffer]
   float* red_max = reinterpret_cast<float*>(segments + kQueries);     // [group][warp][RP]
   float* red_top = red_max + 8 * RP;                           // [group][RP]
-  Cursor* start = reinterpret_cast<Cursor*>(red_top + 2 * RP);
+  int* nan_table = reinterpret_cast<int*>(red_top + 2 * RP);   // [segment parity][head_dim], see clear_nan
+  Cursor* start = reinterpret_cast<Cursor*>(nan_table + 2 * D);
   int64_t* share_smem = reinterpret_cast<int64_t*>(start + 1);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(share_smem + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* ask_flag = abort_flag + 1;                     // [group][2]
-  volatile uint32_t* slot_named = reinterpret_cast<volatile uint32_t*>(ask_flag + 4);  // [slot]
-  static_assert(4096 + kQueries * sizeof(Segment<RP>) + 10 * RP * 4 + sizeof(Cursor) + 16 + 8 + 16 + 64 <=
+  volatile int* nan_flag = ask_flag + 4;                       // [segment parity]
+  volatile uint32_t* slot_named = reinterpret_cast<volatile uint32_t*>(nan_flag + 2);  // [slot]
+  static_assert(4096 + kQueries * sizeof(Segment<RP>) + 10 * RP * 4 + 2 * D * 4 + sizeof(Cursor) + 16 + 8 + 16 + 72 <=
                     C::kFixedBytes,
                 "fixed area");
 
@@ -260,6 +263,7 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   if (threadIdx.x == 0) {
     *abort_flag = 0;
     for (int i = 0; i < 4; ++i) ask_flag[i] = 0;
+    nan_flag[0] = nan_flag[1] = 0;
     for (int s = 0; s < C::kSlots; ++s) {
       ptx::mbar_init(full0 + 8 * s, 2);  // the copies' bytes, and the scales
       ptx::mbar_init(empty0 + 8 * s, 1);
@@ -280,6 +284,7 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
     ptx::prefetch_tensormap(&tm_v);
   }
   if (threadIdx.x < 128) reinterpret_cast<uint32_t*>(ones)[threadIdx.x] = 0x7f7f7f7fu;
+  for (int i = threadIdx.x; i < 2 * D; i += kThreads) nan_table[i] = INT_MAX;
   for (int i = threadIdx.x; i < 512; i += kThreads)
     reinterpret_cast<uint32_t*>(one_values)[i] = 0x38383838u;
   ptx::fence_proxy_async();
@@ -652,7 +657,12 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
                                       in_row * 16) = make_uint4(0, 0, 0, 0);
           }
         }
-        const bool bounded = a.causal && t0 + held - 1 > first_position;
+        const bool bounded = a.causal && t0 + held - 1 > first_position;  // some row does not see all
+        if (bounded) {
+          __syncwarp();
+          clear_nan<D>(slots + slot * C::kSlotBytes, quarter * 32, 32, t0, nan_table + (segment & 1) * D,
+                       nan_flag + (segment & 1), lane);
+        }
         float my_top = -INFINITY;  // of row lane % RP in this warp's 32 tokens
 #pragma unroll
         for (int c0 = 0; c0 < RP; c0 += C::kChunk) {
@@ -784,6 +794,11 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       failed = ptx::barrier_any(3, 2 * kGroupWarps * 32, failed);
       if (failed) break;
       ptx::tc_fence_after();
+      // The table of the segment before this one is of the next.
+      const int* nan_from = nan_table + (segment & 1) * D;
+      const bool nans = nan_flag[segment & 1] != 0;
+      if (threadIdx.x < D) nan_table[(segment + 1 & 1) * D + threadIdx.x] = INT_MAX;
+      if (threadIdx.x == 0) nan_flag[segment + 1 & 1] = 0;
       // Lane r: what row r's two accumulators are multiplied by (RP <= 32).
       float factor_a = 0.0f, factor_b = 0.0f;
       if (lane < RP) {
@@ -840,6 +855,11 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
           }
         }
         const int d = h * 128 + token;
+        if (nans && d < D) {
+#pragma unroll
+          for (int n = 0; n < 8; ++n)
+            if (nan_from[d] <= first_position + (r0 + n) / a.group) v[n] = NAN;
+        }
 #pragma unroll
         for (int n = 0; n < 8; ++n) {
           const int r = r0 + n;

@@ -24,6 +24,7 @@
 //    joins in the order of the tiles.
 #include "kv_attention.cuh"
 
+#include <climits>
 #include <cstdlib>
 
 namespace mx {
@@ -54,7 +55,7 @@ struct PrefillCfg {
   static constexpr int kPBytes = kTmemP ? 0 : TERMS * kRows * kKvTile;
   static constexpr int kStageWarp = kTmemP ? 1024 : 2048;  // bytes a warp stages outputs in
   static constexpr int kStageBytes = kTmemP ? kSoftmaxWarps * kStageWarp : 0;  // else in P
-  static constexpr int kFixedBytes = 11264;
+  static constexpr int kFixedBytes = 12288;
   static constexpr int kBudget = 227 * 1024 - 1024;
   static constexpr int kFit = (kBudget - kFixedBytes - kStageBytes - kQBytes - kBuffers * kPBytes) / (kSlotBytes + 512);
   static constexpr int kSlots = kFit > 8 ? 8 : kFit;
@@ -276,12 +277,14 @@ kv_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   Segment* segments = reinterpret_cast<Segment*>(p_sf + 6 * 512);  // two
   float* row_sum = reinterpret_cast<float*>(segments + 2);         // [block][row]
   float* row_top = row_sum + 4 * kRows;                            // [block][row]
-  Cursor* start = reinterpret_cast<Cursor*>(row_top + 4 * kRows);
+  int* nan_from = reinterpret_cast<int*>(row_top + 4 * kRows);     // [head_dim], see clear_nan
+  Cursor* start = reinterpret_cast<Cursor*>(nan_from + 256);
   int64_t* share_smem = reinterpret_cast<int64_t*>(start + 1);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(share_smem + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* ask_flag = abort_flag + 1;               // [quarter][2]
-  static_assert(512 + 9 * 512 + 2 * sizeof(Segment) + 8 * kRows * 4 + sizeof(Cursor) + 16 + 8 + 32 <=
+  volatile int* nan_seen = ask_flag + 8;
+  static_assert(512 + 9 * 512 + 2 * sizeof(Segment) + 8 * kRows * 4 + 1024 + sizeof(Cursor) + 16 + 8 + 36 <=
                     C::kFixedBytes,
                 "fixed area");
 
@@ -659,6 +662,8 @@ kv_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       for (int n = 0; n < kBatch; ++n) scale[n] = query_scale<T, kPer>(words[n], first_row + n < real);
       failed = ptx::barrier_any(1, kSoftmaxWarps * 32, failed);
       if (failed) return;
+      if (threadIdx.x < D) nan_from[threadIdx.x] = INT_MAX;
+      if (threadIdx.x == 0) *nan_seen = 0;
       float mine = scale[0];
 #pragma unroll
       for (int n = 1; n < kBatch; ++n) mine = lane == n ? scale[n] : mine;
@@ -702,13 +707,16 @@ kv_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       int64_t sees = length;
       if (a.causal) sees = min(sees, seg.first_position + (seg.row0 + row) / a.group + 1);
       const int visible = sees < 0 ? 0 : (int)sees;
+      // All rows of the item see the tokens below this.
+      const int64_t all_see = a.causal ? seg.first_position + seg.row0 / a.group + 1 : length;
       float ref = -INFINITY, sum = 0.0f;
 #pragma unroll 1
       for (int j = 0; j < tiles; ++j) {
         const int i = i0 + j, buffer = i % C::kBuffers;
         const int t0 = (tile0 + j) * kKvTile + block * kKvBlock;  // this thread's first token
         const bool named = all_named || (t0 < length && kv_page(a.batch, a.cache, seg.b, t0 / kKvBlock) >= 0);
-        if (!named || t0 + kKvBlock > length) {
+        const bool partly = (int64_t)(tile0 + j + 1) * kKvTile > all_see;  // the same in all warps
+        if (partly || !named || t0 + kKvBlock > length) {
           // Rows of V without a token may hold anything, NaN among them, and 0 * NaN is NaN: clear
           // them once the tile has landed.  The four warps of a block clear eight rows each.
           const int at = at0 + (j + 1 < tiles ? 2 * j + 2 : 2 * j + 1);
@@ -723,6 +731,9 @@ kv_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
                                         in_row * 16) = make_uint4(0, 0, 0, 0);
             }
           }
+          __syncwarp();
+          if (partly && !failed)
+            clear_nan<D>(v_s, block * kKvBlock + quarter * 8, 8, (tile0 + j) * kKvTile, nan_from, nan_seen, lane);
           ptx::fence_proxy_async();
         }
         wait(sfull0 + 8 * buffer, (uint32_t)(i / C::kBuffers) & 1u, 512);
@@ -850,6 +861,7 @@ kv_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       const bool mine = r < seg.rows;
       // Through shared memory, so that a row's values leave together: each warp has 2 KB of its
       // rows in the first two terms of P, which no product reads any more, or 1 KB apart.
+      const bool nans = *nan_seen != 0;
       constexpr int kMost = C::kStageWarp / 64;                 // 16-bit columns that fit
       constexpr int kCols = D / 4 < kMost ? D / 4 : kMost, kPieces = kCols / 8;  // a pass; 16-byte pieces
       constexpr int kPartCols = kMost / 2, kPartPieces = kPartCols / 4;          // of 32-bit columns
@@ -866,6 +878,11 @@ kv_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
           uint32_t o[kCols];
           ptx::tmem_ld_chunk<kCols>(lane_t + C::kOCol + c0, o);
           ptx::tmem_ld_wait();
+          if (nans) {
+#pragma unroll
+            for (int n = 0; n < kCols; ++n)
+              if (nan_from[c0 + n] < visible) o[n] = 0x7fc00000u;
+          }
           uint32_t w[kCols / 2];
 #pragma unroll
           for (int n = 0; n < kCols / 2; ++n) {
@@ -918,6 +935,11 @@ kv_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
           uint32_t o[kPartCols];
           ptx::tmem_ld_chunk<kPartCols>(lane_t + C::kOCol + c0, o);
           ptx::tmem_ld_wait();
+          if (nans) {
+#pragma unroll
+            for (int n = 0; n < kPartCols; ++n)
+              if (nan_from[c0 + n] < visible) o[n] = 0x7fc00000u;
+          }
 #pragma unroll
           for (int n = 0; n < kPartPieces; ++n)
             *reinterpret_cast<uint4*>(stage + lane * kPartCols * 4 +

@@ -537,3 +537,32 @@ def test_rotary_of_odd_strides_and_no_tokens(mx):
     assert empty[0].shape == (0, 3, 64)
     back = mx.rotary_multi_axis(*want, -pos, f)            # turning back restores the rows
     assert float((back[0].float() - q.float()).abs().max()) <= 2.0 ** -7 * float(q.abs().max()) * 2
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("rows", [4, 150])
+def test_nan_behind_a_row_does_not_reach_it(mx, rows, dim, dtype):
+    """Causal: a NaN value reaches the rows at and behind its token, in its head and column, and a
+    NaN key the rows at and behind it; the rows before stay as they were without them."""
+    n = 300
+    batch = Batch(mx, 42, [n, n], [rows, rows], 2, 64, dim, finite=True)
+    q = torch.randn((2 * rows, 4, dim), generator=_gen(4)).to(dtype).to(DEV)
+    clean = _attend(mx, batch, q, max_query_len=rows)
+    def spot(b, position):
+        return int(batch.table[b, position // 64]), position % 64
+    first = n - rows
+    at_v, at_k = first + rows // 2, first + rows // 2 + 1
+    page, slot = spot(0, at_v)
+    batch.cache.v_values[page, 1, slot, dim - 3] = 0xFF
+    batch.cache.v_values[page, 1, slot, 0] = 0x7F
+    page, slot = spot(1, at_k)
+    batch.cache.k_values[page, 0, slot, 7] = 0x7F
+    got = _attend(mx, batch, q, max_query_len=rows).cpu()
+    want = clean.cpu().clone()
+    for column in (dim - 3, 0):
+        want[at_v - first : rows, 2:, column] = math.nan
+    want[rows + at_k - first :, :2] = math.nan
+    assert torch.equal(got.isnan(), want.isnan())
+    ok = ~want.isnan()
+    assert torch.equal(got[ok], want[ok])
