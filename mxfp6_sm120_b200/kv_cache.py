@@ -35,12 +35,17 @@ _BF16, _F16 = torch.bfloat16, torch.float16
 _SM100_SEEN: set[int] = set()
 
 
+def _raw_stream(index: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 def _launch(device: torch.device, function, *args) -> None:
     """Call a C entry on ``device`` and its current stream.
 
     These operators run several times per decoder layer with microseconds of GPU work each, so the
     argument rules above the call are plain comparisons whose messages are only built to be raised,
-    and the device is switched only when it is not the current one.
+    the device is switched only when it is not the current one, and the stream is asked for by its
+    handle (0.1 us; as an object 1.3 us).
     """
     index = device.index
     if index not in _SM100_SEEN:
@@ -49,10 +54,10 @@ def _launch(device: torch.device, function, *args) -> None:
         _require_sm100(device)
         _SM100_SEEN.add(index)
     if torch.cuda.current_device() == index:
-        status = function(*args, torch.cuda.current_stream(index).cuda_stream)
+        status = function(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
-            status = function(*args, torch.cuda.current_stream(index).cuda_stream)
+            status = function(*args, _raw_stream(index))
     if status != 0:
         check(status)
 
@@ -284,7 +289,7 @@ def kv_cache_attention(q: torch.Tensor, cache: PagedKVCache, block_table: torch.
     query head ``h`` reads key head ``h // (q_heads // kv_heads)``.  A row that sees no token is
     zero.  ``scale`` multiplies the scores (default ``head_dim ** -0.5``).  ``max_query_len``: an
     upper bound of the rows of any sequence (default: 1 without ``cu_seqlens``, else all rows); a
-    tight one picks the better kernel, and rows of a sequence that has more are not written.
+    tight one picks the better kernel, and rows of a sequence that has more may be left unwritten.
     Write the rows' own keys and values first (:func:`kv_cache_write` takes the same
     ``block_table``, ``seq_lens`` and ``cu_seqlens``).
     """

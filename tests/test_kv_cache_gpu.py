@@ -566,3 +566,116 @@ def test_nan_behind_a_row_does_not_reach_it(mx, rows, dim, dtype):
     assert torch.equal(got.isnan(), want.isnan())
     ok = ~want.isnan()
     assert torch.equal(got[ok], want[ok])
+
+
+# ------------------------------------------------------- attention: sizes and scores at the edges
+
+
+def _rescale_blocks(batch, exponent_of_tile, tiles=128):
+    """Key scales of ``2**exponent`` per tile of tokens (scores of about that many nats)."""
+    for b, n in enumerate(batch.lens):
+        for p in range(0, n, 32):
+            page, block = batch.table[b, p // batch.page], p % batch.page // 32
+            batch.scales[0][page, :, block] = 120 + exponent_of_tile[p // tiles % len(exponent_of_tile)]
+    batch.cache.k_scales.copy_(torch.from_numpy(batch.scales[0]))
+
+
+def _check_large_scores(batch, q, got, scale, causal):
+    """As _check_attention, with the rounding of the 32-bit scores written out.  A score is a sum of
+    at most 24 matrix instructions (8 steps along head_dim, 3 terms), each of which may cut off the
+    last bit, 2^-23, of a partial sum of at most S = sum_i |q_i k_i| * scale.  An error of e nats in
+    the scores of numerator and denominator changes the output by at most 2 e of the weighted
+    magnitudes: 2 * 24 * 2^-23 * S more than _delta."""
+    want = batch.oracle_attention(q, scale, causal)
+    weight = batch.weight_of(q, scale, causal)
+    most = 0.0
+    for b, n in enumerate(batch.lens):
+        k = np.abs(kvo.read(batch.values[0], batch.scales[0], batch.table, [(b, p) for p in range(n)]))
+        rows = np.abs(kvo.to_numpy(q[batch.cu[b] : batch.cu[b + 1]]))
+        for h in range(q.shape[1]):
+            most = max(most, float((rows[:, h] @ k[:, h // (q.shape[1] // batch.heads)].T).max()) * abs(scale))
+    half = torch.finfo(q.dtype).eps / 2
+    delta = _delta(q.dtype) + 2 * 24 * 2.0 ** -23 * most
+    assert delta < 0.02                       # the check still tells right from wrong
+    off = np.abs(kvo.to_numpy(got) - want)
+    assert np.isfinite(off).all()
+    assert float((off - (half * np.abs(want) + delta * weight + 1e-7)).max()) <= 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("sequences,rows", [(1, 1), (90, 1), (2, 70)])
+def test_maxima_that_jump_between_tiles(mx, sequences, rows, dtype):
+    """Tiles whose largest scores are tens and hundreds of powers of two above and below the ones
+    before them, in lists that are cut between CTAs and in lists that are not."""
+    lens = [900 - 3 * b for b in range(sequences)]
+    batch = Batch(mx, 51, lens, [rows] * sequences, 2, 32, 64, spread=0)
+    _rescale_blocks(batch, [0, 2, 4, 6, 1, 6, 3, 5])
+    q = torch.randn((batch.tokens, 4, 64), generator=_gen(52))
+    q[:, 1] *= 0.125                          # a row of another range beside it
+    q = q.to(dtype).to(DEV)
+    got = _attend(mx, batch, q, max_query_len=rows)
+    _check_large_scores(batch, q, got, 64 ** -0.5, True)
+
+
+@pytest.mark.parametrize("dim,rows", [(128, 1), (128, 40), (256, 1), (256, 40)])
+def test_maxima_that_jump_in_wide_heads(mx, dim, rows):
+    batch = Batch(mx, 53, [700, 650], [rows, rows], 1, 64, dim, spread=0)
+    _rescale_blocks(batch, [0, 4, 6, 2, 7, 1])
+    q = torch.randn((batch.tokens, 4, dim), generator=_gen(54)).to(torch.bfloat16).to(DEV)
+    got = _attend(mx, batch, q, max_query_len=rows)
+    _check_large_scores(batch, q, got, dim ** -0.5, True)
+
+
+@pytest.mark.parametrize("rows", [1, 50])
+@pytest.mark.parametrize("scale", [0.0, -0.125])
+def test_scale_of_zero_and_below(mx, rows, scale):
+    """Zero: the mean of the values that a row sees.  Negative: the smallest scores weigh most."""
+    batch = Batch(mx, 55, [333, 80], [rows, rows], 2, 32, 64)
+    q = torch.randn((2 * rows, 4, 64), generator=_gen(56)).to(torch.bfloat16).to(DEV)
+    got = _attend(mx, batch, q, max_query_len=rows, scale=scale)
+    _check_attention(batch, q, got, scale, True)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim,group", [(64, 40), (128, 64), (256, 33)])
+def test_many_query_heads_of_one_key_head(mx, dim, group, dtype):
+    """One new token already has more rows than a few: sequences of one and of three tokens."""
+    for news in ([1, 1, 1], [3, 1, 0]):
+        batch = Batch(mx, 57, [300, 1, 45], news, 1, 64, dim)
+        q = torch.randn((batch.tokens, group, dim), generator=_gen(58)).to(dtype).to(DEV)
+        got = _attend(mx, batch, q, max_query_len=max(news))
+        _check_attention(batch, q, got, dim ** -0.5, True)
+
+
+@pytest.mark.parametrize("dim,page", [(64, 128), (128, 32), (256, 64)])
+def test_large_ragged_batch_of_few_and_many_rows(mx, dim, page):
+    """150 sequences: most with one new token, a few with chunks, some empty."""
+    rng = random.Random(59)
+    news = [rng.choice([1, 1, 1, 1, 0, 2, 45]) for _ in range(150)]
+    lens = [max(n, rng.choice([1, 5, 40, 200])) for n in news]
+    batch = Batch(mx, 60, lens, news, 1, page, dim)
+    q = torch.randn((batch.tokens, 2, dim), generator=_gen(61)).to(torch.bfloat16).to(DEV)
+    got = _attend(mx, batch, q, max_query_len=45)
+    _check_attention(batch, q, got, dim ** -0.5, True)
+
+
+def test_offsets_that_make_no_sense_stay_in_bounds(mx):
+    """Descending, negative and too large row offsets; a bound that is too small; lengths below zero
+    and behind the table: rows may be anything or unwritten, but nothing else is touched."""
+    batch = Batch(mx, 62, [100, 64, 3], [30, 1, 2], 2, 32, 64)
+    guard = torch.full((batch.tokens + 40, 6, 64), 9.0, dtype=torch.bfloat16, device=DEV)
+    out = guard[20 : 20 + batch.tokens]
+    q = torch.randn((batch.tokens, 6, 64), generator=_gen(63)).to(torch.bfloat16).to(DEV)
+    for lens, cu, most in (([100, 64, 3], [30, 3, 33, 1], 40), ([100, 64, 3], [-5, -1, 10 ** 6, 2 ** 31 - 1], 40),
+                           ([-7, 2 ** 31 - 1, 10 ** 6], batch.cu, 40), ([-2 ** 31, 64, 0], batch.cu, 40),
+                           (batch.lens, [0, 0, 0, 0], 40), (batch.lens, [2, 33, 33, 33], 1)):
+        mx.kv_cache_attention(q, batch.cache, batch.dev[0], _i32(lens), _i32(cu), max_query_len=most, out=out)
+        assert bool((guard[:20] == 9.0).all()) and bool((guard[20 + batch.tokens :] == 9.0).all())
+    # sequences within a bound that others exceed are right
+    out.fill_(9.0)
+    mx.kv_cache_attention(q, batch.cache, *batch.dev, max_query_len=2, out=out)
+    assert bool((out[:30] == 9.0).all())
+    whole = _attend(mx, batch, q, max_query_len=30)
+    _check_attention(batch, q, whole, 64 ** -0.5, True)
+    part = torch.cat([whole[:30], out[30:]])
+    _check_attention(batch, q, part, 64 ** -0.5, True)
