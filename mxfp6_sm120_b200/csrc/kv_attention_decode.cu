@@ -13,8 +13,9 @@
 //    With at most 96 columns an MMA costs what its 128-row operand costs (about 33 ns).
 //  * Warps: 0-3 and 4-7 softmax (one lane per token; the two groups take alternate tiles, each
 //    with its own running maximum and output accumulator, because one group needs about as long
-//    for a tile as HBM does), 8 TMA, 9 MMAs of the scores (two tiles ahead), 10 MMAs of the
-//    outputs, 11 quantises queries and describes the segments.
+//    for a tile as HBM does), 8 and 9 TMA of K and of V (one warp for both held heads of 128 back:
+//    131072 tokens x 8 heads, 8 rows each: 65 us, with two 55), 10 MMAs of the scores (two tiles
+//    ahead), 11 MMAs of the outputs, 12 and 13 quantise queries and describe the segments.
 //  * The list of (sequence, key head, tile of 128 tokens) is cut into equal shares, one per CTA
 //    (one per SM), whatever the lengths are: the cut follows the lengths on the device.  A CTA
 //    whose share covers all tiles of a (sequence, head) writes its rows; otherwise it leaves
@@ -40,9 +41,9 @@ int* device_status_word(int device);
 
 namespace {
 
-constexpr int kThreads = 416;
+constexpr int kThreads = 448;
 constexpr int kGroupWarps = 4;  // warps of a softmax group, one per 32 lanes of tensor memory
-constexpr int kTmaWarp = 8, kScoreWarp = 9, kOutputWarp = 10, kQueryWarp = 11, kQueryWarps = 2;
+constexpr int kKeyWarp = 8, kValueWarp = 9, kScoreWarp = 10, kOutputWarp = 11, kQueryWarp = 12, kQueryWarps = 2;
 // Query buffers.  Scores run two tiles ahead of the outputs, so a tile of one segment may be
 // waiting for its output while the scores of the second segment behind it are due.
 constexpr int kQueries = 3;
@@ -67,7 +68,9 @@ struct DecodeCfg {
   static constexpr int kFit =
       (kBudget - kFixedBytes - kQueries * kQBytes - 2 * kPBytes) / (kSlotBytes + 512);
   static constexpr int kSlots = kFit > 16 ? 16 : kFit;
-  static_assert(kSlots >= 4, "the ring needs two tiles of K and V");
+  // Two rings: the scores run ahead of the outputs, so K has the odd slot.
+  static constexpr int kKeySlots = (kSlots + 1) / 2, kValueSlots = kSlots / 2;
+  static_assert(kValueSlots >= 2, "the rings need two tiles of K and V");
   static constexpr int kSmemBytes =
       1024 + kSlots * (kSlotBytes + 512) + kQueries * kQBytes + 2 * kPBytes + kFixedBytes;
   // Tensor memory columns: two score tiles; per softmax group an output of one or two halves
@@ -209,12 +212,6 @@ struct Segment {
   int whole;        // all tiles of the item are here
 };
 
-// Place of tile i's K and V (of `count` tiles) in the order of the copies: K0, K1, K2, V0, K3, V1, ...
-__device__ __forceinline__ int slot_of_k(int i) { return i < 2 ? i : 2 * i - 2; }
-__device__ __forceinline__ int slot_of_v(int i, int count) {
-  return i + 2 < count ? 2 * i + 3 : count + i;
-}
-
 template <int D, int RP, int TERMS>
 __global__ void __launch_bounds__(kThreads, 1)
 kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
@@ -319,16 +316,20 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   // E4M3 x E4M3, UE8M0 scales, M = 128, N = kN; K-major unless bit 15 says otherwise for A.
   constexpr uint32_t kIdesc = ((uint32_t)(C::kN >> 3) << 17) | (1u << 23) | ((128u >> 4) << 24);
 
-  if (count > 0 && warp == kTmaWarp) {
-    // ---------------- TMA producer ----------------
-    // Tiles are fetched in the order of their use: K0, K1, K2, V0, K3, V1, ...  Lane l looks up block
-    // l % 4 of tile l / 4 of a group of eight tiles and later issues that block's copies itself;
-    // the next group's lookups are in flight while this group is copied.
+  if (count > 0 && (warp == kKeyWarp || warp == kValueWarp)) {
+    // ---------------- TMA producers, one for K and one for V ----------------
+    // Lane l looks up block l % 4 of tile l / 4 of a group of eight tiles and later issues that
+    // block's copies itself; the next group's lookups are in flight while this group is copied.
+    const bool is_v = warp == kValueWarp;
+    const int first_slot = is_v ? C::kKeySlots : 0;
+    const int end_slot = is_v ? C::kSlots : C::kKeySlots;
+    const CUtensorMap* map = is_v ? &tm_v : &tm_k;
+    const uint8_t* scales = is_v ? a.cache.v_scales : a.cache.k_scales;
     Cursor mine = *start;
     mine.load(a);
     for (int i = 0; i < (lane >> 2); ++i) mine.next(a);
     int64_t page = -1, next_page = -1;  // scale block of this lane's block of tokens, or -1
-    uint32_t k_sf = 127, v_sf = 127, next_k = 127, next_v = 127;
+    uint32_t scale = 127, next_scale = 127;
     auto lookup_page = [&]() -> int64_t {
       const int block = mine.tile * kKvTileBlocks + (lane & 3);
       if (block * kKvBlock >= mine.seq.length) return -1;
@@ -336,84 +337,60 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       return p < 0 ? -1 : (p * a.cache.kv_heads + mine.head) * per_page + block % per_page;
     };
     page = lookup_page();
-    if (page >= 0) {
-      k_sf = a.cache.k_scales[page];
-      v_sf = a.cache.v_scales[page];
-    }
-    // The V tiles of a group's last two tiles are copied after the next group's first K tiles.
-    int64_t last_page = -1;
-    uint32_t last_v = 127;
-    int slot = 0;
+    if (page >= 0) scale = scales[page];
+    int slot = first_slot;
     uint32_t phase = 0;
     bool ok = true;
     const bool leads = (lane & 3) % per_page == 0;  // first block of a page in its tile
     const uint32_t page_bytes = (uint32_t)(a.cache.page_size * D);
     const uint32_t slots_s = ptx::smem_u32(slots) + (lane & 3) * kKvBlock * C::kRowBytes;
-    // Copies one tile whose four blocks are known to lanes src .. src + 3.
-    auto copy = [&](bool is_v, int64_t lane_page, uint32_t lane_sf, int src) {
-      ok = ok && __all_sync(0xffffffffu, bounded_wait(empty0 + 8 * slot, phase ^ 1u, abort_flag,
-                                                      a.status, 401));
-      if (!ok) return;
-      const uint32_t bar = full0 + 8 * slot;
-      // One copy per page and 128 columns; blocks of no page are left as they are.
-      const bool issue = (lane & ~3) == src && leads && lane_page >= 0;
-      const uint32_t pages = __popc(__ballot_sync(0xffffffffu, issue));
-      if (lane == src) ptx::mbar_arrive_expect_tx(bar, pages * page_bytes);
-      __syncwarp();
-      if (issue) {
-#pragma unroll
-        for (int s = 0; s < C::kSubs; ++s)
-          ptx::tma_load_2d(slots_s + slot * C::kSlotBytes + s * C::kSubBytes, is_v ? &tm_v : &tm_k,
-                           s * 128, (int)(lane_page * kKvBlock), bar);
-      }
-      // Scale atom: lane = row % 32.  Keys: row block c of 32 tokens has one factor for all of
-      // head_dim; values: every row has the factors of the four 32-token steps along K.
-      uint32_t sf[kKvTileBlocks];
-#pragma unroll
-      for (int i = 0; i < kKvTileBlocks; ++i) sf[i] = __shfl_sync(0xffffffffu, lane_sf, src + i);
-      const uint32_t all = sf[0] | sf[1] << 8 | sf[2] << 16 | sf[3] << 24;
-      reinterpret_cast<uint4*>(sf_tiles + slot * 512)[lane] =
-          is_v ? make_uint4(all, all, all, all)
-               : make_uint4(sf[0] * 0x01010101u, sf[1] * 0x01010101u, sf[2] * 0x01010101u,
-                            sf[3] * 0x01010101u);
-      const uint32_t named = __ballot_sync(0xffffffffu, lane_page >= 0) >> src & 15u;
-      if (lane == 0) slot_named[slot] = named;
-      ptx::fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(bar);
-      if (++slot == C::kSlots) {
-        slot = 0;
-        phase ^= 1u;
-      }
-    };
     for (int i0 = 0; ok && i0 < count; i0 += 8) {
       const bool more = i0 + 8 < count;
       if (more) {
         for (int i = 0; i < 8; ++i) mine.next(a);
         next_page = lookup_page();
       }
-      for (int j = 0; ok && j < 8 && i0 + j < count; ++j) {
-        copy(false, page, k_sf, 4 * j);
-        if (j > 1) copy(true, page, v_sf, 4 * (j - 2));
-        else if (i0 > 0) copy(true, last_page, last_v, 4 * (j + 6));
-        if (j == 3 && more) {
-          next_k = next_page >= 0 ? a.cache.k_scales[next_page] : 127u;
-          next_v = next_page >= 0 ? a.cache.v_scales[next_page] : 127u;
+      // One copy per page and 128 columns; blocks of no page are left as they are.
+      const bool issue = leads && page >= 0;
+      const uint32_t issued = __ballot_sync(0xffffffffu, issue);
+      const uint32_t named = __ballot_sync(0xffffffffu, page >= 0);
+      for (int j = 0; j < 8 && i0 + j < count; ++j) {
+        const int src = 4 * j;  // lanes src .. src + 3 know the tile's blocks
+        ok = ok && __all_sync(0xffffffffu, bounded_wait(empty0 + 8 * slot, phase ^ 1u, abort_flag,
+                                                        a.status, 401));
+        if (!ok) break;
+        const uint32_t bar = full0 + 8 * slot;
+        if (lane == src) ptx::mbar_arrive_expect_tx(bar, __popc(issued >> src & 15u) * page_bytes);
+        __syncwarp();
+        if (issue && (lane & ~3) == src) {
+#pragma unroll
+          for (int s = 0; s < C::kSubs; ++s)
+            ptx::tma_load_2d(slots_s + slot * C::kSlotBytes + s * C::kSubBytes, map, s * 128,
+                             (int)(page * kKvBlock), bar);
         }
+        // Scale atom: lane = row % 32.  Keys: row block c of 32 tokens has one factor for all of
+        // head_dim; values: every row has the factors of the four 32-token steps along K.
+        uint32_t sf[kKvTileBlocks];
+#pragma unroll
+        for (int i = 0; i < kKvTileBlocks; ++i) sf[i] = __shfl_sync(0xffffffffu, scale, src + i);
+        const uint32_t all = sf[0] | sf[1] << 8 | sf[2] << 16 | sf[3] << 24;
+        reinterpret_cast<uint4*>(sf_tiles + slot * 512)[lane] =
+            is_v ? make_uint4(all, all, all, all)
+                 : make_uint4(sf[0] * 0x01010101u, sf[1] * 0x01010101u, sf[2] * 0x01010101u,
+                              sf[3] * 0x01010101u);
+        if (lane == 0) slot_named[slot] = named >> src & 15u;
+        ptx::fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(bar);
+        if (++slot == end_slot) {
+          slot = first_slot;
+          phase ^= 1u;
+        }
+        if (j == 3 && more) next_scale = next_page >= 0 ? scales[next_page] : 127u;
       }
-      if (!more) break;
-      last_page = page;
-      last_v = v_sf;
       page = next_page;
-      k_sf = next_k;
-      v_sf = next_v;
+      scale = next_scale;
     }
-    if (count > 1) {
-      // The tile before the last one may have been the last of the group before.
-      const bool before = ((count - 1) & 7) == 0;
-      copy(true, before ? last_page : page, before ? last_v : v_sf, 4 * ((count - 2) & 7));
-    }
-    copy(true, page, v_sf, 4 * ((count - 1) & 7));
   } else if (count > 0 && warp == kScoreWarp) {
     // ---------------- scores ----------------
     // Two warps issue MMAs: with one, the scores of a tile waited behind the outputs of the tile
@@ -433,14 +410,13 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         left = segments[segment % kQueries].tiles;
       }
       --left;
-      const int at = slot_of_k(i);
-      const int slot = at % C::kSlots;
+      const int slot = i % C::kKeySlots;
       // The score tile of two tiles ago has been read.
       if (i >= 2)
         ok = ok && __all_sync(0xffffffffu, bounded_wait(sread0 + 8 * (i & 1), (uint32_t)((i - 2) >> 1) & 1u,
                                                         abort_flag, a.status, 415));
       ok = ok && __all_sync(0xffffffffu,
-                            bounded_wait(full0 + 8 * slot, (uint32_t)(at / C::kSlots) & 1u,
+                            bounded_wait(full0 + 8 * slot, (uint32_t)(i / C::kKeySlots) & 1u,
                                          abort_flag, a.status, 403));
       if (!ok) break;
       ptx::tc_fence_after();
@@ -471,12 +447,11 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
     bool ok = true;
     int left = 0, number = 0;  // tiles of the segment that are still to come, that were
     for (int i = 0, segment = -1; i < count; ++i) {
-      const int at = slot_of_v(i, count);
-      const int slot = at % C::kSlots;
+      const int slot = C::kKeySlots + i % C::kValueSlots;
       ok = ok && __all_sync(0xffffffffu, bounded_wait(pfull0 + 8 * (i & 1), (uint32_t)(i >> 1) & 1u,
                                                       abort_flag, a.status, 404));
       ok = ok && __all_sync(0xffffffffu,
-                            bounded_wait(full0 + 8 * slot, (uint32_t)(at / C::kSlots) & 1u,
+                            bounded_wait(full0 + 8 * slot, (uint32_t)(i / C::kValueSlots) & 1u,
                                          abort_flag, a.status, 405));
       if (!ok) break;
       if (left == 0) {
@@ -639,9 +614,8 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         const int t0 = (seg.tile + j) * kKvTile;
         const int held = min(kKvTile, length - t0);  // tokens of this tile that exist
         wait(sfull, done & 1u, 409);
-        const int at = slot_of_v(i, count);
-        const int slot = at % C::kSlots;
-        wait(full0 + 8 * slot, (uint32_t)(at / C::kSlots) & 1u, 408);
+        const int slot = C::kKeySlots + i % C::kValueSlots;
+        wait(full0 + 8 * slot, (uint32_t)(i / C::kValueSlots) & 1u, 408);
         if (failed) break;
         ptx::tc_fence_after();
         const bool named = (slot_named[slot] >> quarter & 1u) != 0;
