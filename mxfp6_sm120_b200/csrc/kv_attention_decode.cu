@@ -614,6 +614,10 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         const int t0 = (seg.tile + j) * kKvTile;
         const int held = min(kKvTile, length - t0);  // tokens of this tile that exist
         wait(sfull, done & 1u, 409);
+        // PV of this group's last tile, i - 2, has read the weights that this tile's replace.  It also
+        // shows that V of tile i - kValueSlots, which had this tile's slot, has landed: copies land
+        // in any order, and one phase further back the parity would be the same.
+        if (done > 0) wait(pvdone, (done - 1) & 1u, 410);
         const int slot = C::kKeySlots + i % C::kValueSlots;
         wait(full0 + 8 * slot, (uint32_t)(i / C::kValueSlots) & 1u, 408);
         if (failed) break;
@@ -670,8 +674,6 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
             for (int r = 0; r < C::kChunk; ++r)
               if (t0 + token > first_position + (c0 + r) / a.group) s[r] = -INFINITY;
           }
-          // PV of this group's last tile has read the weights that this tile's replace.
-          if (c0 == 0 && done > 0) wait(pvdone, (done - 1) & 1u, 410);
 #pragma unroll
           for (int r = 0; r < C::kChunk; r += 4) {
             float p[4];

@@ -59,7 +59,15 @@ struct PrefillCfg {
   static constexpr int kBudget = 227 * 1024 - 1024;
   static constexpr int kFit = (kBudget - kFixedBytes - kStageBytes - kQBytes - kBuffers * kPBytes) / (kSlotBytes + 512);
   static constexpr int kSlots = kFit > 8 ? 8 : kFit;
-  static_assert(kSlots >= 2, "a K and a V tile");
+  static_assert(kSlots >= 3 || (kSlots == 2 && kBuffers == 1), "see kEarlyClear");
+  // The softmax warps wait for a V tile too, where rows of it have to be cleared.  Copies land in
+  // any order, and while the tile that had the slot before is still missing, the slot's barrier
+  // stands one phase further back, where the parity is the same; so they have to know that it has
+  // landed.  Tile i's V has place 2 i + 2 (K0, K1, V0, K2, V1, ...).  Before its scores they know it
+  // of the places up to K of tile i - 1, five places back, and of V of tile i - 2, four places back,
+  // where one buffer made them wait for that output; with its scores, up to its K, three places
+  // back; with the last tile's output, two places back.
+  static constexpr bool kEarlyClear = kSlots >= (kBuffers == 1 ? 4 : 5);
   static constexpr int kSmemBytes =
       1024 + kSlots * (kSlotBytes + 512) + kQBytes + kBuffers * kPBytes + kStageBytes + kFixedBytes;
   static constexpr int kOCol = kBuffers * kKvTile;
@@ -715,10 +723,13 @@ kv_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         const int i = i0 + j, buffer = i % C::kBuffers;
         const int t0 = (tile0 + j) * kKvTile + block * kKvBlock;  // this thread's first token
         const bool named = all_named || (t0 < length && kv_page(a.batch, a.cache, seg.b, t0 / kKvBlock) >= 0);
+        if constexpr (!C::kEarlyClear) wait(sfull0 + 8 * buffer, (uint32_t)(i / C::kBuffers) & 1u, 512);
         const bool partly = (int64_t)(tile0 + j + 1) * kKvTile > all_see;  // the same in all warps
         if (partly || !named || t0 + kKvBlock > length) {
           // Rows of V without a token may hold anything, NaN among them, and 0 * NaN is NaN: clear
           // them once the tile has landed.  The four warps of a block clear eight rows each.
+          if constexpr (C::kSlots == 2)
+            if (i > 0) wait(pvdone0, (uint32_t)(i - 1) & 1u, 517);
           const int at = at0 + (j + 1 < tiles ? 2 * j + 2 : 2 * j + 1);
           const int slot = at % C::kSlots;
           wait(full0 + 8 * slot, (uint32_t)(at / C::kSlots) & 1u, 511);
@@ -736,7 +747,7 @@ kv_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
             clear_nan<D>(v_s, block * kKvBlock + quarter * 8, 8, (tile0 + j) * kKvTile, nan_from, nan_seen, lane);
           ptx::fence_proxy_async();
         }
-        wait(sfull0 + 8 * buffer, (uint32_t)(i / C::kBuffers) & 1u, 512);
+        if constexpr (C::kEarlyClear) wait(sfull0 + 8 * buffer, (uint32_t)(i / C::kBuffers) & 1u, 512);
         if (failed) break;
         ptx::tc_fence_after();
         uint32_t raw[32];
