@@ -63,23 +63,27 @@ struct DecodeCfg {
   static constexpr int kSlotBytes = kKvTile * D;     // a K or V tile
   static constexpr int kQBytes = (kN * D + 1023) / 1024 * 1024;
   static constexpr int kPBytes = kN * kKvTile;
-  static constexpr int kFixedBytes = 7168 + 2 * D * 4;
+  // Weights are buffered twice per softmax group, so that it need not wait for the output of its
+  // last tile (about 0.6 us) before it writes the next; a head of 256 spends the room on its ring.
+  static constexpr int kPBuffers = D < 256 ? 2 : 1;
+  static constexpr int kFixedBytes = 8192 + 2 * D * 4;
   static constexpr int kBudget = 227 * 1024 - 1024;
   static constexpr int kFit =
-      (kBudget - kFixedBytes - kQueries * kQBytes - 2 * kPBytes) / (kSlotBytes + 512);
+      (kBudget - kFixedBytes - kQueries * kQBytes - 2 * kPBuffers * kPBytes) / (kSlotBytes + 512);
   static constexpr int kSlots = kFit > 16 ? 16 : kFit;
   // Two rings: the scores run ahead of the outputs, so K has the odd slot.
   static constexpr int kKeySlots = (kSlots + 1) / 2, kValueSlots = kSlots / 2;
-  static_assert(kValueSlots >= 2, "the rings need two tiles of K and V");
+  static_assert(kValueSlots >= 2 * kPBuffers, "the softmax groups wait for V by the output that far back");
   static constexpr int kSmemBytes =
-      1024 + kSlots * (kSlotBytes + 512) + kQueries * kQBytes + 2 * kPBytes + kFixedBytes;
+      1024 + kSlots * (kSlotBytes + 512) + kQueries * kQBytes + 2 * kPBuffers * kPBytes + kFixedBytes;
   // Tensor memory columns: two score tiles; per softmax group an output of one or two halves
   // and the sums of the weights; scales.
   static constexpr int kHalves = D > 128 ? 2 : 1;
   static constexpr int kOCol = 2 * kN;
   static constexpr int kLCol = kOCol + 2 * kHalves * kN;  // sums of the weights, per group
   static constexpr int kSfCol = kLCol + 2 * kN;
-  static constexpr int kColsUsed = kSfCol + 28;
+  static constexpr int kOnesCol = kSfCol + 2 * kPBuffers * 12;  // a set per group and buffer of weights
+  static constexpr int kColsUsed = kOnesCol + 4;
   static constexpr int kChunk = RP % 16 == 0 ? 16 : 8;  // rows of a score tile held at a time
   static constexpr int kTmemCols = kColsUsed <= 64 ? 64 : kColsUsed <= 128 ? 128 : kColsUsed <= 256 ? 256 : 512;
   static_assert(kColsUsed <= 512, "tensor memory");
@@ -223,14 +227,14 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* slots = smem;
   uint8_t* q_tiles = slots + C::kSlots * C::kSlotBytes;        // [buffer][sub][column][row bytes]
-  uint8_t* p_tiles = q_tiles + kQueries * C::kQBytes;                 // two, [column][128 tokens]
-  uint8_t* sf_tiles = p_tiles + 2 * C::kPBytes;                // scale atom of every slot
+  uint8_t* p_tiles = q_tiles + kQueries * C::kQBytes;                 // [group][buffer][column][128 tokens]
+  uint8_t* sf_tiles = p_tiles + 2 * C::kPBuffers * C::kPBytes;                // scale atom of every slot
   uint8_t* fixed = sf_tiles + C::kSlots * 512;
   uint64_t* bars = reinterpret_cast<uint64_t*>(fixed);
   uint8_t* ones = fixed + 512;                                 // scale atom of factors of one
-  uint8_t* p_sf = fixed + 1024;                                // scale atom of each group's weights
-  uint8_t* one_values = fixed + 1024 + 1024;                   // E4M3 ones, see the sums
-  Segment<RP>* segments = reinterpret_cast<Segment<RP>*>(fixed + 4096);  // [buffer]
+  uint8_t* p_sf = fixed + 1024;                                // scale atoms of the weights, as p_tiles
+  uint8_t* one_values = fixed + 1024 + 2048;                   // E4M3 ones, see the sums
+  Segment<RP>* segments = reinterpret_cast<Segment<RP>*>(fixed + 5120);  // [buffer]
   float* red_max = reinterpret_cast<float*>(segments + kQueries);     // [group][warp][RP]
   float* red_top = red_max + 8 * RP;                           // [group][RP]
   int* nan_table = reinterpret_cast<int*>(red_top + 2 * RP);   // [segment parity][head_dim], see clear_nan
@@ -241,21 +245,21 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   volatile int* ask_flag = abort_flag + 1;                     // [group][2]
   volatile int* nan_flag = ask_flag + 4;                       // [segment parity]
   volatile uint32_t* slot_named = reinterpret_cast<volatile uint32_t*>(nan_flag + 2);  // [slot]
-  static_assert(4096 + kQueries * sizeof(Segment<RP>) + 10 * RP * 4 + 2 * D * 4 + sizeof(Cursor) + 16 + 8 + 16 + 72 <=
+  static_assert(5120 + kQueries * sizeof(Segment<RP>) + 10 * RP * 4 + 2 * D * 4 + sizeof(Cursor) + 16 + 8 + 16 + 72 <=
                     C::kFixedBytes,
                 "fixed area");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t full0 = ptx::smem_u32(bars);
   const uint32_t empty0 = full0 + 8 * C::kSlots;
-  const uint32_t sfull0 = empty0 + 8 * C::kSlots;  // two of each but the query barriers
+  const uint32_t sfull0 = empty0 + 8 * C::kSlots;  // one per group; of the weights', one per buffer
   const uint32_t pfull0 = sfull0 + 16;
-  const uint32_t pvdone0 = pfull0 + 16;
-  const uint32_t qfull0 = pvdone0 + 16;
+  const uint32_t pvdone0 = pfull0 + 16 * C::kPBuffers;
+  const uint32_t qfull0 = pvdone0 + 16 * C::kPBuffers;
   const uint32_t qempty0 = qfull0 + 8 * kQueries;
   const uint32_t vsync0 = qempty0 + 8 * kQueries;
   const uint32_t sread0 = vsync0 + 16;
-  static_assert(8 * (2 * 16 + 10 + 2 * kQueries) <= 512, "barriers");
+  static_assert(8 * (2 * 16 + 6 + 4 * C::kPBuffers + 2 * kQueries) <= 512, "barriers");
 
   if (threadIdx.x == 0) {
     *abort_flag = 0;
@@ -267,8 +271,10 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
     }
     for (int i = 0; i < 2; ++i) {
       ptx::mbar_init(sfull0 + 8 * i, 1);
-      ptx::mbar_init(pfull0 + 8 * i, kGroupWarps);
-      ptx::mbar_init(pvdone0 + 8 * i, 1);
+      for (int b = 0; b < C::kPBuffers; ++b) {
+        ptx::mbar_init(pfull0 + 8 * (i * C::kPBuffers + b), kGroupWarps);
+        ptx::mbar_init(pvdone0 + 8 * (i * C::kPBuffers + b), 1);
+      }
       ptx::mbar_init(vsync0 + 8 * i, kGroupWarps);
       ptx::mbar_init(sread0 + 8 * i, kGroupWarps);
     }
@@ -395,8 +401,7 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
     // ---------------- scores ----------------
     // Two warps issue MMAs: with one, the scores of a tile waited behind the outputs of the tile
     // before it, whose weights are not there yet.
-    const uint32_t sf0 = tmem + C::kSfCol;  // keys, values, weights by tile parity, then ones
-    const uint32_t ones_t = sf0 + 24;
+    const uint32_t sf0 = tmem + C::kSfCol, ones_t = tmem + C::kOnesCol;  // sets of keys, values, weights
     if (ptx::elect_one()) ptx::tc_cp_32x128b_warpx4(ones_t, ptx::smem_desc_scale_atom(ptx::smem_u32(ones)));
     __syncwarp();
     bool ok = true;
@@ -443,13 +448,15 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   } else if (count > 0 && warp == kOutputWarp) {
     // ---------------- outputs and sums ----------------
     const uint32_t sf0 = tmem + C::kSfCol;
-    const uint32_t ones_t = sf0 + 24;  // written before the first scores, which the weights follow
+    const uint32_t ones_t = tmem + C::kOnesCol;  // written before the first scores, which the weights follow
     bool ok = true;
     int left = 0, number = 0;  // tiles of the segment that are still to come, that were
     for (int i = 0, segment = -1; i < count; ++i) {
       const int slot = C::kKeySlots + i % C::kValueSlots;
-      ok = ok && __all_sync(0xffffffffu, bounded_wait(pfull0 + 8 * (i & 1), (uint32_t)(i >> 1) & 1u,
-                                                      abort_flag, a.status, 404));
+      const int weights = (i & 1) * C::kPBuffers + (i >> 1) % C::kPBuffers;
+      ok = ok && __all_sync(0xffffffffu,
+                            bounded_wait(pfull0 + 8 * weights, (uint32_t)((i >> 1) / C::kPBuffers) & 1u,
+                                         abort_flag, a.status, 404));
       ok = ok && __all_sync(0xffffffffu,
                             bounded_wait(full0 + 8 * slot, (uint32_t)(i / C::kValueSlots) & 1u,
                                          abort_flag, a.status, 405));
@@ -461,12 +468,12 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       }
       ptx::tc_fence_after();
       if (ptx::elect_one()) {
-        const uint32_t sf_t = sf0 + 12 * (i & 1) + 4, weight_t = sf_t + 4;
+        const uint32_t sf_t = sf0 + 12 * (i % (2 * C::kPBuffers)) + 4, weight_t = sf_t + 4;
         ptx::tc_cp_32x128b_warpx4(sf_t, ptx::smem_desc_scale_atom(ptx::smem_u32(sf_tiles + slot * 512)));
-        ptx::tc_cp_32x128b_warpx4(weight_t, ptx::smem_desc_scale_atom(ptx::smem_u32(p_sf + (i & 1) * 512)));
+        ptx::tc_cp_32x128b_warpx4(weight_t, ptx::smem_desc_scale_atom(ptx::smem_u32(p_sf + weights * 512)));
         const uint32_t v_s = ptx::smem_u32(slots + slot * C::kSlotBytes);
         const uint64_t bd =
-            ptx::smem_desc(ptx::smem_u32(p_tiles + (i & 1) * C::kPBytes), 0, 1024, ptx::kSwizzle128);
+            ptx::smem_desc(ptx::smem_u32(p_tiles + weights * C::kPBytes), 0, 1024, ptx::kSwizzle128);
         const bool first = number < 2;  // of its group in the segment
 #pragma unroll
         for (int h = 0; h < C::kHalves; ++h) {
@@ -489,7 +496,7 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
           ptx::tc_mma_mxf8f6f4(tmem + C::kLCol + (i & 1) * C::kN, ones_d, bd + 2 * ks,
                                kIdesc | ((uint32_t)ks << 4), ones_t, weight_t,
                                (!first || ks > 0) ? 1u : 0u);
-        ptx::tc_commit(pvdone0 + 8 * (i & 1));
+        ptx::tc_commit(pvdone0 + 8 * weights);
         ptx::tc_commit(empty0 + 8 * slot);
       }
       __syncwarp();
@@ -585,12 +592,10 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
     const int token = quarter * 32 + lane;  // within the tile; quarter = its scale block
     const uint32_t lane_t = tmem + ((uint32_t)(quarter * 32) << 16);
     const uint32_t s_t = lane_t + group * C::kN;
-    const uint32_t sfull = sfull0 + 8 * group, pfull = pfull0 + 8 * group;
-    const uint32_t pvdone = pvdone0 + 8 * group, vsync = vsync0 + 8 * group;
-    const uint32_t sread = sread0 + 8 * group;
+    const uint32_t sfull = sfull0 + 8 * group, vsync = vsync0 + 8 * group, sread = sread0 + 8 * group;
     // Weights are stored four tokens at a time: the lane's are tokens lane & ~3 .. | 3 of row
     // lane % 4 of every four.
-    uint8_t* p_s = p_tiles + group * C::kPBytes + (lane & 3) * 128 + (token & 12);
+    uint8_t* p_s0 = p_tiles + group * C::kPBuffers * C::kPBytes + (lane & 3) * 128 + (token & 12);
     const uint32_t p_chunk = (token & 0x70) ^ ((lane & 3) << 4);
     const uint32_t turn1 = lane & 1 ? 0x3715 : 0x6240, turn2 = lane & 2 ? 0x3276 : 0x5410;
     float* my_max = red_max + group * 4 * RP;
@@ -600,6 +605,10 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
     uint32_t votes = 0;    // of them, to ask for another reference
     auto wait = [&](uint32_t bar, uint32_t parity, int code) {
       if (!failed) failed = !__all_sync(0xffffffffu, bounded_wait(bar, parity, abort_flag, a.status, code));
+    };
+    // The output of the group's tile `number`, one of its last kPBuffers.
+    auto wait_output = [&](uint32_t number, int code) {
+      wait(pvdone0 + 8 * (group * C::kPBuffers + number % C::kPBuffers), number / C::kPBuffers & 1u, code);
     };
     for (int segment = 0, i0 = 0; i0 < count; ++segment) {
       wait(qfull0 + 8 * (segment % kQueries), (uint32_t)(segment / kQueries) & 1u, 407);
@@ -614,10 +623,13 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         const int t0 = (seg.tile + j) * kKvTile;
         const int held = min(kKvTile, length - t0);  // tokens of this tile that exist
         wait(sfull, done & 1u, 409);
-        // PV of this group's last tile, i - 2, has read the weights that this tile's replace.  It also
-        // shows that V of tile i - kValueSlots, which had this tile's slot, has landed: copies land
-        // in any order, and one phase further back the parity would be the same.
-        if (done > 0) wait(pvdone, (done - 1) & 1u, 410);
+        // PV of this group's tile kPBuffers before, i - 2 * kPBuffers, has read the weights that this
+        // tile's replace.  It also shows that V of tile i - kValueSlots, which had this tile's slot,
+        // has landed: copies land in any order, and one phase further back the parity would be the
+        // same.
+        if (done >= C::kPBuffers) wait_output(done - C::kPBuffers, 410);
+        const uint32_t weights = group * C::kPBuffers + done % C::kPBuffers;
+        uint8_t* p_s = p_s0 + done % C::kPBuffers * C::kPBytes;
         const int slot = C::kKeySlots + i % C::kValueSlots;
         wait(full0 + 8 * slot, (uint32_t)(i / C::kValueSlots) & 1u, 408);
         if (failed) break;
@@ -723,7 +735,8 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
           const float f = up ? pow2_whole(ref - m) : 1.0f;
           if (up) ref = m;
           if (j != j0 && !failed) {
-            // What has been added up so far shrinks (PV of this group's last tile is done).
+            // What has been added up so far shrinks.
+            wait_output(done - 1, 412);
             ptx::tc_fence_after();
 #pragma unroll 1
             for (int c0 = 0; c0 < C::kN; c0 += 8) {
@@ -757,16 +770,16 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
           const int col = col0 + lane;
           uint32_t code = my_code;
           if constexpr (RP == 24) code = __shfl_sync(0xffffffffu, my_code, col % RP);
-          if (col < C::kN) p_sf[group * 512 + lane * 16 + (col0 / 32) * 4 + quarter] = (uint8_t)code;
+          if (col < C::kN) p_sf[weights * 512 + lane * 16 + (col0 / 32) * 4 + quarter] = (uint8_t)code;
         }
         ptx::fence_proxy_async();
         ptx::tc_fence_before();
         __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(pfull);
+        if (lane == 0) ptx::mbar_arrive(pfull0 + 8 * weights);
       }
       // ---- the output of this CTA's tiles of the item ----
       if (quarter == 0 && lane < RP) red_top[group * RP + lane] = ref;
-      if (j0 < tiles) wait(pvdone, (done - 1) & 1u, 411);
+      if (j0 < tiles) wait_output(done - 1, 411);
       failed = ptx::barrier_any(3, 2 * kGroupWarps * 32, failed);
       if (failed) break;
       ptx::tc_fence_after();
