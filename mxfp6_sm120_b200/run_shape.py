@@ -5,6 +5,8 @@
     python -m mxfp6_sm120_b200.run_shape --op moe --m 32
     python -m mxfp6_sm120_b200.run_shape --op decode --m 32 --context 4000 --layers 2
     python -m mxfp6_sm120_b200.run_shape --op prefill --m 8192 --layers 1
+    python -m mxfp6_sm120_b200.run_shape --op paged_decode --m 32 --context 4000 --layers 2
+    python -m mxfp6_sm120_b200.run_shape --op paged_prefill --m 8192 --layers 1
 
 Prints the mean device time per call: ``--iters`` calls are captured in one CUDA graph
 and the replay is timed with CUDA events.
@@ -21,7 +23,8 @@ import mxfp6_sm120_b200 as mx
 
 def main() -> None:
     parser = argparse.ArgumentParser()
-    parser.add_argument("--op", default="gemm", choices=["gemm", "quantize", "moe", "decode", "prefill"])
+    parser.add_argument("--op", default="gemm", choices=["gemm", "quantize", "moe", "decode", "prefill",
+                                                          "paged_decode", "paged_prefill"])
     parser.add_argument("--m", type=int, default=16)
     parser.add_argument("--n", type=int, default=34816)
     parser.add_argument("--k", type=int, default=5120)
@@ -63,6 +66,34 @@ def main() -> None:
         else:
             def call():
                 return model.prefill(space)
+    elif args.op in ("paged_decode", "paged_prefill"):
+        # The same over the paged 8-bit cache, with rotary positions; random pages and contents.
+        cfg = mx.DecoderConfig()
+        model = mx.DenseDecoder.random(cfg, device, seed=5000, layers=args.layers)
+        space = model.workspace(args.m)
+        space.x.copy_(torch.randn((args.m, cfg.hidden), generator=gen, device=device).to(torch.bfloat16))
+        sequences, length = (args.m, args.context + 1) if args.op == "paged_decode" else (1, args.m)
+        page = 64
+        width = -(-length // page)
+        table = torch.randperm(sequences * width, generator=gen, device=device).to(torch.int32).view(
+            sequences, width)
+        caches = model.new_paged_cache(sequences * width, page)
+        for cache in caches:
+            cache.k_values.random_(0, 0x70, generator=gen)
+            cache.v_values.random_(0, 0x70, generator=gen)
+            cache.k_scales.fill_(119)
+            cache.v_scales.fill_(119)
+        lengths = torch.full((sequences,), length, dtype=torch.int32, device=device)
+        rotary = mx.rotary_frequencies(cfg.head_dim, device=device)
+        first = length - args.m // sequences
+        positions = torch.arange(args.m, device=device, dtype=torch.int32).div(
+            sequences, rounding_mode="floor") + first
+        offsets = None if args.op == "paged_decode" else torch.tensor([0, args.m], dtype=torch.int32,
+                                                                      device=device)
+
+        def call():
+            return model.paged_step(space, caches, table, lengths, offsets,
+                                    max_query_len=args.m // sequences, rotary=rotary, positions=positions)
     else:
         from mxfp6_sm120_b200.moe_layer import MoeLayer
 
@@ -76,6 +107,7 @@ def main() -> None:
             return layer.forward(state, hidden, logits, gate)
 
     # Time graph replays so that host launch overhead does not hide short kernels.
+    torch.cuda.synchronize()  # the inputs were made on another stream
     stream = torch.cuda.Stream()
     with torch.cuda.stream(stream):
         call()
