@@ -30,6 +30,13 @@
 //    by more than 2^16 the four warps move it and shrink the accumulator.  It is also the more
 //    exact way: each block's largest weight is in (181, 363), so E4M3's smallest step never
 //    reaches a weight that counts.  The sums of the weights are a product with ones.
+//
+// Measured inside a CUDA graph (copy rate 6.57 TB/s): 131072 tokens of one sequence, 4 key heads of
+// 256, 6 rows each: 52 us, 5.2 TB/s; 32 sequences of up to 8192: 53 us, 4.9 TB/s; 32 sequences of
+// 8001: 91 us, 5.8 TB/s.  With more rows the softmax of a tile takes longer than its bytes: 131072
+// tokens, 8 key heads of 128: 55 us with 8 rows, 59 with 16, 79 with 24; 48 sequences of 4 drafted
+// tokens (16 rows, up to 4096 tokens): 68 us, 2.9 TB/s, of which about 3 us for every segment's start
+// and end, where the groups meet.  Tried and left: a third softmax group (78 us for the last case).
 #include "kv_attention.cuh"
 
 #include <climits>
@@ -51,7 +58,10 @@ constexpr float kWeightLog2 = 8.0f;     // weights are scaled by 256 before they
 constexpr float kMostLog2 = 16.0f;      // a tile may exceed the reference by 2^16
 constexpr int kSms = 148;
 constexpr int kJoinThreads = 256;
-constexpr int kWholeTiles = 4;    // items of at most this many tiles are not cut (and not joined)
+// Items of at most this many tiles are not cut, and not joined: 32 sequences of 1000 tokens, 8 key
+// heads of 128: 22 us, cut 27 us; one sequence 10.3 us, cut 11.2 us.  At 16 tiles 32 sequences still
+// gain (35.2 -> 32.7 us), but one sequence loses (11.3 -> 15.3 us).
+constexpr int kWholeTiles = 8;
 constexpr int kMinUnits = 3;      // units that a CTA takes at least
 
 template <int D, int RP, int TERMS>
@@ -202,6 +212,37 @@ __device__ __forceinline__ int64_t warp_locate(const AttentionArgs& a, int64_t a
   return tiles;
 }
 
+// What the joining kernel needs to know about the border behind a CTA's share: the item in which the
+// next share begins.
+struct Border {
+  int64_t row;  // first token row of the item
+  int rows;     // query rows
+  int head;
+  int parts;    // CTAs over which the item goes, 1: nothing to join here
+  int pad[3];
+};
+// With many rows it is told, in the workspace before the partial rows: its CTAs do not fit the GPU at
+// once, and most have nothing to do.  With few it finds out while the main kernel ends.  131072 tokens,
+// 6 rows: told 52.4 us, finding out 51.7; 48 sequences of 16 rows: told 68.0, finding out 71.2.
+template <int RP>
+constexpr bool kToldBorders = RP > 8;
+__device__ __forceinline__ Border* borders_of(const AttentionArgs& a) {
+  return reinterpret_cast<Border*>(a.partials) - kSms;
+}
+__device__ __forceinline__ Border border_of(const AttentionArgs& a, const Share& s, int cta, int64_t begin,
+                                            int b, int head) {
+  Border border{0, 0, head, 1, {}};
+  if (cta + 1 >= s.ctas) return border;
+  const KvSequence seq = kv_sequence(a, b);
+  border.row = seq.row;
+  border.rows = seq.rows * a.group;
+  const int64_t u0 = begin + a.item_units, u1 = u0 + seq.tiles - 1;
+  // CTA of a unit: the last one whose share begins at or before it.
+  if (u1 >= u0 && (int)(((u0 + 1) * s.ctas - 1) / s.total) == cta)
+    border.parts = (int)(((u1 + 1) * s.ctas - 1) / s.total) - cta + 1;
+  return border;
+}
+
 // A segment: the tiles of one item that a CTA takes, and where its rows go.  Filled by the query
 // warps, one segment ahead.
 template <int RP>
@@ -238,14 +279,14 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   float* red_max = reinterpret_cast<float*>(segments + kQueries);     // [group][warp][RP]
   float* red_top = red_max + 8 * RP;                           // [group][RP]
   int* nan_table = reinterpret_cast<int*>(red_top + 2 * RP);   // [segment parity][head_dim], see clear_nan
-  Cursor* start = reinterpret_cast<Cursor*>(nan_table + 2 * D);
-  int64_t* share_smem = reinterpret_cast<int64_t*>(start + 1);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(share_smem + 2);
+  Cursor* start = reinterpret_cast<Cursor*>(nan_table + 2 * D);  // of this share, of the next
+  int64_t* share_smem = reinterpret_cast<int64_t*>(start + 2);  // begin, end, all units, begin of the item at the end
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(share_smem + 4);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* ask_flag = abort_flag + 1;                     // [group][2]
   volatile int* nan_flag = ask_flag + 4;                       // [segment parity]
   volatile uint32_t* slot_named = reinterpret_cast<volatile uint32_t*>(nan_flag + 2);  // [slot]
-  static_assert(5120 + kQueries * sizeof(Segment<RP>) + 10 * RP * 4 + 2 * D * 4 + sizeof(Cursor) + 16 + 8 + 16 + 72 <=
+  static_assert(5120 + kQueries * sizeof(Segment<RP>) + 10 * RP * 4 + 2 * D * 4 + 2 * sizeof(Cursor) + 32 + 8 + 16 + 72 <=
                     C::kFixedBytes,
                 "fixed area");
 
@@ -296,21 +337,25 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
     ptx::tmem_relinquish();
   }
   ptx::grid_dependency_wait();
-  // From here on everything before this kernel has completed, also for the joining kernel, which
-  // reads the same lengths before it waits for this one.
+  // From here on everything before this kernel has completed, also for the joining kernel, which may
+  // read the same lengths before it waits for this one.
   ptx::grid_launch_dependents();
   if (warp < 2) {
     // Warp 0 finds the first tile of this CTA, warp 1 the first of the next.
     const Share s = share_of(warp_total_units(a, lane) * a.cache.kv_heads, (int)gridDim.x);
     const int cta = (int)blockIdx.x + warp;
-    Cursor c;
+    Cursor c{};
     int64_t tile = 0;
-    int64_t begin;
+    int64_t begin = 0;
     if ((int)blockIdx.x < s.ctas)
       tile = warp_locate(a, share_begin(s, cta), a.whole_items != 0, lane, &c, &begin);
     if (lane == 0) {
       share_smem[warp] = tile;
-      if (warp == 0) *start = c;
+      start[warp] = c;
+      if (warp == 1) {
+        share_smem[2] = s.total;
+        share_smem[3] = begin;
+      }
     }
   }
   ptx::tc_fence_before();
@@ -872,6 +917,13 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
     }
   }
 
+  if constexpr (kToldBorders<RP>) {
+    // Now that nothing waits for it.
+    if (warp == kValueWarp && lane == 0 && a.whole_items == 0 && blockIdx.x + 1 < gridDim.x)
+      borders_of(a)[blockIdx.x] = border_of(a, share_of(share_smem[2], (int)gridDim.x), (int)blockIdx.x,
+                                            share_smem[3], start[1].b, start[1].head);
+  }
+
   // ---------------- teardown ----------------
   ptx::tc_fence_before();
   __syncthreads();
@@ -895,36 +947,29 @@ kv_decode_join_kernel(const AttentionArgs a, int grid) {
   using T = typename std::conditional<TERMS == 2, __nv_bfloat16, __half>::type;
   constexpr int kColumns = D / 4;                     // four values a thread
   constexpr int kShares = kJoinThreads / kColumns;    // threads that share a column's parts
-  __shared__ Cursor item;
-  __shared__ int item_parts;
   __shared__ float factor[kSms];
   __shared__ float4 acc[kJoinThreads];
   const int c0 = (int)blockIdx.x, r = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
-  // The item in which the share of CTA c0 + 1 begins, if its first tile is CTA c0's.  The lengths
-  // are final before the main kernel starts.
-  if (tid < 32) {
-    const Share s = share_of(warp_total_units(a, lane) * a.cache.kv_heads, grid);
-    int parts = 1;
-    Cursor c;
-    if (c0 + 1 < s.ctas) {
+  Border item;
+  if constexpr (kToldBorders<RP>) {
+    ptx::grid_dependency_wait();
+    item = borders_of(a)[c0];
+  } else {
+    // The lengths are final before the main kernel starts.
+    __shared__ Border found;
+    if (tid < 32) {
+      const Share s = share_of(warp_total_units(a, lane) * a.cache.kv_heads, grid);
+      Cursor c{};
       int64_t begin = 0;
-      warp_locate(a, share_begin(s, c0 + 1), false, lane, &c, &begin);
-      c.load(a);
-      const int64_t u0 = begin + a.item_units, u1 = u0 + c.seq.tiles - 1;
-      // CTA of a unit: the last one whose share begins at or before it.
-      if (c.seq.tiles > 0 && (int)(((u0 + 1) * s.ctas - 1) / s.total) == c0)
-        parts = (int)(((u1 + 1) * s.ctas - 1) / s.total) - c0 + 1;
+      if (c0 + 1 < s.ctas) warp_locate(a, share_begin(s, c0 + 1), false, lane, &c, &begin);
+      if (lane == 0) found = border_of(a, s, c0, begin, c.b, c.head);
     }
-    if (lane == 0) {
-      item = c;
-      item_parts = parts;
-    }
+    __syncthreads();
+    item = found;
+    ptx::grid_dependency_wait();
   }
-  __syncthreads();
-  const int parts = item_parts, head = item.head;
-  const KvSequence seq = item.seq;
-  ptx::grid_dependency_wait();
-  if (parts == 1 || r >= seq.rows * a.group) return;
+  const int parts = item.parts, head = item.head;
+  if (parts == 1 || r >= item.rows) return;
   // The first CTA began before this item or with it, the others inside it.
   const int64_t first = 2 * c0 + 1, later = 2 * c0;  // slot of part p: p == 0 ? first : later + 2 p
   auto part_of = [&](int p) {
@@ -974,7 +1019,7 @@ kv_decode_join_kernel(const AttentionArgs a, int grid) {
     o.w += v.w;
   }
   const float scale = l == 0.0f ? 0.0f : 1.0f / l;
-  T* out = static_cast<T*>(a.out) + (seq.row + r / a.group) * a.out_token_stride +
+  T* out = static_cast<T*>(a.out) + (item.row + r / a.group) * a.out_token_stride +
            (int64_t)(head * a.group + r % a.group) * a.out_head_stride + column * 4;
   const float v[4] = {o.x * scale, o.y * scale, o.z * scale, o.w * scale};
 #pragma unroll
@@ -1049,16 +1094,18 @@ int64_t kv_decode_workspace(int64_t batch, int kv_heads, int head_dim, int dtype
   const int grid = kv_decode_grid(batch, kv_heads, max_context);
   if (grid == 1 || max_context <= kWholeTiles * kKvTile) return 0;
   const int rp = rows <= 8 ? 8 : rows <= 16 ? 16 : kv_decode_rows(head_dim, dtype);
-  return (int64_t)grid * 2 * (rp * head_dim + 2 * rp) * 4;
+  return kSms * (int64_t)sizeof(Border) + (int64_t)grid * 2 * (rp * head_dim + 2 * rp) * 4;
 }
 
 // Sequences with at most a.max_rows <= kv_decode_rows() rows (tokens x group); others are left
 // alone.
 int launch_kv_decode(const AttentionArgs& args, int dtype, cudaStream_t stream) {
   AttentionArgs a = args;
-  // Measured: about 2.6 us beside 1.5 us a tile of 256, 2.3 us beside 0.8 us a tile of 128.
+  // Measured: about 2.6 us beside 1.5 us a tile of 256, 3.1 us beside 1.1 us a tile of 128.
   a.item_units = a.cache.head_dim == 256 ? 2 : 3;
   a.whole_items = (int64_t)a.batch.table_width * a.cache.page_size <= kWholeTiles * kKvTile;
+  static_assert(sizeof(Border) % 16 == 0, "partial rows stay aligned");
+  a.partials = reinterpret_cast<float*>(reinterpret_cast<Border*>(args.partials) + kSms);
   CUtensorMap tm_k, tm_v;
   if (int rc = make_kv_map(&tm_k, a.cache.k_values, a.cache)) return rc;
   if (int rc = make_kv_map(&tm_v, a.cache.v_values, a.cache)) return rc;

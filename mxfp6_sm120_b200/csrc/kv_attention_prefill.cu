@@ -22,6 +22,14 @@
 //  * Work: the list of (sequence, row tile, key head) with its tiles of cached tokens is cut into
 //    equal shares, one per SM; an item that is cut leaves partial rows, which a second kernel
 //    joins in the order of the tiles.
+//
+// Measured inside a CUDA graph: a prompt of 8192 tokens, 24 query and 4 key heads of 256: 730 to 800 us
+// (boxes and clocks differ), 1.03 to 1.13 PFLOP/s of 16-bit products, tensor pipes 57 % active at
+// 1.67 GHz.  The scores' product reads both operands from shared memory, 128 bytes a clock, which is
+// all it gives, beside the copies into the ring: without any exponential the time is the same, with
+// half the products 690 us.  Five chunks of 1500 tokens over 12000, 8 rows per key head of 128: 330 us,
+// 0.57 PFLOP/s; here the softmax bounds it (without exponentials and E4M3 terms 252 us).  Tried and
+// left: the next rows' terms before the last rows' output (790 against 746 us, heads of 256).
 #include "kv_attention.cuh"
 
 #include <climits>

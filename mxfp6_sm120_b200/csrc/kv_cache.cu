@@ -11,7 +11,10 @@
 //
 // One CTA owns a (block, head, K or V), so no two CTAs touch the same bytes and the result
 // does not depend on their order.  Both kernels move each byte once and compute next to
-// nothing: HBM bounds them, launch latency at decode sizes.
+// nothing: HBM bounds them, launch latency at decode sizes.  Inside a CUDA graph (copy rate
+// 6.57 TB/s): write of 8191 tokens, 4 heads of 256: 14 us, 3.6 TB/s (the first bytes come after
+// the lengths and the page, three loads one after another); of one token for 32 sequences:
+// 3.5 us; read of 12 sequences of up to 6000 tokens: 51 us, 5.4 TB/s; of 77 tokens: 2.7 us.
 #include "kv_cache.cuh"
 
 #include <cuda_fp8.h>

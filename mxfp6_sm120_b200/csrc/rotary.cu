@@ -7,7 +7,8 @@
 // to half a turn there; sine and cosine of what is left are 32-bit, the rotation is a 32-bit
 // multiply-add, rounded once.  All heads of a token share the angles: a CTA computes them once
 // into shared memory and then streams its heads, sixteen bytes a thread and half.
-// Every byte is read and written once: HBM bounds it, launch latency at decode sizes.
+// Every byte is read and written once: HBM bounds it, launch latency at decode sizes.  Inside a
+// CUDA graph: 8192 tokens, 32 + 8 heads of 128: 32 us, 5.3 TB/s of a copy's 6.57; 17 tokens: 2.7 us.
 #include "common.cuh"
 
 #include <type_traits>
