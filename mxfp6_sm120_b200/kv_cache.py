@@ -101,10 +101,13 @@ class PagedKVCache:
             raise ValueError("cache tensors must be on one device")
         if not (k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
             raise ValueError("cache tensors must be contiguous")
-        # What every call passes on.
         object.__setattr__(self, "device", device)
-        object.__setattr__(self, "_arguments", (k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(),
-                                                pages, heads, page, dim))
+        object.__setattr__(self, "_extents", (pages, heads, page, dim))
+
+    def _arguments(self) -> tuple:
+        """What every call passes on."""
+        return (self.k_values.data_ptr(), self.v_values.data_ptr(), self.k_scales.data_ptr(),
+                self.v_scales.data_ptr(), *self._extents)
 
     @classmethod
     def allocate(cls, pages: int, kv_heads: int, page_size: int, head_dim: int,
@@ -119,19 +122,19 @@ class PagedKVCache:
 
     @property
     def pages(self) -> int:
-        return self._arguments[4]
+        return self._extents[0]
 
     @property
     def kv_heads(self) -> int:
-        return self._arguments[5]
+        return self._extents[1]
 
     @property
     def page_size(self) -> int:
-        return self._arguments[6]
+        return self._extents[2]
 
     @property
     def head_dim(self) -> int:
-        return self._arguments[7]
+        return self._extents[3]
 
     def nbytes(self) -> int:
         """Bytes of the values and scales."""
@@ -224,13 +227,13 @@ def kv_cache_write(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor,
     if k.ndim != 3:
         raise ValueError(f"k must be [tokens, kv_heads, head_dim]; got {tuple(k.shape)}")
     batch = _check_batch(cache, block_table, seq_lens, cu_seqlens, k.shape[0])
-    device, arguments = cache.device, cache._arguments
-    heads, dim = arguments[5], arguments[7]
+    device = cache.device
+    _, heads, _, dim = cache._extents
     k_strides = _check_rows(k, "k", heads, dim, device)
     v_strides = _check_rows(v, "v", heads, dim, device)
     if v.shape != k.shape or v.dtype is not k.dtype:
         raise ValueError("k and v must have one shape and dtype")
-    _launch(device, library().mxfp6_kv_cache_write, *arguments, *batch, k.data_ptr(), v.data_ptr(),
+    _launch(device, library().mxfp6_kv_cache_write, *cache._arguments(), *batch, k.data_ptr(), v.data_ptr(),
             _DTYPE_CODE[k.dtype], k_strides[0], k_strides[1], v_strides[0], v_strides[1])
 
 
@@ -248,8 +251,8 @@ def kv_cache_read(cache: PagedKVCache, block_table: torch.Tensor, seq_lens: torc
     """
     if not isinstance(cache, PagedKVCache):
         raise TypeError("cache must be a PagedKVCache instance")
-    device, arguments = cache.device, cache._arguments
-    heads, dim = arguments[5], arguments[7]
+    device = cache.device
+    _, heads, _, dim = cache._extents
     if out is None:
         if dtype not in _DTYPE_CODE:
             raise TypeError(f"dtype must be torch.float16 or torch.bfloat16; got {dtype}")
@@ -273,7 +276,7 @@ def kv_cache_read(cache: PagedKVCache, block_table: torch.Tensor, seq_lens: torc
         raise ValueError("out's tensors must be contiguous")
     if v.shape != k.shape or v.dtype is not k.dtype:
         raise ValueError("the outputs must have one shape and dtype")
-    _launch(device, library().mxfp6_kv_cache_read, *arguments, *batch, k.data_ptr(), v.data_ptr(),
+    _launch(device, library().mxfp6_kv_cache_read, *cache._arguments(), *batch, k.data_ptr(), v.data_ptr(),
             _DTYPE_CODE[k.dtype])
     return k, v
 
@@ -291,15 +294,15 @@ def kv_cache_attention(q: torch.Tensor, cache: PagedKVCache, block_table: torch.
     upper bound of the rows of any sequence (default: 1 without ``cu_seqlens``, else all rows); a
     tight one picks the better kernel, and rows of a sequence that has more may be left unwritten.
     Write the rows' own keys and values first (:func:`kv_cache_write` takes the same
-    ``block_table``, ``seq_lens`` and ``cu_seqlens``).
+    ``block_table``, ``seq_lens`` and ``cu_seqlens``).  ``out`` must not overlap ``q``.
     """
     if q.ndim != 3:
         raise ValueError(f"q must be [tokens, q_heads, head_dim]; got {tuple(q.shape)}")
     tokens, q_heads, dim = q.shape
     batch = _check_batch(cache, block_table, seq_lens, cu_seqlens, tokens)
-    device, arguments = cache.device, cache._arguments
-    heads = arguments[5]
-    q_strides = _check_rows(q, "q", None, arguments[7], device)
+    device = cache.device
+    _, heads, page_size, head_dim = cache._extents
+    q_strides = _check_rows(q, "q", None, head_dim, device)
     if q_heads < 1 or q_heads % heads != 0:
         raise ValueError(f"q_heads ({q_heads}) must be a multiple of the cache's {heads} heads")
     if max_query_len is None:
@@ -318,10 +321,10 @@ def kv_cache_attention(q: torch.Tensor, cache: PagedKVCache, block_table: torch.
     lib = library()
     code = _DTYPE_CODE[q.dtype]
     need = lib.mxfp6_kv_cache_attention_workspace(batch[6], tokens, max_query_len, q_heads, heads, dim,
-                                                  code, batch[5] * arguments[6])
+                                                  code, batch[5] * page_size)
     # Scratch of this call alone: the allocator keeps it apart between streams and graphs.
     workspace = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
-    _launch(device, lib.mxfp6_kv_cache_attention, *arguments, *batch, q.data_ptr(), out.data_ptr(), code,
+    _launch(device, lib.mxfp6_kv_cache_attention, *cache._arguments(), *batch, q.data_ptr(), out.data_ptr(), code,
             q_heads, q_strides[0], q_strides[1], out_strides[0], out_strides[1], max_query_len, scale,
             1 if causal else 0, None if workspace is None else workspace.data_ptr(), need)
     return out

@@ -679,3 +679,44 @@ def test_offsets_that_make_no_sense_stay_in_bounds(mx):
     _check_attention(batch, q, whole, 64 ** -0.5, True)
     part = torch.cat([whole[:30], out[30:]])
     _check_attention(batch, q, part, 64 ** -0.5, True)
+
+
+def test_calls_without_rows(mx):
+    """No tokens in a call: nothing is read, written or launched."""
+    batch = Batch(mx, 70, [40, 3], [0, 0], 2, 32, 64)
+    before = [t.clone() for t in (batch.cache.k_values, batch.cache.k_scales)]
+    empty = torch.empty((0, 2, 64), dtype=torch.bfloat16, device=DEV)
+    mx.kv_cache_write(batch.cache, empty, empty, *batch.dev)
+    k, v = mx.kv_cache_read(batch.cache, *batch.dev, tokens=0)
+    out = mx.kv_cache_attention(torch.empty((0, 6, 64), dtype=torch.bfloat16, device=DEV), batch.cache, *batch.dev)
+    torch.cuda.synchronize()
+    assert k.shape == v.shape == (0, 2, 64) and out.shape == (0, 6, 64)
+    assert torch.equal(before[0], batch.cache.k_values) and torch.equal(before[1], batch.cache.k_scales)
+
+
+@pytest.mark.parametrize("rows", [1, 60])
+def test_a_cache_whose_memory_is_replaced(mx, rows):
+    """A call uses the memory that the cache's tensors have when it is made."""
+    batch = Batch(mx, 71, [150], [rows], 2, 32, 64)
+    q = torch.randn((rows, 4, 64), generator=_gen(72)).to(torch.bfloat16).to(DEV)
+    for t in (batch.cache.k_values, batch.cache.v_values, batch.cache.k_scales, batch.cache.v_scales):
+        old = t.data
+        t.data = old.clone()
+        old.fill_(255)
+    got = _attend(mx, batch, q, max_query_len=rows)
+    _check_attention(batch, q, got, 64 ** -0.5, True)
+
+
+def test_a_table_shared_by_all_sequences(mx):
+    """Sequences that read the same pages (a row of the table expanded, stride zero), and a table
+    whose rows are a slice of wider ones."""
+    batch = Batch(mx, 73, [180], [1], 2, 32, 128)
+    q = torch.randn((5, 4, 128), generator=_gen(74)).to(torch.bfloat16).to(DEV)
+    lens = _i32([180, 100, 7, 33, 128])
+    wide = torch.full((5, batch.width + 9), 2 ** 31 - 1, dtype=torch.int32, device=DEV)
+    wide[:, 4 : 4 + batch.width] = batch.dev[0]
+    for table in (batch.dev[0].expand(5, -1), wide[:, 4 : 4 + batch.width]):
+        got = mx.kv_cache_attention(q, batch.cache, table, lens)
+        for b, n in enumerate((180, 100, 7, 33, 128)):
+            batch.lens = [n]
+            _check_attention(batch, q[b : b + 1], got[b : b + 1], 128 ** -0.5, True)
