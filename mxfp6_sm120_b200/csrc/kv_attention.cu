@@ -8,7 +8,7 @@
 // head): up to kv_decode_rows() go to the decode kernel, whose tiles have the cached tokens as
 // their long side, the others to the prefill kernel, which has 128 rows to a tile.  The border is
 // what the decode kernel's tensor memory holds: it is still the faster one there (65536 tokens, 8
-// key heads of 128: 58 us with 32 rows, the other 74 us with 36; 4 key heads of 256: 50 us with 24,
+// key heads of 128: 49 us with 32 rows, the other 76 us with 36; 4 key heads of 256: 50 us with 24,
 // 65 us with 32).
 #include "kv_attention.cuh"
 

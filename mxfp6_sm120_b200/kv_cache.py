@@ -53,7 +53,7 @@ def _launch(device: torch.device, function, *args) -> None:
             raise ValueError(f"the tensors must be on a CUDA device; got {device}")
         _require_sm100(device)
         _SM100_SEEN.add(index)
-    if torch.cuda.current_device() == index:
+    if torch._C._cuda_getDevice() == index:
         status = function(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):

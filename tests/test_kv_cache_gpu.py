@@ -720,3 +720,17 @@ def test_a_table_shared_by_all_sequences(mx):
         for b, n in enumerate((180, 100, 7, 33, 128)):
             batch.lens = [n]
             _check_attention(batch, q[b : b + 1], got[b : b + 1], 128 ** -0.5, True)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("rows", [7, 8, 9, 16, 17, 24, 25, 32, 33])
+def test_row_counts_around_the_variants(mx, rows, dim, dtype):
+    """New tokens x query heads per key head on both sides of every border between kernels, over
+    sequences short and long enough to be cut."""
+    group = next(g for g in (4, 3, 5, 1) if rows % g == 0) if rows != 7 else 7
+    new = rows // group
+    batch = Batch(mx, 75, [1200, new, 131], [new] * 3, 1, 128, dim)
+    q = torch.randn((batch.tokens, group, dim), generator=_gen(76)).to(dtype).to(DEV)
+    got = _attend(mx, batch, q, max_query_len=new)
+    _check_attention(batch, q, got, dim ** -0.5, True)
