@@ -98,6 +98,8 @@ __device__ __forceinline__ void store8(T* at, const uint4& v) {
   }
 }
 
+__host__ __device__ __forceinline__ int kept_items(int dim, int half) { return (dim - 2 * half + 15) / 16; }
+
 template <class T, bool kVector>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryArgs a) {
   __shared__ __align__(16) float cosines[kMostTokens * kMaxHalf];
@@ -118,10 +120,9 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryArgs a) {
     cosines[n] = c;
   }
   __syncthreads();
-  // Work items: eight pairs of a head, then eight untouched values behind rotary_dim.
+  // Work items: eight pairs of a head, then up to sixteen untouched values behind rotary_dim.
   const int turned = a.half / 8;
-  const int kept = (a.dim - 2 * a.half) / 8;
-  const int per_head = turned + kept;
+  const int per_head = turned + kept_items(a.dim, a.half);
   const int total = (a.heads[0] + a.heads[1]) * per_head;
 #pragma unroll 2
   for (int n = blockIdx.y * kThreads + threadIdx.x; n < total * tokens; n += gridDim.y * kThreads) {
@@ -137,8 +138,11 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryArgs a) {
     T* y = static_cast<T*>(a.out[which]) + token * a.out_token[which] + head * a.out_head[which];
     if (item >= turned) {
       if (x != y) {
-        const int at = 2 * a.half + (item - turned) * 8;
-        store8<T, kVector>(y + at, load8<T, kVector>(x + at));
+        const int at = 2 * a.half + (item - turned) * 16;
+        const bool two = at + 8 < a.dim;
+        const uint4 u = load8<T, kVector>(x + at), v = load8<T, kVector>(x + (two ? at + 8 : at));
+        store8<T, kVector>(y + at, u);
+        if (two) store8<T, kVector>(y + at + 8, v);
       }
       continue;
     }
@@ -223,14 +227,21 @@ int rotary_multi_axis(const void* q, void* q_out, int q_heads, const int64_t q_s
   a.dim = dim;
   a.wide_positions = wide_positions;
   a.adjacent = adjacent;
-  // A token's heads are dealt to several CTAs while the tokens alone leave SMs idle; four tokens
-  // share a CTA where there are enough, so that its angles and its last items fill the threads
-  // (8192 tokens x 40 heads of 128: 34.9 us with one).
-  const int items = (q_heads + k_heads) * (half / 8 + (dim - 2 * half) / 8);
-  int parts = (int)ceil_div64(items, kThreads);
-  if (tokens * parts > 2 * 148) parts = tokens >= 2 * 148 ? 1 : (int)ceil_div64(2 * 148, tokens);
+  // Four tokens share a CTA where there are enough, so that its angles and its last items fill the
+  // threads (8192 tokens x 40 heads of 128: 34.9 us with one).  A CTA's items are dealt to several
+  // while CTAs alone leave SMs idle, and, in shares of two passes or more, while there are fewer than
+  // eight an SM (1924 tokens x 28 heads of 256, 64 turned: 15 us, with a CTA for four tokens 26).
+  const int items = (q_heads + k_heads) * (half / 8 + kept_items(dim, half));
   a.cta_tokens = tokens >= 8 * 148 ? kMostTokens : 1;
-  const dim3 grid((unsigned)ceil_div64(tokens, a.cta_tokens), (unsigned)parts);
+  const int64_t groups = ceil_div64(tokens, a.cta_tokens);
+  const int64_t cta_items = (int64_t)items * a.cta_tokens;
+  int64_t parts = ceil_div64(cta_items, kThreads);
+  if (groups * parts > 2 * 148) {
+    const int64_t most = cta_items / (2 * kThreads), want = ceil_div64(8 * 148, groups);
+    parts = most < want ? most : want;
+    if (parts < 1) parts = 1;
+  }
+  const dim3 grid((unsigned)groups, (unsigned)parts);
   if (dtype == kBF16) {
     if (vector) rotary_kernel<__nv_bfloat16, true><<<grid, kThreads, 0, stream>>>(a);
     else rotary_kernel<__nv_bfloat16, false><<<grid, kThreads, 0, stream>>>(a);

@@ -734,3 +734,15 @@ def test_row_counts_around_the_variants(mx, rows, dim, dtype):
     q = torch.randn((batch.tokens, group, dim), generator=_gen(76)).to(dtype).to(DEV)
     got = _attend(mx, batch, q, max_query_len=new)
     _check_attention(batch, q, got, dim ** -0.5, True)
+
+
+@pytest.mark.parametrize("tokens,q_heads,k_heads,dim,rotary_dim", [
+    (3, 5, 1, 72, 16),          # seven groups of eight behind the turned values: an odd one is left
+    (1303, 2, 1, 24, 16),       # one group of eight, four tokens a CTA, three in the last
+    (1303, 24, 4, 256, 64),     # several CTAs for four tokens
+    (700, 9, 2, 160, 96),
+])
+def test_rotary_of_partial_heads(mx, tokens, q_heads, k_heads, dim, rotary_dim):
+    half = rotary_dim // 2
+    test_rotary_matches_definition(mx, torch.bfloat16, tokens, q_heads, k_heads, dim, rotary_dim,
+                                   [half - half // 3, half // 3], False, tokens % 2 == 0)
