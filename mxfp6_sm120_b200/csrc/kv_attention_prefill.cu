@@ -295,12 +295,13 @@ kv_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   float* row_top = row_sum + 4 * kRows;                            // [block][row]
   int* nan_from = reinterpret_cast<int*>(row_top + 4 * kRows);     // [head_dim], see clear_nan
   Cursor* start = reinterpret_cast<Cursor*>(nan_from + 256);
-  int64_t* share_smem = reinterpret_cast<int64_t*>(start + 1);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(share_smem + 2);
+  int64_t* share_smem = reinterpret_cast<int64_t*>(start + 1);  // begin, end, all units, begin of the item at the end
+  Place* next = reinterpret_cast<Place*>(share_smem + 4);  // where the next share begins
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(next + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* ask_flag = abort_flag + 1;               // [quarter][2]
   volatile int* nan_seen = ask_flag + 8;
-  static_assert(512 + 9 * 512 + 2 * sizeof(Segment) + 8 * kRows * 4 + 1024 + sizeof(Cursor) + 16 + 8 + 36 <=
+  static_assert(512 + 9 * 512 + 2 * sizeof(Segment) + 8 * kRows * 4 + 1024 + sizeof(Cursor) + 32 + sizeof(Place) + 8 + 36 <=
                     C::kFixedBytes,
                 "fixed area");
 
@@ -358,21 +359,13 @@ kv_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
     if ((int)blockIdx.x < s.ctas && s.total > 0) tile = warp_locate(a, share_begin(s, cta), lane, &p, &begin);
     if (lane == 0) {
       share_smem[warp] = tile;
-      if (warp == 0) start->at = p;
-    }
-    if (warp == 1 && (int)gridDim.x > 1 && (int)blockIdx.x + 1 < (int)gridDim.x) {
-      // For the joining kernel: the item in which the next share begins, and over how many CTAs
-      // it goes if its first tile is this CTA's.
-      Border* border = borders_of(a) + blockIdx.x;
-      int parts = 1;
-      if (cta < s.ctas && s.total > 0) {
-        const Sequence q = load_sequence(a, p.b);
-        const int64_t u0 = begin + kItemUnits, u1 = u0 + tiles_of(a, q, p.t) - 1;
-        // CTA of a unit: the last one whose share begins at or before it.
-        if ((int)(((u0 + 1) * s.ctas - 1) / s.total) == (int)blockIdx.x)
-          parts = (int)(((u1 + 1) * s.ctas - 1) / s.total) - (int)blockIdx.x + 1;
+      if (warp == 0) {
+        start->at = p;
+      } else {
+        share_smem[2] = s.total;
+        share_smem[3] = begin;
+        *next = p;
       }
-      if (lane == 0) *border = Border{p.b, p.t, p.head, parts};
     }
   }
   ptx::tc_fence_before();
@@ -994,6 +987,22 @@ kv_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       if (i0 < count) turn_rows(segment + 1);
       if (failed) break;
     }
+  }
+
+  if (warp == kTmaWarp && lane == 0 && blockIdx.x + 1 < gridDim.x) {
+    // For the joining kernel, now that nothing waits for it: the item in which the next share begins,
+    // and over how many CTAs it goes if its first tile is this CTA's.
+    const Share s = share_of(share_smem[2], (int)gridDim.x);
+    const int cta = (int)blockIdx.x;
+    int parts = 1;
+    if (cta + 1 < s.ctas && s.total > 0) {
+      const Sequence q = load_sequence(a, next->b);
+      const int64_t u0 = share_smem[3] + kItemUnits, u1 = u0 + tiles_of(a, q, next->t) - 1;
+      // CTA of a unit: the last one whose share begins at or before it.
+      if ((int)(((u0 + 1) * s.ctas - 1) / s.total) == cta)
+        parts = (int)(((u1 + 1) * s.ctas - 1) / s.total) - cta + 1;
+    }
+    borders_of(a)[cta] = Border{next->b, next->t, next->head, parts};
   }
 
   // ---------------- teardown ----------------
