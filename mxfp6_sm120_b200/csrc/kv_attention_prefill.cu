@@ -23,12 +23,12 @@
 //    equal shares, one per SM; an item that is cut leaves partial rows, which a second kernel
 //    joins in the order of the tiles.
 //
-// Measured inside a CUDA graph: a prompt of 8192 tokens, 24 query and 4 key heads of 256: 730 to 800 us
-// (boxes and clocks differ), 1.03 to 1.13 PFLOP/s of 16-bit products, tensor pipes 57 % active at
+// Measured inside a CUDA graph: a prompt of 8192 tokens, 24 query and 4 key heads of 256: 710 to 770 us
+// (boxes and clocks differ), 1.07 to 1.16 PFLOP/s of 16-bit products, tensor pipes 57 % active at
 // 1.67 GHz.  The scores' product reads both operands from shared memory, 128 bytes a clock, which is
 // all it gives, beside the copies into the ring: without any exponential the time is the same, with
-// half the products 690 us.  Five chunks of 1500 tokens over 12000, 8 rows per key head of 128: 330 us,
-// 0.57 PFLOP/s; here the softmax bounds it (without exponentials and E4M3 terms 252 us).  Tried and
+// half the products 690 us.  Five chunks of 1500 tokens over 12000, 8 rows per key head of 128: 320 us,
+// 0.59 PFLOP/s; here the softmax bounds it (without exponentials and E4M3 terms 252 us).  Tried and
 // left: the next rows' terms before the last rows' output (790 against 746 us, heads of 256).
 #include "kv_attention.cuh"
 
@@ -45,7 +45,9 @@ constexpr int kRows = 128;            // rows of an item
 constexpr float kWeightLog2 = 8.0f;   // weights are scaled by 256 before they become E4M3 terms
 constexpr float kMostLog2 = 16.0f;    // a block may exceed the reference by 2^16
 constexpr int kSms = 148;
-constexpr int kItemUnits = 5;         // what an item costs beside its tiles: about 8 us, a tile 1.7 us
+// What an item costs beside its tiles: about 8 us, a tile 1.7 us.  8192-token prompt, heads of 256: with
+// 3 units 940 us, 4 810, 5 740, 6 750; five chunks, heads of 128: 329, 322, 327, 329 us.
+constexpr int kItemUnits = 5;
 constexpr int kMinUnits = 4;          // units a CTA takes at least
 
 template <int D, int TERMS>
