@@ -499,8 +499,9 @@ int64_t mxfp6_kv_cache_attention_workspace(int64_t batch, int64_t tokens, int64_
                                            int q_heads, int kv_heads, int head_dim, int dtype,
                                            int64_t max_context);
 /* softmax(scale * q k^T) v per query head over the cached tokens of its sequence (up to the
- * row's own position when causal != 0); strides in elements.  The workspace needs no
- * initialisation; concurrent calls need one each. */
+ * row's own position when causal != 0); strides in elements.  max_query_len: an upper bound of the
+ * rows of any sequence; rows of a sequence that has more may be left unwritten.  `out` must not
+ * overlap q.  The workspace needs no initialisation; concurrent calls need one each. */
 int mxfp6_kv_cache_attention(const uint8_t* k_values, const uint8_t* v_values,
                              const uint8_t* k_scales, const uint8_t* v_scales, int64_t pages,
                              int kv_heads, int page_size, int head_dim,

@@ -12,6 +12,8 @@
 // 65 us with 32).
 #include "kv_attention.cuh"
 
+#include <cmath>
+
 namespace mx {
 
 int launch_kv_decode(const AttentionArgs& a, int dtype, cudaStream_t stream);
@@ -121,6 +123,8 @@ int kv_cache_attention(const KvCache& cache, const KvBatch& batch, const void* q
   MX_REQUIRE(q_heads > 0 && q_heads <= 65535 && q_heads % cache.kv_heads == 0,
              "q_heads (%d) must be a multiple of the cache's %d heads", q_heads, cache.kv_heads);
   MX_REQUIRE(max_query_len >= 1, "max_query_len must be positive");
+  const float scale_log2 = scale * 1.4426950408889634f;
+  MX_REQUIRE(std::isfinite(scale_log2), "scale must be finite, and still be so times log2(e)");
   if (batch.tokens == 0) return kOk;
   MX_REQUIRE(q != nullptr && out != nullptr, "q and out must not be null");
   const int group = q_heads / cache.kv_heads;
@@ -146,7 +150,7 @@ int kv_cache_attention(const KvCache& cache, const KvBatch& batch, const void* q
   a.out_head_stride = strides[3];
   a.q_heads = q_heads;
   a.group = group;
-  a.scale_log2 = scale * 1.4426950408889634f;
+  a.scale_log2 = scale_log2;
   a.causal = causal;
   a.vector = aligned16(q) && strides[0] % 8 == 0 && strides[1] % 8 == 0;
   a.vector_out = aligned16(out) && strides[2] % 8 == 0 && strides[3] % 8 == 0;

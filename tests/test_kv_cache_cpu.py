@@ -187,3 +187,33 @@ def test_c_entries_refuse_before_any_launch():
         assert write(**kwargs) == 1, message
         assert message in lib.mxfp6_b200_last_error(), message
     assert lib.mxfp6_kv_cache_attention_workspace(2, 2, 1, 3, 2, 64, 1, 64) in (-1, 0)
+
+
+def test_c_attention_refuses_before_any_launch():
+    from mxfp6_sm120_b200._loader import library
+
+    lib = library()
+    p = 4096
+
+    def attend(batch=(p, p, None, 2, 2, 64, 2), q=p, dtype=1, heads=4, most=1, scale=0.125, workspace=(p, 1 << 40)):
+        return lib.mxfp6_kv_cache_attention(p, p, p, p, 4, 2, 32, 64, *batch, q, p, dtype, heads, 256, 64, 256, 64,
+                                            most, scale, 1, *workspace, None)
+
+    for message, kwargs in (
+        (b"float16 or bfloat16", dict(dtype=2)),
+        (b"multiple of the cache", dict(heads=3)),
+        (b"multiple of the cache", dict(heads=0)),
+        (b"max_query_len", dict(most=0)),
+        (b"scale must be finite", dict(scale=math.inf)),
+        (b"scale must be finite", dict(scale=math.nan)),
+        (b"scale must be finite", dict(scale=3.0e38)),
+        (b"must not be null", dict(q=None)),
+        (b"2^30 rows", dict(batch=(p, p, p, 2, 1 << 30, 64, 2))),
+        (b"workspace must be", dict(workspace=(p, 16))),
+        (b"workspace must be", dict(workspace=(p + 4, 1 << 40))),
+        (b"workspace must be", dict(workspace=(None, 1 << 40))),
+    ):
+        assert attend(**kwargs) == 1, message
+        assert message in lib.mxfp6_b200_last_error(), (message, lib.mxfp6_b200_last_error())
+    # no rows: nothing to do
+    assert attend(batch=(p, p, p, 2, 0, 64, 2)) == 0
