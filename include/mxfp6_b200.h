@@ -478,7 +478,8 @@ int mxfp6_workspace_reset(void);
  * including the rows of this call, cu_seqlens [batch + 1] int32 or NULL (one row a sequence):
  * rows [cu_seqlens[b], cu_seqlens[b + 1]) of the token tensors are the last positions of
  * sequence b.  `tokens` = rows of the token tensors; rows behind cu_seqlens[batch] stay as they
- * were.  The three arrays are device memory; no content of theirs leads out of bounds. */
+ * were.  The three arrays are device memory; no content of theirs leads out of bounds, as long as it
+ * does not change while a call that reads it runs. */
 int mxfp6_kv_cache_write(uint8_t* k_values, uint8_t* v_values, uint8_t* k_scales,
                          uint8_t* v_scales, int64_t pages, int kv_heads, int page_size,
                          int head_dim, const int32_t* block_table, const int32_t* seq_lens,

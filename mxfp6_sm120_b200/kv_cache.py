@@ -13,8 +13,9 @@ Every operator takes the same description of a batch:
 ``cu_seqlens``   ``[batch + 1]`` int32, rows ``cu_seqlens[b] : cu_seqlens[b + 1]`` of the token
                  tensors are the last positions of sequence ``b``; None: one row per sequence
 
-All three live on the device and are read there, so a captured CUDA graph follows them; rows
-behind ``cu_seqlens[batch]`` are left as they were.
+All three live on the device and are read there while the call runs (they must not change
+meanwhile), so a captured CUDA graph follows them; rows behind ``cu_seqlens[batch]`` are left as
+they were.
 """
 
 from __future__ import annotations
