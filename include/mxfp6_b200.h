@@ -516,7 +516,8 @@ int mxfp6_kv_cache_attention(const uint8_t* k_values, const uint8_t* v_values,
 /* Turns pair i of every head of q [tokens, q_heads, dim] and k [tokens, k_heads, dim] by
  * positions[axis[i], token] * inv_freq[i] radians, i < half; out may be the input.  Pairs are
  * (i, i + half), or (2 i, 2 i + 1) when adjacent != 0.  positions: int32, or int64 when
- * wide_positions != 0.  Either tensor may have zero heads. */
+ * wide_positions != 0.  Either tensor may have zero heads.  axis[i] (device memory) must be in
+ * [0, axes); a pair whose axis is not becomes NaN. */
 int mxfp6_rotary_multi_axis(const void* q, void* q_out, int q_heads, int64_t q_token_stride,
                             int64_t q_head_stride, int64_t q_out_token_stride,
                             int64_t q_out_head_stride, const void* k, void* k_out, int k_heads,

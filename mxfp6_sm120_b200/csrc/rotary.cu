@@ -108,14 +108,15 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryArgs a) {
   const int tokens = (int)(a.tokens - token0 < a.cta_tokens ? a.tokens - token0 : a.cta_tokens);
   for (int n = threadIdx.x; n < tokens * a.half; n += kThreads) {
     const int i = n % a.half;
-    int axis = a.axis[i];
-    axis = axis < 0 || axis >= a.axes ? 0 : axis;
-    const int64_t at = axis * a.position_stride + token0 + n / a.half;
-    const int64_t position = a.wide_positions ? static_cast<const int64_t*>(a.positions)[at]
-                                              : static_cast<const int32_t*>(a.positions)[at];
-    const double turns = (double)position * (a.inv_freq[i] * 0.15915494309189533577);
-    float s, c;
-    sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
+    const int axis = a.axis[i];
+    float s = NAN, c = NAN;  // no row of positions for the axis: no angle to turn by
+    if (axis >= 0 && axis < a.axes) {
+      const int64_t at = axis * a.position_stride + token0 + n / a.half;
+      const int64_t position = a.wide_positions ? static_cast<const int64_t*>(a.positions)[at]
+                                                : static_cast<const int32_t*>(a.positions)[at];
+      const double turns = (double)position * (a.inv_freq[i] * 0.15915494309189533577);
+      sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
+    }
     sines[n] = s;
     cosines[n] = c;
   }

@@ -338,11 +338,15 @@ def kv_cache_attention(q: torch.Tensor, cache: PagedKVCache, block_table: torch.
 class RotaryFrequencies:
     """``inv_freq``: float64 ``[rotary_dim / 2]``, radians per position of every pair;
     ``axis``: int32 ``[rotary_dim / 2]``, the row of ``positions`` that turns it;
-    ``adjacent``: pairs are ``(2i, 2i + 1)`` instead of ``(i, i + rotary_dim / 2)``."""
+    ``adjacent``: pairs are ``(2i, 2i + 1)`` instead of ``(i, i + rotary_dim / 2)``;
+    ``axes``: rows that ``positions`` must have, the largest ``axis`` and one, so that a call with
+    fewer is refused without reading the device (:func:`rotary_frequencies` knows it; None: a pair
+    whose axis has no row becomes NaN)."""
 
     inv_freq: torch.Tensor
     axis: torch.Tensor
     adjacent: bool = False
+    axes: int | None = None
 
     def __post_init__(self) -> None:
         inv, axis = self.inv_freq, self.axis
@@ -360,6 +364,8 @@ class RotaryFrequencies:
             raise ValueError("axis must be on inv_freq's device")
         if not (inv.is_contiguous() and axis.is_contiguous()):
             raise ValueError("inv_freq and axis must be contiguous")
+        if self.axes is not None and not 1 <= self.axes <= 8:
+            raise ValueError(f"axes must be 1 to 8; got {self.axes}")
 
     @property
     def rotary_dim(self) -> int:
@@ -392,7 +398,8 @@ def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, sections: list[i
         axis = [a for a, count in enumerate(sections) for _ in range(count)]
     inv = [theta ** (-i / half) for i in range(half)]
     return RotaryFrequencies(torch.tensor(inv, dtype=torch.float64, device=device),
-                             torch.tensor(axis, dtype=torch.int32, device=device), adjacent)
+                             torch.tensor(axis, dtype=torch.int32, device=device), adjacent,
+                             max(axis) + 1)
 
 
 def rotary_multi_axis(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
@@ -402,7 +409,7 @@ def rotary_multi_axis(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
 
     ``positions``: int32 or int64 ``[axes, tokens]`` (or ``[tokens]`` for one axis); pair ``i`` of
     every head turns by ``positions[axis[i], token] * inv_freq[i]`` radians, computed in 64 bits.
-    Values behind ``rotary_dim`` are copied.  ``q_out`` / ``k_out`` may be ``q`` / ``k``
+    ``positions`` may have more rows than ``frequencies.axes``, not fewer.  Values behind ``rotary_dim`` are copied.  ``q_out`` / ``k_out`` may be ``q`` / ``k``
     themselves (in place); other overlaps are not allowed.
     """
     if not isinstance(frequencies, RotaryFrequencies):
@@ -430,6 +437,9 @@ def rotary_multi_axis(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
     if len(shape) != 2 or not 1 <= shape[0] <= 8 or shape[1] != tokens or (
             tokens > 1 and positions.stride(1) != 1):
         raise ValueError(f"positions must be [axes, {tokens}] with contiguous rows, 1 to 8 axes")
+    if frequencies.axes is not None and shape[0] < frequencies.axes:
+        raise ValueError(f"positions must have a row for each of the frequencies' {frequencies.axes} axes; "
+                         f"got {shape[0]}")
     if positions.device != device:
         raise ValueError("positions must be on q's device")
     if q_out is None:

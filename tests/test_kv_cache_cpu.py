@@ -217,3 +217,27 @@ def test_c_attention_refuses_before_any_launch():
         assert message in lib.mxfp6_b200_last_error(), (message, lib.mxfp6_b200_last_error())
     # no rows: nothing to do
     assert attend(batch=(p, p, p, 2, 0, 64, 2)) == 0
+
+
+def test_rotary_refuses_positions_with_too_few_axes():
+    """Frequencies of three sections need three rows of positions, whichever way they are laid out;
+    rows that no pair follows are not asked for."""
+    q = torch.zeros((3, 4, 64), dtype=torch.float16)
+    pos = torch.zeros((3, 3), dtype=torch.int64)
+    for sections, interleaved, axes in (([8, 4, 4], False, 3), ([8, 4, 4], True, 3), ([8, 8], False, 2),
+                                        ([8, 8, 0], False, 2), ([0, 16], False, 2), (None, False, 1)):
+        f = mx.rotary_frequencies(32, 1.0e4, sections, interleaved=interleaved, device="cpu")
+        assert f.axes == axes
+        for rows in range(1, 4):
+            match = "a row for each" if rows < axes else "CUDA device"
+            with pytest.raises(ValueError, match=match):
+                mx.rotary_multi_axis(q, q.clone(), pos[:rows], f)
+        with pytest.raises(ValueError, match="a row for each" if axes > 1 else "CUDA device"):
+            mx.rotary_multi_axis(q, q.clone(), pos[0], f)
+    f = mx.rotary_frequencies(32, 1.0e4, [8, 8], device="cpu")
+    for bad in (0, 9):
+        with pytest.raises(ValueError, match="axes must be 1 to 8"):
+            mx.RotaryFrequencies(f.inv_freq, f.axis, axes=bad)
+    with pytest.raises(ValueError, match="a row for each"):
+        mx.rotary_multi_axis(q, q.clone(), pos[:2], mx.RotaryFrequencies(f.inv_freq, f.axis, False, 3))
+    assert mx.RotaryFrequencies(f.inv_freq, f.axis).axes is None      # nothing is read from the device

@@ -746,3 +746,22 @@ def test_rotary_of_partial_heads(mx, tokens, q_heads, k_heads, dim, rotary_dim):
     half = rotary_dim // 2
     test_rotary_matches_definition(mx, torch.bfloat16, tokens, q_heads, k_heads, dim, rotary_dim,
                                    [half - half // 3, half // 3], False, tokens % 2 == 0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("adjacent", [False, True])
+def test_pairs_without_a_row_of_positions_are_nan(mx, adjacent, dtype):
+    """Frequencies whose axes the host does not know: pairs whose axis has no row become NaN, the
+    others turn as ever and the values behind rotary_dim stay."""
+    f = mx.rotary_frequencies(32, 1.0e4, [8, 8], adjacent=adjacent, device=DEV)
+    axis = f.axis.clone()
+    axis[[3, 4, 12]] = _i32([2, -1, 2 ** 31 - 1])
+    q = torch.randn((5, 3, 48), generator=_gen(1)).to(dtype).to(DEV)
+    pos = torch.randint(0, 1000, (2, 5), generator=_gen(2)).to(DEV)
+    want = [t.clone() for t in mx.rotary_multi_axis(q, q[:, :1], pos, f)]
+    got = mx.rotary_multi_axis(q, q[:, :1], pos, mx.RotaryFrequencies(f.inv_freq, axis, adjacent))
+    lost = [i for pair in (3, 4, 12) for i in ((2 * pair, 2 * pair + 1) if adjacent else (pair, pair + 16))]
+    for g, w in zip(got, want):
+        w[..., lost] = math.nan
+        assert torch.equal(g.isnan(), w.isnan())
+        assert torch.equal(g.nan_to_num(), w.nan_to_num())
