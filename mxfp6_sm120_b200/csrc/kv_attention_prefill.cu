@@ -722,7 +722,7 @@ kv_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       const int tiles = failed ? 0 : seg.tiles, length = seg.length, tile0 = seg.tile;
       const bool all_named = seg.all_named != 0;
       // Above zero, so that a masked score (-inf) stays one where the scale is zero.
-      const float factor = seg.scale[row] < 1e-30f ? 1e-30f : seg.scale[row];
+      const float row_factor = seg.scale[row] < 1e-30f ? 1e-30f : seg.scale[row];
       // Cached tokens that this row sees.
       int64_t sees = length;
       if (a.causal) sees = min(sees, seg.first_position + (seg.row0 + row) / a.group + 1);
@@ -768,11 +768,14 @@ kv_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         ptx::tc_fence_before();
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(sread0 + 8 * buffer);
+        float factor = row_factor;
         if (!named || !__all_sync(0xffffffffu, t0 + kKvBlock <= visible)) {
           const int n = named ? visible - t0 : 0;
 #pragma unroll
           for (int e = 0; e < 32; ++e)
             if (e >= n) raw[e] = 0xff800000u;  // -inf
+          // A row whose query has an infinity or NaN has a factor of NaN: not where it sees nothing.
+          if (n <= 0) factor = 1.0f;
         }
         float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll

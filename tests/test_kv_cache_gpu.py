@@ -765,3 +765,25 @@ def test_pairs_without_a_row_of_positions_are_nan(mx, adjacent, dtype):
         w[..., lost] = math.nan
         assert torch.equal(g.isnan(), w.isnan())
         assert torch.equal(g.nan_to_num(), w.nan_to_num())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dim,group", [(64, 4), (128, 3), (256, 2)])
+@pytest.mark.parametrize("rows", [4, 70])
+def test_rows_that_see_nothing_are_zero_whatever_they_hold(mx, rows, dim, group, causal, dtype):
+    """NaN and infinities in the query rows of a padded sequence, of positions below zero and of a
+    sequence without pages; the other rows keep their bits."""
+    batch = Batch(mx, 80, [0, rows - 1, 300, 2 * rows], [rows] * 4, 2, 32, dim)
+    batch.table[3, :] = -1
+    batch.dev = (torch.from_numpy(batch.table).to(DEV), *batch.dev[1:])
+    q = torch.randn((batch.tokens, 2 * group, dim), generator=_gen(81)).to(dtype).to(DEV)
+    want = _attend(mx, batch, q, max_query_len=rows, causal=causal)
+    _check_attention(batch, q, want, dim ** -0.5, causal)
+    blind = torch.tensor([*range(rows + (1 if causal else 0)), *range(3 * rows, 4 * rows)], device=DEV)
+    q[blind[0::3], :, 7] = math.nan
+    q[blind[1::3], :, 0] = math.inf
+    q[blind[2::3]] = -math.inf
+    got = _attend(mx, batch, q, max_query_len=rows, causal=causal)
+    assert bool((got[blind] == 0).all())
+    assert torch.equal(got, want)
