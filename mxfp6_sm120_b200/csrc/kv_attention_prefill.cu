@@ -32,6 +32,7 @@
 // left: the next rows' terms before the last rows' output (790 against 746 us, heads of 256).
 #include "kv_attention.cuh"
 
+#include <cfloat>
 #include <climits>
 #include <cstdlib>
 
@@ -721,8 +722,9 @@ kv_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       wait(qfull, (uint32_t)segment & 1u, 520);  // the other warps' scales
       const int tiles = failed ? 0 : seg.tiles, length = seg.length, tile0 = seg.tile;
       const bool all_named = seg.all_named != 0;
-      // Above zero, so that a masked score (-inf) stays one where the scale is zero.
-      const float row_factor = seg.scale[row] < 1e-30f ? 1e-30f : seg.scale[row];
+      // Above zero, so that a masked score (-inf) stays one where the scale is zero; the smallest
+      // normal number is far below any factor of a score that counts.
+      const float row_factor = seg.scale[row] < FLT_MIN ? FLT_MIN : seg.scale[row];
       // Cached tokens that this row sees.
       int64_t sees = length;
       if (a.causal) sees = min(sees, seg.first_position + (seg.row0 + row) / a.group + 1);

@@ -787,3 +787,17 @@ def test_rows_that_see_nothing_are_zero_whatever_they_hold(mx, rows, dim, group,
     got = _attend(mx, batch, q, max_query_len=rows, causal=causal)
     assert bool((got[blind] == 0).all())
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("rows", [1, 60])
+def test_small_scales_of_large_keys(mx, rows, sign, dtype):
+    """Keys of about 2^98 under a scale of 2^-101: ordinary scores, though the factor of a row's
+    scores is below 2^-100."""
+    batch = Batch(mx, 84, [333, 80], [rows, rows], 2, 32, 64)
+    batch.scales[0] = np.where(batch.scales[0] == 255, 255, batch.scales[0].astype(np.int32) + 98).astype(np.uint8)
+    batch.cache.k_scales.copy_(torch.from_numpy(batch.scales[0]))
+    q = torch.randn((2 * rows, 4, 64), generator=_gen(85)).to(dtype).to(DEV)
+    got = _attend(mx, batch, q, max_query_len=rows, scale=sign * 2.0 ** -101)
+    _check_attention(batch, q, got, sign * 2.0 ** -101, True)
