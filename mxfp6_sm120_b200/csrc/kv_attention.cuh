@@ -46,17 +46,22 @@ int make_kv_map(CUtensorMap* map, const uint8_t* values, const KvCache& cache);
 
 #ifdef __CUDACC__
 // E4M3 terms of two FP16 numbers: codes[t] holds both in its low sixteen bits.  The remainders
-// are exact in FP16.
+// are exact in FP16.  Returns what the terms add up to, exact in FP16 as well: it is a multiple of
+// x's last place, or of the second term's smallest step.  Three terms leave at most 2^-18 of x.
 template <int kTerms>
-__device__ __forceinline__ void e4m3_terms_half(__half2 x, uint32_t (&codes)[kTerms]) {
+__device__ __forceinline__ __half2 e4m3_terms_half(__half2 x, uint32_t (&codes)[kTerms]) {
+  const __half2 whole = x;
+  __half2 first{};
 #pragma unroll
   for (int t = 0; t < kTerms; ++t) {
     codes[t] = __nv_cvt_halfraw2_to_fp8x2(static_cast<__half2_raw>(x), __NV_SATFINITE, __NV_E4M3);
-    if (t + 1 < kTerms) {
-      const __half2 v(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)codes[t], __NV_E4M3));
-      x = __hmul2(__hsub2(x, v), __float2half2_rn(16.0f));
-    }
+    if (kTerms == 3 && t == 2) return whole;
+    const __half2 v(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)codes[t], __NV_E4M3));
+    if (t == 0) first = v;
+    else if (kTerms == 2) return __hfma2(v, __float2half2_rn(0.0625f), first);
+    x = __hmul2(__hsub2(x, v), __float2half2_rn(16.0f));
   }
+  return whole;
 }
 
 // 2^v of a whole v up to 127 (below -126: 2^-126): adding 1.5 * 2^23 leaves v in the low bits.

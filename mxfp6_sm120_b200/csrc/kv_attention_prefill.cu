@@ -804,11 +804,12 @@ kv_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
 #pragma unroll
           for (int n = 0; n < 4; ++n)
             p[n] = ptx::exp2_approx(__uint_as_float(raw[e + n]) * factor - base);
-          s0 += p[0] + p[2];
-          s1 += p[1] + p[3];
           uint32_t lo[TERMS], hi[TERMS];
-          e4m3_terms_half<TERMS>(__floats2half2_rn(p[0], p[1]), lo);
-          e4m3_terms_half<TERMS>(__floats2half2_rn(p[2], p[3]), hi);
+          const __half2 w0 = e4m3_terms_half<TERMS>(__floats2half2_rn(p[0], p[1]), lo);
+          const __half2 w1 = e4m3_terms_half<TERMS>(__floats2half2_rn(p[2], p[3]), hi);
+          // The sums are of the weights as they were rounded, so that they add up to one.
+          s0 = ptx::add_halves(s0, *reinterpret_cast<const uint32_t*>(&w0));
+          s1 = ptx::add_halves(s1, *reinterpret_cast<const uint32_t*>(&w1));
 #pragma unroll
           for (int k = 0; k < TERMS; ++k) codes[k][e / 4] = __byte_perm(lo[k], hi[k], 0x5410);
         }

@@ -57,6 +57,16 @@ __device__ __forceinline__ float exp2_approx(float v) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
+// s + low half + high half, in 32 bits.
+__device__ __forceinline__ float add_halves(float s, uint32_t halves) {
+  asm("{\n\t.reg .f16 lo, hi;\n\t"
+      "mov.b32 {lo, hi}, %1;\n\t"
+      "add.f32.f16 %0, lo, %0;\n\t"
+      "add.f32.f16 %0, hi, %0;\n\t}"
+      : "+f"(s)
+      : "r"(halves));
+  return s;
+}
 // Largest value over the warp, NaN ignored.
 __device__ __forceinline__ float warp_max(float v) {
   float r;

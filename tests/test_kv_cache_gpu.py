@@ -801,3 +801,33 @@ def test_small_scales_of_large_keys(mx, rows, sign, dtype):
     q = torch.randn((2 * rows, 4, 64), generator=_gen(85)).to(dtype).to(DEV)
     got = _attend(mx, batch, q, max_query_len=rows, scale=sign * 2.0 ** -101)
     _check_attention(batch, q, got, sign * 2.0 ** -101, True)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("page,dim,group", [(32, 64, 8), (128, 64, 3), (64, 128, 4), (32, 256, 6)])
+def test_first_row_of_a_prompt_is_its_value(mx, page, dim, group, dtype):
+    """The first row of a prompt sees one token, whose weight is one: its output is the token's value,
+    rounded once.  Values have four significant bits, so both types hold them."""
+    lens = [300, 64, 129, 45, 70]
+    batch = Batch(mx, 82, lens, lens, 2, page, dim)
+    for seed in (83, 84, 85):
+        q = (torch.randn((batch.tokens, 2 * group, dim), generator=_gen(seed)) * 2).to(dtype).to(DEV)
+        got = _attend(mx, batch, q, max_query_len=300)[batch.cu[:-1]]
+        want = kvo.read(batch.values[1], batch.scales[1], batch.table, [(b, 0) for b in range(5)])
+        want = torch.from_numpy(want).repeat_interleave(group, dim=1).to(dtype)
+        assert torch.equal(got.cpu(), want)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("rows", [1, 60])
+def test_weights_add_up_to_one(mx, rows, dim, dtype):
+    """Values that are all one: whatever the weights were rounded to, their mean is one.  Sums of at
+    most 400 weights in 32 bits, a reciprocal and a product are off by less than 2^-14, which rounds
+    back to one in both types."""
+    batch = Batch(mx, 86, [400, 77], [rows, rows], 2, 32, dim, finite=True)
+    batch.cache.v_values.fill_(0x38)
+    batch.cache.v_scales.fill_(127)
+    q = (torch.randn((2 * rows, 6, dim), generator=_gen(87)) * 3).to(dtype).to(DEV)
+    got = _attend(mx, batch, q, max_query_len=rows)
+    assert bool((got == 1).all())
