@@ -12,6 +12,7 @@
 // 65 us with 32).
 #include "kv_attention.cuh"
 
+#include <climits>
 #include <cmath>
 
 namespace mx {
@@ -26,6 +27,11 @@ int64_t kv_prefill_workspace(int64_t batch, int64_t tokens, int kv_heads, int gr
 int* device_status_word(int device);
 
 namespace {
+
+// Limits of a call: query heads, rows (token rows, and times the query heads of a key head), and cached
+// tokens that a block table can name (check_kv).
+constexpr int kMostHeads = 65535;
+constexpr int64_t kMostRows = int64_t(1) << 30, kMostContext = int64_t(1) << 30;
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
@@ -103,9 +109,12 @@ static AttentionPlan plan_attention(int64_t batch, int64_t tokens, int64_t max_q
 int64_t kv_cache_attention_workspace(int64_t batch, int64_t tokens, int64_t max_query_len,
                                      int q_heads, int kv_heads, int head_dim, int dtype,
                                      int64_t max_context) {
-  if (batch < 1 || tokens < 0 || max_query_len < 1 || q_heads < 1 || kv_heads < 1 ||
-      q_heads % kv_heads != 0 || (head_dim != 64 && head_dim != 128 && head_dim != 256) ||
-      (dtype != kF16 && dtype != kBF16) || max_context < 1) {
+  // The call's own limits.
+  if (batch < 1 || batch > INT_MAX || tokens < 0 || tokens > kMostRows || max_query_len < 1 ||
+      q_heads < 1 || q_heads > kMostHeads || kv_heads < 1 || q_heads % kv_heads != 0 ||
+      tokens * (q_heads / kv_heads) > kMostRows ||
+      (head_dim != 64 && head_dim != 128 && head_dim != 256) || (dtype != kF16 && dtype != kBF16) ||
+      max_context < 1 || max_context > kMostContext) {
     return -1;
   }
   if (tokens == 0) return 0;
@@ -120,7 +129,7 @@ int kv_cache_attention(const KvCache& cache, const KvBatch& batch, const void* q
                        cudaStream_t stream) {
   if (int rc = check_kv(cache, batch)) return rc;
   MX_REQUIRE(dtype == kF16 || dtype == kBF16, "q must be float16 or bfloat16");
-  MX_REQUIRE(q_heads > 0 && q_heads <= 65535 && q_heads % cache.kv_heads == 0,
+  MX_REQUIRE(q_heads > 0 && q_heads <= kMostHeads && q_heads % cache.kv_heads == 0,
              "q_heads (%d) must be a multiple of the cache's %d heads", q_heads, cache.kv_heads);
   MX_REQUIRE(max_query_len >= 1, "max_query_len must be positive");
   const float scale_log2 = scale * 1.4426950408889634f;
@@ -128,7 +137,7 @@ int kv_cache_attention(const KvCache& cache, const KvBatch& batch, const void* q
   if (batch.tokens == 0) return kOk;
   MX_REQUIRE(q != nullptr && out != nullptr, "q and out must not be null");
   const int group = q_heads / cache.kv_heads;
-  MX_REQUIRE(batch.tokens * group <= (int64_t(1) << 30), "at most 2^30 rows (tokens x group) a call");
+  MX_REQUIRE(batch.tokens * group <= kMostRows, "at most 2^30 rows (tokens x group) a call");
   const AttentionPlan plan =
       plan_attention(batch.batch, batch.tokens, max_query_len, group, cache.kv_heads,
                      cache.head_dim, dtype, (int64_t)batch.table_width * cache.page_size);

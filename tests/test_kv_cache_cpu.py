@@ -241,3 +241,27 @@ def test_rotary_refuses_positions_with_too_few_axes():
     with pytest.raises(ValueError, match="a row for each"):
         mx.rotary_multi_axis(q, q.clone(), pos[:2], mx.RotaryFrequencies(f.inv_freq, f.axis, False, 3))
     assert mx.RotaryFrequencies(f.inv_freq, f.axis).axes is None      # nothing is read from the device
+
+
+def test_workspace_query_refuses_what_the_call_refuses():
+    """-1 for sizes that the call would refuse, 0 where it needs no scratch, else its bytes."""
+    from mxfp6_sm120_b200._loader import library
+
+    query = library().mxfp6_kv_cache_attention_workspace
+    good = dict(batch=2, tokens=2, most=1, q_heads=4, kv_heads=2, dim=64, dtype=1, context=4096)
+
+    def ask(**kwargs):
+        return query(*{**good, **kwargs}.values())
+
+    # 32 tiles of 128 tokens: 4 sequences x heads of 33 units cut into shares of 3 = 44 CTAs, each with two
+    # ends of 8 rows x 64 values, a maximum and a sum; before them 148 borders of 32 bytes
+    assert ask() == 148 * 32 + 44 * 2 * (8 * 64 + 2 * 8) * 4
+    assert ask(context=1024) == 0 and ask(tokens=0) == 0
+    for bad in (dict(batch=0), dict(batch=-1), dict(batch=1 << 31), dict(tokens=-1), dict(tokens=(1 << 30) + 1, q_heads=2),
+                dict(tokens=(1 << 29) + 1), dict(tokens=1 << 62), dict(most=0), dict(q_heads=0), dict(q_heads=-2),
+                dict(q_heads=3), dict(q_heads=65536), dict(kv_heads=0), dict(kv_heads=3), dict(dim=80),
+                dict(dtype=2), dict(context=0), dict(context=(1 << 30) + 32)):
+        assert ask(**bad) == -1, bad
+        if "context" not in bad:
+            assert ask(**bad, context=64) == -1, bad
+    assert ask(tokens=1 << 29, most=1 << 29) > 0 and ask(context=1 << 30) > 0 and ask(q_heads=65534) > 0
