@@ -743,7 +743,7 @@ kv_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
           // Rows of V without a token may hold anything, NaN among them, and 0 * NaN is NaN: clear
           // them once the tile has landed.  The four warps of a block clear eight rows each.
           if constexpr (C::kSlots == 2)
-            if (i > 0) wait(pvdone0, (uint32_t)(i - 1) & 1u, 517);
+            if (i > 0) wait(pvdone0, (uint32_t)(i - 1) & 1u, 521);
           const int at = at0 + (j + 1 < tiles ? 2 * j + 2 : 2 * j + 1);
           const int slot = at % C::kSlots;
           wait(full0 + 8 * slot, (uint32_t)(at / C::kSlots) & 1u, 511);

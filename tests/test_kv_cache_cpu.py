@@ -265,3 +265,21 @@ def test_workspace_query_refuses_what_the_call_refuses():
         if "context" not in bad:
             assert ask(**bad, context=64) == -1, bad
     assert ask(tokens=1 << 29, most=1 << 29) > 0 and ask(context=1 << 30) > 0 and ask(q_heads=65534) > 0
+
+
+@pytest.mark.parametrize("name,hundred", [("kv_attention_decode", 4), ("kv_attention_prefill", 5)])
+def test_a_status_code_names_one_wait(name, hundred):
+    """The code that a wait leaves when it runs out tells which barrier was waited for where: no two
+    waits of a kernel share one, but for the two places of which a variant compiles one."""
+    import re
+    from pathlib import Path
+
+    text = (Path(mx.__file__).parent / "csrc" / f"{name}.cu").read_text()
+    calls = re.findall(rf"\b(bounded_wait|wait|wait_output|meet)\(((?:[^;{{}}]*?,)?\s*({hundred}\d\d))\)", text)
+    places: dict[str, list[str]] = {}
+    for _, arguments, code in calls:
+        places.setdefault(code, []).append(re.sub(r"\s+", " ", arguments))
+    assert len(places) >= 14
+    for code, found in places.items():
+        assert len(set(found)) == 1, (code, found)
+        assert len(found) == 1 or all("sfull0" in f for f in found), (code, found)
