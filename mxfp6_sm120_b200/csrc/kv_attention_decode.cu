@@ -39,6 +39,7 @@
 // and end, where the groups meet.  Tried and left: a third softmax group (78 us for the last case).
 #include "kv_attention.cuh"
 
+#include <cfloat>
 #include <climits>
 #include <cstdlib>
 
@@ -742,10 +743,11 @@ kv_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
             float p[4];
 #pragma unroll
             for (int n = 0; n < 4; ++n) {
-              // To the nearest power of two: the largest weight is in (181, 363).
+              // To the nearest power of two: the largest weight is in (181, 363).  Where nothing is
+              // seen (-inf) the lowest finite base keeps the weights zero.
               const float top = rintf(ptx::warp_max(s[r + n]));
               if (lane % RP == c0 + r + n) my_top = top;
-              p[n] = ptx::exp2_approx(s[r + n] - (fmaxf(top, -1e30f) - kWeightLog2));
+              p[n] = ptx::exp2_approx(s[r + n] - (fmaxf(top, -FLT_MAX) - kWeightLog2));
             }
             uint32_t lo[TERMS], hi[TERMS];
             e4m3_terms_half<TERMS>(__floats2half2_rn(p[0], p[1]), lo);

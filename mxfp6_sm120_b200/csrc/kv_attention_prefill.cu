@@ -795,7 +795,8 @@ kv_prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
           if (ask) *asked = 1;
           ptx::mbar_arrive(vsync);
         }
-        const float base = fmaxf(top, -1e30f) - kWeightLog2;
+        // Where nothing is seen (-inf) the lowest finite base keeps the weights zero.
+        const float base = fmaxf(top, -FLT_MAX) - kWeightLog2;
         uint32_t codes[TERMS][8];
         float s0 = 0.0f, s1 = 0.0f;
 #pragma unroll

@@ -831,3 +831,18 @@ def test_weights_add_up_to_one(mx, rows, dim, dtype):
     q = (torch.randn((2 * rows, 6, dim), generator=_gen(87)) * 3).to(dtype).to(DEV)
     got = _attend(mx, batch, q, max_query_len=rows)
     assert bool((got == 1).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [64, 256])
+@pytest.mark.parametrize("rows", [1, 60])
+def test_equal_scores_far_below_zero(mx, rows, dim, dtype):
+    """Scores of about -2^115 (2^13 * 2^98 * dim / sqrt(dim)), the same for every token: the weights are
+    equal, not all zero."""
+    batch = Batch(mx, 88, [300, 70], [rows, rows], 1, 32, dim, finite=True)
+    batch.values[0][:], batch.scales[0][:] = 0x38, 127 + 98
+    batch.cache.k_values.fill_(0x38)
+    batch.cache.k_scales.fill_(127 + 98)
+    q = torch.full((2 * rows, 4, dim), -(2.0 ** 13), dtype=dtype, device=DEV)
+    got = _attend(mx, batch, q, max_query_len=rows)
+    _check_attention(batch, q, got, dim ** -0.5, True)
