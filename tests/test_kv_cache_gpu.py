@@ -846,3 +846,60 @@ def test_equal_scores_far_below_zero(mx, rows, dim, dtype):
     q = torch.full((2 * rows, 4, dim), -(2.0 ** 13), dtype=dtype, device=DEV)
     got = _attend(mx, batch, q, max_query_len=rows)
     _check_attention(batch, q, got, dim ** -0.5, True)
+
+
+def _check_rounded_weights(batch, q, got, scale):
+    """As _check_attention, from what the weights are held in.  Each is off by a factor 1 + d_j, |d_j| <= d,
+    and the row is divided by the sum of the weights as they were rounded: with o the exact output,
+
+        sum_j p_j (1 + d_j) v_j / sum_j p_j (1 + d_j) - o = sum_j p_j d_j (v_j - o) / (1 + sum_j p_j d_j)
+
+    which is at most d / (1 - d) * sum_j p_j |v_j - o|.  d = 2^-11 for the rounding to FP16, and for BF16
+    2^-9 more for the second E4M3 term; 2^-13 more covers 32-bit scores below 40 (24 sums of 2^-24 each)
+    and exponentials, and the division.  Weights below 2^-3 (2^-7 with three terms) of the 181 and more
+    that the largest of their block is scaled to are off by 2^-14 (2^-18) instead: less than 2^-21 (2^-25)
+    of the sum a token, times twice the largest value.  The output is rounded once more, by half a step."""
+    want = batch.oracle_attention(q, scale, True)
+    rows = kvo.to_numpy(q)
+    bf16 = q.dtype is torch.bfloat16
+    d = 2.0 ** -11 + 2.0 ** -13 + (2.0 ** -9 if bf16 else 0.0)
+    group = q.shape[1] // batch.heads
+    for b, length in enumerate(batch.lens):
+        where = [(b, p) for p in range(length)]
+        k = kvo.read(batch.values[0], batch.scales[0], batch.table, where)
+        v = kvo.read(batch.values[1], batch.scales[1], batch.table, where)
+        n = batch.cu[b + 1] - batch.cu[b]
+        for i in range(n):
+            sees = length - n + i + 1
+            for h in range(q.shape[1]):
+                s = k[:sees, h // group] @ rows[batch.cu[b] + i, h] * scale
+                p = np.exp(s - s.max())
+                o, seen = want[batch.cu[b] + i, h], v[:sees, h // group]
+                apart = (p[:, None] * np.abs(seen - o)).sum(0) / p.sum()
+                few = sees * (2.0 ** -21 if bf16 else 2.0 ** -25) * 2 * np.abs(seen).max()
+                limit = torch.finfo(q.dtype).eps / 2 * np.abs(o) + d / (1 - d) * apart + few
+                off = np.abs(kvo.to_numpy(got[batch.cu[b] + i, h]) - o)
+                assert np.all(off <= limit + 2.0 ** -25), (b, i, h, float((off - limit).max()))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim,group", [(64, 129), (128, 200), (256, 256)])
+def test_more_query_heads_than_a_tile_has_rows(mx, dim, group, dtype):
+    """The query heads of one token fill a row tile and more; whole vectors and odd strides."""
+    for news in ([1, 1, 1], [2, 5, 1]):
+        batch = Batch(mx, 89, [300, 5, 45], news, 1, 64, dim)
+        wide = torch.randn((batch.tokens, group * dim + 1), generator=_gen(90)).to(dtype).to(DEV)
+        for q in (wide[:, :-1].contiguous().view(batch.tokens, group, dim),
+                  wide[:, 1:].view(batch.tokens, group, dim)):
+            got = _attend(mx, batch, q, max_query_len=max(news))
+            _check_rounded_weights(batch, q, got, dim ** -0.5)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("rows", [2, 45])
+def test_rows_within_what_their_weights_are_held_in(mx, rows, dim, dtype):
+    batch = Batch(mx, 91, [260, rows, 97], [rows] * 3, 2, 32, dim)
+    q = torch.randn((batch.tokens, 8, dim), generator=_gen(92)).to(dtype).to(DEV)
+    got = _attend(mx, batch, q, max_query_len=rows)
+    _check_rounded_weights(batch, q, got, dim ** -0.5)
