@@ -5,9 +5,19 @@
 // block scales, kind::mxf8f6f4).  The other operand of each product, 16-bit queries and 32-bit
 // weights, becomes a sum of E4M3 terms x = t0 + t1 / 16 (+ t2 / 256): a term keeps four
 // significant bits, rounding to nearest makes the remainder at most half a step (2^-4 relative to
-// the binade), so each further term takes four more.  Two terms hold a BF16 query (8 bits)
-// exactly, three an FP16 one (11 bits); for the weights the error is at most 2^-9 and 2^-14.  The
-// products of all terms accumulate in 32 bits.
+// the binade), so each further term takes four more.  Below E4M3's smallest normal number a term's
+// step is fixed, so that two terms leave up to 2^-14 of a small x and three up to 2^-18.
+//  * Queries are scaled so that a row's largest magnitude is in (224, 448].  Two terms hold a BF16
+//    query (8 bits) exactly from 2^-6 on, three an FP16 one (11 bits) from 2^-7 on; what is smaller
+//    is off by at most 2^-14 and 2^-18: 2^-21 and 2^-25 of the row's largest.
+//  * Weights (largest of a block in (181, 363)) are rounded to FP16 first, where two of them become
+//    terms with one instruction a step: off by up to 2^-11.  Two terms leave 2^-9 of the binade
+//    beside it, three nothing.  2^-9 + 2^-11 for BF16 and 2^-11 for FP16 are chosen: no more than
+//    the half step (2^-8, 2^-11) that the output is rounded by, and rows are divided by the sum of
+//    the weights as they were rounded, so that a row is not off as a whole.  A third term for BF16
+//    would be half as many matrix instructions again.
+// The products of all terms accumulate in 32 bits, weights 2^8 times and, where a block exceeds its
+// row's reference, 2^24 times their size: values up to 2^80 in magnitude cannot overflow.
 #pragma once
 
 #include "kv_cache.cuh"

@@ -3,9 +3,9 @@
 // S = Q K^T and O = P V on 128 rows (new tokens x query heads of a key head, flattened) by 128
 // cached tokens.  K and V are read by tcgen05.mma as they lie in the pages (TMA tiles, block
 // scales in hardware, V as an MN-major operand); Q and P are E4M3 terms (kv_attention.cuh): a
-// product is two passes (BF16; three for FP16) at the 8-bit rate, so the tensor cores bound it at
-// what they give 16-bit operands, with half the bytes per cached token and no conversion of a
-// cached value anywhere.
+// BF16 product is two passes at the 8-bit rate, so the tensor cores bound it at what they give 16-bit
+// operands, with half the bytes per cached token and no conversion of a cached value anywhere.  An
+// FP16 product is three passes, half as much again.
 //
 //  * The terms of a product accumulate into the same tensor memory: their factors 1, 1/16, 1/256
 //    are block scales of the A operand.
@@ -23,13 +23,16 @@
 //    equal shares, one per SM; an item that is cut leaves partial rows, which a second kernel
 //    joins in the order of the tiles.
 //
-// Measured inside a CUDA graph: a prompt of 8192 tokens, 24 query and 4 key heads of 256: 710 to 770 us
-// (boxes and clocks differ), 1.07 to 1.16 PFLOP/s of 16-bit products, tensor pipes 57 % active at
-// 1.67 GHz.  The scores' product reads both operands from shared memory, 128 bytes a clock, which is
+// Measured inside a CUDA graph: a prompt of 8192 tokens, 24 query and 4 key heads of 256: 710 to 770 us,
+// back to back 830 (boxes and clocks differ), 0.99 to 1.16 PFLOP/s of 16-bit products, tensor pipes 57 %
+// active at 1.64 GHz; in FP16 1040 to 1100 us.  The scores' product reads both operands from shared memory, 128 bytes a clock, which is
 // all it gives, beside the copies into the ring: without any exponential the time is the same, with
-// half the products 690 us.  Five chunks of 1500 tokens over 12000, 8 rows per key head of 128: 320 us,
-// 0.59 PFLOP/s; here the softmax bounds it (without exponentials and E4M3 terms 252 us).  Tried and
-// left: the next rows' terms before the last rows' output (790 against 746 us, heads of 256).
+// half the products 690 us.  Five chunks of 1500 tokens over 12000, 8 rows per key head of 128:
+// 306 to 325 us, 0.58 to 0.62 PFLOP/s (FP16 390 to 400 us).  Here no unit is at its limit: issue slots
+// 64 %, ALU 56 %, special functions 32 %, tensor pipes 31 %, shared memory 17 % of their peaks; four
+// softmax warps a scheduler do not cover the chain of a tile (scores, maximum, exponentials, conversions,
+// weights through shared memory, product).  Without exponentials and E4M3 terms 252 us.  Tried and left:
+// the next rows' terms before the last rows' output (790 against 746 us, heads of 256).
 #include "kv_attention.cuh"
 
 #include <cfloat>
@@ -47,7 +50,8 @@ constexpr float kWeightLog2 = 8.0f;   // weights are scaled by 256 before they b
 constexpr float kMostLog2 = 16.0f;    // a block may exceed the reference by 2^16
 constexpr int kSms = 148;
 // What an item costs beside its tiles: about 8 us, a tile 1.7 us.  8192-token prompt, heads of 256: with
-// 3 units 940 us, 4 810, 5 740, 6 750; five chunks, heads of 128: 329, 322, 327, 329 us.
+// 3 units 940 us, 4 810, 5 740, 6 750; five chunks, heads of 128: 329, 322, 327, 329 us.  Other lengths
+// were not tried; part of the first row may be how 8192 tokens divide.
 constexpr int kItemUnits = 5;
 constexpr int kMinUnits = 4;          // units a CTA takes at least
 

@@ -16,6 +16,9 @@ Every operator takes the same description of a batch:
 All three live on the device and are read there while the call runs (they must not change
 meanwhile), so a captured CUDA graph follows them; rows behind ``cu_seqlens[batch]`` are left as
 they were.
+
+These are serving operators without a backward pass: results carry no gradient, whatever their
+inputs require.
 """
 
 from __future__ import annotations
@@ -69,7 +72,8 @@ class PagedKVCache:
 
     ``k_values`` / ``v_values``: uint8 E4M3 codes ``[pages, kv_heads, page_size, head_dim]``;
     ``k_scales`` / ``v_scales``: uint8 UE8M0 codes ``[pages, kv_heads, page_size // 32]``, one per
-    32 tokens of a page and head: a value is ``code * 2**(scale - 127)``.
+    32 tokens of a page and head: a value is ``code * 2**(scale - 127)``.  Scale codes of blocks that
+    hold tokens are 0 to 254 (:func:`kv_cache_write` makes 28 to 253); 255 is no number.
     """
 
     k_values: torch.Tensor
@@ -295,7 +299,9 @@ def kv_cache_attention(q: torch.Tensor, cache: PagedKVCache, block_table: torch.
     upper bound of the rows of any sequence (default: 1 without ``cu_seqlens``, else all rows); a
     tight one picks the better kernel, and rows of a sequence that has more may be left unwritten.
     Write the rows' own keys and values first (:func:`kv_cache_write` takes the same
-    ``block_table``, ``seq_lens`` and ``cu_seqlens``).  ``out`` must not overlap ``q``.
+    ``block_table``, ``seq_lens`` and ``cu_seqlens``).  ``out`` must not overlap ``q``.  Sums are
+    32-bit: values up to 2^80 in magnitude cannot overflow them, nor scores that fit 32 bits.  A block
+    table that names at most 1024 tokens a sequence takes a form for short ones.
     """
     if q.ndim != 3:
         raise ValueError(f"q must be [tokens, q_heads, head_dim]; got {tuple(q.shape)}")
