@@ -25,14 +25,15 @@
 //
 // Measured inside a CUDA graph: a prompt of 8192 tokens, 24 query and 4 key heads of 256: 710 to 770 us,
 // back to back 830 (boxes and clocks differ), 0.99 to 1.16 PFLOP/s of 16-bit products, tensor pipes 57 %
-// active at 1.64 GHz; in FP16 1040 to 1100 us.  The scores' product reads both operands from shared memory, 128 bytes a clock, which is
-// all it gives, beside the copies into the ring: without any exponential the time is the same, with
-// half the products 690 us.  Five chunks of 1500 tokens over 12000, 8 rows per key head of 128:
-// 306 to 325 us, 0.58 to 0.62 PFLOP/s (FP16 390 to 400 us).  Here no unit is at its limit: issue slots
-// 64 %, ALU 56 %, special functions 32 %, tensor pipes 31 %, shared memory 17 % of their peaks; four
-// softmax warps a scheduler do not cover the chain of a tile (scores, maximum, exponentials, conversions,
-// weights through shared memory, product).  Without exponentials and E4M3 terms 252 us.  Tried and left:
-// the next rows' terms before the last rows' output (790 against 746 us, heads of 256).
+// active at 1.64 GHz; in FP16 1040 to 1100 us.  The scores' product reads both operands from shared
+// memory, 128 bytes a clock, which is all it gives, beside the copies into the ring: without any
+// exponential the time is the same, with half the products 690 us.
+// Five chunks of 1500 tokens over 12000, 8 rows per key head of 128: 306 to 325 us, 0.58 to 0.62 PFLOP/s
+// (FP16 390 to 400 us).  Here no unit is at its limit: issue slots 64 %, ALU 56 %, special functions 32 %,
+// tensor pipes 31 %, shared memory 17 % of their peaks; four softmax warps a scheduler do not cover the
+// chain of a tile (scores, maximum, exponentials, conversions, weights through shared memory, product).
+// Without exponentials and E4M3 terms 252 us.
+// Tried and left: the next rows' terms before the last rows' output (790 against 746 us, heads of 256).
 #include "kv_attention.cuh"
 
 #include <cfloat>

@@ -300,8 +300,8 @@ def kv_cache_attention(q: torch.Tensor, cache: PagedKVCache, block_table: torch.
     tight one picks the better kernel, and rows of a sequence that has more may be left unwritten.
     Write the rows' own keys and values first (:func:`kv_cache_write` takes the same
     ``block_table``, ``seq_lens`` and ``cu_seqlens``).  ``out`` must not overlap ``q``.  Sums are
-    32-bit: values up to 2^80 in magnitude cannot overflow them, nor scores that fit 32 bits.  A block
-    table that names at most 1024 tokens a sequence takes a form for short ones.
+    32-bit: keys and values up to 2^80 in magnitude overflow none of them while the scores fit 32
+    bits.  A block table that names at most 1024 tokens a sequence takes a form for short ones.
     """
     if q.ndim != 3:
         raise ValueError(f"q must be [tokens, q_heads, head_dim]; got {tuple(q.shape)}")
@@ -415,8 +415,9 @@ def rotary_multi_axis(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
 
     ``positions``: int32 or int64 ``[axes, tokens]`` (or ``[tokens]`` for one axis); pair ``i`` of
     every head turns by ``positions[axis[i], token] * inv_freq[i]`` radians, computed in 64 bits.
-    ``positions`` may have more rows than ``frequencies.axes``, not fewer.  Values behind ``rotary_dim`` are copied.  ``q_out`` / ``k_out`` may be ``q`` / ``k``
-    themselves (in place); other overlaps are not allowed.
+    ``positions`` may have more rows than ``frequencies.axes``, not fewer.  Values behind
+    ``rotary_dim`` are copied.  ``q_out`` / ``k_out`` may be ``q`` / ``k`` themselves (in place);
+    other overlaps are not allowed.
     """
     if not isinstance(frequencies, RotaryFrequencies):
         raise TypeError("frequencies must be a RotaryFrequencies instance")
